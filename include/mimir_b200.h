@@ -6,12 +6,14 @@
  * mimir_b200_last_error() gives a thread-local message.  The library never throws and never
  * falls back to the CPU: an op it cannot run returns MIMIR_B200_E_UNSUPPORTED.
  *
- * Three groups of entry points:
+ * Four groups of entry points:
  *   1. life cycle and device-memory budget  (mirror of MemoryGuard's verbs)
  *   2. per-op calls with HOST pointers      (mirror of ComputeEngine::linearForward,
  *      one call per `case LayerType::X` of Model::forwardPassView)
  *   3. whole-graph calls                    (mirror of Model::forwardPassView itself: the
  *      layer list is translated once, weights are uploaded once, activations stay in HBM)
+ *   4. serving calls with DEVICE pointers   (rotary positions, a paged key / value cache, attention
+ *      over it, sampling)
  *
  * Layout conventions are the reference's: every activation is a flat row-major fp32 vector for
  * one sample (images CHW, sequences [seq, dim]); `batch` is a leading dimension added by this
@@ -458,7 +460,8 @@ int mimir_b200_argmax_rows_device(const float* x_dev, int32_t* ids_dev, long lon
                                   void* stream);
 int mimir_b200_get_stats(MimirB200Stats* out);
 /* Reads (and clears) the device word that bounded in-kernel waits set when they give up:
- * OK, or E_TIMEOUT.  model_forward and the host-pointer calls check it themselves. */
+ * OK, or E_TIMEOUT.  model_forward and the host-pointer calls check it themselves.  Also reads (and clears) what the calls of
+ * section 4 found in device memory that does not fit: E_INVALID. */
 int mimir_b200_check_device(void* stream);
 /* Runs the give-up path of the kernels' bounded waits on purpose: one thread block waits `limit_ns` (at most 100 ms)
  * on a barrier that nothing arrives on, then sets the device error word, drains and returns normally.  The next
@@ -510,6 +513,138 @@ int mimir_b200_dev_softmax(const float* x, float* y, int batch, long long n, int
                            void* stream);
 int mimir_b200_dev_eltwise(int op, const float* a, const float* b, float* y, int batch, long long n,
                            long long nb, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * 4. Serving: rotary positions, a paged key / value cache, attention over it, a token from logits
+ *
+ * What a host that generates text for many users at once needs next to the layer ops; no counterpart in the reference, whose
+ * generation re-runs the prefix.  Device pointers, asynchronous on `stream` (a cudaStream_t of the calling thread's current
+ * device, which the pointers belong to).  Nothing is allocated, nothing synchronises: the calls can be captured into a CUDA
+ * graph (lengths, page tables, positions and random numbers are read when the graph runs; the host numbers n_seqs, n_rows,
+ * max_rows and max_kv are limits that size the launch).  Calls that run at the same time must not share a workspace.
+ * Sizes and pointers that the host can see are checked (E_INVALID, E_UNSUPPORTED).  Numbers in device memory are checked by the
+ * kernels before they index anything: a sequence whose rows or length do not fit has its rows left as they are (rows) or sees no
+ * keys (length), a page number outside the cache has its keys left out, and the next mimir_b200_check_device reports E_INVALID.
+ * ------------------------------------------------------------------------------------------ */
+
+#define MIMIR_B200_MAX_ROPE_PAIRS 128
+
+typedef enum MimirB200Type {
+  MIMIR_B200_T_F32 = 0,
+  MIMIR_B200_T_F16 = 1,
+  MIMIR_B200_T_BF16 = 2,
+  MIMIR_B200_T_I8 = 3,  /* caches: code * scale, scale = (largest magnitude of the vector) * (1 / 127 in fp32) */
+  MIMIR_B200_T_E4M3 = 4 /* caches: likewise with 448, codes are 8-bit floats of 4 exponent and 3 mantissa bits */
+} MimirB200Type;
+
+/* Rotary positions.  Pair i of the first rot_dim elements of a head is turned by position * f_i, f_i = base^(-2 i / rot_dim);
+ * its elements are 2 i and 2 i + 1 (interleaved) or i and i + rot_dim / 2.  The other elements pass unchanged.
+ *   LINEAR  f_i / factor.
+ *   BANDS   r = original_len * f_i / (2 pi) turns over the original length: f_i from r = high on, f_i / factor up to r = low, linear
+ *           in r in between.
+ *   RAMP    f_i ((1 - w) + w / factor), w = (i - a) / (b - a) within 0 .. 1, where a = max(floor d(high), 0), b = min(ceil d(low),
+ *           rot_dim - 1), d(r) = rot_dim ln(original_len / (2 pi r)) / (2 ln base); b - a = 0.001 where they are equal. */
+typedef enum MimirB200RopeScaling {
+  MIMIR_B200_ROPE_NONE = 0,
+  MIMIR_B200_ROPE_LINEAR = 1,
+  MIMIR_B200_ROPE_BANDS = 2,
+  MIMIR_B200_ROPE_RAMP = 3
+} MimirB200RopeScaling;
+
+typedef struct MimirRopeSpec {
+  int32_t rot_dim, interleaved, scaling, inverse; /* inverse != 0: turns back (also the gradient's way) */
+  double base, factor, low, high, original_len;   /* the last four as the scaling needs them */
+  double magnitude;                               /* multiplies cosines and sines; 0 = 1 */
+} MimirRopeSpec;
+
+typedef struct MimirRopePlan {
+  uint64_t step[MIMIR_B200_MAX_ROPE_PAIRS]; /* f_i in turns, modulo whole turns, times 2^64 */
+  float magnitude;
+  int32_t rot_dim, interleaved, reserved;
+} MimirRopePlan;
+
+/* The plan of a specification (host arithmetic, no device); a program keeps it. */
+int mimir_b200_rope_plan(const MimirRopeSpec* spec, MimirRopePlan* plan);
+/* y = x turned by the rows' positions (any int32).  x and y are [rows][heads][head_dim] with strides in elements (queries and keys of
+ * one projection are one call, heads counted together), type F32, F16 or BF16.  y == x with equal strides works in place; other
+ * overlaps are not allowed. */
+int mimir_b200_dev_rope(const MimirRopePlan* plan, const int32_t* positions, const void* x, void* y, long long rows, int heads,
+                        int head_dim, long long x_row_stride, long long x_head_stride, long long y_row_stride,
+                        long long y_head_stride, int type, void* stream);
+
+/* A cache of pages.  Element d of the key of a slot and head lies at page * page_stride + slot * slot_stride + head * head_stride + d
+ * (elements), values likewise, so both [page][slot][head][d] and [page][head][slot][d] are caches.  page_size is a multiple of
+ * 8, head_dim a multiple of 8 up to 256, strides multiples of 8, pointers 16-byte aligned.  I8 and E4M3 have one scale per slot and
+ * head, [page][head][slot] without gaps. */
+typedef struct MimirPagedCache {
+  void* k;
+  void* v;
+  float* k_scale; /* I8 and E4M3 only */
+  float* v_scale;
+  int64_t page_stride, slot_stride, head_stride;
+  int32_t type, n_pages, page_size, kv_heads, head_dim;
+} MimirPagedCache;
+
+/* A ragged batch: sequence s has the new rows row_start[s] .. row_start[s + 1] - 1 of the row tensors and kv_len[s] keys, its new ones
+ * included (the last of them are the new rows'), key j in page page_table[s * table_stride + j / page_size].  Rows of no sequence are
+ * left as they are.  Entries of the table that no call reads may hold anything. */
+typedef struct MimirPagedBatch {
+  const int32_t* row_start;  /* device [n_seqs + 1] */
+  const int32_t* kv_len;     /* device [n_seqs] */
+  const int32_t* page_table; /* device [n_seqs][table_stride] */
+  int64_t table_stride;
+  int32_t n_seqs, n_rows;    /* n_rows: rows of the row tensors */
+  int32_t max_rows, max_kv;  /* most new rows and most keys that a sequence has */
+} MimirPagedBatch;
+
+/* The new rows' keys and values, [n_rows][kv_heads][head_dim] of type F32, F16 or BF16 with strides in elements (multiples of 8,
+ * pointers 16-byte aligned), into the pages: rounded to the cache's type to nearest, or as codes (IEEE division by the scale, to
+ * nearest).  The largest magnitude is over finite elements; infinities become the largest code, and what is not a number 0 (I8)
+ * or not a number (E4M3).  A row before its sequence's first key (more rows than keys) is not stored.  Slots of other rows keep their
+ * contents.  Two rows that share a slot leave either's code. */
+int mimir_b200_dev_cache_write(const MimirPagedCache* cache, const MimirPagedBatch* batch, const void* k, const void* v, int type,
+                               long long row_stride, long long head_stride, void* stream);
+/* Every sequence's keys and values out of the pages: key j of sequence s to row out_start[s] + j of k and v, [out_rows][kv_heads][head_dim]
+ * (batch: kv_len, page_table, n_seqs and max_kv are read).  out_start (device, [n_seqs + 1]) ascends; of a range shorter than the
+ * sequence only its rows are written, of a longer one only the sequence's. */
+int mimir_b200_dev_cache_read(const MimirPagedCache* cache, const MimirPagedBatch* batch, const int32_t* out_start, int out_rows, void* k,
+                              void* v, int type, long long row_stride, long long head_stride, void* stream);
+
+/* Attention of the new rows over their sequences' cached keys (the new rows' own are written first, by dev_cache_write):
+ * out = softmax(scale q k^T) v per head, query head h with key head h / (heads / kv_heads).  New row i of a sequence has position
+ * kv_len - rows + i; causal: it sees keys up to its position; window > 0: keys above position - window.  A row that sees no key is
+ * zero and its lse -infinity.  Keys and values that no row of the sequence's call sees are not used whatever they hold.
+ * type (of q and out): F32, F16 or BF16 on caches of type F16, I8, E4M3; BF16 on BF16; F32 on F32 (whose keys and values have the
+ * range of the default operand planes, +-65504).  Scores, sums and results are kept in fp32. */
+typedef struct MimirPagedAttention {
+  const void* q;                              /* [n_rows][heads][head_dim], strides in elements, multiples of 8, 16-byte aligned */
+  void* out;                                  /* the same shape */
+  float* lse;                                 /* [n_rows][heads] natural logarithms of the sums of exponentials, or NULL */
+  void* workspace;                            /* mimir_b200_paged_attention_workspace bytes, 16-byte aligned; contents do not matter */
+  uint64_t workspace_bytes;
+  int64_t row_stride, head_stride, out_row_stride, out_head_stride;
+  int32_t type, heads, causal, window;
+  float scale;
+  int32_t reserved;
+} MimirPagedAttention;
+/* Bytes of workspace that a call with these sizes needs (0: none).  Pointers are not looked at. */
+int mimir_b200_paged_attention_workspace(const MimirPagedCache* cache, const MimirPagedBatch* batch, const MimirPagedAttention* attention,
+                                         uint64_t* bytes);
+int mimir_b200_dev_paged_attention(const MimirPagedCache* cache, const MimirPagedBatch* batch, const MimirPagedAttention* attention,
+                                   void* stream);
+
+/* A token from each row of n logits (F32, F16 or BF16, row_stride elements apart) by a given random number; beside
+ * mimir_b200_argmax_rows_device.  w_i = exp((x_i - max) / temperature).  Of the logits in the order (larger first, then lower
+ * index) the first top_k (<= 0 or >= n: all), of those the shortest beginning with at least top_p of their mass (>= 1: all; at least
+ * one), of those the ones with w_i >= min_p stay.  The token is the first index at which the running sum of w (in index order)
+ * exceeds uniform * (sum of w).  temperature <= 0: the largest logit's first index.  A logit of -infinity or not a number is never
+ * taken; +infinity is taken at once; a row without any gives id -1.  Sums are exact integers of w in units of 2^-45 (n up to 131 072)
+ * or finer, so that a result does not depend on how the work is divided.
+ * temperature, top_k, top_p, min_p: one per row in device memory, or NULL (1, all, 1, 0).  uniform: one per row, in [0, 1).
+ * logprob (or NULL): the logarithm of the taken token's share of what stayed.  n up to 2^24. */
+int mimir_b200_dev_sample_rows(const void* logits, int type, long long rows, int n, long long row_stride, const float* temperature,
+                               const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* ids,
+                               float* logprob, void* stream);
 
 #ifdef __cplusplus
 }

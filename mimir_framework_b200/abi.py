@@ -1,7 +1,7 @@
 """ctypes view of ``include/mimir_b200.h``.
 
 Only declarations live here: the structs (``MimirLayerDesc``, ``MimirNamedInput``,
-``MimirB200Stats``), the status codes and the loader of ``libmimir_b200.so``.  The loader raises
+``MimirB200Stats``, those of the serving calls), the status codes and the loader of ``libmimir_b200.so``.  The loader raises
 if the library has not been built — there is no Python or CPU stand-in for any op.
 """
 from __future__ import annotations
@@ -19,6 +19,11 @@ STATUS_NAMES = ["OK", "E_INVALID", "E_UNSUPPORTED", "E_OOM_BUDGET", "E_CUDA", "E
 PREC_BF16X2, PREC_BF16W, PREC_BF16 = 0, 1, 2
 ELT_ADD, ELT_MULTIPLY, ELT_GELU, ELT_SILU, ELT_RELU, ELT_TANH, ELT_SIGMOID = range(7)
 ELT_LEAKY_RELU, ELT_SOFTPLUS, ELT_MISH, ELT_HARD_SIGMOID, ELT_HARD_SWISH, ELT_SUBTRACT, ELT_DIVIDE, ELT_ELU = range(7, 15)
+
+
+T_F32, T_F16, T_BF16, T_I8, T_E4M3 = range(5)  # MimirB200Type
+ROPE_SCALING = {"none": 0, "linear": 1, "bands": 2, "ramp": 3}
+MAX_ROPE_PAIRS = 128
 
 
 class MimirLayerDesc(C.Structure):
@@ -93,6 +98,33 @@ class MimirB200Stats(C.Structure):
         ("bytes_last_forward", C.c_uint64),
         ("ms_last_forward", C.c_float),
     ]
+
+
+class MimirRopeSpec(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rot_dim", "interleaved", "scaling", "inverse")] + [
+        (n, C.c_double) for n in ("base", "factor", "low", "high", "original_len", "magnitude")]
+
+
+class MimirRopePlan(C.Structure):
+    _fields_ = [("step", C.c_uint64 * MAX_ROPE_PAIRS), ("magnitude", C.c_float), ("rot_dim", C.c_int32), ("interleaved", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class MimirPagedCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_int64) for n in ("page_stride", "slot_stride", "head_stride")] + [
+        (n, C.c_int32) for n in ("type", "n_pages", "page_size", "kv_heads", "head_dim")]
+
+
+class MimirPagedBatch(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("row_start", "kv_len", "page_table")] + [("table_stride", C.c_int64)] + [
+        (n, C.c_int32) for n in ("n_seqs", "n_rows", "max_rows", "max_kv")]
+
+
+class MimirPagedAttention(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "lse", "workspace")] + [("workspace_bytes", C.c_uint64)] + [
+        (n, C.c_int64) for n in ("row_stride", "head_stride", "out_row_stride", "out_head_stride")] + [
+        (n, C.c_int32) for n in ("type", "heads", "causal", "window")] + [("scale", C.c_float), ("reserved", C.c_int32)]
 
 
 # Defaults of the reference's `struct Layer` (Layers.hpp:86-219) for the fields the descriptor

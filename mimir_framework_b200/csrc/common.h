@@ -95,6 +95,7 @@ struct Context {
   std::vector<uint8_t*> stage_blocks;      // page-locked blocks of STAGE_BYTES, likewise (StageBlock, ops.h)
   std::atomic<uint64_t> error_clears{0};
   int last_error_site = 0;
+  std::atomic<bool> paged_used{false};     // a call of the serving group has run: the word behind dev_error_word may hold its findings
   // Optional live timing of the contraction kernel: pairs of events recorded on the launching
   // stream around every GEMM launch while enabled (read back by mimir_b200_profile_read).
   bool prof_gemm = false;
@@ -160,6 +161,9 @@ int launch_stage_copy(const StageItems& items, cudaStream_t st);
 // src -> device -> dst through a copier of its own that meets failures on the host: `inject` 1 page-locked memory, 2 a second thread,
 // are not to be had
 int host_copy_selftest(int inject, const float* src, float* dst, size_t n, int* ring_copies);
+// E_INVALID where a kernel of the serving group found device-side numbers that do not fit since the last call (serve.cu); the stream
+// has drained
+int paged_flags_read(cudaStream_t st);
 // Frees every buffer of the RuntimeAllocator verbs on the current device (shutdown).
 void release_owned_buffers();
 

@@ -2381,7 +2381,8 @@ int mimir_b200_check_device(void* stream) {
   ErrorWatch errors;
   MB_TRY(errors.enqueue(st));
   MB_CUDA(cudaStreamSynchronize(st));
-  return errors.read(st);
+  MB_TRY(errors.read(st));
+  return paged_flags_read(st);
 }
 
 // Live timing of the contraction kernel with CUDA events on the launching stream.

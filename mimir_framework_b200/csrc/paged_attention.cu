@@ -1,0 +1,649 @@
+// paged_attention.cu — attention of new tokens over a paged key / value cache: softmax(scale q k^T + mask) v per head, the heads of a
+// group sharing their key head, each sequence with its own lengths.
+//
+// One token a sequence reads every cached key and value once and computes little: the cache's bytes at the memory rate are the
+// floor.  So K and V go from global memory straight into the registers that feed the tensor instruction (mma.sync m16n8k16), with no
+// shared memory between: the contraction index of Q K^T may be permuted (Q's fragments are laid out the same way), and so may the
+// columns of P V, so that a lane reads eight consecutive elements of a row each time and a warp whole sectors.
+//   rows     16 (token, head of the group) pairs of one key head are a tile: heads that share keys share the read
+//   keys     a warp takes blocks of KB keys with a running maximum and sum per row; warps, and the CTAs of a cluster, split the blocks and
+//            meet in (distributed) shared memory in a fixed order
+//   K        lane (g, t) holds elements 8 t .. 8 t + 7 of each 32 of key g:  two contraction steps
+//   V        lane (g, t) holds elements 8 g .. 8 g + 7 of each 64 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: eight column tiles
+// fp32 queries and probabilities are two IEEE-half terms (hi + lo, 22 bits): queries after a power of two per row has brought their
+// largest to [1, 2).  Codes of eight bits are exact in half; their scales multiply scores and probabilities.  Each block's P V starts from
+// zero and is added in fp32, because the tensor core's accumulation truncates.
+#include <cmath>
+
+#include "common.h"
+#include "paged.cuh"
+#include "paged_attention.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_ROWS = 16;
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+template <bool BF>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  if constexpr (BF) mma_bf16(c, a, b0, b1);
+  else mma_f16(c, a, b0, b1);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (BF) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<BF>(x, y);
+  const float2 h = unpack2<BF>(hi);
+  lo = pack2<BF>(x - h.x, y - h.y);
+}
+
+// eight elements of a cache type as four pairs in the tensor type (and, of fp32, what those leave in a second four)
+template <int CT>
+__device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  if constexpr (CT == MIMIR_B200_T_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2<false>(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]), hi[i], lo[i]);
+  } else if constexpr (CT == MIMIR_B200_T_I8) {
+    // 0x6400 | (code + 128) is 1024 + 128 + code as a half
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = r.w[i / 2] ^ 0x80808080u;
+      const uint32_t w = __byte_perm(b, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
+      const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), off);
+      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else if constexpr (CT == MIMIR_B200_T_E4M3) {
+    // sign, exponent and mantissa moved to a half's places: the value times 2^-8 (the exponents' biases are 7 and 15), subnormals too;
+    // the codes 0x7f and 0xff (not a number) would be 480
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = __byte_perm(r.w[i / 2], 0, (i & 1) ? 0x3424 : 0x1404);  // the code in the high byte of each half
+      uint32_t h = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+      const uint32_t nan = __vcmpeq2(w & 0x7f007f00u, 0x7f007f00u);
+      hi[i] = h | (nan & 0x7e007e00u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = r.w[i];
+  }
+}
+
+// dst in shared memory of cluster rank `rank`
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+template <int CT, int NQ, int DP>
+struct PagedShape {
+  static constexpr bool BF = CT == MIMIR_B200_T_BF16;
+  static constexpr int KB = type_bytes(CT) == 1 ? 32 : 16;              // keys of a block
+  static constexpr int UD = CT == MIMIR_B200_T_F32 ? 64 : DP < 128 ? DP : 128;  // head elements loaded at a time
+  static constexpr int Q_BYTES = NQ * (DP / 16) * 32 * 16;
+  static constexpr int O_STRIDE = DP + 4;
+  static constexpr int SMEM = Q_BYTES + PA_WARPS * PA_ROWS * (O_STRIDE + 2) * 4 + 2 * PA_ROWS * 4;
+};
+
+template <int CT, int NQ, int DP>
+__global__ void __launch_bounds__(PA_THREADS, (DP > 128 || CT == MIMIR_B200_T_F32) ? 2 : 3)
+paged_attention_kernel(const __grid_constant__ AttendArgs a) {
+  using S = PagedShape<CT, NQ, DP>;
+  constexpr bool BF = S::BF, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3, WIDE = CT == MIMIR_B200_T_F32;
+  constexpr int KB = S::KB, NG = KB / 8, UD = S::UD, NU = DP / UD;
+  constexpr float LOG2E = 1.4426950408889634f;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* sq = reinterpret_cast<uint4*>(smem);                        // [NQ][DP / 16][32 lanes]
+  float* so = reinterpret_cast<float*>(smem + S::Q_BYTES);           // [warp][16][O_STRIDE]
+  float* sm = so + PA_WARPS * PA_ROWS * S::O_STRIDE;                 // [warp][16] maxima, then [warp][16] sums
+  float* sl = sm + PA_WARPS * PA_ROWS;
+  float* sscale = sl + PA_WARPS * PA_ROWS;                           // [16]
+  const PagedView& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rank = static_cast<int>(blockIdx.x) % a.cluster;
+  const int part = static_cast<int>(blockIdx.x) / a.cluster;
+  const int split = part % a.splits, unit = part / a.splits;
+  const int tile = unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
+  const PagedSeq q = paged_seq(p, s);
+  const int r0 = tile * PA_ROWS, n_rows = q.rows * a.group;
+  if (r0 >= n_rows) return;  // (the whole cluster)
+  const int r_end = min(r0 + PA_ROWS, n_rows);
+  const int pos0 = q.kv - q.rows;  // of the sequence's first new token
+  const int pos_first = pos0 + r0 / a.group, pos_last = pos0 + (r_end - 1) / a.group;
+  const int k_end = a.causal ? min(q.kv, pos_last + 1) : q.kv;
+  const int k_begin = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
+  const int b_first = k_begin / KB, blocks = k_end > k_begin ? (k_end + KB - 1) / KB - b_first : 0;
+  const int workers = a.splits * a.cluster * PA_WARPS, me = (split * a.cluster + rank) * PA_WARPS + warp;
+  const int b0 = b_first + static_cast<int>(static_cast<long long>(blocks) * me / workers);
+  const int b1 = b_first + static_cast<int>(static_cast<long long>(blocks) * (me + 1) / workers);
+
+  // ---- the queries of the tile as fragments, hi (+ lo): a warp takes four rows -------------------------------------------------
+#pragma unroll
+  for (int i = 0; i < PA_ROWS / PA_WARPS; ++i) {
+    const int row = warp * (PA_ROWS / PA_WARPS) + i, r = r0 + row;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+    const int d = lane * 8;
+    if (r < r_end && d < p.head_dim) {
+      const int tok = r / a.group, h = head * a.group + r - tok * a.group;
+      const char* src = static_cast<const char*>(a.q) + ((q.row0 + tok) * a.q_row + h * a.q_head + d) * static_cast<long long>(type_bytes(a.type));
+      if (a.type == MIMIR_B200_T_F32) unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(src), f);
+      else if (a.type == MIMIR_B200_T_F16) unpack8<MIMIR_B200_T_F16>(load8<MIMIR_B200_T_F16>(src), f);
+      else unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(src), f);
+    }
+    float scale = 1.0f;
+    if (!BF && a.type != MIMIR_B200_T_F16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // two to the exponent of the largest, in [2^-126, 2^126] (an infinity stays one)
+      const int e2 = min(252, max(1, static_cast<int>(__float_as_uint(top) >> 23)));
+      scale = __uint_as_float(static_cast<uint32_t>(e2) << 23);
+      const float inv = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= inv;
+    }
+    if (lane == 0) sscale[row] = scale;
+    if (d < DP) {
+      // elements 8 c .. 8 c + 7 belong to lane (row % 8, c % 4) of steps 2 (c / 4) and 2 (c / 4) + 1: registers row / 8 and row / 8 + 2
+      const int c = lane;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi0, lo0, hi1, lo1;
+        split2<BF>(f[4 * half], f[4 * half + 1], hi0, lo0);
+        split2<BF>(f[4 * half + 2], f[4 * half + 3], hi1, lo1);
+        const int step = 2 * (c / 4) + half, to = (row & 7) * 4 + (c & 3), reg = row >> 3;
+        uint32_t* w = reinterpret_cast<uint32_t*>(sq + step * 32 + to);
+        w[reg] = hi0, w[reg + 2] = hi1;
+        if constexpr (NQ == 2) {
+          w = reinterpret_cast<uint32_t*>(sq + (DP / 16 + step) * 32 + to);
+          w[reg] = lo0, w[reg + 2] = lo1;
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // scores in the exponent's base two, and the positions of this lane's two rows
+  float c2[2];
+  int lim_hi[2], lim_lo[2];  // keys lim_lo .. lim_hi - 1 are seen
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    c2[i] = a.scale * LOG2E * sscale[g + 8 * i];
+    if (CT == MIMIR_B200_T_E4M3) c2[i] *= 256.0f;
+    const int pos = pos0 + min(r0 + g + 8 * i, r_end - 1) / a.group;
+    lim_hi[i] = a.causal ? min(q.kv, pos + 1) : q.kv;
+    lim_lo[i] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  }
+  const int all_lo = a.window > 0 ? max(0, pos_last - a.window + 1) : 0, all_hi = a.causal ? min(q.kv, pos_first + 1) : q.kv;
+
+  float o[DP / 8][4];
+#pragma unroll
+  for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+  // ---- pages of a block's groups of eight keys (a page holds a multiple of eight) ----------------------------------------------------
+  int page_next[NG];
+  auto fetch_pages = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int key = b * KB + 8 * j;
+      page_next[j] = (b < b1 && key < k_end && key + 7 >= k_begin) ? paged_page(p, s, p.by_page.div(key)) : -1;
+    }
+  };
+  long long off[NG];  // of a group's first key in the pages, -1: none
+  long long soff[NG];  // and in the scales
+  auto place_pages = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int key = b * KB + 8 * j, slot = key - p.by_page.div(key) * p.page_size;
+      off[j] = page_next[j] < 0 ? -1 : page_next[j] * p.page_stride + slot * p.slot_stride + head * p.head_stride;
+      soff[j] = (static_cast<long long>(page_next[j]) * p.kv_heads + head) * p.page_size + slot;
+    }
+  };
+  Raw8<CT> kr[NG][UD / 32], vr[KB / 16][4][(UD + 63) / 64];
+  float2 ks[NG], vs[NG];
+  auto load_k = [&](int b, int u) {
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int key = b * KB + 8 * j + g;
+      const bool go = off[j] >= 0 && key < k_end;
+      const char* base = static_cast<const char*>(p.k) + (off[j] + g * p.slot_stride + u * UD + 8 * t) * type_bytes(CT);
+#pragma unroll
+      for (int c = 0; c < UD / 32; ++c) {
+        if (go && u * UD + 32 * c + 8 * t < p.head_dim) kr[j][c] = load8<CT>(base + 32 * c * type_bytes(CT));
+        else
+#pragma unroll
+          for (uint32_t& w : kr[j][c].w) w = 0;
+      }
+      if (CODED && u == 0) {
+        ks[j] = make_float2(0.0f, 0.0f);
+        if (off[j] >= 0) ks[j] = *reinterpret_cast<const float2*>(p.k_scale + soff[j] + 2 * t);
+      }
+    }
+  };
+  auto load_v = [&](int b, int u) {
+#pragma unroll
+    for (int k16 = 0; k16 < KB / 16; ++k16)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        const int j = 2 * k16 + (i >> 1), in = 2 * t + (i & 1), key = b * KB + 8 * j + in;
+        const bool go = off[j] >= 0 && key < k_end && key >= k_begin;  // (a key that no row sees is zero whatever its slot holds)
+        const char* base = static_cast<const char*>(p.v) + (off[j] + in * p.slot_stride + u * UD + 8 * g) * type_bytes(CT);
+#pragma unroll
+        for (int c = 0; c < (UD + 63) / 64; ++c) {
+          if (go && u * UD + 64 * c + 8 * g < p.head_dim) vr[k16][i][c] = load8<CT>(base + 64 * c * type_bytes(CT));
+          else
+#pragma unroll
+            for (uint32_t& w : vr[k16][i][c].w) w = 0;
+        }
+      }
+    if (CODED && u == 0) {
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const int key = b * KB + 8 * j + 2 * t;
+        vs[j] = make_float2(0.0f, 0.0f);
+        if (off[j] >= 0) vs[j] = *reinterpret_cast<const float2*>(p.v_scale + soff[j] + 2 * t);
+        if (key >= k_end || key < k_begin) vs[j].x = 0.0f;
+        if (key + 1 >= k_end || key + 1 < k_begin) vs[j].y = 0.0f;
+      }
+    }
+  };
+
+  if (b0 < b1) {
+    fetch_pages(b0);
+    place_pages(b0);
+    load_k(b0, 0);
+    load_v(b0, 0);
+    fetch_pages(b0 + 1);
+  }
+  for (int b = b0; b < b1; ++b) {
+    // ---- scores ----------------------------------------------------------------------------------------------------------------
+    float sc[NG][4];
+    bool there[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      there[j] = off[j] >= 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
+    }
+    float2 ks_now[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) ks_now[j] = ks[j];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int c = 0; c < UD / 32; ++c) {
+        uint4 qa[2], ql[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int step = (u * UD + 32 * c) / 16 + h;
+          qa[h] = sq[step * 32 + lane];
+          if constexpr (NQ == 2) ql[h] = sq[(DP / 16 + step) * 32 + lane];
+        }
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          uint32_t hi[4], lo[4];
+          to_pairs<CT>(kr[j][c], hi, lo);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            mma16<BF>(sc[j], qa[h], hi[2 * h], hi[2 * h + 1]);
+            if constexpr (NQ == 2) mma16<BF>(sc[j], ql[h], hi[2 * h], hi[2 * h + 1]);
+            if constexpr (WIDE) mma16<BF>(sc[j], qa[h], lo[2 * h], lo[2 * h + 1]);
+          }
+        }
+      }
+      if (u + 1 < NU) load_k(b, u + 1);
+    }
+    // the next block's keys are on their way while this one's values are used
+    if constexpr (NU == 1) {
+      if (b + 1 < b1) {
+        place_pages(b + 1);
+        load_k(b + 1, 0);
+        fetch_pages(b + 2);
+      }
+    }
+    // ---- running maximum and sum -----------------------------------------------------------------------------------------------------
+    bool full = b * KB >= all_lo && b * KB + KB <= all_hi;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) full = full && there[j];
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = sc[j][i] * c2[i >> 1];
+        if constexpr (CODED) v *= (i & 1) ? ks_now[j].y : ks_now[j].x;
+        if (!full) {
+          const int key = b * KB + 8 * j + 2 * t + (i & 1);
+          if (!(there[j] && key < lim_hi[i >> 1] && key >= lim_lo[i >> 1])) v = -INFINITY;
+        }
+        sc[j][i] = v;
+        mx[i >> 1] = fmaxf(mx[i >> 1], v);
+      }
+    float alpha[2], base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      const float mn = fmaxf(m[i], mx[i]);
+      base[i] = mn == -INFINITY ? 0.0f : mn;  // (a row that has seen nothing yet)
+      alpha[i] = exp2f(m[i] - base[i]);
+      m[i] = mn;
+      l[i] *= alpha[i];
+    }
+    // codes' scales move into the probabilities, which a power of two keeps near one: halves have little range
+    float back = 1.0f;
+    float2 vf[NG];
+    if constexpr (CODED) {
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) top = fmaxf(top, fmaxf(fabsf(vs[j].x), fabsf(vs[j].y)));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e2 = min(240, max(14, static_cast<int>(__float_as_uint(top) >> 23)));
+      back = __uint_as_float(static_cast<uint32_t>(e2) << 23);
+      const float inv = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) vf[j] = make_float2(vs[j].x * inv, vs[j].y * inv);
+      if (CT == MIMIR_B200_T_E4M3) back *= 256.0f;
+    }
+    uint4 ph[KB / 16], pl[KB / 16];
+#pragma unroll
+    for (int k16 = 0; k16 < KB / 16; ++k16) {
+      uint32_t hi[2][2], lo[2][2];  // [group of eight keys][row]
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int j = 2 * k16 + x;
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = exp2f(sc[j][i] - base[i >> 1]);
+          l[i >> 1] += e[i];
+          if constexpr (CODED) e[i] *= (i & 1) ? vf[j].y : vf[j].x;
+        }
+        split2<BF>(e[0], e[1], hi[x][0], lo[x][0]);
+        split2<BF>(e[2], e[3], hi[x][1], lo[x][1]);
+      }
+      ph[k16] = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
+      pl[k16] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
+    }
+    // ---- values ------------------------------------------------------------------------------------------------------------------------
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int c = 0; c < (UD + 63) / 64; ++c) {
+#pragma unroll
+        for (int pr = 0; pr < 4; ++pr) {  // column tiles 2 pr and 2 pr + 1
+          float acc[2][4] = {};
+#pragma unroll
+          for (int k16 = 0; k16 < KB / 16; ++k16) {
+            uint32_t hi[4], lo[4];  // the pair of this lane's four keys
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t h4[4], l4[4];
+              to_pairs<CT>(vr[k16][i][c], h4, l4);
+              hi[i] = h4[pr];
+              if constexpr (WIDE) lo[i] = l4[pr];
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t sel = x ? 0x7632 : 0x5410;
+              const uint32_t v0 = __byte_perm(hi[0], hi[1], sel), v1 = __byte_perm(hi[2], hi[3], sel);
+              mma16<BF>(acc[x], ph[k16], v0, v1);
+              mma16<BF>(acc[x], pl[k16], v0, v1);
+              if constexpr (WIDE) mma16<BF>(acc[x], ph[k16], __byte_perm(lo[0], lo[1], sel), __byte_perm(lo[2], lo[3], sel));
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float(&oo)[4] = o[(u * UD + 64 * c) / 8 + 2 * pr + x];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (CODED) oo[i] = fmaf(acc[x][i], back, oo[i] * alpha[i >> 1]);
+              else oo[i] = fmaf(oo[i], alpha[i >> 1], acc[x][i]);
+            }
+          }
+        }
+      }
+      if constexpr (NU > 1) {
+        if (u + 1 < NU) load_v(b, u + 1);
+      }
+    }
+    if constexpr (NU > 1) {
+      if (b + 1 < b1) {
+        place_pages(b + 1);
+        load_k(b + 1, 0);
+        fetch_pages(b + 2);
+      }
+    }
+    if (b + 1 < b1) load_v(b + 1, 0);
+  }
+
+  // ---- warps, then the cluster's CTAs, meet -------------------------------------------------------------------------------------------
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    const int row = g + 8 * i;
+    if (t == 0) sm[warp * PA_ROWS + row] = m[i], sl[warp * PA_ROWS + row] = l[i];
+    float* w = so + (warp * PA_ROWS + row) * S::O_STRIDE;
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j) {  // tile (c, j % 8) has columns 64 c + 16 t + j % 8 and 8 more
+      const int d = (j / 8) * 64 + 16 * t + (j & 7);
+      w[d] = o[j][2 * i];
+      w[d + 8] = o[j][2 * i + 1];
+    }
+  }
+  __syncthreads();
+  // this CTA's rows: (max, sum, O) into warp 0's place
+  for (int i = threadIdx.x; i < PA_ROWS * DP; i += PA_THREADS) {
+    const int row = i / DP, d = i - row * DP;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, sm[w * PA_ROWS + row]);
+    float sum = 0.0f;
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) sum = fmaf(so[(w * PA_ROWS + row) * S::O_STRIDE + d], exp2f(sm[w * PA_ROWS + row] - base), sum);
+    so[row * S::O_STRIDE + d] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x < PA_ROWS) {
+    const int row = threadIdx.x;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, sm[w * PA_ROWS + row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) sum = fmaf(sl[w * PA_ROWS + row], exp2f(sm[w * PA_ROWS + row] - base), sum);
+    sm[row] = top, sl[row] = sum;
+  }
+  if (a.cluster > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  // each CTA finishes its share of the rows
+  for (int row = rank; row < r_end - r0; row += a.cluster) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int c = 0; c < a.cluster; ++c) top = fmaxf(top, a.cluster > 1 ? ld_cluster(sm + row, c) : sm[row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (int c = 0; c < a.cluster; ++c) {
+      const float mc = a.cluster > 1 ? ld_cluster(sm + row, c) : sm[row], lc = a.cluster > 1 ? ld_cluster(sl + row, c) : sl[row];
+      sum = fmaf(lc, exp2f(mc - base), sum);
+    }
+    for (int d = threadIdx.x; d < p.head_dim; d += PA_THREADS) {
+      float v = 0.0f;
+      for (int c = 0; c < a.cluster; ++c) {
+        const float mc = a.cluster > 1 ? ld_cluster(sm + row, c) : sm[row];
+        const float oc = a.cluster > 1 ? ld_cluster(so + row * S::O_STRIDE + d, c) : so[row * S::O_STRIDE + d];
+        v = fmaf(oc, exp2f(mc - base), v);
+      }
+      if (a.splits > 1) {
+        a.part_o[(static_cast<long long>(part) * PA_ROWS + row) * p.head_dim + d] = v;
+      } else {
+        store_out(a, q.row0, r0 + row, head, d, sum == 0.0f ? 0.0f : v / sum);
+      }
+    }
+    if (threadIdx.x == 0) {
+      if (a.splits > 1) a.part_ml[static_cast<long long>(part) * PA_ROWS + row] = make_float2(top, sum);
+      else store_lse(a, q.row0, r0 + row, head, top, sum);
+    }
+  }
+  if (a.cluster > 1) {  // no CTA leaves while others read its shared memory
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+// The parts of a tile that several clusters computed, in order.
+__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ AttendArgs a) {
+  const PagedView& p = a.p;
+  const int unit = blockIdx.x / PA_ROWS, row = blockIdx.x % PA_ROWS;
+  const int tile = unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
+  const PagedSeq q = paged_seq(p, s);
+  const int r = tile * PA_ROWS + row;
+  if (r >= q.rows * a.group) return;
+  const float2* ml = a.part_ml + static_cast<long long>(unit) * a.splits * PA_ROWS + row;
+  const float* po = a.part_o + (static_cast<long long>(unit) * a.splits * PA_ROWS + row) * p.head_dim;
+  float top = -INFINITY, sum = 0.0f;
+  for (int c = 0; c < a.splits; ++c) top = fmaxf(top, ml[c * PA_ROWS].x);
+  const float base = top == -INFINITY ? 0.0f : top;
+  for (int c = 0; c < a.splits; ++c) sum = fmaf(ml[c * PA_ROWS].y, exp2f(ml[c * PA_ROWS].x - base), sum);
+  for (int d = threadIdx.x; d < p.head_dim; d += 128) {
+    float v = 0.0f;
+    for (int c = 0; c < a.splits; ++c) v = fmaf(po[static_cast<long long>(c) * PA_ROWS * p.head_dim + d], exp2f(ml[c * PA_ROWS].x - base), v);
+    store_out(a, q.row0, r, head, d, sum == 0.0f ? 0.0f : v / sum);
+  }
+  if (threadIdx.x == 0) store_lse(a, q.row0, r, head, top, sum);
+}
+
+struct RowSplit {
+  int tiles = 1, cluster = 1, splits = 1;
+  long long units = 0;
+};
+// How the keys of a tile are shared out.  A cluster of up to eight CTAs meets through shared memory at no extra launch; beyond that
+// (few tiles, long sequences) clusters leave parts in the workspace for a second launch.
+RowSplit row_split(const AttendLaunch& a) {
+  RowSplit r;
+  const int group = a.heads / a.p.kv_heads;
+  r.tiles = static_cast<int>((static_cast<long long>(a.p.max_rows) * group + PA_ROWS - 1) / PA_ROWS);
+  r.units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tiles;
+  const long long slots = 2LL * ctx().sm_count;
+  const int keys = a.window > 0 && a.window < a.p.max_kv ? a.window : a.p.max_kv;
+  while (r.cluster < 8 && r.units * r.cluster < 4 * slots && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
+  while (r.units * r.cluster * r.splits < slots && keys >= 512 * 2 * r.cluster * r.splits) r.splits *= 2;
+  return r;
+}
+
+template <int CT, int NQ, int DP>
+int launch_rows_as(const AttendArgs& a, long long grid, cudaStream_t st) {
+  using S = PagedShape<CT, NQ, DP>;
+  static PerDeviceOnce once;
+  MB_TRY(once.run([]() -> int {
+    MB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<CT, NQ, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    return MIMIR_B200_OK;
+  }));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(PA_THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  if (a.cluster > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(a.cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  MB_CUDA(cudaLaunchKernelEx(&cfg, paged_attention_kernel<CT, NQ, DP>, a));
+  count_launch();
+  return MIMIR_B200_OK;
+}
+template <int CT, int NQ>
+int launch_rows_dim(const AttendArgs& a, long long grid, cudaStream_t st) {
+  if (a.p.head_dim <= 64) return launch_rows_as<CT, NQ, 64>(a, grid, st);
+  if (a.p.head_dim <= 128) return launch_rows_as<CT, NQ, 128>(a, grid, st);
+  return launch_rows_as<CT, NQ, 256>(a, grid, st);
+}
+
+}  // namespace
+
+size_t paged_attention_ws_bytes(const AttendLaunch& a) {
+  const RowSplit r = row_split(a);
+  if (r.splits <= 1) return 0;
+  return static_cast<size_t>(r.units) * r.splits * PA_ROWS * (a.p.head_dim * sizeof(float) + sizeof(float2));
+}
+
+int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
+  const RowSplit r = row_split(l);
+  const size_t need = paged_attention_ws_bytes(l);
+  if (need > 0 && (!l.ws || l.ws_bytes < need))
+    return fail(MIMIR_B200_E_INVALID, "paged_attention: a workspace of %zu bytes is needed (paged_attention_workspace), got %zu", need, l.ws ? l.ws_bytes : 0);
+  const long long grid = r.units * r.splits * r.cluster;
+  if (grid > 0x7fffffffLL || r.units * PA_ROWS > 0x7fffffffLL) return fail(MIMIR_B200_E_INVALID, "paged_attention: too many rows and heads for one call");
+  AttendArgs a = {};
+  a.p = l.p;
+  a.q = l.q, a.out = l.out, a.lse = l.lse;
+  a.q_row = l.q_row, a.q_head = l.q_head, a.o_row = l.o_row, a.o_head = l.o_head;
+  a.type = l.type, a.heads = l.heads, a.group = l.heads / l.p.kv_heads, a.causal = l.causal, a.window = l.window, a.scale = l.scale;
+  a.tiles = r.tiles, a.cluster = r.cluster, a.splits = r.splits;
+  if (need) {
+    a.part_o = static_cast<float*>(l.ws);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(r.units) * r.splits * PA_ROWS * l.p.head_dim);
+  }
+  int s;
+  const bool two = l.type == MIMIR_B200_T_F32;
+  switch (l.cache_type) {
+    case MIMIR_B200_T_F32: s = launch_rows_dim<MIMIR_B200_T_F32, 2>(a, grid, st); break;
+    case MIMIR_B200_T_BF16: s = launch_rows_dim<MIMIR_B200_T_BF16, 1>(a, grid, st); break;
+    case MIMIR_B200_T_F16: s = two ? launch_rows_dim<MIMIR_B200_T_F16, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_F16, 1>(a, grid, st); break;
+    case MIMIR_B200_T_I8: s = two ? launch_rows_dim<MIMIR_B200_T_I8, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_I8, 1>(a, grid, st); break;
+    default: s = two ? launch_rows_dim<MIMIR_B200_T_E4M3, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_E4M3, 1>(a, grid, st); break;
+  }
+  MB_TRY(s);
+  if (r.splits > 1) {
+    paged_merge_kernel<<<static_cast<unsigned>(r.units * PA_ROWS), 128, 0, st>>>(a);
+    MB_CUDA(cudaGetLastError());
+    count_launch();
+  }
+  return MIMIR_B200_OK;
+}
+
+}  // namespace mb

@@ -1,0 +1,172 @@
+// paged_cache.cu — new keys and values into the pages of a cache, and sequences back out of it.
+//
+// Pure data movement: rows in, codes (and a scale per row and head in 8 bits) out, each once.  A vector of head_dim elements belongs to a
+// group of lanes with eight elements each, so that a group's largest magnitude is a few shuffles and loads are 16 bytes.  A CTA looks
+// up where its rows go once, in shared memory, and then moves all their heads.
+//   I8:   scale = amax * (1 / 127), code = x / scale to nearest (ties to even)      E4M3: scale = amax * (1 / 448), likewise
+// amax is over the finite elements; 1 / 127 and 1 / 448 are fp32 constants and the division is the IEEE one, so that codes are what any
+// fp32 program gets that computes them so.
+#include "common.h"
+#include "paged.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int PC_THREADS = 256;
+constexpr int PC_ROWS = 32;     // most rows a CTA looks up
+constexpr int PC_STARTS = 1024;  // sequence starts kept in shared memory
+
+// the last s of 0 .. n with start[s] <= row, -1 if none (starts ascend; entries that do not are found out by the caller)
+__device__ __forceinline__ int last_start(const int* start, int n, int row) {
+  int lo = -1, hi = n + 1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct CacheMove {
+  PagedView p;
+  const int* start;  // [n_seqs + 1] row_start (write) or out_start (read)
+  int rows;
+  void* k;
+  void* v;
+  long long row_stride, head_stride;
+  int per_cta, group;  // rows of a CTA; lanes of a vector, a power of two
+};
+
+template <int CT, int T, bool WRITE>
+__global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_constant__ CacheMove a) {
+  constexpr bool CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3;
+  constexpr float TOP = CT == MIMIR_B200_T_I8 ? 127.0f : 448.0f, PART = 1.0f / TOP;
+  __shared__ int starts[PC_STARTS];
+  __shared__ long long at[PC_ROWS];     // of a row's slot in the pages, -1: the row is none of a sequence
+  __shared__ long long scale_at[PC_ROWS];
+  const PagedView& p = a.p;
+  const int row0 = blockIdx.x * a.per_cta, rows = min(a.per_cta, a.rows - row0);
+  const bool kept = p.n_seqs < PC_STARTS;
+  if (kept) {
+    for (int i = threadIdx.x; i <= p.n_seqs; i += PC_THREADS) starts[i] = __ldg(a.start + i);
+    __syncthreads();
+  }
+  if (static_cast<int>(threadIdx.x) < rows) {
+    const int row = row0 + threadIdx.x, s = last_start(kept ? starts : a.start, p.n_seqs, row);
+    long long where = -1, sc = 0;
+    if (s >= 0 && s < p.n_seqs) {
+      const int first = a.start[s], end = a.start[s + 1], kv = __ldg(p.kv_len + s);
+      // (out_start of a read: as many rows as keys, the last ones of a longer range stay as they are)
+      const int pos = WRITE ? kv - (end - row) : row - first;
+      if (first < 0 || row < first || row >= end || end > a.rows || (WRITE && end - first > p.max_rows)) {
+        atomicOr(p.flags, PAGED_BAD_ROWS);
+      } else if (kv < 0 || kv > p.max_kv || kv > p.table_stride * p.page_size) {
+        atomicOr(p.flags, PAGED_BAD_LEN);
+      } else if (pos >= 0 && pos < kv) {
+        const int pi = p.by_page.div(pos), slot = pos - pi * p.page_size, page = paged_page(p, s, pi);
+        if (page >= 0) {
+          where = page * p.page_stride + slot * p.slot_stride;
+          sc = static_cast<long long>(page) * p.kv_heads * p.page_size + slot;
+        }
+      }
+    }
+    at[threadIdx.x] = where;
+    scale_at[threadIdx.x] = sc;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & (a.group - 1), d = lane * 8;
+  const bool mine = d < p.head_dim;
+  const int groups = PC_THREADS / a.group, vectors = rows * 2 * p.kv_heads;
+  // (whole warps stay in the loop for the shuffles)
+  for (int i0 = 0; i0 < vectors; i0 += groups) {
+    const int i = i0 + threadIdx.x / a.group;
+    const bool there = i < vectors;
+    const int row = there ? i / (2 * p.kv_heads) : 0, j = there ? i - row * 2 * p.kv_heads : 0;
+    const bool is_v = j >= p.kv_heads;
+    const int head = is_v ? j - p.kv_heads : j;
+    const bool go = there && mine && at[row] >= 0;
+    const long long user = (row0 + row) * a.row_stride + head * a.head_stride + d, slot = at[row] + head * p.head_stride + d;
+    char* mem = static_cast<char*>(is_v ? a.v : a.k) + user * type_bytes(T);
+    char* pool = static_cast<char*>(is_v ? p.v : p.k) + slot * type_bytes(CT);
+    float* scales = is_v ? p.v_scale : p.k_scale;
+    const long long si = scale_at[row] + static_cast<long long>(head) * p.page_size;
+    float f[8];
+    if constexpr (WRITE) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+      if (go) unpack8<T>(load8<T>(mem), f);
+      if constexpr (CODED) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = fabsf(f[e]);
+          if (v < INFINITY) amax = fmaxf(amax, v);
+        }
+        for (int o = a.group >> 1; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const float scale = __fmul_rn(amax, PART);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // (a scale of zero: nothing but zeros, infinities and magnitudes whose scale is below fp32's smallest)
+          const float v = scale > 0.0f ? __fdiv_rn(f[e], scale) : 0.0f;
+          f[e] = CT != MIMIR_B200_T_I8 ? v : v == v ? fmaxf(-TOP, fminf(TOP, v)) : 0.0f;
+        }
+        if (go && lane == 0) scales[si] = scale;
+      }
+      if (go) store8<CT>(pool, pack8<CT>(f));
+    } else if (go) {
+      unpack8<CT>(load8<CT>(pool), f);
+      if constexpr (CODED) {
+        const float scale = scales[si];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= scale;
+      }
+      store8<T>(mem, pack8<T>(f));
+    }
+  }
+}
+
+template <bool WRITE, int CT>
+int launch_move_as(const CacheMove& a, int type, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>((a.rows + a.per_cta - 1) / a.per_cta);
+  if (type == MIMIR_B200_T_F32) cache_move_kernel<CT, MIMIR_B200_T_F32, WRITE><<<grid, PC_THREADS, 0, st>>>(a);
+  else if (type == MIMIR_B200_T_F16) cache_move_kernel<CT, MIMIR_B200_T_F16, WRITE><<<grid, PC_THREADS, 0, st>>>(a);
+  else cache_move_kernel<CT, MIMIR_B200_T_BF16, WRITE><<<grid, PC_THREADS, 0, st>>>(a);
+  MB_CUDA(cudaGetLastError());
+  count_launch();
+  return MIMIR_B200_OK;
+}
+
+template <bool WRITE>
+int launch_move(CacheMove a, int cache_type, int type, cudaStream_t st) {
+  a.group = 1;
+  while (a.group * 8 < a.p.head_dim) a.group *= 2;
+  // rows of a CTA: enough for a pass of its threads, and no fewer CTAs than SMs for that
+  a.per_cta = 1;
+  while (a.per_cta < PC_ROWS && a.rows >= 8LL * ctx().sm_count * a.per_cta) a.per_cta *= 2;
+  switch (cache_type) {
+    case MIMIR_B200_T_F32: return launch_move_as<WRITE, MIMIR_B200_T_F32>(a, type, st);
+    case MIMIR_B200_T_F16: return launch_move_as<WRITE, MIMIR_B200_T_F16>(a, type, st);
+    case MIMIR_B200_T_BF16: return launch_move_as<WRITE, MIMIR_B200_T_BF16>(a, type, st);
+    case MIMIR_B200_T_I8: return launch_move_as<WRITE, MIMIR_B200_T_I8>(a, type, st);
+    default: return launch_move_as<WRITE, MIMIR_B200_T_E4M3>(a, type, st);
+  }
+}
+
+}  // namespace
+
+int launch_cache_write(const PagedView& p, int cache_type, const void* k, const void* v, int type, long long row_stride, long long head_stride,
+                       cudaStream_t st) {
+  CacheMove a = {};
+  a.p = p, a.start = p.row_start, a.rows = p.n_rows, a.k = const_cast<void*>(k), a.v = const_cast<void*>(v);
+  a.row_stride = row_stride, a.head_stride = head_stride;
+  return launch_move<true>(a, cache_type, type, st);
+}
+int launch_cache_read(const PagedView& p, int cache_type, const int* out_start, int out_rows, void* k, void* v, int type, long long row_stride,
+                      long long head_stride, cudaStream_t st) {
+  CacheMove a = {};
+  a.p = p, a.start = out_start, a.rows = out_rows, a.k = k, a.v = v;
+  a.row_stride = row_stride, a.head_stride = head_stride;
+  return launch_move<false>(a, cache_type, type, st);
+}
+
+}  // namespace mb

@@ -118,6 +118,13 @@ _SIGS = {
     "mimir_b200_dev_groupnorm": [_P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, _P],
     "mimir_b200_dev_softmax": [_P, _P, C.c_int, C.c_longlong, C.c_int, _P],
     "mimir_b200_dev_eltwise": [C.c_int, _P, _P, _P, C.c_int, C.c_longlong, C.c_longlong, _P],
+    "mimir_b200_rope_plan": [_P, _P],
+    "mimir_b200_dev_rope": [_P, _P, _P, _P, C.c_longlong, C.c_int, C.c_int] + [C.c_longlong] * 4 + [C.c_int, _P],
+    "mimir_b200_dev_cache_write": [_P, _P, _P, _P, C.c_int, C.c_longlong, C.c_longlong, _P],
+    "mimir_b200_dev_cache_read": [_P, _P, _P, C.c_int, _P, _P, C.c_int, C.c_longlong, C.c_longlong, _P],
+    "mimir_b200_paged_attention_workspace": [_P, _P, _P, _P],
+    "mimir_b200_dev_paged_attention": [_P, _P, _P, _P],
+    "mimir_b200_dev_sample_rows": [_P, C.c_int, C.c_longlong, C.c_int, C.c_longlong] + [_P] * 8,
 }
 
 EXPORTED_SYMBOLS = sorted(list(_SIGS) + ["mimir_b200_last_error"])
@@ -575,6 +582,61 @@ class GraphModel:
         check(lib().mimir_b200_model_forward_device(self._h, C.addressof(arr), len(spec), batch, out_ptr, out_capacity,
                                                     C.byref(n), stream))
         return n.value
+
+
+# ---- serving calls: device addresses, asynchronous on ``stream`` ------------------------------------
+def check_device(stream: int = 0):
+    check(lib().mimir_b200_check_device(stream))
+
+
+def rope_plan(rot_dim, base=10000.0, interleaved=False, scaling="none", factor=0.0, low=0.0, high=0.0, original_len=0.0, magnitude=0.0,
+              inverse=False) -> abi.MimirRopePlan:
+    spec = abi.MimirRopeSpec(rot_dim, int(interleaved), abi.ROPE_SCALING[scaling], int(inverse), base, factor, low, high, original_len, magnitude)
+    plan = abi.MimirRopePlan()
+    check(lib().mimir_b200_rope_plan(C.addressof(spec), C.addressof(plan)))
+    return plan
+
+
+def dev_rope(plan, positions, x, y, rows, heads, head_dim, x_strides, y_strides, type, stream: int = 0):
+    """x_strides, y_strides: (row, head) in elements."""
+    check(lib().mimir_b200_dev_rope(C.byref(plan), positions, x, y, rows, heads, head_dim, *x_strides, *y_strides, type, stream))
+
+
+def paged_cache(k, v, type, n_pages, page_size, kv_heads, head_dim, page_stride, slot_stride, head_stride, k_scale=None, v_scale=None):
+    return abi.MimirPagedCache(k, v, k_scale, v_scale, page_stride, slot_stride, head_stride, type, n_pages, page_size, kv_heads, head_dim)
+
+
+def paged_batch(row_start, kv_len, page_table, table_stride, n_seqs, n_rows, max_rows, max_kv):
+    return abi.MimirPagedBatch(row_start, kv_len, page_table, table_stride, n_seqs, n_rows, max_rows, max_kv)
+
+
+def paged_attention(q, out, type, heads, row_stride, head_stride, out_row_stride, out_head_stride, scale, causal=True, window=0, lse=None,
+                    workspace=None, workspace_bytes=0):
+    return abi.MimirPagedAttention(q, out, lse, workspace, workspace_bytes, row_stride, head_stride, out_row_stride, out_head_stride, type, heads,
+                                   int(causal), window, scale, 0)
+
+
+def paged_attention_workspace(cache, batch, attention) -> int:
+    n = C.c_uint64(0)
+    check(lib().mimir_b200_paged_attention_workspace(C.byref(cache), C.byref(batch), C.byref(attention), C.byref(n)))
+    return n.value
+
+
+def dev_cache_write(cache, batch, k, v, type, row_stride, head_stride, stream: int = 0):
+    check(lib().mimir_b200_dev_cache_write(C.byref(cache), C.byref(batch), k, v, type, row_stride, head_stride, stream))
+
+
+def dev_cache_read(cache, batch, out_start, out_rows, k, v, type, row_stride, head_stride, stream: int = 0):
+    check(lib().mimir_b200_dev_cache_read(C.byref(cache), C.byref(batch), out_start, out_rows, k, v, type, row_stride, head_stride, stream))
+
+
+def dev_paged_attention(cache, batch, attention, stream: int = 0):
+    check(lib().mimir_b200_dev_paged_attention(C.byref(cache), C.byref(batch), C.byref(attention), stream))
+
+
+def dev_sample_rows(logits, type, rows, n, row_stride, temperature, top_k, top_p, min_p, uniform, ids, logprob=None, stream: int = 0):
+    """temperature, top_k, top_p, min_p and logprob may be None."""
+    check(lib().mimir_b200_dev_sample_rows(logits, type, rows, n, row_stride, temperature, top_k, top_p, min_p, uniform, ids, logprob, stream))
 
 
 class Replicas:
