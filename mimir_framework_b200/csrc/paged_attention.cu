@@ -39,60 +39,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint4& a, uint32_t b0
   if constexpr (BF) mma_bf16(c, a, b0, b1);
   else mma_f16(c, a, b0, b1);
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  if constexpr (BF) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-template <bool BF>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <bool BF>
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = pack2<BF>(x, y);
-  const float2 h = unpack2<BF>(hi);
-  lo = pack2<BF>(x - h.x, y - h.y);
-}
-
-// eight elements of a cache type as four pairs in the tensor type (and, of fp32, what those leave in a second four)
-template <int CT>
-__device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-  if constexpr (CT == MIMIR_B200_T_F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) split2<false>(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]), hi[i], lo[i]);
-  } else if constexpr (CT == MIMIR_B200_T_I8) {
-    // 0x6400 | (code + 128) is 1024 + 128 + code as a half
-    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b = r.w[i / 2] ^ 0x80808080u;
-      const uint32_t w = __byte_perm(b, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
-      const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), off);
-      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  } else if constexpr (CT == MIMIR_B200_T_E4M3) {
-    // sign, exponent and mantissa moved to a half's places: the value times 2^-8 (the exponents' biases are 7 and 15), subnormals too;
-    // the codes 0x7f and 0xff (not a number) would be 480
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = __byte_perm(r.w[i / 2], 0, (i & 1) ? 0x3424 : 0x1404);  // the code in the high byte of each half
-      uint32_t h = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
-      const uint32_t nan = __vcmpeq2(w & 0x7f007f00u, 0x7f007f00u);
-      hi[i] = h | (nan & 0x7e007e00u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) hi[i] = r.w[i];
-  }
-}
-
 // dst in shared memory of cluster rank `rank`
 __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
   uint32_t a;
@@ -133,7 +79,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   const int tile = unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
   const PagedSeq q = paged_seq(p, s);
   const int r0 = tile * PA_ROWS, n_rows = q.rows * a.group;
-  if (r0 >= n_rows) return;  // (the whole cluster)
+  if (r0 >= n_rows || n_rows > a.few) return;  // (the whole cluster)
   const int r_end = min(r0 + PA_ROWS, n_rows);
   const int pos0 = q.kv - q.rows;  // of the sequence's first new token
   const int pos_first = pos0 + r0 / a.group, pos_last = pos0 + (r_end - 1) / a.group;
@@ -530,43 +476,67 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   }
 }
 
-// The parts of a tile that several clusters computed, in order.
+// The parts of a tile that several CTAs or clusters computed, in order.
 __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ AttendArgs a) {
   const PagedView& p = a.p;
-  const int unit = blockIdx.x / PA_ROWS, row = blockIdx.x % PA_ROWS;
-  const int tile = unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
+  const int unit = blockIdx.x / a.part_rows, row = blockIdx.x % a.part_rows;
+  const int at = unit % a.tiles, tile = a.last_first ? a.tiles - 1 - at : at, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
   const PagedSeq q = paged_seq(p, s);
-  const int r = tile * PA_ROWS + row;
-  if (r >= q.rows * a.group) return;
-  const float2* ml = a.part_ml + static_cast<long long>(unit) * a.splits * PA_ROWS + row;
-  const float* po = a.part_o + (static_cast<long long>(unit) * a.splits * PA_ROWS + row) * p.head_dim;
+  const int r = tile * a.part_rows + row, n_rows = q.rows * a.group;
+  if (r >= n_rows || (a.last_first ? n_rows <= a.few : n_rows > a.few)) return;
+  const float2* ml = a.part_ml + static_cast<long long>(unit) * a.splits * a.part_rows + row;
+  const float* po = a.part_o + (static_cast<long long>(unit) * a.splits * a.part_rows + row) * p.head_dim;
   float top = -INFINITY, sum = 0.0f;
-  for (int c = 0; c < a.splits; ++c) top = fmaxf(top, ml[c * PA_ROWS].x);
+  for (int c = 0; c < a.splits; ++c) top = fmaxf(top, ml[c * a.part_rows].x);
   const float base = top == -INFINITY ? 0.0f : top;
-  for (int c = 0; c < a.splits; ++c) sum = fmaf(ml[c * PA_ROWS].y, exp2f(ml[c * PA_ROWS].x - base), sum);
+  for (int c = 0; c < a.splits; ++c) sum = fmaf(ml[c * a.part_rows].y, exp2f(ml[c * a.part_rows].x - base), sum);
   for (int d = threadIdx.x; d < p.head_dim; d += 128) {
     float v = 0.0f;
-    for (int c = 0; c < a.splits; ++c) v = fmaf(po[static_cast<long long>(c) * PA_ROWS * p.head_dim + d], exp2f(ml[c * PA_ROWS].x - base), v);
+    for (int c = 0; c < a.splits; ++c)
+      v = fmaf(po[static_cast<long long>(c) * a.part_rows * p.head_dim + d], exp2f(ml[c * a.part_rows].x - base), v);
     store_out(a, q.row0, r, head, d, sum == 0.0f ? 0.0f : v / sum);
   }
   if (threadIdx.x == 0) store_lse(a, q.row0, r, head, top, sum);
 }
 
-struct RowSplit {
-  int tiles = 1, cluster = 1, splits = 1;
-  long long units = 0;
+// How a call is shared out between the two kernels, and each one's tiles over CTAs.
+struct Share {
+  bool rows = true, chunks = false;  // which kernels run
+  int few = 0x7fffffff;
+  int tiles = 1, cluster = 1, splits = 1;   // row kernel
+  int tc_tiles = 1, tc_splits = 1;
+  long long units = 0, tc_units = 0;
+  size_t bytes = 0, tc_bytes = 0;
 };
-// How the keys of a tile are shared out.  A cluster of up to eight CTAs meets through shared memory at no extra launch; beyond that
-// (few tiles, long sequences) clusters leave parts in the workspace for a second launch.
-RowSplit row_split(const AttendLaunch& a) {
-  RowSplit r;
+// Queries of 16 bits and more rows than a tile of the tensor cores is worth.
+constexpr int TC_FEW = 64;
+Share share_out(const AttendLaunch& a) {
+  Share r;
   const int group = a.heads / a.p.kv_heads;
-  r.tiles = static_cast<int>((static_cast<long long>(a.p.max_rows) * group + PA_ROWS - 1) / PA_ROWS);
+  const long long most = static_cast<long long>(a.p.max_rows) * group;
+  const int keys = a.window > 0 && a.window < a.p.max_kv ? a.window : a.p.max_kv;  // (of a row; a chunk sees a little more)
+  const size_t row_bytes = a.p.head_dim * sizeof(float) + sizeof(float2);
+  if (a.type != MIMIR_B200_T_F32 && most > TC_FEW) {
+    r.chunks = true;
+    // (one sequence: its rows are many; of several, some may have few)
+    r.rows = a.p.n_seqs > 1;
+    r.few = r.rows ? TC_FEW : 0;
+    const int per = tc_tile_rows(a.p.head_dim);
+    r.tc_tiles = static_cast<int>((most + per - 1) / per);
+    r.tc_units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tc_tiles;
+    while (r.tc_units * r.tc_splits * 2 <= ctx().sm_count && keys >= 1024 * r.tc_splits) r.tc_splits *= 2;
+    if (r.tc_splits > 1) r.tc_bytes = static_cast<size_t>(r.tc_units) * r.tc_splits * per * row_bytes;
+  }
+  if (!r.rows) return r;
+  // A cluster of up to eight CTAs meets through shared memory at no extra launch; beyond that (few tiles, long sequences) clusters
+  // leave parts in the workspace for a second launch.
+  const long long few = r.chunks ? TC_FEW : most;
+  r.tiles = static_cast<int>((few + PA_ROWS - 1) / PA_ROWS);
   r.units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tiles;
   const long long slots = 2LL * ctx().sm_count;
-  const int keys = a.window > 0 && a.window < a.p.max_kv ? a.window : a.p.max_kv;
   while (r.cluster < 8 && r.units * r.cluster < 4 * slots && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
   while (r.units * r.cluster * r.splits < slots && keys >= 512 * 2 * r.cluster * r.splits) r.splits *= 2;
+  if (r.splits > 1) r.bytes = static_cast<size_t>(r.units) * r.splits * PA_ROWS * row_bytes;
   return r;
 }
 
@@ -606,43 +576,57 @@ int launch_rows_dim(const AttendArgs& a, long long grid, cudaStream_t st) {
 }  // namespace
 
 size_t paged_attention_ws_bytes(const AttendLaunch& a) {
-  const RowSplit r = row_split(a);
-  if (r.splits <= 1) return 0;
-  return static_cast<size_t>(r.units) * r.splits * PA_ROWS * (a.p.head_dim * sizeof(float) + sizeof(float2));
+  const Share r = share_out(a);
+  return r.bytes + r.tc_bytes;
 }
 
+namespace {
+int launch_merge(const AttendArgs& a, long long units, cudaStream_t st) {
+  paged_merge_kernel<<<static_cast<unsigned>(units * a.part_rows), 128, 0, st>>>(a);
+  MB_CUDA(cudaGetLastError());
+  count_launch();
+  return MIMIR_B200_OK;
+}
+}  // namespace
+
 int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
-  const RowSplit r = row_split(l);
-  const size_t need = paged_attention_ws_bytes(l);
+  const Share r = share_out(l);
+  const size_t need = r.bytes + r.tc_bytes;
   if (need > 0 && (!l.ws || l.ws_bytes < need))
     return fail(MIMIR_B200_E_INVALID, "paged_attention: a workspace of %zu bytes is needed (paged_attention_workspace), got %zu", need, l.ws ? l.ws_bytes : 0);
   const long long grid = r.units * r.splits * r.cluster;
-  if (grid > 0x7fffffffLL || r.units * PA_ROWS > 0x7fffffffLL) return fail(MIMIR_B200_E_INVALID, "paged_attention: too many rows and heads for one call");
+  if (grid > 0x7fffffffLL || r.units * PA_ROWS > 0x7fffffffLL || r.tc_units * r.tc_splits > 0x7fffffffLL)
+    return fail(MIMIR_B200_E_INVALID, "paged_attention: too many rows and heads for one call");
   AttendArgs a = {};
   a.p = l.p;
   a.q = l.q, a.out = l.out, a.lse = l.lse;
   a.q_row = l.q_row, a.q_head = l.q_head, a.o_row = l.o_row, a.o_head = l.o_head;
   a.type = l.type, a.heads = l.heads, a.group = l.heads / l.p.kv_heads, a.causal = l.causal, a.window = l.window, a.scale = l.scale;
-  a.tiles = r.tiles, a.cluster = r.cluster, a.splits = r.splits;
-  if (need) {
-    a.part_o = static_cast<float*>(l.ws);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(r.units) * r.splits * PA_ROWS * l.p.head_dim);
+  a.few = r.few;
+  a.err_word = ctx().dev_error_word;
+  auto parts = [&](size_t offset, long long units, int splits, int rows) {
+    a.splits = splits, a.part_rows = rows;
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(l.ws) + offset);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(units) * splits * rows * l.p.head_dim);
+  };
+  if (r.chunks) {
+    a.tiles = r.tc_tiles, a.last_first = 1;
+    parts(r.bytes, r.tc_units, r.tc_splits, tc_tile_rows(l.p.head_dim));
+    MB_TRY(launch_paged_attention_tc(a, l.cache_type, st));
+    if (r.tc_splits > 1) MB_TRY(launch_merge(a, r.tc_units, st));
   }
-  int s;
+  if (!r.rows) return MIMIR_B200_OK;
+  a.tiles = r.tiles, a.cluster = r.cluster, a.last_first = 0;
+  parts(0, r.units, r.splits, PA_ROWS);
   const bool two = l.type == MIMIR_B200_T_F32;
   switch (l.cache_type) {
-    case MIMIR_B200_T_F32: s = launch_rows_dim<MIMIR_B200_T_F32, 2>(a, grid, st); break;
-    case MIMIR_B200_T_BF16: s = launch_rows_dim<MIMIR_B200_T_BF16, 1>(a, grid, st); break;
-    case MIMIR_B200_T_F16: s = two ? launch_rows_dim<MIMIR_B200_T_F16, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_F16, 1>(a, grid, st); break;
-    case MIMIR_B200_T_I8: s = two ? launch_rows_dim<MIMIR_B200_T_I8, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_I8, 1>(a, grid, st); break;
-    default: s = two ? launch_rows_dim<MIMIR_B200_T_E4M3, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_E4M3, 1>(a, grid, st); break;
+    case MIMIR_B200_T_F32: MB_TRY((launch_rows_dim<MIMIR_B200_T_F32, 2>(a, grid, st))); break;
+    case MIMIR_B200_T_BF16: MB_TRY((launch_rows_dim<MIMIR_B200_T_BF16, 1>(a, grid, st))); break;
+    case MIMIR_B200_T_F16: MB_TRY((two ? launch_rows_dim<MIMIR_B200_T_F16, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_F16, 1>(a, grid, st))); break;
+    case MIMIR_B200_T_I8: MB_TRY((two ? launch_rows_dim<MIMIR_B200_T_I8, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_I8, 1>(a, grid, st))); break;
+    default: MB_TRY((two ? launch_rows_dim<MIMIR_B200_T_E4M3, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_E4M3, 1>(a, grid, st))); break;
   }
-  MB_TRY(s);
-  if (r.splits > 1) {
-    paged_merge_kernel<<<static_cast<unsigned>(r.units * PA_ROWS), 128, 0, st>>>(a);
-    MB_CUDA(cudaGetLastError());
-    count_launch();
-  }
+  if (r.splits > 1) MB_TRY(launch_merge(a, r.units, st));
   return MIMIR_B200_OK;
 }
 

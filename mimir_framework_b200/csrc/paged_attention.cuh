@@ -13,12 +13,73 @@ struct AttendArgs {
   long long q_row, q_head, o_row, o_head;  // elements
   int type, heads, group, causal, window;
   float scale;
+  int few;                                 // (token, head) rows of a sequence and key head: up to so many are the row kernel's
   int tiles, cluster, splits;              // of the rows of a sequence; CTAs and clusters that share a tile's keys
-  float* part_o;                           // [unit][split][16][head_dim], [unit][split][16] (max, sum): splits > 1
+  int part_rows, last_first;               // rows of a tile; tiles are numbered from the last
+  float* part_o;                           // [unit][split][part_rows][head_dim], [unit][split][part_rows] (max, sum): splits > 1
   float2* part_ml;
+  int* err_word;
 };
+// paged_attention_tc.cu: chunks of many rows; queries of 16 bits
+constexpr int TC_KEYS = 128, TC_ROWS = 128;
+inline int tc_tile_rows(int head_dim) { return head_dim <= 128 ? 2 * TC_ROWS : TC_ROWS; }
+int launch_paged_attention_tc(const AttendArgs& a, int cache_type, cudaStream_t st);
 
 namespace {
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (BF) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<BF>(x, y);
+  const float2 h = unpack2<BF>(hi);
+  lo = pack2<BF>(x - h.x, y - h.y);
+}
+
+// eight elements of a cache type as four pairs in the tensor type (and, of fp32, what those leave in a second four)
+template <int CT>
+__device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  if constexpr (CT == MIMIR_B200_T_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2<false>(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]), hi[i], lo[i]);
+  } else if constexpr (CT == MIMIR_B200_T_I8) {
+    // 0x6400 | (code + 128) is 1024 + 128 + code as a half
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = r.w[i / 2] ^ 0x80808080u;
+      const uint32_t w = __byte_perm(b, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
+      const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), off);
+      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else if constexpr (CT == MIMIR_B200_T_E4M3) {
+    // sign, exponent and mantissa moved to a half's places: the value times 2^-8 (the exponents' biases are 7 and 15), subnormals too;
+    // the codes 0x7f and 0xff (not a number) would be 480
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = __byte_perm(r.w[i / 2], 0, (i & 1) ? 0x3424 : 0x1404);  // the code in the high byte of each half
+      uint32_t h = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+      const uint32_t nan = __vcmpeq2(w & 0x7f007f00u, 0x7f007f00u);
+      hi[i] = h | (nan & 0x7e007e00u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = r.w[i];
+  }
+}
 
 __device__ __forceinline__ void store_out(const AttendArgs& a, int row0, int r, int kv_head, int d, float v) {
   const int tok = r / a.group, h = kv_head * a.group + r - tok * a.group;

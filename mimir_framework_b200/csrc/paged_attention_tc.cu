@@ -1,0 +1,557 @@
+// paged_attention_tc.cu — attention over a paged cache for chunks of many new tokens, on tcgen05.
+//
+// A chunk's rows times the cached keys are two matrix products of 2 head_dim operations a pair each, with a softmax between: the
+// tensor cores bound it, and the exponentials come close behind (16 of them a cycle and SM against 128 x 128 x 128 products in
+// 512 cycles).  A CTA owns 256 (token, head of the group) rows of one key head in two tiles of 128 and walks the keys in tiles of
+// 128, so that one tile's softmax runs while the tensor cores work on the other:
+//   warps 0-3, 4-7   softmax of row tile 0 and 1: a thread has a row, reads its 128 scores from tensor memory and writes the probabilities
+//                    back over them as 16-bit pairs, from where P V reads them (A operand in tensor memory)
+//   warp 8           issues the tensor instructions: per key tile P_0 V, Q_0 K', P_1 V, Q_1 K' (K' the next tile)
+//   warps 9-11       bring K and V tiles out of the pages into a ring, rows found through the page table, 8-bit codes as halves
+// Heads of over 128 elements have one tile of 128 rows (O takes 256 columns of tensor memory) and two score tiles that alternate.
+// K and V tiles lie in the same layout, [64 elements][key] rows of 128 swizzled bytes: K-major for Q K^T, MN-major for P V.
+// The running maximum is raised only when a score outgrows it by 2^8, so O in tensor memory is rescaled a few times a row.
+// Probabilities of a bfloat16 cache are rounded to bfloat16 (8 bits, relative to each probability), else to half (11 bits); their sum is
+// of the unrounded ones, in fp32.  Scores, maxima, sums and O are fp32.
+#include <cmath>
+
+#include "common.h"
+#include "launch.cuh"
+#include "paged.cuh"
+#include "paged_attention.cuh"
+#include "sm100_ptx.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int TC_LOADERS = 96, TC_TMEM = 512;
+
+template <int DP, int CT>
+struct TcShape {
+  static constexpr bool BF = CT == MIMIR_B200_T_BF16, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3;
+  static constexpr int NT = DP <= 128 ? 2 : 1;         // row tiles
+  static constexpr int SUB = DP / 64;                  // 64-element columns of a tile
+  static constexpr int TILE = SUB * TC_KEYS * 128;     // bytes of a K or V tile, and of a Q tile
+  static constexpr int NS = DP == 64 ? 6 : DP == 128 ? 4 : 2;
+  static constexpr int SCALES = CODED ? NS / 2 * 2 * TC_KEYS * 4 : 0;  // [V stage][key, value][key]
+  static constexpr int OFFS = 2 * TC_KEYS * 8;         // where the rows of a key tile lie, two tiles
+  static constexpr int SMEM = NT * TILE + NS * TILE + SCALES + OFFS + 512;
+  static constexpr int THREADS = NT * 128 + 128;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {  // zeros where there is nothing
+  const int n = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// MN-major operand of 64-element columns `column` bytes apart, 16 keys (two groups of eight 128-byte rows) an instruction
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t column) {
+  return static_cast<uint64_t>((saddr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(column >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+template <int DP, int CT>
+__global__ void __launch_bounds__(TcShape<DP, CT>::THREADS, 1)
+paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
+  using S = TcShape<DP, CT>;
+  constexpr bool BF = S::BF, CODED = S::CODED;
+  constexpr int NT = S::NT, NS = S::NS, TILE = S::TILE, SUB = S::SUB;
+  constexpr float LOG2E = 1.4426950408889634f;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it
+    if (threadIdx.x == 0) atomicExch(a.err_word, 60);
+    return;
+  }
+  uint8_t* sq = smem;
+  uint8_t* ring = sq + NT * TILE;
+  float* scales = reinterpret_cast<float*>(ring + NS * TILE);
+  long long* offs = reinterpret_cast<long long*>(ring + NS * TILE + S::SCALES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * TILE + S::SCALES + S::OFFS);
+  uint64_t *kv_full = bars, *kv_empty = bars + NS, *s_full = bars + 2 * NS /*[2]*/, *p_full = s_full + 2 /*[2]*/, *pv_done = s_full + 4 /*[2]*/, *drained = s_full + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 7);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* missing = abort_flag + 1;  // the loaders met a page outside the cache
+
+  const PagedView& p = a.p;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int split = static_cast<int>(blockIdx.x) % a.splits, unit = static_cast<int>(blockIdx.x) / a.splits;
+  // (the last rows see the most keys: their CTAs start first)
+  const int tile = a.tiles - 1 - unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
+  const PagedSeq seq = paged_seq(p, s);
+  const int n_rows = seq.rows * a.group, r0 = tile * NT * TC_ROWS;
+  if (n_rows <= a.few || r0 >= n_rows) return;
+  const int r_end = min(r0 + NT * TC_ROWS, n_rows), tiles_here = (r_end - r0 + TC_ROWS - 1) / TC_ROWS;
+  const int pos0 = seq.kv - seq.rows;
+  const int pos_first = pos0 + r0 / a.group, pos_last = pos0 + (r_end - 1) / a.group;
+  const int k_end = a.causal ? min(seq.kv, pos_last + 1) : seq.kv;
+  const int k_begin = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
+  const int t_first = k_begin / TC_KEYS, t_all = k_end > k_begin ? (k_end + TC_KEYS - 1) / TC_KEYS - t_first : 0;
+  const int kt0 = t_first + static_cast<int>(static_cast<long long>(t_all) * split / a.splits);
+  const int n_kt = t_first + static_cast<int>(static_cast<long long>(t_all) * (split + 1) / a.splits) - kt0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(kv_full + i, TC_LOADERS);
+      mbar_init(kv_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(pv_done + i, 1);
+    }
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    *missing = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == NT * 4) {
+    tmem_alloc(tmem_slot, TC_TMEM);
+    tmem_relinquish();
+  }
+
+  // ---- queries: a softmax thread lays its row out, 8 elements to a 16-byte chunk ---------------------------------------------------------
+  float c2 = 0.0f;
+  const int t = warp >> 2, r_local = static_cast<int>(threadIdx.x) & 127, r = r0 + t * TC_ROWS + r_local;
+  const int tok = r / a.group;
+  if (t < NT) {
+    const int h = head * a.group + r - tok * a.group;
+    const bool there = r < r_end;
+    const char* src = static_cast<const char*>(a.q) + ((seq.row0 + tok) * a.q_row + h * a.q_head) * 2;
+    const bool from_bf = a.type == MIMIR_B200_T_BF16;
+    auto read = [&](int c, float (&f)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+      if (there && 8 * c < p.head_dim) {
+        if (from_bf) unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(src + 16 * c), f);
+        else unpack8<MIMIR_B200_T_F16>(load8<MIMIR_B200_T_F16>(src + 16 * c), f);
+      }
+    };
+    // bfloat16 as half: the row times a power of two that brings its largest to [1, 2) (bits below 2^-24 of that are lost)
+    float up = 1.0f, down = 1.0f;
+    if (!BF && from_bf) {
+      float top = 0.0f;
+      for (int c = 0; c < DP / 8; ++c) {
+        float f[8];
+        read(c, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+      }
+      const int e2 = min(252, max(1, static_cast<int>(__float_as_uint(top) >> 23)));
+      up = __uint_as_float(static_cast<uint32_t>(e2) << 23);
+      down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+    }
+    c2 = fabsf(a.scale) * LOG2E * up * (CT == MIMIR_B200_T_E4M3 ? 256.0f : 1.0f);
+    if (a.scale < 0.0f) down = -down;  // (the largest product is then the smallest score's)
+    for (int c = 0; c < DP / 8; ++c) {
+      float f[8];
+      read(c, f);
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack2<BF>(f[2 * e] * down, f[2 * e + 1] * down);
+      *reinterpret_cast<uint4*>(sq + t * TILE + (c >> 3) * (TC_ROWS * 128) + r_local * 128 + (((c & 7) ^ (r_local & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    fence_proxy_async_smem();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem_o = tmem + 2 * TC_KEYS;  // tile t at + t * DP
+
+  if (warp > NT * 4) {
+    // ---- loaders -----------------------------------------------------------------------------------------------------------------------------
+    const int id = static_cast<int>(threadIdx.x) - (NT * 128 + 32);
+    const uint32_t ring_at = smem_u32(ring);
+    bool ok = true, pending = false;
+    for (int j = 0; j < n_kt; ++j) {  // (a thread whose wait gave up keeps coming to the barrier)
+      const int key0 = (kt0 + j) * TC_KEYS;
+      long long* at = offs + (j & 1) * TC_KEYS;
+      float* sc = scales + (j % (NS / 2)) * 2 * TC_KEYS;
+      long long scale_at[2] = {-1, -1};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = id + i * TC_LOADERS, key = key0 + k;
+        if (k < TC_KEYS) {
+          long long where = -1;
+          if (key >= k_begin && key < k_end) {
+            const int pi = p.by_page.div(key), slot = key - pi * p.page_size, page = paged_page(p, s, pi);
+            if (page >= 0) {
+              where = page * p.page_stride + slot * p.slot_stride + head * p.head_stride;
+              scale_at[i] = (static_cast<long long>(page) * p.kv_heads + head) * p.page_size + slot;
+            } else {
+              *missing = 1;
+            }
+          }
+          at[k] = where;
+        }
+      }
+      __syncwarp();
+      asm volatile("barrier.sync 1, 96;" ::: "memory");
+#pragma unroll
+      for (int kv = 0; kv < 2 && ok; ++kv) {
+        const int i = 2 * j + kv, st = i % NS;
+        const uint32_t round = static_cast<uint32_t>((i / NS) & 1) ^ 1;
+        if (!CODED && pending && !mbar_test(kv_empty + st, round)) {
+          // no stage free: the tile on its way is handed over first (what frees a stage may be waiting for it)
+          copies_wait<0>();
+          fence_proxy_async_smem();
+          mbar_arrive(kv_full + (i - 1) % NS);
+          pending = false;
+        }
+        if (!mbar_wait(kv_empty + st, round, abort_flag, a.err_word, 61)) { ok = false; break; }
+        const uint32_t dst = ring_at + st * TILE;
+        const char* src = static_cast<const char*>(kv ? p.v : p.k);
+        if constexpr (!CODED) {
+          // the copies of one tile are on their way while the next one's are issued; a tile is handed over when its own are there
+#pragma unroll 4
+          for (int x = id; x < TC_KEYS * (DP / 8); x += TC_LOADERS) {
+            const int k = x / (DP / 8), c = x % (DP / 8);
+            const bool there = at[k] >= 0 && 8 * c < p.head_dim;
+            copy16(dst + (c >> 3) * (TC_KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), there ? src + (at[k] + 8 * c) * 2 : src, there);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (pending) {
+            copies_wait<1>();
+            fence_proxy_async_smem();
+            mbar_arrive(kv_full + (i - 1) % NS);
+          }
+          pending = true;
+        } else {
+          constexpr int U = 4;
+          for (int x0 = id; x0 < TC_KEYS * (DP / 8); x0 += U * TC_LOADERS) {
+            Raw8<CT> raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int x = x0 + u * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
+              raw[u].w[0] = raw[u].w[1] = 0;
+              if (k < TC_KEYS && at[k] >= 0 && 8 * c < p.head_dim) raw[u] = load8<CT>(src + at[k] + 8 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int x = x0 + u * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
+              uint32_t hi[4], lo[4];
+              to_pairs<CT>(raw[u], hi, lo);
+              if (k < TC_KEYS)
+                *reinterpret_cast<uint4*>(ring + st * TILE + (c >> 3) * (TC_KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            }
+          }
+          if (kv) {  // both scales with the values, whose stage is let go of last
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const int k = id + n * TC_LOADERS;
+              if (k < TC_KEYS) {
+                sc[k] = scale_at[n] >= 0 ? __ldg(p.k_scale + scale_at[n]) : 0.0f;
+                sc[TC_KEYS + k] = scale_at[n] >= 0 ? __ldg(p.v_scale + scale_at[n]) : 0.0f;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(kv_full + st);
+        }
+      }
+    }
+    if constexpr (!CODED) {
+      copies_wait<0>();
+      fence_proxy_async_smem();
+      if (ok && pending) mbar_arrive(kv_full + (2 * n_kt - 1) % NS);
+    }
+  } else if (warp == NT * 4) {
+    // ---- tensor instructions -------------------------------------------------------------------------------------------------------------------
+    const uint32_t idesc_s = make_idesc(TC_ROWS, TC_KEYS, BF ? 0 : 1), idesc_o = make_idesc(TC_ROWS, DP, BF ? 0 : 1) | (1u << 16);
+    const uint32_t q_at = smem_u32(sq), ring_at = smem_u32(ring);
+    auto scores = [&](int tt, int j) {  // S = Q_tt K_j^T
+      const uint32_t k_at = ring_at + ((2 * j) % NS) * TILE, d = tmem + (NT == 2 ? tt : (j & 1)) * TC_KEYS;
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t o = (k >> 2) * (TC_KEYS * 128) + (k & 3) * 32;
+          umma_bf16(d, make_smem_desc(q_at + tt * TILE + o, 128), make_smem_desc(k_at + o, 128), idesc_s, k != 0 ? 1u : 0u);
+        }
+        umma_commit(s_full + (NT == 2 ? tt : (j & 1)));
+      }
+      __syncwarp();
+    };
+    auto values = [&](int tt, int j) {  // O_tt (+)= P V_j
+      const uint32_t v_at = ring_at + ((2 * j + 1) % NS) * TILE, pa = tmem + (NT == 2 ? tt : (j & 1)) * TC_KEYS, d = tmem_o + tt * DP;
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < TC_KEYS / 16; ++k) umma_f16_ts(d, pa + 8 * k, desc_mn(v_at + k * 2048, TC_KEYS * 128), idesc_o, (j | k) != 0 ? 1u : 0u);
+        umma_commit(pv_done + tt);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int i) {
+      if (elect_one()) umma_commit(kv_empty + i % NS);
+      __syncwarp();
+    };
+    auto full = [&](int i, int where) {
+      const bool ok = mbar_wait_warp(kv_full + i % NS, static_cast<uint32_t>((i / NS) & 1), abort_flag, a.err_word, where);
+      tcgen05_fence_after();
+      return ok;
+    };
+    auto ready = [&](int tt, int j) {
+      const bool ok = mbar_wait_warp(p_full + (NT == 2 ? tt : (j & 1)), static_cast<uint32_t>((NT == 2 ? j : j >> 1) & 1), abort_flag, a.err_word, 64);
+      tcgen05_fence_after();
+      return ok;
+    };
+    bool ok = n_kt > 0 && full(0, 62);
+    if (ok) {
+      for (int tt = 0; tt < tiles_here; ++tt) scores(tt, 0);
+      release(0);
+    }
+    for (int j = 0; j < n_kt && ok; ++j) {
+      const bool more = j + 1 < n_kt;
+      if constexpr (NT == 2) {
+        for (int tt = 0; tt < tiles_here && ok; ++tt) {
+          ok = ready(tt, j);
+          if (ok && tt == 0) ok = full(2 * j + 1, 63);
+          if (!ok) break;
+          values(tt, j);
+          if (tt == tiles_here - 1) release(2 * j + 1);
+          if (more) {
+            if (tt == 0) ok = full(2 * j + 2, 62);
+            if (!ok) break;
+            scores(tt, j + 1);
+            if (tt == tiles_here - 1) release(2 * j + 2);
+          }
+        }
+      } else {
+        if (more) {
+          ok = full(2 * j + 2, 62);
+          if (!ok) break;
+          scores(0, j + 1);
+          release(2 * j + 2);
+        }
+        ok = ready(0, j) && full(2 * j + 1, 63);
+        if (!ok) break;
+        values(0, j);
+        release(2 * j + 1);
+      }
+    }
+    // everything issued has finished before tensor memory is let go of
+    if (elect_one()) umma_commit(drained);
+    __syncwarp();
+    int drain_abort = 0;
+    mbar_wait_warp(drained, 0, &drain_abort, a.err_word, 65);
+  } else if (t < tiles_here) {
+    // ---- softmax: a thread a row -------------------------------------------------------------------------------------------------------------------
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int pos = pos0 + min(tok, (r_end - 1) / a.group);
+    const int lim_hi = a.causal ? min(seq.kv, pos + 1) : seq.kv, lim_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    // of all of this warp's rows: keys that every row sees (positions ascend with the rows)
+    const int w_first = __shfl_sync(0xffffffffu, pos, 0), w_last = __shfl_sync(0xffffffffu, pos, 31);
+    const int all_hi = a.causal ? min(seq.kv, w_first + 1) : seq.kv, all_lo = a.window > 0 ? max(0, w_last - a.window + 1) : 0;
+    float base = -INFINITY, sum = 0.0f;
+    float v_unit = 0.0f;  // codes: the power of two that O's values are in
+    bool alive = true;
+    for (int j = 0; j < n_kt; ++j) {
+      const int buf = NT == 2 ? t : (j & 1);
+      const uint32_t ts = tmem + buf * TC_KEYS + lanes;
+      alive = mbar_wait_warp(s_full + buf, static_cast<uint32_t>((NT == 2 ? j : j >> 1) & 1), abort_flag, a.err_word, 66);
+      const float* sc = scales + (j % (NS / 2)) * 2 * TC_KEYS;
+      if (CODED && alive) alive = mbar_wait_warp(kv_full + (2 * j + 1) % NS, static_cast<uint32_t>(((2 * j + 1) / NS) & 1), abort_flag, a.err_word, 67);
+      if (!alive) break;
+      tcgen05_fence_after();
+      uint32_t w[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32_nowait(ts + 32 * c, w[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld_regs(w[c]);
+      const int key0 = (kt0 + j) * TC_KEYS;
+      if constexpr (CODED) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(sc + 32 * c + i);
+            w[c][i] = __float_as_uint(__uint_as_float(w[c][i]) * k4.x);
+            w[c][i + 1] = __float_as_uint(__uint_as_float(w[c][i + 1]) * k4.y);
+            w[c][i + 2] = __float_as_uint(__uint_as_float(w[c][i + 2]) * k4.z);
+            w[c][i + 3] = __float_as_uint(__uint_as_float(w[c][i + 3]) * k4.w);
+          }
+      }
+      if (key0 < all_lo || key0 + TC_KEYS > all_hi) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int key = key0 + 32 * c + i;
+            if (key < lim_lo || key >= lim_hi) w[c][i] = 0xff800000u;
+          }
+      }
+      if (*missing) {  // a page of this sequence is none of the cache's: which keys are out is looked up again
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            const int key = key0 + 32 * c + i;
+            if (key + 7 >= k_begin && key < k_end && paged_page(p, s, p.by_page.div(key)) < 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[c][i + e] = 0xff800000u;
+            }
+          }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) mx = max3(mx, __uint_as_float(w[c][i]), __uint_as_float(w[c][i + 1]));
+      mx *= c2;
+      float grow = 0.0f;
+      if constexpr (CODED) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(sc[TC_KEYS + 32 * i + lane]));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int e2 = min(240, max(14, static_cast<int>(__float_as_uint(top) >> 23)));
+        grow = __uint_as_float(static_cast<uint32_t>(e2) << 23);
+      }
+      const bool raise = mx > base + 8.0f || (CODED && grow > v_unit);
+      if (__any_sync(0xffffffffu, raise)) {
+        const float nb = fmaxf(base, mx);
+        float f = base == -INFINITY ? 0.0f : ex2(base - nb);
+        sum *= f;
+        base = nb;
+        if constexpr (CODED) {
+          const float nu = fmaxf(v_unit, grow);
+          f *= v_unit / nu;
+          v_unit = nu;
+        }
+        if (j > 0) {
+          if (!mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(j - 1) & 1, abort_flag, a.err_word, 68)) { alive = false; break; }
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32_nowait(tmem_o + t * DP + lanes + 32 * c, o);
+            tmem_wait_ld_regs(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_32x32(tmem_o + t * DP + lanes + 32 * c, o);
+          }
+        }
+      }
+      const float sub = base == -INFINITY ? 0.0f : base, inv_unit = CODED ? 1.0f / v_unit : 1.0f;
+      float part[4] = {};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float e[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            e[n] = ex2(fmaf(__uint_as_float(w[c][i + n]), c2, -sub));
+            part[n] += e[n];
+          }
+          if constexpr (CODED) {
+            const float4 v4 = *reinterpret_cast<const float4*>(sc + TC_KEYS + 32 * c + i);
+            e[0] *= v4.x * inv_unit, e[1] *= v4.y * inv_unit, e[2] *= v4.z * inv_unit, e[3] *= v4.w * inv_unit;
+          }
+          pk[i / 2] = pack2<BF>(e[0], e[1]);
+          pk[i / 2 + 1] = pack2<BF>(e[2], e[3]);
+        }
+        tmem_st_32x16(ts + 16 * c, pk);
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + buf);
+    }
+    if (alive && n_kt > 0) alive = mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(n_kt - 1) & 1, abort_flag, a.err_word, 69);
+    if (alive) {
+      tcgen05_fence_after();
+      const bool there = r < r_end;
+      const float unit_v = (CODED ? v_unit : 1.0f) * (CT == MIMIR_B200_T_E4M3 ? 256.0f : 1.0f);
+      const float inv = a.splits > 1 ? unit_v : sum == 0.0f ? 0.0f : unit_v / sum;
+      const int h = head * a.group + r - tok * a.group;
+      const long long part_row = static_cast<long long>(blockIdx.x) * (NT * TC_ROWS) + t * TC_ROWS + r_local;
+      char* dst = static_cast<char*>(a.out) + ((seq.row0 + tok) * a.o_row + h * a.o_head) * 2;
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0;
+        if (n_kt > 0) {
+          tmem_ld_32x32_nowait(tmem_o + t * DP + lanes + 32 * c, o);
+          tmem_wait_ld_regs(o);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          const int d = 32 * c + i;
+          if (!there || d >= p.head_dim) continue;
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[i + e]) * inv;
+          if (a.splits > 1) {
+            store8<MIMIR_B200_T_F32>(a.part_o + part_row * p.head_dim + d, pack8<MIMIR_B200_T_F32>(f));
+          } else if (a.type == MIMIR_B200_T_BF16) {
+            store8<MIMIR_B200_T_BF16>(dst + 2 * d, pack8<MIMIR_B200_T_BF16>(f));
+          } else {
+            store8<MIMIR_B200_T_F16>(dst + 2 * d, pack8<MIMIR_B200_T_F16>(f));
+          }
+        }
+        __syncwarp();
+      }
+      if (there) {
+        if (a.splits > 1) a.part_ml[part_row] = make_float2(base, sum);
+        else store_lse(a, seq.row0, r, head, base, sum);
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == NT * 4) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, TC_TMEM);
+  }
+}
+
+template <int DP, int CT>
+int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
+  using S = TcShape<DP, CT>;
+  static PerDeviceOnce once;
+  MB_TRY(once.run([]() -> int {
+    MB_CUDA(cudaFuncSetAttribute(paged_attention_tc_kernel<DP, CT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    return MIMIR_B200_OK;
+  }));
+  const long long grid = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * a.tiles * a.splits;
+  paged_attention_tc_kernel<DP, CT><<<static_cast<unsigned>(grid), S::THREADS, S::SMEM, st>>>(a);
+  MB_CUDA(cudaGetLastError());
+  count_launch();
+  return MIMIR_B200_OK;
+}
+template <int CT>
+int launch_tc_dim(const AttendArgs& a, cudaStream_t st) {
+  if (a.p.head_dim <= 64) return launch_tc_as<64, CT>(a, st);
+  if (a.p.head_dim <= 128) return launch_tc_as<128, CT>(a, st);
+  return launch_tc_as<256, CT>(a, st);
+}
+
+}  // namespace
+
+int launch_paged_attention_tc(const AttendArgs& a, int cache_type, cudaStream_t st) {
+  switch (cache_type) {
+    case MIMIR_B200_T_F16: return launch_tc_dim<MIMIR_B200_T_F16>(a, st);
+    case MIMIR_B200_T_BF16: return launch_tc_dim<MIMIR_B200_T_BF16>(a, st);
+    case MIMIR_B200_T_I8: return launch_tc_dim<MIMIR_B200_T_I8>(a, st);
+    default: return launch_tc_dim<MIMIR_B200_T_E4M3>(a, st);
+  }
+}
+
+}  // namespace mb

@@ -161,7 +161,8 @@ def check_attention(p, q, out, lse, type_, causal, window):
     n = p.n_rows
     want, want_lse, weight, reach = attention(p, q[:n, :, : p.dim].double().cpu().numpy(), 1 / math.sqrt(p.dim), causal, window)
     # bf16 and e4m3 / i8 tensors meet bf16 or half terms; the bound goes by the result's type
-    bound, lse_bound = attention_bounds(want, weight, reach, p.dim, max(p.kv, default=0), BF16 if p.type == BF16 else type_)
+    chunk = type_ != F32 and q.shape[1] // p.heads * max(p.rows, default=0) > 64
+    bound, lse_bound = attention_bounds(want, weight, reach, p.dim, max(p.kv, default=0), BF16 if p.type == BF16 else type_, chunk)
     err = np.abs(out[:n, :, : p.dim].double().cpu().numpy() - want)
     assert np.all(err <= bound), f"{np.max(err / np.maximum(bound, 1e-300))} of the bound"
     got = lse[:n].double().cpu().numpy()
@@ -191,6 +192,53 @@ def test_attention(backend, rows, kv, kv_heads, group, dim, page, causal, window
     q, out, lse = attend(backend, p, heads, type_, causal, window, gap=8 if dim == 80 else 0, extra_rows=2)
     backend.check_device()
     check_attention(p, q, out, lse, type_, causal, window)
+
+
+@pytest.mark.parametrize("cache,type_", [pair for pair in PAIRS if pair[1] != F32])
+@pytest.mark.parametrize("rows,kv,kv_heads,group,dim,page,causal,window", [
+    ([65], [65], 1, 1, 64, 16, True, 0),                                   # one row over; a tile mostly empty
+    ([257, 1, 64, 130], [300, 700, 64, 130], 1, 1, 128, 24, True, 0),      # many and few rows in one batch
+    ([200, 90], [900, 50], 2, 2, 64, 8, True, 0),                          # more rows than keys
+    ([100, 0, 70], [0, 40, 71], 1, 4, 96, 128, False, 0),                  # no keys; no rows; not causal
+    ([300], [1111], 1, 1, 128, 64, True, 77),                              # a window narrower than a tile
+    ([129], [2000], 1, 2, 256, 16, True, 300),
+    ([80], [9000], 1, 2, 256, 64, True, 0),                                # few tiles, many keys: parts in the workspace
+    ([80, 5], [9000, 3000], 1, 2, 40, 56, False, 0)])
+def test_attention_of_chunks(backend, rows, kv, kv_heads, group, dim, page, causal, window, cache, type_):
+    p = Pages(rows, kv, kv_heads, dim, page, cache, "head" if group == 2 else "slot", seed=dim, gap=24 if dim == 96 else 0)
+    p.fill()
+    q, out, lse = attend(backend, p, kv_heads * group, type_, causal, window, gap=8 if dim == 40 else 0, extra_rows=3)
+    backend.check_device()
+    check_attention(p, q, out, lse, type_, causal, window)
+
+
+@pytest.mark.parametrize("cache,type_", [(BF16, BF16), (E4M3, F16), (F16, BF16)])
+def test_chunks_with_a_negative_scale_a_bad_page_and_large_scores(backend, cache, type_):
+    p = Pages([150, 70], [400, 90], 2, 64, 16, cache, seed=2)
+    p.fill(spread=2.0)
+    q, out, lse = attend(backend, p, 4, type_, spread=20.0)
+    check_attention(p, q, out, lse, type_, True, 0)
+    a = backend.paged_attention(q.data_ptr(), out.data_ptr(), type_, 4, 256, 64, 256, 64, -0.02, lse=lse.data_ptr())
+    backend.dev_paged_attention(p.cache(), p.batch(), a)
+    want, want_lse, weight, reach = attention(p, q.double().cpu().numpy(), -0.02, True, 0)
+    bound, lse_bound = attention_bounds(want, weight, reach, 64, 400, BF16 if cache == BF16 else type_, True)
+    assert np.all(np.abs(out.double().cpu().numpy() - want) <= bound)
+    # keys 32 .. 47 of the first sequence are in no page
+    bad = p.dev[2].clone()
+    bad[0, 2] = -1
+    backend.dev_paged_attention(p.cache(), p.batch(page_table=bad.data_ptr()), a)
+    with pytest.raises(backend.MimirB200Error, match="page number"):
+        backend.check_device()
+    kept = [j for j in range(400) if not 32 <= j < 48]
+    r = Pages([150, 70], [384, 90], 2, 64, 16, cache, seed=3)
+    for w in range(2):
+        r.put(w, 0, np.arange(384), torch.from_numpy(p.get(w, 0)[kept]).cuda())
+        r.put(w, 1, np.arange(90), torch.from_numpy(p.get(w, 1)).cuda())
+    for w in range(2):  # (stored as the same codes and scales: nothing is rounded again)
+        assert np.abs(r.get(w, 0) - p.get(w, 0)[kept]).max() <= 2.0**-20 * np.abs(p.get(w, 0)).max()
+    want, _, weight, reach = attention(r, q.double().cpu().numpy(), -0.02, True, 0)
+    bound, _ = attention_bounds(want, weight, reach, 64, 400, BF16 if cache == BF16 else type_, True)
+    assert np.all(np.abs(out.double().cpu().numpy() - want) <= bound + 2.0**-18 * np.abs(weight))
 
 
 @pytest.mark.parametrize("cache,type_", [(BF16, BF16), (F16, F32), (E4M3, BF16), (I8, F16)])
