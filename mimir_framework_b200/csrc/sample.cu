@@ -4,16 +4,29 @@
 //   beginning that holds top_p of their mass; of those w_i >= min_p.  The token is the first index (in index order) at which the running
 //   sum of the candidates' w exceeds u times their whole sum.
 //
-// A sum is compared with a border, so every w is a 64-bit integer (w times a power of two that leaves room for n of them): sums of
-// integers are the same in every order.  The borders of top_k and top_p are found digit by digit of the logits' order (their
-// bits, as unsigned integers that ascend with the value): counts and masses of 256 digits at a time, four rounds.
+// A row is read once: a cluster of CTAs keeps it in shared memory, a slice each, and meets through distributed shared memory.
+//   1. the largest logit
+//   2. with top_k or top_p: counts and masses of 1024 intervals of (max - x) / T, the interval in which the border lies, and in it the
+//      border itself: up to 1024 logits of it are sorted in one CTA, more are divided again by their bits
+//   3. masses of the warps' stretches of the row in index order; the stretch in which u falls is walked
+// Sums are compared with borders, so every w is an integer (w times a power of two that leaves room for n of them): sums of integers are
+// the same in every order and division of the work.  w comes from a table of 2^(k / 64) and four terms of the exponential series in
+// fp64, relative error under 2^-44: the fp64 lanes (64 a cycle and SM, eleven operations a logit) are what a large batch waits for.
+#include <cooperative_groups.h>
+
+#include <cmath>
+
 #include "common.h"
 #include "paged.cuh"
 
 namespace mb {
 namespace {
 
-constexpr int SA_THREADS = 1024, SA_WARPS = SA_THREADS / 32;
+namespace cg = cooperative_groups;
+
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 1024, SA_LIST = 1024;
+constexpr size_t SA_SLICE = size_t(70) << 10;   // bytes of a row in a CTA's shared memory: two CTAs to an SM
+constexpr size_t SA_LARGE = size_t(180) << 10;  // the most: one
 
 // ascending in the value; 0: not a candidate (not a number, -infinity)
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -23,12 +36,89 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
+// elements of 16 bytes
 template <int T>
-__device__ __forceinline__ float logit(const void* row, int i) {
+struct Vec {
+  static constexpr int N = 16 / type_bytes(T);
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (T == MIMIR_B200_T_F32) {
+        f[i] = __uint_as_float(w[i]);
+      } else if constexpr (T == MIMIR_B200_T_F16) {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = p.x, f[2 * i + 1] = p.y;
+      } else {
+        f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+};
+template <int T>
+__device__ __forceinline__ float logit(const void* row, long long i) {
   if constexpr (T == MIMIR_B200_T_F32) return __ldg(static_cast<const float*>(row) + i);
   else if constexpr (T == MIMIR_B200_T_F16) return __half2float(static_cast<const __half*>(row)[i]);
   else return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
 }
+
+using u64 = unsigned long long;
+
+struct Border {          // candidates: order > order, and the first `ties` of order == order
+  uint32_t order;
+  int ties;
+};
+struct Found {
+  int bin;               // -1: the candidates do not reach the border
+  uint32_t above_n, in_n;
+  u64 above, in;
+};
+
+struct SampleShared {
+  double table[64];
+  uint32_t count[SA_BINS], mass_lo[SA_BINS], mass_hi[SA_BINS];  // of this CTA's slice
+  uint32_t before_n[SA_BINS];                                   // of the row: counts and masses ahead of this CTA's share of the intervals
+  u64 before[SA_BINS];
+  uint32_t bin_n[SA_BINS];
+  u64 bin[SA_BINS];
+  uint32_t list[SA_LIST];
+  uint32_t list_n;
+  u64 scan64[33];
+  uint32_t scan32[33];
+  // read by the cluster's other CTAs
+  float top;
+  int first;
+  uint32_t low, high;
+  uint32_t total_n;
+  u64 total;
+  Found found;
+  Border border;
+  u64 above_border;                                             // mass of candidates above it
+  uint32_t above_border_n;
+  u64 warp_mass[SA_WARPS];
+  uint32_t warp_ties[SA_WARPS];
+};
+
+struct Weigh {
+  double top, scale;  // log2(e) / T
+  double one, magic;  // what a weight of 1 is as an integer, 2^52
+  const double* table;
+  // x <= top; not infinite
+  __device__ __forceinline__ u64 operator()(float x) const {
+    const double y = (static_cast<double>(x) - top) * scale;
+    if (!(y > -64.0)) return 0;
+    const double s = y + 105553116266496.0;  // 1.5 * 2^46: y rounded to 64ths in the low bits
+    const int k = __double2loint(s);
+    const double r = (y - (s - 105553116266496.0)) * 0.69314718055994530942;
+    double p = fma(r, 1.0 / 24, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const double t = table[k & 63];
+    const double w = __hiloint2double(__double2hiint(t) + ((k >> 6) << 20), __double2loint(t)) * p;
+    return static_cast<u64>(__double_as_longlong(fma(w, one, magic)) & 0xfffffffffffffll);
+  }
+};
 
 template <class V>
 __device__ __forceinline__ V warp_scan(V v, int lane) {  // inclusive
@@ -48,7 +138,7 @@ __device__ __forceinline__ V block_scan(V v, V* scratch, V* total) {
   if (lane == 31) scratch[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    const V w = scratch[lane];
+    const V w = lane < SA_WARPS ? scratch[lane] : 0;
     const V s = warp_scan(w, lane);
     scratch[lane] = s - w;
     if (lane == 31) scratch[32] = s;
@@ -58,192 +148,502 @@ __device__ __forceinline__ V block_scan(V v, V* scratch, V* total) {
   return scratch[warp] + inc - v;
 }
 
-struct Weigh {
-  double top, inv_t, one;  // one: what a weight of 1 is as an integer
-  __device__ __forceinline__ unsigned long long operator()(float x) const {
-    return static_cast<unsigned long long>(__double2ull_rn(exp((static_cast<double>(x) - top) * inv_t) * one));
-  }
-};
-
-template <int T>
-__global__ void __launch_bounds__(SA_THREADS) sample_rows_kernel(const __grid_constant__ SampleLaunch a) {
-  static_assert(SA_WARPS == 32, "block_scan");
-  __shared__ unsigned long long mass[256];
-  __shared__ unsigned count[256];
-  __shared__ unsigned long long s64[33];
-  __shared__ int s32[33];
-  __shared__ uint32_t s_order;
-  __shared__ int s_index;
-  const int tid = threadIdx.x, lane = tid & 31, n = a.n;
-  const long long row = blockIdx.x;
+template <int T, bool KEPT>
+__global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid_constant__ SampleLaunch a, int slice) {
+  constexpr int V = Vec<T>::N;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ SampleShared sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n;
+  const long long row = blockIdx.x / ranks;
   const char* x = static_cast<const char*>(a.x) + row * a.row_stride * type_bytes(T);
+  const int first = min(n, rank * slice), mine = min(n, first + slice) - first;  // this CTA's stretch (slice: a multiple of 32 V)
   const float t = a.temperature ? __ldg(a.temperature + row) : 1.0f;
   const int top_k = a.top_k ? __ldg(a.top_k + row) : 0;
   const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f, min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   const float u = __ldg(a.uniform + row);
+  const int vecs = (mine + V - 1) / V;
 
-  // the largest logit, and the first index that has it
-  uint32_t best = 0;
-  int at = n;
-  for (int i = tid; i < n; i += SA_THREADS) {
-    const uint32_t o = order_of(logit<T>(x, i));
-    if (o > best) best = o, at = i;
+  // ---- vector i of the stretch; absent elements are not numbers -------------------------------------------------------------------------
+  auto from_global = [&](int i, float (&f)[V]) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;  // (stretches start on whole vectors)
+    if (aligned && (i + 1) * V <= mine) {
+      Vec<T>::unpack(__ldg(reinterpret_cast<const uint4*>(x) + first / V + i), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = i * V + e < mine ? logit<T>(x, first + i * V + e) : __uint_as_float(0x7fc00000u);
+    }
+  };
+  auto read = [&](int i, float (&f)[V]) {
+    if constexpr (KEPT) Vec<T>::unpack(reinterpret_cast<const uint4*>(dyn)[i], f);
+    else from_global(i, f);
+  };
+
+  // ---- 1. the largest -------------------------------------------------------------------------------------------------------------------
+  float top = -INFINITY;
+  if constexpr (KEPT) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < vecs; i0 += U * SA_THREADS) {
+      uint4 v[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * SA_THREADS;
+        if (i >= vecs) continue;
+        if (aligned && (i + 1) * V <= mine) {
+          v[j] = __ldg(reinterpret_cast<const uint4*>(x) + first / V + i);
+        } else {
+          float f[V];
+          from_global(i, f);
+          if constexpr (T == MIMIR_B200_T_F32) {
+            v[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+          } else {
+            const Raw8<T> r = pack8<T>(f);
+            v[j] = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * SA_THREADS;
+        if (i >= vecs) continue;
+        reinterpret_cast<uint4*>(dyn)[i] = v[j];
+        float f[V];
+        Vec<T>::unpack(v[j], f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = fmaxf(top, f[e]);
+      }
+    }
+  } else {
+    for (int i = tid; i < vecs; i += SA_THREADS) {
+      float f[V];
+      read(i, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = fmaxf(top, f[e]);
+    }
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-    if (ob > best || (ob == best && oi < at)) best = ob, at = oi;
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (tid < 64) sh.table[tid] = exp2(tid * (1.0 / 64));
+  if (tid == 0) sh.list_n = 0;
+  if (lane == 0) reinterpret_cast<float*>(sh.scan32)[warp] = top;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < SA_WARPS; ++w) top = fmaxf(top, reinterpret_cast<float*>(sh.scan32)[w]);
+    sh.top = top;
   }
-  if (tid == 0) s_order = 0, s_index = n;
-  __syncthreads();
-  if (lane == 0) atomicMax(&s_order, best);
-  __syncthreads();
-  if (lane == 0 && best == s_order) atomicMin(&s_index, at);
-  __syncthreads();
-  best = s_order;
-  at = s_index;
-  const float top = value_of(best);
-  if (best == 0 || top == INFINITY || !(t > 0.0f)) {
-    if (tid == 0) {
-      a.ids[row] = best == 0 ? -1 : at;
-      if (a.logprob) a.logprob[row] = best == 0 ? -INFINITY : 0.0f;
+  cluster.sync();
+  top = -INFINITY;
+  for (int c = 0; c < ranks; ++c) top = fmaxf(top, *cluster.map_shared_rank(&sh.top, c));
+
+  if (top == -INFINITY || top == INFINITY || !(t > 0.0f)) {  // the largest's first index, or none
+    int at = 0x7fffffff;
+    if (top > -INFINITY)
+      for (int i = tid; i < vecs && at == 0x7fffffff; i += SA_THREADS) {
+        float f[V];
+        read(i, f);
+#pragma unroll
+        for (int e = V - 1; e >= 0; --e)
+          if (f[e] == top) at = first + i * V + e;
+      }
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (tid == 0) sh.first = 0x7fffffff;
+    __syncthreads();
+    if (lane == 0) atomicMin(&sh.first, at);
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int c = 0; c < ranks; ++c) at = min(at, *cluster.map_shared_rank(&sh.first, c));
+      a.ids[row] = top == -INFINITY ? -1 : at;
+      if (a.logprob) a.logprob[row] = top == -INFINITY ? -INFINITY : 0.0f;
     }
+    cluster.sync();  // (no CTA leaves while others read its shared memory)
     return;
   }
   int room = 0;  // n <= 2^room
   while ((1ll << room) < n) ++room;
   Weigh weigh;
   weigh.top = top;
-  weigh.inv_t = 1.0 / static_cast<double>(t);
-  weigh.one = static_cast<double>(1ull << min(62 - room, 52));
+  weigh.scale = 1.4426950408889634074 / static_cast<double>(t);
+  weigh.one = static_cast<double>(1ull << min(62 - room, 51));
+  weigh.magic = 4503599627370496.0;
+  weigh.table = sh.table;
 
-  // candidates: order > border, and the first `ties` of order == border
-  uint32_t border = 0;
-  int ties = 0;
-  unsigned long long whole = 0;  // their mass
-  auto rounds = [&](bool by_count, long long want_count, unsigned long long want_mass) {
-    // the largest border whose candidates with that order or more are at least want_count many, or have want_mass; among orders >= floor_order
-    uint32_t prefix = 0;
-    unsigned long long above = 0;
-    long long above_n = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+  // ---- 2. the border ---------------------------------------------------------------------------------------------------------------------
+  const bool by_count = top_k > 0 && top_k < n, by_mass = top_p < 1.0f;
+  Border border = {0, 0};
+  if (by_count || by_mass) {
+    const float width = static_cast<float>(32.0 * weigh.scale);  // of (max - x), in intervals
+    const int share = SA_BINS / ranks;                           // intervals that this CTA adds up
+    auto interval = [&](float v) { return min(SA_BINS - 1, __float2int_rz((top - v) * width)); };
+    auto add = [&](int bin, float v, bool weighed) {
+      atomicAdd(&sh.count[bin], 1u);
+      if (!weighed) return;
+      const u64 w = weigh(v);
+      const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&sh.mass_lo[bin], lo);
+      const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
+      if (hi) atomicAdd(&sh.mass_hi[bin], hi);
+    };
+    auto clear = [&]() {
+      for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.count[i] = sh.mass_lo[i] = sh.mass_hi[i] = 0;
       __syncthreads();
-      if (tid < 256) mass[tid] = 0, count[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += SA_THREADS) {
-        const float v = logit<T>(x, i);
-        const uint32_t o = order_of(v);
-        if (o == 0 || o < border) continue;
-        if (shift < 24 && (o >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-        atomicAdd(&count[(o >> shift) & 255], 1u);
-        if (!by_count) atomicAdd(&mass[(o >> shift) & 255], weigh(v));
-      }
-      __syncthreads();
-      // thread d: what orders of digits above d hold
-      const int d = 255 - tid;
-      unsigned long long all;
-      int all_n;
-      const unsigned long long m_here = tid < 256 ? mass[d] : 0;
-      const int c_here = tid < 256 ? static_cast<int>(count[d]) : 0;
-      const unsigned long long m_before = block_scan(m_here, s64, &all) + above;
-      const long long c_before = block_scan(c_here, s32, &all_n) + above_n;
-      if (tid == 0) s_index = -1;
-      __syncthreads();
-      if (tid < 256 && c_here > 0) {
-        const bool crosses = by_count ? (c_before < want_count && c_before + c_here >= want_count)
-                                      : (m_before < want_mass && m_before + m_here >= want_mass);
-        if (crosses) {
-          s_index = d;
-          s64[0] = m_before;
-          s32[0] = static_cast<int>(c_before);
+    };
+    // counts and masses of the row's intervals in this CTA's share, and what lies ahead of each
+    auto gather = [&]() {
+      cluster.sync();
+      u64 m[2] = {0, 0};
+      uint32_t c[2] = {0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = 2 * tid + h;
+        if (i >= share) continue;
+        for (int q = 0; q < ranks; ++q) {
+          const SampleShared* s = cluster.map_shared_rank(&sh, q);
+          c[h] += s->count[rank * share + i];
+          m[h] += (static_cast<u64>(s->mass_hi[rank * share + i]) << 32) + s->mass_lo[rank * share + i];
         }
       }
+      u64 all;
+      uint32_t all_n;
+      u64 mb = block_scan(m[0] + m[1], sh.scan64, &all);
+      uint32_t cb = block_scan(c[0] + c[1], sh.scan32, &all_n);
+      if (tid == 0) sh.total = all, sh.total_n = all_n;
+      cluster.sync();
+      for (int q = 0; q < rank; ++q) {
+        const SampleShared* s = cluster.map_shared_rank(&sh, q);
+        mb += s->total, cb += s->total_n;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = 2 * tid + h;
+        if (i < share) sh.before[i] = mb, sh.before_n[i] = cb, sh.bin[i] = m[h], sh.bin_n[i] = c[h];
+        mb += m[h], cb += c[h];
+      }
       __syncthreads();
-      if (s_index < 0) return false;  // fewer than that: all of them
-      prefix |= static_cast<uint32_t>(s_index) << shift;
-      above = s64[0];
-      above_n = s32[0];
+    };
+    // the interval in which the candidates reach want_n in number or want in mass, counted from (above_n, above)
+    auto find = [&](bool number, uint32_t want_n, u64 want, uint32_t above_n, u64 above) {
+      __syncthreads();
+      if (tid == 0) sh.found.bin = -1;
+      cluster.sync();
+      for (int i = tid; i < share; i += SA_THREADS) {
+        const u64 b = above + sh.before[i], m = sh.bin[i];
+        const uint32_t bn = above_n + sh.before_n[i], c = sh.bin_n[i];
+        if (c > 0 && (number ? bn < want_n && bn + c >= want_n : b < want && b + m >= want)) {
+          Found f;
+          f.bin = rank * share + i;
+          f.above = b, f.above_n = bn, f.in = m, f.in_n = c;
+          for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->found = f;
+        }
+      }
+      cluster.sync();
+      return sh.found;
+    };
+    // mass of candidates up to a border
+    u64 whole = 0;
+    auto settle = [&](bool number, uint32_t want_n, u64 want) {
+      Found f = find(number, want_n, want, 0, 0);
+      if (f.bin < 0) return;  // all of them
+      // logits of the interval: the level's own division of them
+      uint32_t low = 0;
+      int shift = -1;  // -1: intervals of values; else (order - low) >> shift
+      uint32_t range_lo = 1, range_hi = 0xffffffffu;
+      const int value_bin = f.bin;
+      auto member = [&](uint32_t o, float v) { return o >= range_lo && o <= range_hi && interval(v) == value_bin; };
+      while (f.in_n > SA_LIST && shift != 0) {
+        // their range of orders, divided evenly, the largest first
+        uint32_t lo = 0xffffffffu, hi = 0;
+        for (int i = tid; i < vecs; i += SA_THREADS) {
+          float v[V];
+          read(i, v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const uint32_t o = order_of(v[e]);
+            if (o && member(o, v[e])) lo = min(lo, o), hi = max(hi, o);
+          }
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+        __syncthreads();
+        if (tid == 0) sh.low = 0xffffffffu, sh.high = 0;
+        clear();
+        if (lane == 0) atomicMin(&sh.low, lo), atomicMax(&sh.high, hi);
+        cluster.sync();
+        lo = 0xffffffffu, hi = 0;
+        for (int q = 0; q < ranks; ++q) lo = min(lo, *cluster.map_shared_rank(&sh.low, q)), hi = max(hi, *cluster.map_shared_rank(&sh.high, q));
+        shift = 0;
+        while (((hi - lo) >> shift) >= SA_BINS) ++shift;
+        low = lo;
+        for (int i = tid; i < vecs; i += SA_THREADS) {
+          float v[V];
+          read(i, v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const uint32_t o = order_of(v[e]);
+            if (o && member(o, v[e])) add(static_cast<int>((hi - o) >> shift), v[e], by_mass);
+          }
+        }
+        gather();
+        const uint32_t above_n = f.above_n;
+        const u64 above = f.above;
+        f = find(number, want_n, want, above_n, above);
+        if (f.bin < 0) return;  // (never: the sums are exact)
+        range_hi = hi - (static_cast<uint32_t>(f.bin) << shift);
+        const uint32_t span = (1u << shift) - 1;
+        range_lo = range_hi - low < span ? low : range_hi - span;
+      }
+      if (f.in_n <= SA_LIST && shift != 0) {
+        // sorted in the first CTA
+        SampleShared* home = cluster.map_shared_rank(&sh, 0);
+        for (int i = tid; i < vecs; i += SA_THREADS) {
+          float v[V];
+          read(i, v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const uint32_t o = order_of(v[e]);
+            if (o && member(o, v[e])) {
+              const uint32_t at = atomicAdd(&home->list_n, 1u);
+              if (at < SA_LIST) home->list[at] = o;
+            }
+          }
+        }
+        cluster.sync();
+        if (rank == 0) {
+          const int have = static_cast<int>(min(sh.list_n, static_cast<uint32_t>(SA_LIST)));
+          for (int i = tid; i < SA_LIST; i += SA_THREADS)
+            if (i >= have) sh.list[i] = 0;
+          int size = 32;
+          while (size < have) size *= 2;
+          __syncthreads();
+          for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j; j >>= 1) {
+              for (int i = tid; i < size / 2; i += SA_THREADS) {
+                const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1));
+                const uint32_t a0 = sh.list[p], a1 = sh.list[p | j];
+                if ((a0 < a1) == ((p & k) == 0)) sh.list[p] = a1, sh.list[p | j] = a0;  // descending
+              }
+              __syncthreads();
+            }
+          // a thread has two neighbours of the sorted list
+          const uint32_t o0 = sh.list[2 * tid], o1 = sh.list[2 * tid + 1];
+          const u64 w0 = o0 ? weigh(value_of(o0)) : 0, w1 = o1 ? weigh(value_of(o1)) : 0;
+          u64 all;
+          const u64 b0 = f.above + block_scan(w0 + w1, sh.scan64, &all);
+          const uint32_t n0 = f.above_n + 2 * tid;
+          auto test = [&](uint32_t o, u64 b, uint32_t bn, u64 w) {
+            if (o && (number ? bn + 1 == want_n : b < want && b + w >= want)) sh.found.bin = static_cast<int>(bn - f.above_n);
+          };
+          test(o0, b0, n0, w0);
+          test(o1, b0 + w0, n0 + 1, w1);
+          __syncthreads();
+          if (tid == 0) {
+            // its equals ahead of it are candidates too
+            const int at = sh.found.bin;
+            int from = at;
+            while (from > 0 && sh.list[from - 1] == sh.list[at]) --from;
+            sh.border.order = sh.list[at];
+            sh.border.ties = at - from + 1;
+            sh.found.in_n = static_cast<uint32_t>(from);
+          }
+          __syncthreads();
+          // what lies above it
+          const uint32_t from = sh.found.in_n;
+          const u64 part = (2u * tid < from ? w0 : 0) + (2u * tid + 1 < from ? w1 : 0);
+          block_scan(part, sh.scan64, &all);
+          if (tid == 0) {
+            sh.above_border = f.above + all;
+            sh.above_border_n = f.above_n + from;
+            sh.list_n = 0;
+          }
+        }
+        cluster.sync();
+        border = home->border;
+        whole = home->above_border + static_cast<u64>(border.ties) * weigh(value_of(border.order));
+        cluster.sync();
+      } else {
+        // one order alone
+        border.order = range_hi;
+        const u64 w = weigh(value_of(border.order));
+        if (number) {
+          border.ties = static_cast<int>(want_n - f.above_n);
+        } else {
+          const u64 left = want - f.above, need = w ? (left + w - 1) / w : 1;  // tie j (from 0) is kept while what is ahead is less
+          border.ties = need < f.in_n ? static_cast<int>(need) : static_cast<int>(f.in_n);
+        }
+        whole = f.above + static_cast<u64>(border.ties) * w;
+      }
+    };
+    auto first_level = [&]() {
+      clear();
+      for (int i = tid; i < vecs; i += SA_THREADS) {
+        float v[V];
+        read(i, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (v[e] > -INFINITY) add(interval(v[e]), v[e], by_mass);
+      }
+      gather();
+      whole = 0;
+      for (int q = 0; q < ranks; ++q) whole += cluster.map_shared_rank(&sh, q)->total;
+    };
+    first_level();
+    if (by_count) settle(true, static_cast<uint32_t>(top_k), 0);
+    if (by_mass) {
+      const Border counted = border;
+      const u64 of = whole;
+      if (counted.order) first_level();  // (the intervals may have been divided since)
+      const double want = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(of));
+      border = {0, 0};
+      settle(false, 0, want >= 1.0 ? static_cast<u64>(want) : 1ull);
+      // never past the counted ones
+      if (border.order < counted.order || (border.order == counted.order && counted.order && border.ties > counted.ties)) border = counted;
     }
-    const unsigned long long w = weigh(value_of(prefix));
-    int many = static_cast<int>(count[prefix & 255]);
-    if (by_count) {
-      many = static_cast<int>(want_count - above_n);
-    } else {
-      // tie j (from 0) is kept while what is ahead of it is less than want_mass
-      const unsigned long long left = want_mass - above, need = w ? (left + w - 1) / w : 1;
-      if (need < static_cast<unsigned long long>(many)) many = static_cast<int>(need);
-      if (prefix == border && ties > 0 && ties < many) many = ties;
-    }
-    border = prefix;
-    ties = many;
-    __syncthreads();
-    return true;
-  };
-  if (top_k > 0 && top_k < n) rounds(true, top_k, 0);
-  if (top_p < 1.0f) {
-    // the mass of the candidates so far
-    unsigned long long part = 0;
-    for (int i = tid; i < n; i += SA_THREADS) {
-      const float v = logit<T>(x, i);
-      const uint32_t o = order_of(v);
-      if (o > border) part += weigh(v);
-    }
-    block_scan(part, s64, &whole);
-    if (border) whole += static_cast<unsigned long long>(ties) * weigh(value_of(border));
-    const double want = ceil(static_cast<double>(top_p) * static_cast<double>(whole));
-    rounds(false, 0, want >= 1.0 ? static_cast<unsigned long long>(want) : 1ull);
   }
 
-  // running sums in index order: a thread has a stretch of the row
-  const unsigned long long least = min_p > 0.0f ? static_cast<unsigned long long>(ceil(fmin(static_cast<double>(min_p), 1.0) * weigh.one)) : 0;
-  const int stretch = (n + SA_THREADS - 1) / SA_THREADS;
-  const int i0 = min(n, tid * stretch), i1 = min(n, i0 + stretch);
-  int my_ties = 0, all_ties;
-  if (border)
-    for (int i = i0; i < i1; ++i) my_ties += order_of(logit<T>(x, i)) == border;
-  const int ties_before = block_scan(my_ties, s32, &all_ties);
-  auto walk = [&](unsigned long long from, unsigned long long until, unsigned long long* w_at) {
-    int seen = ties_before;
-    for (int i = i0; i < i1; ++i) {
-      const float v = logit<T>(x, i);
-      const uint32_t o = order_of(v);
-      if (o == 0 || o < border) continue;
-      if (border && o == border && seen++ >= ties) continue;
-      const unsigned long long w = weigh(v);
-      if (w < least) continue;
-      from += w;
-      *w_at = w;
-      if (from > until) return i;
+  // ---- 3. running sums in index order --------------------------------------------------------------------------------------------------------
+  // logits surely below min_p are left out before they are weighed (2^-10 of slack for the fp32 product)
+  const double least_w = min_p > 0.0f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  const u64 least = static_cast<u64>(ceil(least_w * weigh.one));
+  const float sure = min_p > 0.0f ? static_cast<float>((log2(least_w) - 1e-3) / weigh.scale * 1.0001) : -INFINITY;  // of x - max
+  const int per_warp = (vecs + SA_WARPS - 1) / SA_WARPS, v0 = min(vecs, warp * per_warp), v1 = min(vecs, v0 + per_warp);
+  auto weight = [&](float v, bool* tie) -> u64 {
+    *tie = false;
+    if (!(v - top >= sure) || !(v > -INFINITY)) return 0;
+    const uint32_t o = order_of(v);
+    if (o < border.order) return 0;
+    if (o == border.order) {
+      *tie = true;
+      return 0;
     }
-    *w_at = from;
-    return -1;
+    const u64 w = weigh(v);
+    return w < least ? 0 : w;
   };
-  unsigned long long mine, total;
-  walk(0, ~0ull, &mine);
-  const unsigned long long before = block_scan(mine, s64, &total);
-  // u times the sum, rounded down; below the sum
-  double goal = floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(total));
-  unsigned long long until = static_cast<unsigned long long>(goal);
-  if (until >= total) until = total - 1;
-  if (before <= until && until < before + mine) {
-    unsigned long long w;
-    const int id = walk(before, until, &w);
-    a.ids[row] = id;
-    if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+  u64 mass = 0;
+  uint32_t ties = 0;
+  for (int i = v0 + lane; i < v1; i += 32) {
+    float v[V];
+    read(i, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      bool tie;
+      mass += weight(v[e], &tie);
+      ties += tie;
+    }
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  if (lane == 0) sh.warp_mass[warp] = mass, sh.warp_ties[warp] = ties;
+  cluster.sync();
+  u64 tie_w = border.order ? weigh(value_of(border.order)) : 0;
+  if (tie_w < least) tie_w = 0;
+  const uint32_t allowed = static_cast<uint32_t>(border.ties);
+  // sums ahead of this warp, and of all
+  u64 ahead = 0, total = 0;
+  uint32_t ahead_t = 0, total_t = 0;
+  for (int i = lane; i < ranks * SA_WARPS; i += 32) {
+    const SampleShared* s = cluster.map_shared_rank(&sh, i / SA_WARPS);
+    const u64 m = s->warp_mass[i % SA_WARPS];
+    const uint32_t tt = s->warp_ties[i % SA_WARPS];
+    total += m, total_t += tt;
+    if (i < rank * SA_WARPS + warp) ahead += m, ahead_t += tt;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+  total_t = __reduce_add_sync(0xffffffffu, total_t), ahead_t = __reduce_add_sync(0xffffffffu, ahead_t);
+  total += static_cast<u64>(min(total_t, allowed)) * tie_w;
+  ahead += static_cast<u64>(min(ahead_t, allowed)) * tie_w;
+  const u64 warp_all = mass + static_cast<u64>(min(ahead_t + ties, allowed) - min(ahead_t, allowed)) * tie_w;
+  // u times the sum, rounded down; below the sum
+  u64 until = static_cast<u64>(floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(total)));
+  if (until >= total) until = total - 1;
+  if (ahead <= until && until < ahead + warp_all) {  // (one warp of the cluster)
+    u64 run = ahead;
+    uint32_t seen = ahead_t;
+    for (int i0 = v0; i0 < v1; i0 += 32) {
+      float v[V];
+      u64 w[V], sum = 0;
+      uint32_t mine_t = 0;
+      bool tie[V];
+      const bool there = i0 + lane < v1;
+      if (there) read(i0 + lane, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        tie[e] = false;
+        w[e] = there ? weight(v[e], &tie[e]) : 0;
+        mine_t += tie[e];
+      }
+      uint32_t t_at = seen + warp_scan(mine_t, lane) - mine_t;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (tie[e] && t_at++ < allowed) w[e] = tie_w;
+        sum += w[e];
+      }
+      const u64 inc = warp_scan(sum, lane);
+      u64 at = run + inc - sum;
+      if (at <= until && until < run + inc) {
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          at += w[e];
+          if (!done && at > until) {
+            done = true;
+            a.ids[row] = first + (i0 + lane) * V + e;
+            if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w[e]) / static_cast<double>(total)));
+          }
+        }
+      }
+      run = __shfl_sync(0xffffffffu, run + inc, 31);
+      seen += __reduce_add_sync(0xffffffffu, mine_t);
+      if (run > until) break;
+    }
+  }
+  cluster.sync();
+}
+
+template <int T, bool KEPT>
+int launch_as(const SampleLaunch& s, int cluster, int slice, cudaStream_t st) {
+  const size_t smem = KEPT ? static_cast<size_t>(slice) * type_bytes(T) : 0;
+  static PerDeviceOnce once;
+  MB_TRY(once.run([]() -> int {
+    MB_CUDA(cudaFuncSetAttribute(sample_rows_kernel<T, KEPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SA_LARGE)));
+    return MIMIR_B200_OK;
+  }));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(s.rows * cluster));
+  cfg.blockDim = dim3(SA_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MB_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel<T, KEPT>, s, slice));
+  count_launch();
+  return MIMIR_B200_OK;
+}
+template <int T>
+int launch_t(const SampleLaunch& s, cudaStream_t st) {
+  constexpr int STEP = 32 * Vec<T>::N;  // a warp's vectors
+  // as few CTAs as hold the row two to an SM, more while SMs would be idle and each keeps a few thousand logits
+  const int fits = static_cast<int>(SA_SLICE) / type_bytes(T);
+  int cluster = 1;
+  while (cluster < 8 && (static_cast<long long>(cluster) * fits < s.n || (s.rows * cluster < 2LL * ctx().sm_count && s.n / cluster >= 4096))) cluster *= 2;
+  const long long each = (s.n + cluster - 1) / cluster;
+  const int slice = static_cast<int>((each + STEP - 1) / STEP * STEP);
+  if (s.rows * cluster > 0x7fffffffLL) return fail(MIMIR_B200_E_INVALID, "sample_rows: too many rows for one call");
+  return static_cast<size_t>(slice) * type_bytes(T) <= SA_LARGE ? launch_as<T, true>(s, cluster, slice, st) : launch_as<T, false>(s, cluster, slice, st);
 }
 
 }  // namespace
 
 int launch_sample_rows(const SampleLaunch& s, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>(s.rows);
-  if (s.type == MIMIR_B200_T_F32) sample_rows_kernel<MIMIR_B200_T_F32><<<grid, SA_THREADS, 0, st>>>(s);
-  else if (s.type == MIMIR_B200_T_F16) sample_rows_kernel<MIMIR_B200_T_F16><<<grid, SA_THREADS, 0, st>>>(s);
-  else sample_rows_kernel<MIMIR_B200_T_BF16><<<grid, SA_THREADS, 0, st>>>(s);
-  MB_CUDA(cudaGetLastError());
-  count_launch();
-  return MIMIR_B200_OK;
+  if (s.type == MIMIR_B200_T_F32) return launch_t<MIMIR_B200_T_F32>(s, st);
+  if (s.type == MIMIR_B200_T_F16) return launch_t<MIMIR_B200_T_F16>(s, st);
+  return launch_t<MIMIR_B200_T_BF16>(s, st);
 }
 
 }  // namespace mb
