@@ -6,12 +6,15 @@
 //
 // A row is read once: a cluster of CTAs keeps it in shared memory, a slice each, and meets through distributed shared memory.
 //   1. the largest logit
-//   2. with top_k or top_p: counts and masses of 1024 intervals of (max - x) / T, the interval in which the border lies, and in it the
-//      border itself: up to 1024 logits of it are sorted in one CTA, more are divided again by their bits
+//   2. with top_k or top_p: counts (and masses) of 1024 intervals of (max - x) / T, and the interval in which the border lies.  Where
+//      what can still be taken is at most 1024 logits, they are gathered, sorted and finished in one CTA.  Else the border itself is found:
+//      the interval's logits are sorted, or divided again by their bits while they are more than 1024
 //   3. masses of the warps' stretches of the row in index order; the stretch in which u falls is walked
 // Sums are compared with borders, so every w is an integer (w times a power of two that leaves room for n of them): sums of integers are
 // the same in every order and division of the work.  w comes from a table of 2^(k / 64) and four terms of the exponential series in
-// fp64, relative error under 2^-44: the fp64 lanes (64 a cycle and SM, eleven operations a logit) are what a large batch waits for.
+// fp64, relative error under 2^-44.  A large batch waits for the arithmetic: the weights (eleven fp64 operations each), and the two
+// to three additions in shared memory of each logit that an interval of its own is kept for; those whose mass cannot reach the border
+// are added up in registers (an fp32 sum of the weights says which).
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -25,7 +28,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 1024, SA_LIST = 1024;
-constexpr size_t SA_SLICE = size_t(70) << 10;   // bytes of a row in a CTA's shared memory: two CTAs to an SM
+constexpr size_t SA_SLICE = size_t(88) << 10;   // bytes of a row in a CTA's shared memory: two CTAs to an SM
 constexpr size_t SA_LARGE = size_t(180) << 10;  // the most: one
 
 // ascending in the value; 0: not a candidate (not a number, -infinity)
@@ -64,9 +67,9 @@ __device__ __forceinline__ float logit(const void* row, long long i) {
 
 using u64 = unsigned long long;
 
-struct Border {          // candidates: order > order, and the first `ties` of order == order
+struct Border {          // candidates: order > order, and the first `ties` (of `equals`) of order == order
   uint32_t order;
-  int ties;
+  uint32_t ties, equals;
 };
 struct Found {
   int bin;               // -1: the candidates do not reach the border
@@ -77,11 +80,7 @@ struct Found {
 struct SampleShared {
   double table[64];
   uint32_t count[SA_BINS], mass_lo[SA_BINS], mass_hi[SA_BINS];  // of this CTA's slice
-  uint32_t before_n[SA_BINS];                                   // of the row: counts and masses ahead of this CTA's share of the intervals
-  u64 before[SA_BINS];
-  uint32_t bin_n[SA_BINS];
-  u64 bin[SA_BINS];
-  uint32_t list[SA_LIST];
+  u64 list[SA_LIST];  // order in the high half; below it the index's complement where indices matter
   uint32_t list_n;
   u64 scan64[33];
   uint32_t scan32[33];
@@ -93,8 +92,8 @@ struct SampleShared {
   u64 total;
   Found found;
   Border border;
-  u64 above_border;                                             // mass of candidates above it
-  uint32_t above_border_n;
+  uint32_t least_n;                                             // candidates up to the last interval that min_p leaves
+  float rough;
   u64 warp_mass[SA_WARPS];
   uint32_t warp_ties[SA_WARPS];
 };
@@ -103,10 +102,9 @@ struct Weigh {
   double top, scale;  // log2(e) / T
   double one, magic;  // what a weight of 1 is as an integer, 2^52
   const double* table;
-  // x <= top; not infinite
+  // x <= top; 0 for what is not a candidate
   __device__ __forceinline__ u64 operator()(float x) const {
-    const double y = (static_cast<double>(x) - top) * scale;
-    if (!(y > -64.0)) return 0;
+    const double y = fmax((static_cast<double>(x) - top) * scale, -600.0);  // (what is not a number becomes 2^-600, zero)
     const double s = y + 105553116266496.0;  // 1.5 * 2^46: y rounded to 64ths in the low bits
     const int k = __double2loint(s);
     const double r = (y - (s - 105553116266496.0)) * 0.69314718055994530942;
@@ -269,28 +267,36 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   weigh.one = static_cast<double>(1ull << min(62 - room, 51));
   weigh.magic = 4503599627370496.0;
   weigh.table = sh.table;
+  // logits surely below min_p are left out before they are weighed (2^-10 of slack for the fp32 product)
+  const double least_w = min_p > 0.0f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  const u64 least = static_cast<u64>(ceil(least_w * weigh.one));
+  const float sure = min_p > 0.0f ? static_cast<float>((log2(least_w) - 1e-3) / weigh.scale * 1.0001) : -INFINITY;  // of x - max
 
   // ---- 2. the border ---------------------------------------------------------------------------------------------------------------------
   const bool by_count = top_k > 0 && top_k < n, by_mass = top_p < 1.0f;
-  Border border = {0, 0};
+  Border border = {0, 0, 0};
   if (by_count || by_mass) {
     const float width = static_cast<float>(32.0 * weigh.scale);  // of (max - x), in intervals
     const int share = SA_BINS / ranks;                           // intervals that this CTA adds up
-    auto interval = [&](float v) { return min(SA_BINS - 1, __float2int_rz((top - v) * width)); };
-    auto add = [&](int bin, float v, bool weighed) {
-      atomicAdd(&sh.count[bin], 1u);
-      if (!weighed) return;
-      const u64 w = weigh(v);
+    int cut = SA_BINS - 1;                                       // from this one on they are one
+    auto interval = [&](float v) {
+      const int i = __float2int_rz((top - v) * width);
+      return i < cut ? i : SA_BINS - 1;
+    };
+    auto add_mass = [&](int bin, u64 w) {
       const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&sh.mass_lo[bin], lo);
       const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
       if (hi) atomicAdd(&sh.mass_hi[bin], hi);
     };
     auto clear = [&]() {
+      __syncthreads();
       for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.count[i] = sh.mass_lo[i] = sh.mass_hi[i] = 0;
+      if (tid == 0) sh.found.bin = -1;
       __syncthreads();
     };
-    // counts and masses of the row's intervals in this CTA's share, and what lies ahead of each
-    auto gather = [&]() {
+    // the interval in which the candidates reach want_n in number or a part of the mass, counted from (above_n, above)
+    u64 whole = 0, want = 0;
+    auto find = [&](bool number, uint32_t want_n, uint32_t above_n, u64 above, int last) {
       cluster.sync();
       u64 m[2] = {0, 0};
       uint32_t c[2] = {0, 0};
@@ -301,55 +307,92 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         for (int q = 0; q < ranks; ++q) {
           const SampleShared* s = cluster.map_shared_rank(&sh, q);
           c[h] += s->count[rank * share + i];
-          m[h] += (static_cast<u64>(s->mass_hi[rank * share + i]) << 32) + s->mass_lo[rank * share + i];
+          if (!number) m[h] += (static_cast<u64>(s->mass_hi[rank * share + i]) << 32) + s->mass_lo[rank * share + i];
         }
       }
-      u64 all;
+      u64 all = 0, mb = 0;
       uint32_t all_n;
-      u64 mb = block_scan(m[0] + m[1], sh.scan64, &all);
+      if (!number) mb = block_scan(m[0] + m[1], sh.scan64, &all);
       uint32_t cb = block_scan(c[0] + c[1], sh.scan32, &all_n);
       if (tid == 0) sh.total = all, sh.total_n = all_n;
       cluster.sync();
-      for (int q = 0; q < rank; ++q) {
+      u64 sum = 0;
+      for (int q = 0; q < ranks; ++q) {
         const SampleShared* s = cluster.map_shared_rank(&sh, q);
-        mb += s->total, cb += s->total_n;
+        const u64 mq = s->total;
+        if (q < rank) mb += mq, cb += s->total_n;
+        sum += mq;
+      }
+      if (!number && want == 0) {  // (the first of the mass's levels)
+        const Border& k = border;  // equals of the counted border that are not candidates
+        whole = sum - (k.order ? static_cast<u64>(k.equals - k.ties) * weigh(value_of(k.order)) : 0);
+        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(whole));
+        want = part >= 1.0 ? static_cast<u64>(part) : 1ull;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = 2 * tid + h;
-        if (i < share) sh.before[i] = mb, sh.before_n[i] = cb, sh.bin[i] = m[h], sh.bin_n[i] = c[h];
-        mb += m[h], cb += c[h];
-      }
-      __syncthreads();
-    };
-    // the interval in which the candidates reach want_n in number or want in mass, counted from (above_n, above)
-    auto find = [&](bool number, uint32_t want_n, u64 want, uint32_t above_n, u64 above) {
-      __syncthreads();
-      if (tid == 0) sh.found.bin = -1;
-      cluster.sync();
-      for (int i = tid; i < share; i += SA_THREADS) {
-        const u64 b = above + sh.before[i], m = sh.bin[i];
-        const uint32_t bn = above_n + sh.before_n[i], c = sh.bin_n[i];
-        if (c > 0 && (number ? bn < want_n && bn + c >= want_n : b < want && b + m >= want)) {
-          Found f;
-          f.bin = rank * share + i;
-          f.above = b, f.above_n = bn, f.in = m, f.in_n = c;
-          for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->found = f;
+        if (i < share && c[h] > 0) {
+          const u64 ahead = above + mb;
+          const uint32_t ahead_n = above_n + cb;
+          if (number ? ahead_n < want_n && ahead_n + c[h] >= want_n : ahead < want && ahead + m[h] >= want) {
+            Found f;
+            f.bin = rank * share + i;
+            f.above = ahead, f.above_n = ahead_n, f.in = m[h], f.in_n = c[h];
+            for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->found = f;
+          }
         }
+        mb += m[h], cb += c[h];
+        if (i < share && rank * share + i == last)
+          for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->least_n = above_n + cb;
       }
       cluster.sync();
       return sh.found;
     };
-    // mass of candidates up to a border
-    u64 whole = 0;
-    auto settle = [&](bool number, uint32_t want_n, u64 want) {
-      Found f = find(number, want_n, want, 0, 0);
-      if (f.bin < 0) return;  // all of them
-      // logits of the interval: the level's own division of them
-      uint32_t low = 0;
-      int shift = -1;  // -1: intervals of values; else (order - low) >> shift
-      uint32_t range_lo = 1, range_hi = 0xffffffffu;
+    auto sort = [&](int size) {  // sh.list, descending
+      for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+          for (int i = tid; i < size / 2; i += SA_THREADS) {
+            const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1));
+            const u64 a0 = sh.list[p], a1 = sh.list[p | j];
+            if ((a0 < a1) == ((p & k) == 0)) sh.list[p] = a1, sh.list[p | j] = a0;
+          }
+          __syncthreads();
+        }
+    };
+    // what `pick` says yes to into the first CTA's list; true there, whose list is filled up with zeros to a power of two
+    int size = 32;
+    auto collect = [&](auto&& pick) {
+      SampleShared* home = cluster.map_shared_rank(&sh, 0);
+      for (int i = tid; i < vecs; i += SA_THREADS) {
+        float v[V];
+        read(i, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const uint32_t o = order_of(v[e]);
+          if (o && pick(o, v[e])) {
+            const uint32_t at = atomicAdd(&home->list_n, 1u);
+            if (at < SA_LIST) home->list[at] = (static_cast<u64>(o) << 32) | ~static_cast<uint32_t>(first + i * V + e);
+          }
+        }
+      }
+      cluster.sync();
+      if (rank != 0) return false;
+      const int have = static_cast<int>(min(sh.list_n, static_cast<uint32_t>(SA_LIST)));
+      while (size < have) size *= 2;
+      for (int i = tid; i < SA_LIST; i += SA_THREADS)
+        if (i >= have) sh.list[i] = 0;
+      __syncthreads();
+      if (tid == 0) sh.list_n = 0;
+      sort(size);
+      return true;
+    };
+
+    // The border in an interval found: level by level, then sorted or a single order.
+    auto settle = [&](bool number, uint32_t want_n, Found f) {
       const int value_bin = f.bin;
+      uint32_t range_lo = max(1u, border.order), range_hi = 0xffffffffu;  // (what top_k left out is no member)
+      int shift = -1;
       auto member = [&](uint32_t o, float v) { return o >= range_lo && o <= range_hi && interval(v) == value_bin; };
       while (f.in_n > SA_LIST && shift != 0) {
         // their range of orders, divided evenly, the largest first
@@ -373,28 +416,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         for (int q = 0; q < ranks; ++q) lo = min(lo, *cluster.map_shared_rank(&sh.low, q)), hi = max(hi, *cluster.map_shared_rank(&sh.high, q));
         shift = 0;
         while (((hi - lo) >> shift) >= SA_BINS) ++shift;
-        low = lo;
-        for (int i = tid; i < vecs; i += SA_THREADS) {
-          float v[V];
-          read(i, v);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const uint32_t o = order_of(v[e]);
-            if (o && member(o, v[e])) add(static_cast<int>((hi - o) >> shift), v[e], by_mass);
-          }
-        }
-        gather();
-        const uint32_t above_n = f.above_n;
-        const u64 above = f.above;
-        f = find(number, want_n, want, above_n, above);
-        if (f.bin < 0) return;  // (never: the sums are exact)
-        range_hi = hi - (static_cast<uint32_t>(f.bin) << shift);
-        const uint32_t span = (1u << shift) - 1;
-        range_lo = range_hi - low < span ? low : range_hi - span;
-      }
-      if (f.in_n <= SA_LIST && shift != 0) {
-        // sorted in the first CTA
-        SampleShared* home = cluster.map_shared_rank(&sh, 0);
         for (int i = tid; i < vecs; i += SA_THREADS) {
           float v[V];
           read(i, v);
@@ -402,116 +423,194 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
           for (int e = 0; e < V; ++e) {
             const uint32_t o = order_of(v[e]);
             if (o && member(o, v[e])) {
-              const uint32_t at = atomicAdd(&home->list_n, 1u);
-              if (at < SA_LIST) home->list[at] = o;
+              atomicAdd(&sh.count[(hi - o) >> shift], 1u);
+              if (!number) add_mass(static_cast<int>((hi - o) >> shift), weigh(v[e]));
             }
           }
         }
-        cluster.sync();
-        if (rank == 0) {
-          const int have = static_cast<int>(min(sh.list_n, static_cast<uint32_t>(SA_LIST)));
-          for (int i = tid; i < SA_LIST; i += SA_THREADS)
-            if (i >= have) sh.list[i] = 0;
-          int size = 32;
-          while (size < have) size *= 2;
-          __syncthreads();
-          for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j; j >>= 1) {
-              for (int i = tid; i < size / 2; i += SA_THREADS) {
-                const int p = ((i & ~(j - 1)) << 1) | (i & (j - 1));
-                const uint32_t a0 = sh.list[p], a1 = sh.list[p | j];
-                if ((a0 < a1) == ((p & k) == 0)) sh.list[p] = a1, sh.list[p | j] = a0;  // descending
-              }
-              __syncthreads();
-            }
+        f = find(number, want_n, f.above_n, f.above, -1);
+        if (f.bin < 0) return;  // (never: the sums are exact)
+        range_hi = hi - (static_cast<uint32_t>(f.bin) << shift);
+        const uint32_t span = (1u << shift) - 1;
+        range_lo = range_hi - lo < span ? lo : range_hi - span;
+      }
+      if (f.in_n <= SA_LIST && shift != 0) {
+        if (collect(member)) {
           // a thread has two neighbours of the sorted list
-          const uint32_t o0 = sh.list[2 * tid], o1 = sh.list[2 * tid + 1];
+          const uint32_t o0 = static_cast<uint32_t>(sh.list[2 * tid] >> 32), o1 = static_cast<uint32_t>(sh.list[2 * tid + 1] >> 32);
           const u64 w0 = o0 ? weigh(value_of(o0)) : 0, w1 = o1 ? weigh(value_of(o1)) : 0;
           u64 all;
           const u64 b0 = f.above + block_scan(w0 + w1, sh.scan64, &all);
           const uint32_t n0 = f.above_n + 2 * tid;
-          auto test = [&](uint32_t o, u64 b, uint32_t bn, u64 w) {
-            if (o && (number ? bn + 1 == want_n : b < want && b + w >= want)) sh.found.bin = static_cast<int>(bn - f.above_n);
-          };
-          test(o0, b0, n0, w0);
-          test(o1, b0 + w0, n0 + 1, w1);
-          __syncthreads();
-          if (tid == 0) {
+          auto test = [&](int at, u64 b, uint32_t bn, u64 w) {
+            const uint32_t o = static_cast<uint32_t>(sh.list[at] >> 32);
+            if (!o || !(number ? bn + 1 == want_n : b < want && b + w >= want)) return;
             // its equals ahead of it are candidates too
-            const int at = sh.found.bin;
-            int from = at;
-            while (from > 0 && sh.list[from - 1] == sh.list[at]) --from;
-            sh.border.order = sh.list[at];
-            sh.border.ties = at - from + 1;
-            sh.found.in_n = static_cast<uint32_t>(from);
-          }
-          __syncthreads();
-          // what lies above it
-          const uint32_t from = sh.found.in_n;
-          const u64 part = (2u * tid < from ? w0 : 0) + (2u * tid + 1 < from ? w1 : 0);
-          block_scan(part, sh.scan64, &all);
-          if (tid == 0) {
-            sh.above_border = f.above + all;
-            sh.above_border_n = f.above_n + from;
-            sh.list_n = 0;
-          }
+            int from = at, to = at;
+            while (from > 0 && static_cast<uint32_t>(sh.list[from - 1] >> 32) == o) --from;
+            while (to + 1 < SA_LIST && static_cast<uint32_t>(sh.list[to + 1] >> 32) == o) ++to;
+            sh.border.order = o;
+            sh.border.ties = static_cast<uint32_t>(at - from + 1);
+            sh.border.equals = static_cast<uint32_t>(to - from + 1);
+          };
+          test(2 * tid, b0, n0, w0);
+          test(2 * tid + 1, b0 + w0, n0 + 1, w1);
         }
         cluster.sync();
-        border = home->border;
-        whole = home->above_border + static_cast<u64>(border.ties) * weigh(value_of(border.order));
-        cluster.sync();
+        border = *cluster.map_shared_rank(&sh.border, 0);
       } else {
         // one order alone
         border.order = range_hi;
+        border.equals = f.in_n;
         const u64 w = weigh(value_of(border.order));
         if (number) {
-          border.ties = static_cast<int>(want_n - f.above_n);
+          border.ties = want_n - f.above_n;
         } else {
           const u64 left = want - f.above, need = w ? (left + w - 1) / w : 1;  // tie j (from 0) is kept while what is ahead is less
-          border.ties = need < f.in_n ? static_cast<int>(need) : static_cast<int>(f.in_n);
+          border.ties = need < f.in_n ? static_cast<uint32_t>(need) : f.in_n;
         }
-        whole = f.above + static_cast<u64>(border.ties) * w;
       }
     };
-    auto first_level = [&]() {
+    // The few that can still be taken, in the first CTA: top_k, top_p and min_p in the sorted list, then u in index order.
+    auto finish = [&](int last) {
+      if (!collect([&](uint32_t, float v) { return interval(v) <= last; })) return;
+      const u64 e0 = sh.list[2 * tid], e1 = sh.list[2 * tid + 1];
+      const uint32_t o0 = static_cast<uint32_t>(e0 >> 32), o1 = static_cast<uint32_t>(e1 >> 32);
+      const uint32_t most = by_count ? static_cast<uint32_t>(top_k) : 0xffffffffu;
+      const u64 w0 = o0 && 2u * tid < most ? weigh(value_of(o0)) : 0, w1 = o1 && 2u * tid + 1 < most ? weigh(value_of(o1)) : 0;
+      u64 all, limit = ~0ull;
+      const u64 b0 = block_scan(w0 + w1, sh.scan64, &all);
+      if (by_mass) {
+        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(by_count ? all : whole));
+        limit = part >= 1.0 ? static_cast<u64>(part) : 1ull;
+      }
+      const bool k0 = o0 && 2u * tid < most && b0 < limit && w0 >= least, k1 = o1 && 2u * tid + 1 < most && b0 + w0 < limit && w1 >= least;
+      // index order: the kept ones by their index's complement, descending
+      sh.list[2 * tid] = k0 ? (e0 << 32) | o0 : 0;
+      sh.list[2 * tid + 1] = k1 ? (e1 << 32) | o1 : 0;
+      __syncthreads();
+      sort(size);
+      const u64 i0 = sh.list[2 * tid], i1 = sh.list[2 * tid + 1];
+      const u64 x0 = i0 ? weigh(value_of(static_cast<uint32_t>(i0))) : 0, x1 = i1 ? weigh(value_of(static_cast<uint32_t>(i1))) : 0;
+      const u64 at = block_scan(x0 + x1, sh.scan64, &all);
+      u64 until = static_cast<u64>(floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(all)));
+      if (until >= all) until = all - 1;
+      auto take = [&](u64 item, u64 from, u64 w) {
+        if (!(from <= until && until < from + w)) return;
+        a.ids[row] = static_cast<int>(~static_cast<uint32_t>(item >> 32));
+        if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all)));
+      };
+      take(i0, at, x0);
+      take(i1, at + x0, x1);
+    };
+
+    const int last_min = min_p > 0.0f ? interval(top + sure) : SA_BINS - 1;  // intervals behind it are below min_p
+    bool done = false;
+    if (by_count) {
       clear();
       for (int i = tid; i < vecs; i += SA_THREADS) {
         float v[V];
         read(i, v);
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (v[e] > -INFINITY) add(interval(v[e]), v[e], by_mass);
+          if (v[e] > -INFINITY) atomicAdd(&sh.count[interval(v[e])], 1u);
       }
-      gather();
-      whole = 0;
-      for (int q = 0; q < ranks; ++q) whole += cluster.map_shared_rank(&sh, q)->total;
-    };
-    first_level();
-    if (by_count) settle(true, static_cast<uint32_t>(top_k), 0);
-    if (by_mass) {
+      const Found f = find(true, static_cast<uint32_t>(top_k), 0, 0, last_min);
+      if (f.bin >= 0) {
+        if (f.above_n + f.in_n <= SA_LIST) {
+          finish(f.bin);
+          done = true;
+        } else {
+          settle(true, static_cast<uint32_t>(top_k), f);
+        }
+      }
+    }
+    if (by_mass && !done) {
       const Border counted = border;
-      const u64 of = whole;
-      if (counted.order) first_level();  // (the intervals may have been divided since)
-      const double want = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(of));
-      border = {0, 0};
-      settle(false, 0, want >= 1.0 ? static_cast<u64>(want) : 1ull);
-      // never past the counted ones
-      if (border.order < counted.order || (border.order == counted.order && counted.order && border.ties > counted.ties)) border = counted;
+      if (!counted.order && slice >= 4096) {
+        // a rough sum first: intervals whose whole mass cannot reach what top_p leaves out need not be kept apart
+        const float s = static_cast<float>(weigh.scale);
+        float sum = 0.0f;
+        for (int i = tid; i < vecs; i += SA_THREADS) {
+          float v[V];
+          read(i, v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            float w;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf((v[e] - top) * s, -200.0f)));
+            sum += w;
+          }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        __syncthreads();
+        if (lane == 0) reinterpret_cast<float*>(sh.scan32)[warp] = sum;
+        __syncthreads();
+        if (tid == 0) {
+          for (int w = 1; w < SA_WARPS; ++w) sum += reinterpret_cast<float*>(sh.scan32)[w];
+          sh.rough = sum;
+        }
+        cluster.sync();
+        sum = 0.0f;
+        for (int q = 0; q < ranks; ++q) sum += *cluster.map_shared_rank(&sh.rough, q);
+        const float bits = log2f(static_cast<float>(n) / ((1.0f - top_p) * sum)) + 1.0f;  // n weights of 2^-bits are half of what is left out
+        cut = bits < 31.0f ? max(1, static_cast<int>(bits * 32.0f) + 1) : SA_BINS - 1;
+      }
+      clear();
+      const float from = counted.order ? value_of(counted.order) : -INFINITY;
+      u64 rest = 0;
+      uint32_t rest_n = 0;
+      for (int i = tid; i < vecs; i += SA_THREADS) {
+        float v[V];
+        read(i, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (counted.order && !(v[e] >= from)) continue;
+          const u64 w = weigh(v[e]);
+          const int bin = interval(v[e]);
+          if (bin < SA_BINS - 1 && v[e] > -INFINITY) {
+            atomicAdd(&sh.count[bin], 1u);
+            add_mass(bin, w);
+          } else {
+            rest += w;
+            rest_n += v[e] > -INFINITY;
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+      rest_n = __reduce_add_sync(0xffffffffu, rest_n);
+      if (lane == 0 && rest_n) {
+        atomicAdd(&sh.count[SA_BINS - 1], rest_n);
+        add_mass(SA_BINS - 1, rest);
+      }
+      const int last = min_p > 0.0f ? interval(top + sure) : SA_BINS - 1;
+      const Found f = find(false, 0, 0, 0, last);
+      if (f.bin >= 0) {
+        const bool least_first = last < f.bin;  // min_p leaves nothing near top_p's border
+        if (!counted.order && (least_first ? sh.least_n : f.above_n + f.in_n) <= SA_LIST) {
+          finish(least_first ? last : f.bin);
+          done = true;
+        } else if (!least_first || counted.order) {
+          settle(false, 0, f);
+          // never past the counted ones
+          if (border.order < counted.order || (border.order == counted.order && border.ties > counted.ties && counted.order)) border = counted;
+        }
+      }
+    }
+    if (done) {
+      cluster.sync();  // (no CTA leaves while others read its shared memory)
+      return;
     }
   }
 
   // ---- 3. running sums in index order --------------------------------------------------------------------------------------------------------
-  // logits surely below min_p are left out before they are weighed (2^-10 of slack for the fp32 product)
-  const double least_w = min_p > 0.0f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
-  const u64 least = static_cast<u64>(ceil(least_w * weigh.one));
-  const float sure = min_p > 0.0f ? static_cast<float>((log2(least_w) - 1e-3) / weigh.scale * 1.0001) : -INFINITY;  // of x - max
+  const float border_x = border.order ? value_of(border.order) : -INFINITY;
   const int per_warp = (vecs + SA_WARPS - 1) / SA_WARPS, v0 = min(vecs, warp * per_warp), v1 = min(vecs, v0 + per_warp);
   auto weight = [&](float v, bool* tie) -> u64 {
     *tie = false;
-    if (!(v - top >= sure) || !(v > -INFINITY)) return 0;
-    const uint32_t o = order_of(v);
-    if (o < border.order) return 0;
-    if (o == border.order) {
+    if (!(v - top >= sure) || !(v >= border_x)) return 0;
+    if (v == border_x && border.order) {
       *tie = true;
       return 0;
     }
@@ -537,7 +636,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   cluster.sync();
   u64 tie_w = border.order ? weigh(value_of(border.order)) : 0;
   if (tie_w < least) tie_w = 0;
-  const uint32_t allowed = static_cast<uint32_t>(border.ties);
+  const uint32_t allowed = border.ties;
   // sums ahead of this warp, and of all
   u64 ahead = 0, total = 0;
   uint32_t ahead_t = 0, total_t = 0;
