@@ -5,16 +5,18 @@
 //   sum of the candidates' w exceeds u times their whole sum.
 //
 // A row is read once: a cluster of CTAs keeps it in shared memory, a slice each, and meets through distributed shared memory.
-//   1. the largest logit
-//   2. with top_k or top_p: counts (and masses) of 1024 intervals of (max - x) / T, and the interval in which the border lies.  Where
-//      what can still be taken is at most 1024 logits, they are gathered, sorted and finished in one CTA.  Else the border itself is found:
-//      the interval's logits are sorted, or divided again by their bits while they are more than 1024
+//   1. the largest logit, and in fp32 about how much all weights are
+//   2. top_k: counts of 1024 intervals of (max - x) / T and the interval in which the border lies.  Up to 1024 logits down to that
+//      are gathered, sorted and finished in one CTA; else the border itself is found among the interval's
+//      top_p: rough masses of the intervals (one 32-bit addition in shared memory a logit) say between which two the border lies, a
+//      part in 2^10 of the mass to either side.  Where min_p ends before them, top_p takes nothing away.  Else every weight is taken
+//      exactly, what lies between the two is listed, and the border found among it.
+//      A border among logits: up to 1024 are sorted in one CTA; more are divided by their bits until they are fewer or all the same
 //   3. masses of the warps' stretches of the row in index order; the stretch in which u falls is walked
 // Sums are compared with borders, so every w is an integer (w times a power of two that leaves room for n of them): sums of integers are
 // the same in every order and division of the work.  w comes from a table of 2^(k / 64) and four terms of the exponential series in
-// fp64, relative error under 2^-44.  A large batch waits for the arithmetic: the weights (eleven fp64 operations each), and the two
-// to three additions in shared memory of each logit that an interval of its own is kept for; those whose mass cannot reach the border
-// are added up in registers (an fp32 sum of the weights says which).
+// fp64, relative error under 2^-44.  A large batch waits for instructions: about 8 a logit to load and sum it roughly, 12 for the
+// intervals, 36 for an exact weight.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -67,6 +69,12 @@ __device__ __forceinline__ float logit(const void* row, long long i) {
 
 using u64 = unsigned long long;
 
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct Border {          // candidates: order > order, and the first `ties` (of `equals`) of order == order
   uint32_t order;
   uint32_t ties, equals;
@@ -87,34 +95,37 @@ struct SampleShared {
   // read by the cluster's other CTAs
   float top;
   int first;
-  uint32_t low, high;
   uint32_t total_n;
   u64 total;
   Found found;
   Border border;
-  uint32_t least_n;                                             // candidates up to the last interval that min_p leaves
+  int window[2];                                                // intervals between which top_p's border lies
+  u64 above, inside;                                            // masses ahead of them and in them
+  uint32_t inside_n;
   float rough;
   u64 warp_mass[SA_WARPS];
   uint32_t warp_ties[SA_WARPS];
+  float warp_top[SA_WARPS], warp_sum[SA_WARPS];
 };
 
+// w of a candidate (what is none gets some w of its own: callers leave it out)
 struct Weigh {
   double top, scale;  // log2(e) / T
-  double one, magic;  // what a weight of 1 is as an integer, 2^52
+  double one;         // what a weight of 1 is as an integer
+  float least_x;      // w is zero there and below
   const double* table;
-  // x <= top; 0 for what is not a candidate
   __device__ __forceinline__ u64 operator()(float x) const {
-    const double y = fmax((static_cast<double>(x) - top) * scale, -600.0);  // (what is not a number becomes 2^-600, zero)
+    const double y = (static_cast<double>(fmaxf(x, least_x)) - top) * scale;
     const double s = y + 105553116266496.0;  // 1.5 * 2^46: y rounded to 64ths in the low bits
     const int k = __double2loint(s);
-    const double r = (y - (s - 105553116266496.0)) * 0.69314718055994530942;
-    double p = fma(r, 1.0 / 24, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
+    const double r = y - (s - 105553116266496.0);
+    double p = fma(r, 9.618129107628477e-3, 5.5504108664821580e-2);  // ln(2)^i / i!
+    p = fma(p, r, 2.4022650695910071e-1);
+    p = fma(p, r, 6.9314718055994531e-1);
     p = fma(p, r, 1.0);
     const double t = table[k & 63];
     const double w = __hiloint2double(__double2hiint(t) + ((k >> 6) << 20), __double2loint(t)) * p;
-    return static_cast<u64>(__double_as_longlong(fma(w, one, magic)) & 0xfffffffffffffll);
+    return static_cast<u64>(__double_as_longlong(fma(w, one, 4503599627370496.0)) & 0xfffffffffffffll);  // (2^52: the integer in the low bits)
   }
 };
 
@@ -178,8 +189,25 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     else from_global(i, f);
   };
 
-  // ---- 1. the largest -------------------------------------------------------------------------------------------------------------------
-  float top = -INFINITY;
+  // ---- 1. the largest, and a rough sum of the weights (a thread's by its own largest, which it raises as it goes) ------------------------
+  const float s2 = t > 0.0f ? 1.4426950408889634f / t : 0.0f;
+  float top = -INFINITY, rough = 0.0f;
+  const bool by_count = top_k > 0 && top_k < n, by_mass = top_p < 1.0f, sum_now = by_mass && !by_count;
+  auto take_in = [&](const float (&f)[V]) {
+    float m = f[0];
+#pragma unroll
+    for (int e = 1; e < V; ++e) m = fmaxf(m, f[e]);
+    if (!sum_now) {
+      top = fmaxf(top, m);
+      return;
+    }
+    if (m > top) {
+      rough *= ex2f(fmaxf((top - m) * s2, -200.0f));
+      top = m;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) rough += ex2f(fmaxf((f[e] - top) * s2, -200.0f));
+  };
   if constexpr (KEPT) {
     const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     constexpr int U = 4;
@@ -209,31 +237,39 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         reinterpret_cast<uint4*>(dyn)[i] = v[j];
         float f[V];
         Vec<T>::unpack(v[j], f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) top = fmaxf(top, f[e]);
+        take_in(f);
       }
     }
   } else {
     for (int i = tid; i < vecs; i += SA_THREADS) {
       float f[V];
       read(i, f);
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = fmaxf(top, f[e]);
+      take_in(f);
     }
   }
+  // sums of parts that have their own largest
+  auto join = [&](float& m, float& s, float om, float os) {
+    const float mm = fmaxf(m, om);
+    if (mm > -INFINITY) s = s * ex2f(fmaxf((m - mm) * s2, -200.0f)) + os * ex2f(fmaxf((om - mm) * s2, -200.0f));
+    m = mm;
+  };
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 16; o; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, rough, o);
+    join(top, rough, om, os);
+  }
   if (tid < 64) sh.table[tid] = exp2(tid * (1.0 / 64));
   if (tid == 0) sh.list_n = 0;
-  if (lane == 0) reinterpret_cast<float*>(sh.scan32)[warp] = top;
+  if (lane == 0) sh.warp_top[warp] = top, sh.warp_sum[warp] = rough;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < SA_WARPS; ++w) top = fmaxf(top, reinterpret_cast<float*>(sh.scan32)[w]);
+    for (int w = 1; w < SA_WARPS; ++w) join(top, rough, sh.warp_top[w], sh.warp_sum[w]);
     sh.top = top;
+    sh.rough = rough;
   }
   cluster.sync();
-  top = -INFINITY;
-  for (int c = 0; c < ranks; ++c) top = fmaxf(top, *cluster.map_shared_rank(&sh.top, c));
+  top = -INFINITY, rough = 0.0f;
+  for (int c = 0; c < ranks; ++c) join(top, rough, *cluster.map_shared_rank(&sh.top, c), *cluster.map_shared_rank(&sh.rough, c));
 
   if (top == -INFINITY || top == INFINITY || !(t > 0.0f)) {  // the largest's first index, or none
     int at = 0x7fffffff;
@@ -265,7 +301,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   weigh.top = top;
   weigh.scale = 1.4426950408889634074 / static_cast<double>(t);
   weigh.one = static_cast<double>(1ull << min(62 - room, 51));
-  weigh.magic = 4503599627370496.0;
+  {
+    // 600 powers of two down; where that is no smaller float, every other logit is further down than that
+    float low = static_cast<float>(fmax(static_cast<double>(top) - 600.0 / weigh.scale, -3.4028234e38));
+    if ((static_cast<double>(top) - low) * weigh.scale > 900.0 || low >= top) {
+      low = fmaxf(value_of(order_of(top) - 1), -3.4028235e38f);
+      weigh.scale = fmin(weigh.scale, 600.0 / (static_cast<double>(top) - low));
+    }
+    weigh.least_x = low;
+  }
   weigh.table = sh.table;
   // logits surely below min_p are left out before they are weighed (2^-10 of slack for the fp32 product)
   const double least_w = min_p > 0.0f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
@@ -273,16 +317,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   const float sure = min_p > 0.0f ? static_cast<float>((log2(least_w) - 1e-3) / weigh.scale * 1.0001) : -INFINITY;  // of x - max
 
   // ---- 2. the border ---------------------------------------------------------------------------------------------------------------------
-  const bool by_count = top_k > 0 && top_k < n, by_mass = top_p < 1.0f;
   Border border = {0, 0, 0};
   if (by_count || by_mass) {
     const float width = static_cast<float>(32.0 * weigh.scale);  // of (max - x), in intervals
     const int share = SA_BINS / ranks;                           // intervals that this CTA adds up
-    int cut = SA_BINS - 1;                                       // from this one on they are one
-    auto interval = [&](float v) {
-      const int i = __float2int_rz((top - v) * width);
-      return i < cut ? i : SA_BINS - 1;
-    };
+    // rounded in the low bits of 2^23 + it; what is not a number is in the last one
+    auto interval = [&](float v) { return static_cast<int>(__float_as_uint(fminf((top - v) * width, SA_BINS - 1.0f) + 8388608.0f) & (2 * SA_BINS - 1)); };
     auto add_mass = [&](int bin, u64 w) {
       const uint32_t lo = static_cast<uint32_t>(w), old = atomicAdd(&sh.mass_lo[bin], lo);
       const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
@@ -291,12 +331,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     auto clear = [&]() {
       __syncthreads();
       for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.count[i] = sh.mass_lo[i] = sh.mass_hi[i] = 0;
-      if (tid == 0) sh.found.bin = -1;
+      if (tid == 0) sh.found.bin = -1, sh.window[0] = sh.window[1] = SA_BINS - 1;
       __syncthreads();
     };
-    // the interval in which the candidates reach want_n in number or a part of the mass, counted from (above_n, above)
-    u64 whole = 0, want = 0;
-    auto find = [&](bool number, uint32_t want_n, uint32_t above_n, u64 above, int last) {
+    // the interval in which the candidates reach want_n in number, or `want` in mass, counted from (above_n, above)
+    u64 want = 0;
+    auto find = [&](bool number, uint32_t want_n, uint32_t above_n, u64 above) {
       cluster.sync();
       u64 m[2] = {0, 0};
       uint32_t c[2] = {0, 0};
@@ -316,18 +356,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       uint32_t cb = block_scan(c[0] + c[1], sh.scan32, &all_n);
       if (tid == 0) sh.total = all, sh.total_n = all_n;
       cluster.sync();
-      u64 sum = 0;
-      for (int q = 0; q < ranks; ++q) {
+      for (int q = 0; q < rank; ++q) {
         const SampleShared* s = cluster.map_shared_rank(&sh, q);
-        const u64 mq = s->total;
-        if (q < rank) mb += mq, cb += s->total_n;
-        sum += mq;
-      }
-      if (!number && want == 0) {  // (the first of the mass's levels)
-        const Border& k = border;  // equals of the counted border that are not candidates
-        whole = sum - (k.order ? static_cast<u64>(k.equals - k.ties) * weigh(value_of(k.order)) : 0);
-        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(whole));
-        want = part >= 1.0 ? static_cast<u64>(part) : 1ull;
+        mb += s->total, cb += s->total_n;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -343,8 +374,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
           }
         }
         mb += m[h], cb += c[h];
-        if (i < share && rank * share + i == last)
-          for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->least_n = above_n + cb;
       }
       cluster.sync();
       return sh.found;
@@ -369,10 +398,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         read(i, v);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const uint32_t o = order_of(v[e]);
-          if (o && pick(o, v[e])) {
+          if (pick(v[e])) {
             const uint32_t at = atomicAdd(&home->list_n, 1u);
-            if (at < SA_LIST) home->list[at] = (static_cast<u64>(o) << 32) | ~static_cast<uint32_t>(first + i * V + e);
+            if (at < SA_LIST) home->list[at] = (static_cast<u64>(order_of(v[e])) << 32) | ~static_cast<uint32_t>(first + i * V + e);
           }
         }
       }
@@ -388,51 +416,35 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       return true;
     };
 
-    // The border in an interval found: level by level, then sorted or a single order.
-    auto settle = [&](bool number, uint32_t want_n, Found f) {
+    // The border among the logits of orders range_lo .. range_hi, and of the interval f.bin where `number` says so (f: what lies ahead of
+    // them and in them): level by level, then sorted or a single order.
+    auto settle = [&](bool number, uint32_t want_n, Found f, uint32_t range_lo, uint32_t range_hi) {
       const int value_bin = f.bin;
-      uint32_t range_lo = max(1u, border.order), range_hi = 0xffffffffu;  // (what top_k left out is no member)
       int shift = -1;
-      auto member = [&](uint32_t o, float v) { return o >= range_lo && o <= range_hi && interval(v) == value_bin; };
+      float x_lo = value_of(range_lo), x_hi = value_of(range_hi);
+      auto member = [&](float v) { return v >= x_lo && v <= x_hi && (!number || interval(v) == value_bin); };
       while (f.in_n > SA_LIST && shift != 0) {
         // their range of orders, divided evenly, the largest first
-        uint32_t lo = 0xffffffffu, hi = 0;
-        for (int i = tid; i < vecs; i += SA_THREADS) {
-          float v[V];
-          read(i, v);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const uint32_t o = order_of(v[e]);
-            if (o && member(o, v[e])) lo = min(lo, o), hi = max(hi, o);
-          }
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
-        __syncthreads();
-        if (tid == 0) sh.low = 0xffffffffu, sh.high = 0;
-        clear();
-        if (lane == 0) atomicMin(&sh.low, lo), atomicMax(&sh.high, hi);
-        cluster.sync();
-        lo = 0xffffffffu, hi = 0;
-        for (int q = 0; q < ranks; ++q) lo = min(lo, *cluster.map_shared_rank(&sh.low, q)), hi = max(hi, *cluster.map_shared_rank(&sh.high, q));
         shift = 0;
-        while (((hi - lo) >> shift) >= SA_BINS) ++shift;
+        while (((range_hi - range_lo) >> shift) >= SA_BINS) ++shift;
+        clear();
         for (int i = tid; i < vecs; i += SA_THREADS) {
           float v[V];
           read(i, v);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const uint32_t o = order_of(v[e]);
-            if (o && member(o, v[e])) {
-              atomicAdd(&sh.count[(hi - o) >> shift], 1u);
-              if (!number) add_mass(static_cast<int>((hi - o) >> shift), weigh(v[e]));
-            }
+            if (!member(v[e])) continue;
+            const int bin = static_cast<int>((range_hi - order_of(v[e])) >> shift);
+            atomicAdd(&sh.count[bin], 1u);
+            if (!number) add_mass(bin, weigh(v[e]));
           }
         }
-        f = find(number, want_n, f.above_n, f.above, -1);
+        f = find(number, want_n, f.above_n, f.above);
         if (f.bin < 0) return;  // (never: the sums are exact)
-        range_hi = hi - (static_cast<uint32_t>(f.bin) << shift);
+        range_hi -= static_cast<uint32_t>(f.bin) << shift;
         const uint32_t span = (1u << shift) - 1;
-        range_lo = range_hi - lo < span ? lo : range_hi - span;
+        if (range_hi - range_lo > span) range_lo = range_hi - span;
+        x_lo = value_of(range_lo), x_hi = value_of(range_hi);
       }
       if (f.in_n <= SA_LIST && shift != 0) {
         if (collect(member)) {
@@ -471,17 +483,17 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         }
       }
     };
-    // The few that can still be taken, in the first CTA: top_k, top_p and min_p in the sorted list, then u in index order.
+    // The few down to top_k's interval, in the first CTA: top_k, top_p and min_p in the sorted list, then u in index order.
     auto finish = [&](int last) {
-      if (!collect([&](uint32_t, float v) { return interval(v) <= last; })) return;
+      if (!collect([&](float v) { return v > -INFINITY && interval(v) <= last; })) return;
       const u64 e0 = sh.list[2 * tid], e1 = sh.list[2 * tid + 1];
       const uint32_t o0 = static_cast<uint32_t>(e0 >> 32), o1 = static_cast<uint32_t>(e1 >> 32);
-      const uint32_t most = by_count ? static_cast<uint32_t>(top_k) : 0xffffffffu;
+      const uint32_t most = static_cast<uint32_t>(top_k);
       const u64 w0 = o0 && 2u * tid < most ? weigh(value_of(o0)) : 0, w1 = o1 && 2u * tid + 1 < most ? weigh(value_of(o1)) : 0;
       u64 all, limit = ~0ull;
       const u64 b0 = block_scan(w0 + w1, sh.scan64, &all);
       if (by_mass) {
-        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(by_count ? all : whole));
+        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all));
         limit = part >= 1.0 ? static_cast<u64>(part) : 1ull;
       }
       const bool k0 = o0 && 2u * tid < most && b0 < limit && w0 >= least, k1 = o1 && 2u * tid + 1 < most && b0 + w0 < limit && w1 >= least;
@@ -504,7 +516,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       take(i1, at + x0, x1);
     };
 
-    const int last_min = min_p > 0.0f ? interval(top + sure) : SA_BINS - 1;  // intervals behind it are below min_p
     bool done = false;
     if (by_count) {
       clear();
@@ -515,87 +526,138 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         for (int e = 0; e < V; ++e)
           if (v[e] > -INFINITY) atomicAdd(&sh.count[interval(v[e])], 1u);
       }
-      const Found f = find(true, static_cast<uint32_t>(top_k), 0, 0, last_min);
+      const Found f = find(true, static_cast<uint32_t>(top_k), 0, 0);
       if (f.bin >= 0) {
         if (f.above_n + f.in_n <= SA_LIST) {
           finish(f.bin);
           done = true;
         } else {
-          settle(true, static_cast<uint32_t>(top_k), f);
+          settle(true, static_cast<uint32_t>(top_k), f, order_of(-3.4028235e38f), order_of(top));
         }
       }
     }
     if (by_mass && !done) {
       const Border counted = border;
-      if (!counted.order && slice >= 4096) {
-        // a rough sum first: intervals whose whole mass cannot reach what top_p leaves out need not be kept apart
-        const float s = static_cast<float>(weigh.scale);
-        float sum = 0.0f;
+      const float from = counted.order ? value_of(counted.order) : -3.4028235e38f;
+      auto sum_up = [&](float v) {  // over the cluster
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        if (lane == 0) sh.warp_sum[warp] = v;
+        __syncthreads();
+        if (tid == 0) {
+          for (int w = 1; w < SA_WARPS; ++w) v += sh.warp_sum[w];
+          sh.rough = v;
+        }
+        cluster.sync();
+        v = 0.0f;
+        for (int q = 0; q < ranks; ++q) v += *cluster.map_shared_rank(&sh.rough, q);
+        return v;
+      };
+      if (!sum_now) {
+        rough = 0.0f;
         for (int i = tid; i < vecs; i += SA_THREADS) {
           float v[V];
           read(i, v);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            float w;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf((v[e] - top) * s, -200.0f)));
-            sum += w;
-          }
+          for (int e = 0; e < V; ++e)
+            if (v[e] >= from) rough += ex2f(fmaxf((v[e] - top) * s2, -200.0f));
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        __syncthreads();
-        if (lane == 0) reinterpret_cast<float*>(sh.scan32)[warp] = sum;
-        __syncthreads();
-        if (tid == 0) {
-          for (int w = 1; w < SA_WARPS; ++w) sum += reinterpret_cast<float*>(sh.scan32)[w];
-          sh.rough = sum;
-        }
-        cluster.sync();
-        sum = 0.0f;
-        for (int q = 0; q < ranks; ++q) sum += *cluster.map_shared_rank(&sh.rough, q);
-        const float bits = log2f(static_cast<float>(n) / ((1.0f - top_p) * sum)) + 1.0f;  // n weights of 2^-bits are half of what is left out
-        cut = bits < 31.0f ? max(1, static_cast<int>(bits * 32.0f) + 1) : SA_BINS - 1;
+        rough = sum_up(rough);
       }
+      // rough masses of the intervals, in units of 2^-30 of all.  Those whose whole mass is a small part of what top_p leaves out are
+      // not looked at (n weights of 2^-bits are 2^-12 of that): behind the window's end, if not behind its start
       clear();
-      const float from = counted.order ? value_of(counted.order) : -INFINITY;
-      u64 rest = 0;
-      uint32_t rest_n = 0;
+      const float unit = log2f(rough) - 30.0f;
+      const float bits = log2f(static_cast<float>(n)) - log2f(fmaxf(1.0f - top_p, 0x1p-24f) * rough) + 12.0f;
+      const int cut = bits < 31.0f ? max(1, static_cast<int>(bits * 32.0f) + 1) : SA_BINS - 1;
       for (int i = tid; i < vecs; i += SA_THREADS) {
         float v[V];
         read(i, v);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          if (counted.order && !(v[e] >= from)) continue;
-          const u64 w = weigh(v[e]);
           const int bin = interval(v[e]);
-          if (bin < SA_BINS - 1 && v[e] > -INFINITY) {
-            atomicAdd(&sh.count[bin], 1u);
-            add_mass(bin, w);
-          } else {
-            rest += w;
-            rest_n += v[e] > -INFINITY;
+          const uint32_t w = __float2uint_rn(ex2f(fmaf(v[e] - top, s2, -unit)));
+          if (bin < cut && v[e] >= from) atomicAdd(&sh.mass_lo[bin], w);
+        }
+      }
+      cluster.sync();
+      {
+        u64 m[2] = {0, 0}, all;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = 2 * tid + h;
+          if (i >= share) continue;
+          for (int q = 0; q < ranks; ++q) m[h] += cluster.map_shared_rank(&sh, q)->mass_lo[rank * share + i];
+        }
+        u64 ahead = block_scan(m[0] + m[1], sh.scan64, &all);
+        if (tid == 0) sh.total = all;
+        cluster.sync();
+        for (int q = 0; q < rank; ++q) ahead += cluster.map_shared_rank(&sh, q)->total;
+        const double near = static_cast<double>(top_p) * 0x1p30;
+        const double low = near - 0x1p20, high = near + 0x1p20;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = 2 * tid + h;
+          const double b = static_cast<double>(ahead), e = static_cast<double>(ahead + m[h]);
+          if (i < share) {
+            if (rank * share + i == 0 ? e >= low : b < low && e >= low)
+              for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->window[0] = rank * share + i;
+            if (b < high && e >= high)
+              for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->window[1] = rank * share + i;
+          }
+          ahead += m[h];
+        }
+        cluster.sync();
+      }
+      const int bin0 = sh.window[0], bin1 = sh.window[1];
+      // min_p ends before top_p does: top_p takes nothing away
+      if (!(min_p > 0.0f && !counted.order && interval(top + sure) < bin0)) {
+        // the window as logits (its edges as near as fp32 has them: the part of the mass to either side is for that as well)
+        float x_hi = bin0 == 0 ? top : fminf(top, top - (bin0 - 0.5f) / width), x_lo = bin1 == SA_BINS - 1 ? from : fmaxf(from, top - (bin1 + 0.5f) / width);
+        // every weight exactly: ahead of the window, in it, all of them; how many in it
+        u64 ahead = 0, in = 0, all = 0;
+        uint32_t in_n = 0;
+        for (int i = tid; i < vecs; i += SA_THREADS) {
+          float v[V];
+          read(i, v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const u64 w = v[e] >= from ? weigh(v[e]) : 0;
+            all += w;
+            if (v[e] > x_hi) ahead += w;
+            else if (v[e] >= x_lo) in += w, ++in_n;
           }
         }
-      }
 #pragma unroll
-      for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
-      rest_n = __reduce_add_sync(0xffffffffu, rest_n);
-      if (lane == 0 && rest_n) {
-        atomicAdd(&sh.count[SA_BINS - 1], rest_n);
-        add_mass(SA_BINS - 1, rest);
-      }
-      const int last = min_p > 0.0f ? interval(top + sure) : SA_BINS - 1;
-      const Found f = find(false, 0, 0, 0, last);
-      if (f.bin >= 0) {
-        const bool least_first = last < f.bin;  // min_p leaves nothing near top_p's border
-        if (!counted.order && (least_first ? sh.least_n : f.above_n + f.in_n) <= SA_LIST) {
-          finish(least_first ? last : f.bin);
-          done = true;
-        } else if (!least_first || counted.order) {
-          settle(false, 0, f);
-          // never past the counted ones
-          if (border.order < counted.order || (border.order == counted.order && border.ties > counted.ties && counted.order)) border = counted;
+        for (int o = 16; o; o >>= 1) {
+          ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+          in += __shfl_xor_sync(0xffffffffu, in, o);
+          all += __shfl_xor_sync(0xffffffffu, all, o);
         }
+        in_n = __reduce_add_sync(0xffffffffu, in_n);
+        __syncthreads();
+        if (tid == 0) sh.above = sh.inside = sh.total = 0, sh.inside_n = 0;
+        __syncthreads();
+        if (lane == 0) atomicAdd(&sh.above, ahead), atomicAdd(&sh.inside, in), atomicAdd(&sh.total, all), atomicAdd(&sh.inside_n, in_n);
+        cluster.sync();
+        Found f = {0, 0, 0, 0, 0};
+        all = 0;
+        for (int q = 0; q < ranks; ++q) {
+          const SampleShared* s = cluster.map_shared_rank(&sh, q);
+          f.above += s->above, f.in += s->inside, f.in_n += s->inside_n, all += s->total;
+        }
+        // (equals of the counted border that are no candidates)
+        const u64 surplus = counted.order ? static_cast<u64>(counted.equals - counted.ties) * weigh(value_of(counted.order)) : 0;
+        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all - surplus));
+        want = part >= 1.0 ? static_cast<u64>(part) : 1ull;
+        if (!(f.above < want && want <= f.above + f.in)) {  // (the rough masses were further off than they can be)
+          f.in_n = 0xffffffffu, f.above = 0;
+          x_lo = from, x_hi = top;
+        }
+        settle(false, 0, f, order_of(x_lo), order_of(x_hi));
+        // never past the counted ones
+        if (border.order < counted.order || (border.order == counted.order && border.ties > counted.ties && counted.order)) border = counted;
       }
     }
     if (done) {
@@ -605,15 +667,18 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   }
 
   // ---- 3. running sums in index order --------------------------------------------------------------------------------------------------------
-  const float border_x = border.order ? value_of(border.order) : -INFINITY;
+  const float border_x = border.order ? value_of(border.order) : -3.4028235e38f;
+  const float least_x = fmaxf(border_x, top + sure);  // (top + sure rounds to no more than the least logit that min_p may leave)
   const int per_warp = (vecs + SA_WARPS - 1) / SA_WARPS, v0 = min(vecs, warp * per_warp), v1 = min(vecs, v0 + per_warp);
+  auto any = [&](const float (&v)[V]) {
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < V; ++e) m = fmaxf(m, v[e]);
+    return m >= least_x;
+  };
   auto weight = [&](float v, bool* tie) -> u64 {
-    *tie = false;
-    if (!(v - top >= sure) || !(v >= border_x)) return 0;
-    if (v == border_x && border.order) {
-      *tie = true;
-      return 0;
-    }
+    *tie = v == border_x && border.order;
+    if (!(v >= least_x) || *tie) return 0;
     const u64 w = weigh(v);
     return w < least ? 0 : w;
   };
@@ -622,6 +687,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   for (int i = v0 + lane; i < v1; i += 32) {
     float v[V];
     read(i, v);
+    if (!any(v)) continue;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       bool tie;
@@ -664,8 +730,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       u64 w[V], sum = 0;
       uint32_t mine_t = 0;
       bool tie[V];
-      const bool there = i0 + lane < v1;
-      if (there) read(i0 + lane, v);
+      bool there = i0 + lane < v1;
+      if (there) {
+        read(i0 + lane, v);
+        there = any(v);
+      }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         tie[e] = false;
