@@ -75,6 +75,10 @@ __device__ __forceinline__ float ex2f(float x) {
   return y;
 }
 
+struct Powers {
+  double v[64];  // 2^(k / 64)
+};
+
 struct Border {          // candidates: order > order, and the first `ties` (of `equals`) of order == order
   uint32_t order;
   uint32_t ties, equals;
@@ -93,7 +97,6 @@ struct SampleShared {
   u64 scan64[33];
   uint32_t scan32[33];
   // read by the cluster's other CTAs
-  float top;
   int first;
   uint32_t total_n;
   u64 total;
@@ -102,10 +105,10 @@ struct SampleShared {
   int window[2];                                                // intervals between which top_p's border lies
   u64 above, inside;                                            // masses ahead of them and in them
   uint32_t inside_n;
-  float rough;
   u64 warp_mass[SA_WARPS];
   uint32_t warp_ties[SA_WARPS];
   float warp_top[SA_WARPS], warp_sum[SA_WARPS];
+  double scale;
 };
 
 // w of a candidate (what is none gets some w of its own: callers leave it out)
@@ -128,6 +131,12 @@ struct Weigh {
     return static_cast<u64>(__double_as_longlong(fma(w, one, 4503599627370496.0)) & 0xfffffffffffffll);  // (2^52: the integer in the low bits)
   }
 };
+
+// the logarithm of w / total, to fp32's last bits near one too
+__device__ __forceinline__ float log_share(u64 w, u64 total) {
+  const u64 left = total - w;
+  return left < w ? log1pf(-(static_cast<float>(left) / static_cast<float>(total))) : logf(static_cast<float>(w) / static_cast<float>(total));
+}
 
 template <class V>
 __device__ __forceinline__ V warp_scan(V v, int lane) {  // inclusive
@@ -158,7 +167,7 @@ __device__ __forceinline__ V block_scan(V v, V* scratch, V* total) {
 }
 
 template <int T, bool KEPT>
-__global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid_constant__ SampleLaunch a, int slice) {
+__global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid_constant__ SampleLaunch a, int slice, const __grid_constant__ Powers powers) {
   constexpr int V = Vec<T>::N;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ SampleShared sh;
@@ -191,6 +200,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
 
   // ---- 1. the largest, and a rough sum of the weights (a thread's by its own largest, which it raises as it goes) ------------------------
   const float s2 = t > 0.0f ? 1.4426950408889634f / t : 0.0f;
+  if (tid == SA_THREADS - 1) sh.scale = 1.4426950408889634074 / static_cast<double>(t);  // (one thread: a fp64 division of all took as long as a pass)
   float top = -INFINITY, rough = 0.0f;
   const bool by_count = top_k > 0 && top_k < n, by_mass = top_p < 1.0f, sum_now = by_mass && !by_count;
   auto take_in = [&](const float (&f)[V]) {
@@ -258,18 +268,22 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     const float om = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, rough, o);
     join(top, rough, om, os);
   }
-  if (tid < 64) sh.table[tid] = exp2(tid * (1.0 / 64));
+  if (tid < 64) sh.table[tid] = powers.v[tid];
   if (tid == 0) sh.list_n = 0;
   if (lane == 0) sh.warp_top[warp] = top, sh.warp_sum[warp] = rough;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < SA_WARPS; ++w) join(top, rough, sh.warp_top[w], sh.warp_sum[w]);
-    sh.top = top;
-    sh.rough = rough;
-  }
   cluster.sync();
-  top = -INFINITY, rough = 0.0f;
-  for (int c = 0; c < ranks; ++c) join(top, rough, *cluster.map_shared_rank(&sh.top, c), *cluster.map_shared_rank(&sh.rough, c));
+  {  // every warp joins the parts of all
+    top = -INFINITY, rough = 0.0f;
+    for (int i = lane; i < ranks * SA_WARPS; i += 32) {
+      const SampleShared* s = cluster.map_shared_rank(&sh, i / SA_WARPS);
+      join(top, rough, s->warp_top[i % SA_WARPS], s->warp_sum[i % SA_WARPS]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, rough, o);
+      join(top, rough, om, os);
+    }
+  }
 
   if (top == -INFINITY || top == INFINITY || !(t > 0.0f)) {  // the largest's first index, or none
     int at = 0x7fffffff;
@@ -299,11 +313,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   while ((1ll << room) < n) ++room;
   Weigh weigh;
   weigh.top = top;
-  weigh.scale = 1.4426950408889634074 / static_cast<double>(t);
+  weigh.scale = sh.scale;
   weigh.one = static_cast<double>(1ull << min(62 - room, 51));
   {
     // 600 powers of two down; where that is no smaller float, every other logit is further down than that
-    float low = static_cast<float>(fmax(static_cast<double>(top) - 600.0 / weigh.scale, -3.4028234e38));
+    float low = static_cast<float>(fmax(static_cast<double>(top) - 415.888 * static_cast<double>(t), -3.4028234e38));
     if ((static_cast<double>(top) - low) * weigh.scale > 900.0 || low >= top) {
       low = fmaxf(value_of(order_of(top) - 1), -3.4028235e38f);
       weigh.scale = fmin(weigh.scale, 600.0 / (static_cast<double>(top) - low));
@@ -311,11 +325,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     weigh.least_x = low;
   }
   weigh.table = sh.table;
-  // logits surely below min_p are left out before they are weighed (2^-10 of slack for the fp32 product)
-  const double least_w = min_p > 0.0f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
-  const u64 least = static_cast<u64>(ceil(least_w * weigh.one));
-  const float sure = min_p > 0.0f ? static_cast<float>((log2(least_w) - 1e-3) / weigh.scale * 1.0001) : -INFINITY;  // of x - max
-
+  // logits surely below min_p are left out before they are weighed (2e-3 and a part in 10 000 of slack for the fp32 product)
+  const float least_w = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
+  const u64 least = static_cast<u64>(ceil(static_cast<double>(least_w) * weigh.one));
+  const float sure = min_p > 0.0f ? (log2f(least_w) - 2e-3f) * (t * 0.69321f) : -INFINITY;  // of x - max
   // ---- 2. the border ---------------------------------------------------------------------------------------------------------------------
   Border border = {0, 0, 0};
   if (by_count || by_mass) {
@@ -510,7 +523,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       auto take = [&](u64 item, u64 from, u64 w) {
         if (!(from <= until && until < from + w)) return;
         a.ids[row] = static_cast<int>(~static_cast<uint32_t>(item >> 32));
-        if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all)));
+        if (a.logprob) a.logprob[row] = log_share(w, all);
       };
       take(i0, at, x0);
       take(i1, at + x0, x1);
@@ -542,16 +555,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       auto sum_up = [&](float v) {  // over the cluster
 #pragma unroll
         for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        __syncthreads();
         if (lane == 0) sh.warp_sum[warp] = v;
-        __syncthreads();
-        if (tid == 0) {
-          for (int w = 1; w < SA_WARPS; ++w) v += sh.warp_sum[w];
-          sh.rough = v;
-        }
         cluster.sync();
         v = 0.0f;
-        for (int q = 0; q < ranks; ++q) v += *cluster.map_shared_rank(&sh.rough, q);
+        for (int i = lane; i < ranks * SA_WARPS; i += 32) v += cluster.map_shared_rank(&sh, i / SA_WARPS)->warp_sum[i % SA_WARPS];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
       };
       if (!sum_now) {
@@ -669,7 +678,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   // ---- 3. running sums in index order --------------------------------------------------------------------------------------------------------
   const float border_x = border.order ? value_of(border.order) : -3.4028235e38f;
   const float least_x = fmaxf(border_x, top + sure);  // (top + sure rounds to no more than the least logit that min_p may leave)
-  const int per_warp = (vecs + SA_WARPS - 1) / SA_WARPS, v0 = min(vecs, warp * per_warp), v1 = min(vecs, v0 + per_warp);
+  // a thread's own stretch of vectors: an odd number, so that a warp's reads fall into different banks
+  const int stretch = ((vecs + SA_THREADS - 1) / SA_THREADS) | 1, v0 = min(vecs, tid * stretch), v1 = min(vecs, v0 + stretch);
   auto any = [&](const float (&v)[V]) {
     float m = v[0];
 #pragma unroll
@@ -684,7 +694,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   };
   u64 mass = 0;
   uint32_t ties = 0;
-  for (int i = v0 + lane; i < v1; i += 32) {
+  for (int i = v0; i < v1; ++i) {
     float v[V];
     read(i, v);
     if (!any(v)) continue;
@@ -695,10 +705,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       ties += tie;
     }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-  ties = __reduce_add_sync(0xffffffffu, ties);
-  if (lane == 0) sh.warp_mass[warp] = mass, sh.warp_ties[warp] = ties;
+  const u64 mass_inc = warp_scan(mass, lane);
+  const uint32_t ties_inc = warp_scan(ties, lane);
+  if (lane == 31) sh.warp_mass[warp] = mass_inc, sh.warp_ties[warp] = ties_inc;
   cluster.sync();
   u64 tie_w = border.order ? weigh(value_of(border.order)) : 0;
   if (tie_w < least) tie_w = 0;
@@ -718,51 +727,42 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   total_t = __reduce_add_sync(0xffffffffu, total_t), ahead_t = __reduce_add_sync(0xffffffffu, ahead_t);
   total += static_cast<u64>(min(total_t, allowed)) * tie_w;
   ahead += static_cast<u64>(min(ahead_t, allowed)) * tie_w;
-  const u64 warp_all = mass + static_cast<u64>(min(ahead_t + ties, allowed) - min(ahead_t, allowed)) * tie_w;
   // u times the sum, rounded down; below the sum
   u64 until = static_cast<u64>(floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(total)));
   if (until >= total) until = total - 1;
-  if (ahead <= until && until < ahead + warp_all) {  // (one warp of the cluster)
-    u64 run = ahead;
-    uint32_t seen = ahead_t;
-    for (int i0 = v0; i0 < v1; i0 += 32) {
-      float v[V];
-      u64 w[V], sum = 0;
-      uint32_t mine_t = 0;
-      bool tie[V];
-      bool there = i0 + lane < v1;
-      if (there) {
-        read(i0 + lane, v);
-        there = any(v);
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        tie[e] = false;
-        w[e] = there ? weight(v[e], &tie[e]) : 0;
-        mine_t += tie[e];
-      }
-      uint32_t t_at = seen + warp_scan(mine_t, lane) - mine_t;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (tie[e] && t_at++ < allowed) w[e] = tie_w;
-        sum += w[e];
-      }
-      const u64 inc = warp_scan(sum, lane);
-      u64 at = run + inc - sum;
-      if (at <= until && until < run + inc) {
-        bool done = false;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          at += w[e];
-          if (!done && at > until) {
-            done = true;
-            a.ids[row] = first + (i0 + lane) * V + e;
-            if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w[e]) / static_cast<double>(total)));
-          }
+  // this thread's stretch: masses and equals of the border ahead of it
+  const uint32_t t_from = ahead_t + ties_inc - ties;
+  const u64 above_ahead = ahead - static_cast<u64>(min(ahead_t, allowed)) * tie_w + mass_inc - mass;
+  const u64 from = above_ahead + static_cast<u64>(min(t_from, allowed)) * tie_w;
+  const u64 to = above_ahead + mass + static_cast<u64>(min(t_from + ties, allowed)) * tie_w;
+  const unsigned who = __ballot_sync(0xffffffffu, from <= until && until < to);
+  if (who) {  // (one thread of the cluster): its warp walks its stretch, an element a lane
+    const int l = __ffs(who) - 1;
+    u64 run = __shfl_sync(0xffffffffu, from, l);
+    uint32_t seen = __shfl_sync(0xffffffffu, t_from, l);
+    const int e0 = __shfl_sync(0xffffffffu, v0, l) * V, e1 = __shfl_sync(0xffffffffu, v1, l) * V;
+    for (int e = e0; e < e1; e += 32) {
+      float v = __uint_as_float(0x7fc00000u);
+      if constexpr (KEPT) {
+        if (e + lane < e1) {
+          if constexpr (T == MIMIR_B200_T_F32) v = reinterpret_cast<const float*>(dyn)[e + lane];
+          else if constexpr (T == MIMIR_B200_T_F16) v = __half2float(reinterpret_cast<const __half*>(dyn)[e + lane]);
+          else v = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(dyn)[e + lane]);
         }
+      } else {
+        if (e + lane < min(e1, mine)) v = logit<T>(x, first + e + lane);
       }
-      run = __shfl_sync(0xffffffffu, run + inc, 31);
-      seen += __reduce_add_sync(0xffffffffu, mine_t);
+      bool tie;
+      u64 w = weight(v, &tie);
+      const unsigned equal = __ballot_sync(0xffffffffu, tie);
+      if (tie && seen + __popc(equal & ((1u << lane) - 1)) < allowed) w = tie_w;
+      const u64 inc = warp_scan(w, lane);
+      if (run + inc - w <= until && until < run + inc) {
+        a.ids[row] = first + e + lane;
+        if (a.logprob) a.logprob[row] = log_share(w, total);
+      }
+      run += __shfl_sync(0xffffffffu, inc, 31);
+      seen += __popc(equal);
       if (run > until) break;
     }
   }
@@ -789,7 +789,12 @@ int launch_as(const SampleLaunch& s, int cluster, int slice, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  MB_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel<T, KEPT>, s, slice));
+  static const Powers powers = [] {
+    Powers p;
+    for (int k = 0; k < 64; ++k) p.v[k] = std::exp2(k / 64.0);
+    return p;
+  }();
+  MB_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel<T, KEPT>, s, slice, powers));
   count_launch();
   return MIMIR_B200_OK;
 }
