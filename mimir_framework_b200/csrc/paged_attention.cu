@@ -11,8 +11,9 @@
 //   K        lane (g, t) holds elements 8 t .. 8 t + 7 of each 32 of key g:  two contraction steps
 //   V        lane (g, t) holds elements 8 g .. 8 g + 7 of each 64 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: eight column tiles
 // fp32 queries and probabilities are two IEEE-half terms (hi + lo, 22 bits): queries after a power of two per row has brought their
-// largest to [1, 2).  Codes of eight bits are exact in half; their scales multiply scores and probabilities.  Each block's P V starts from
-// zero and is added in fp32, because the tensor core's accumulation truncates.
+// largest to [1, 2).  Probabilities are two terms for bfloat16 caches too (16 bits), one half (11 bits) where only the result is bfloat16.
+// Codes of eight bits are exact in half; their scales multiply scores and probabilities.  For fp32 results each block's P V starts from
+// zero and is added in fp32, because the tensor core's accumulation truncates (1.5e-8 of the value an instruction).
 #include <cmath>
 
 #include "common.h"
@@ -39,18 +40,27 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint4& a, uint32_t b0
   if constexpr (BF) mma_bf16(c, a, b0, b1);
   else mma_f16(c, a, b0, b1);
 }
-// dst in shared memory of cluster rank `rank`
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+// shared memory of cluster rank `rank`
+__device__ __forceinline__ uint32_t cluster_address(const float* p, uint32_t rank) {
   uint32_t a;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return a;
+}
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_address(p, rank)) : "memory");
   return v;
 }
 
-template <int CT, int NQ, int DP>
+template <int CT, int NQ, int NP, int DP>  // terms of a query and of a probability
 struct PagedShape {
   static constexpr bool BF = CT == MIMIR_B200_T_BF16;
+  static constexpr bool FRESH = NQ == 2;                                // P V of a block apart from O
   static constexpr int KB = type_bytes(CT) == 1 ? 32 : 16;              // keys of a block
   static constexpr int UD = CT == MIMIR_B200_T_F32 ? 64 : DP < 128 ? DP : 128;  // head elements loaded at a time
   static constexpr int Q_BYTES = NQ * (DP / 16) * 32 * 16;
@@ -58,10 +68,10 @@ struct PagedShape {
   static constexpr int SMEM = Q_BYTES + PA_WARPS * PA_ROWS * (O_STRIDE + 2) * 4 + 2 * PA_ROWS * 4;
 };
 
-template <int CT, int NQ, int DP>
-__global__ void __launch_bounds__(PA_THREADS, (DP > 128 || CT == MIMIR_B200_T_F32) ? 2 : 3)
+template <int CT, int NQ, int NP, int DP>
+__global__ void __launch_bounds__(PA_THREADS, (DP > 128 || CT == MIMIR_B200_T_F32 || (DP > 64 && type_bytes(CT) == 1)) ? 2 : 3)
 paged_attention_kernel(const __grid_constant__ AttendArgs a) {
-  using S = PagedShape<CT, NQ, DP>;
+  using S = PagedShape<CT, NQ, NP, DP>;
   constexpr bool BF = S::BF, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3, WIDE = CT == MIMIR_B200_T_F32;
   constexpr int KB = S::KB, NG = KB / 8, UD = S::UD, NU = DP / UD;
   constexpr float LOG2E = 1.4426950408889634f;
@@ -93,7 +103,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   // ---- the queries of the tile as fragments, hi (+ lo): a warp takes four rows -------------------------------------------------
 #pragma unroll
   for (int i = 0; i < PA_ROWS / PA_WARPS; ++i) {
-    const int row = warp * (PA_ROWS / PA_WARPS) + i, r = r0 + row;
+    const int row = i * PA_WARPS + warp, r = r0 + row;
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = 0.0f;
@@ -146,7 +156,6 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     c2[i] = a.scale * LOG2E * sscale[g + 8 * i];
-    if (CT == MIMIR_B200_T_E4M3) c2[i] *= 256.0f;
     const int pos = pos0 + min(r0 + g + 8 * i, r_end - 1) / a.group;
     lim_hi[i] = a.causal ? min(q.kv, pos + 1) : q.kv;
     lim_lo[i] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
@@ -161,32 +170,39 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
   // ---- pages of a block's groups of eight keys (a page holds a multiple of eight) ----------------------------------------------------
-  int page_next[NG];
+  int page_next[NG], slot_next[NG];
+  bool whole_next = false;  // every key of the block is there
   auto fetch_pages = [&](int b) {
+    whole_next = b * KB >= k_begin && b * KB + KB <= k_end;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const int key = b * KB + 8 * j;
-      page_next[j] = (b < b1 && key < k_end && key + 7 >= k_begin) ? paged_page(p, s, p.by_page.div(key)) : -1;
+      const int pi = p.by_page.div(key);
+      slot_next[j] = key - pi * p.page_size;
+      page_next[j] = (b < b1 && key < k_end && key + 7 >= k_begin) ? paged_page(p, s, pi) : -1;
     }
   };
-  long long off[NG];  // of a group's first key in the pages, -1: none
+  long long off[NG];   // of a group's first key in the pages, -1: none
   long long soff[NG];  // and in the scales
-  auto place_pages = [&](int b) {
+  bool whole = false;
+  auto place_pages = [&]() {
+    whole = whole_next;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const int key = b * KB + 8 * j, slot = key - p.by_page.div(key) * p.page_size;
-      off[j] = page_next[j] < 0 ? -1 : page_next[j] * p.page_stride + slot * p.slot_stride + head * p.head_stride;
-      soff[j] = (static_cast<long long>(page_next[j]) * p.kv_heads + head) * p.page_size + slot;
+      whole = whole && page_next[j] >= 0;
+      off[j] = page_next[j] < 0 ? -1 : page_next[j] * p.page_stride + slot_next[j] * p.slot_stride + head * p.head_stride;
+      if constexpr (CODED) soff[j] = (static_cast<long long>(page_next[j]) * p.kv_heads + head) * p.page_size + slot_next[j] + 2 * t;
     }
   };
   Raw8<CT> kr[NG][UD / 32], vr[KB / 16][4][(UD + 63) / 64];
   float2 ks[NG], vs[NG];
+  const long long k_lane = (g * p.slot_stride + 8 * t) * type_bytes(CT), v_lane = (2 * t * p.slot_stride + 8 * g) * type_bytes(CT), row_bytes = p.slot_stride * type_bytes(CT);
   auto load_k = [&](int b, int u) {
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const int key = b * KB + 8 * j + g;
-      const bool go = off[j] >= 0 && key < k_end;
-      const char* base = static_cast<const char*>(p.k) + (off[j] + g * p.slot_stride + u * UD + 8 * t) * type_bytes(CT);
+      const bool go = whole || (off[j] >= 0 && key < k_end);
+      const char* base = static_cast<const char*>(p.k) + off[j] * type_bytes(CT) + k_lane + u * UD * type_bytes(CT);
 #pragma unroll
       for (int c = 0; c < UD / 32; ++c) {
         if (go && u * UD + 32 * c + 8 * t < p.head_dim) kr[j][c] = load8<CT>(base + 32 * c * type_bytes(CT));
@@ -196,7 +212,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       }
       if (CODED && u == 0) {
         ks[j] = make_float2(0.0f, 0.0f);
-        if (off[j] >= 0) ks[j] = *reinterpret_cast<const float2*>(p.k_scale + soff[j] + 2 * t);
+        if (off[j] >= 0) ks[j] = __ldg(reinterpret_cast<const float2*>(p.k_scale + soff[j]));
       }
     }
   };
@@ -205,9 +221,9 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     for (int k16 = 0; k16 < KB / 16; ++k16)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        const int j = 2 * k16 + (i >> 1), in = 2 * t + (i & 1), key = b * KB + 8 * j + in;
-        const bool go = off[j] >= 0 && key < k_end && key >= k_begin;  // (a key that no row sees is zero whatever its slot holds)
-        const char* base = static_cast<const char*>(p.v) + (off[j] + in * p.slot_stride + u * UD + 8 * g) * type_bytes(CT);
+        const int j = 2 * k16 + (i >> 1), key = b * KB + 8 * j + 2 * t + (i & 1);
+        const bool go = whole || (off[j] >= 0 && key < k_end && key >= k_begin);  // (a key that no row sees is zero whatever its slot holds)
+        const char* base = static_cast<const char*>(p.v) + off[j] * type_bytes(CT) + v_lane + ((i & 1) ? row_bytes : 0) + u * UD * type_bytes(CT);
 #pragma unroll
         for (int c = 0; c < (UD + 63) / 64; ++c) {
           if (go && u * UD + 64 * c + 8 * g < p.head_dim) vr[k16][i][c] = load8<CT>(base + 64 * c * type_bytes(CT));
@@ -221,16 +237,19 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       for (int j = 0; j < NG; ++j) {
         const int key = b * KB + 8 * j + 2 * t;
         vs[j] = make_float2(0.0f, 0.0f);
-        if (off[j] >= 0) vs[j] = *reinterpret_cast<const float2*>(p.v_scale + soff[j] + 2 * t);
-        if (key >= k_end || key < k_begin) vs[j].x = 0.0f;
-        if (key + 1 >= k_end || key + 1 < k_begin) vs[j].y = 0.0f;
+        if (off[j] >= 0) vs[j] = __ldg(reinterpret_cast<const float2*>(p.v_scale + soff[j]));
+        if (!whole) {
+          if (key >= k_end || key < k_begin) vs[j].x = 0.0f;
+          if (key + 1 >= k_end || key + 1 < k_begin) vs[j].y = 0.0f;
+        }
       }
     }
   };
 
+  float v_unit = 0.0f;  // codes: the power of two that O's values are in
   if (b0 < b1) {
     fetch_pages(b0);
-    place_pages(b0);
+    place_pages();
     load_k(b0, 0);
     load_v(b0, 0);
     fetch_pages(b0 + 1);
@@ -239,15 +258,15 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     // ---- scores ----------------------------------------------------------------------------------------------------------------
     float sc[NG][4];
     bool there[NG];
+    const bool full = whole && b * KB >= all_lo && b * KB + KB <= all_hi;
+    float2 ks_now[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       there[j] = off[j] >= 0;
+      if constexpr (CODED) ks_now[j] = ks[j];
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
     }
-    float2 ks_now[NG];
-#pragma unroll
-    for (int j = 0; j < NG; ++j) ks_now[j] = ks[j];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
@@ -276,15 +295,12 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     // the next block's keys are on their way while this one's values are used
     if constexpr (NU == 1) {
       if (b + 1 < b1) {
-        place_pages(b + 1);
+        place_pages();
         load_k(b + 1, 0);
         fetch_pages(b + 2);
       }
     }
     // ---- running maximum and sum -----------------------------------------------------------------------------------------------------
-    bool full = b * KB >= all_lo && b * KB + KB <= all_hi;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) full = full && there[j];
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j = 0; j < NG; ++j)
@@ -300,18 +316,19 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
         mx[i >> 1] = fmaxf(mx[i >> 1], v);
       }
     float alpha[2], base[2];
+    bool raise = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
       const float mn = fmaxf(m[i], mx[i]);
+      raise = raise || mn > m[i];
       base[i] = mn == -INFINITY ? 0.0f : mn;  // (a row that has seen nothing yet)
-      alpha[i] = exp2f(m[i] - base[i]);
+      alpha[i] = ex2f(m[i] - base[i]);
       m[i] = mn;
       l[i] *= alpha[i];
     }
     // codes' scales move into the probabilities, which a power of two keeps near one: halves have little range
-    float back = 1.0f;
     float2 vf[NG];
     if constexpr (CODED) {
       float top = 0.0f;
@@ -320,11 +337,22 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e2 = min(240, max(14, static_cast<int>(__float_as_uint(top) >> 23)));
-      back = __uint_as_float(static_cast<uint32_t>(e2) << 23);
-      const float inv = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+      const float unit = fmaxf(v_unit, __uint_as_float(static_cast<uint32_t>(e2) << 23));
+      const float inv = __uint_as_float(0x7f000000u - __float_as_uint(unit));  // (a power of two's reciprocal)
+      if (unit > v_unit) {
+        raise = true;
+        const float f = v_unit * inv;
+        alpha[0] *= f, alpha[1] *= f;
+        v_unit = unit;
+      }
 #pragma unroll
       for (int j = 0; j < NG; ++j) vf[j] = make_float2(vs[j].x * inv, vs[j].y * inv);
-      if (CT == MIMIR_B200_T_E4M3) back *= 256.0f;
+    }
+    if (!S::FRESH && __any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[j][i] *= alpha[i >> 1];
     }
     uint4 ph[KB / 16], pl[KB / 16];
 #pragma unroll
@@ -336,52 +364,56 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = exp2f(sc[j][i] - base[i >> 1]);
+          e[i] = ex2f(sc[j][i] - base[i >> 1]);
           l[i >> 1] += e[i];
           if constexpr (CODED) e[i] *= (i & 1) ? vf[j].y : vf[j].x;
         }
-        split2<BF>(e[0], e[1], hi[x][0], lo[x][0]);
-        split2<BF>(e[2], e[3], hi[x][1], lo[x][1]);
+        if constexpr (NP == 2) {
+          split2<BF>(e[0], e[1], hi[x][0], lo[x][0]);
+          split2<BF>(e[2], e[3], hi[x][1], lo[x][1]);
+        } else {
+          hi[x][0] = pack2<BF>(e[0], e[1]);
+          hi[x][1] = pack2<BF>(e[2], e[3]);
+        }
       }
       ph[k16] = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
-      pl[k16] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
+      if constexpr (NP == 2) pl[k16] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
     }
     // ---- values ------------------------------------------------------------------------------------------------------------------------
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
       for (int c = 0; c < (UD + 63) / 64; ++c) {
+        float acc[8][4];
+        if constexpr (S::FRESH) {
 #pragma unroll
-        for (int pr = 0; pr < 4; ++pr) {  // column tiles 2 pr and 2 pr + 1
-          float acc[2][4] = {};
+          for (int n = 0; n < 8; ++n)
 #pragma unroll
-          for (int k16 = 0; k16 < KB / 16; ++k16) {
-            uint32_t hi[4], lo[4];  // the pair of this lane's four keys
+            for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+        }
+#pragma unroll
+        for (int k16 = 0; k16 < KB / 16; ++k16) {
+          uint32_t h4[4][4], l4[4][4];  // [this lane's four keys][pair of columns]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to_pairs<CT>(vr[k16][i][c], h4[i], l4[i]);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {  // column tiles
+            float(&to)[4] = S::FRESH ? acc[n] : o[(u * UD + 64 * c) / 8 + n];
+            const uint32_t sel = (n & 1) ? 0x7632 : 0x5410;
+            const uint32_t w0 = __byte_perm(h4[0][n / 2], h4[1][n / 2], sel), w1 = __byte_perm(h4[2][n / 2], h4[3][n / 2], sel);
+            mma16<BF>(to, ph[k16], w0, w1);
+            if constexpr (NP == 2) mma16<BF>(to, pl[k16], w0, w1);
+            if constexpr (WIDE) mma16<BF>(to, ph[k16], __byte_perm(l4[0][n / 2], l4[1][n / 2], sel), __byte_perm(l4[2][n / 2], l4[3][n / 2], sel));
+          }
+        }
+        if constexpr (S::FRESH) {
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              uint32_t h4[4], l4[4];
-              to_pairs<CT>(vr[k16][i][c], h4, l4);
-              hi[i] = h4[pr];
-              if constexpr (WIDE) lo[i] = l4[pr];
+              float& oo = o[(u * UD + 64 * c) / 8 + n][i];
+              oo = fmaf(oo, alpha[i >> 1], acc[n][i]);
             }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint32_t sel = x ? 0x7632 : 0x5410;
-              const uint32_t v0 = __byte_perm(hi[0], hi[1], sel), v1 = __byte_perm(hi[2], hi[3], sel);
-              mma16<BF>(acc[x], ph[k16], v0, v1);
-              mma16<BF>(acc[x], pl[k16], v0, v1);
-              if constexpr (WIDE) mma16<BF>(acc[x], ph[k16], __byte_perm(lo[0], lo[1], sel), __byte_perm(lo[2], lo[3], sel));
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float(&oo)[4] = o[(u * UD + 64 * c) / 8 + 2 * pr + x];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (CODED) oo[i] = fmaf(acc[x][i], back, oo[i] * alpha[i >> 1]);
-              else oo[i] = fmaf(oo[i], alpha[i >> 1], acc[x][i]);
-            }
-          }
         }
       }
       if constexpr (NU > 1) {
@@ -390,52 +422,38 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     }
     if constexpr (NU > 1) {
       if (b + 1 < b1) {
-        place_pages(b + 1);
+        place_pages();
         load_k(b + 1, 0);
         fetch_pages(b + 2);
       }
     }
     if (b + 1 < b1) load_v(b + 1, 0);
   }
+  if constexpr (CODED) {
+    const float f = v_unit;
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] *= f;
+  }
 
-  // ---- warps, then the cluster's CTAs, meet -------------------------------------------------------------------------------------------
+  // ---- warps, then the cluster's CTAs, meet: only the tile's rows --------------------------------------------------------------------
+  const int rows = r_end - r0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     const int row = g + 8 * i;
-    if (t == 0) sm[warp * PA_ROWS + row] = m[i], sl[warp * PA_ROWS + row] = l[i];
-    float* w = so + (warp * PA_ROWS + row) * S::O_STRIDE;
+    if (row < rows) {
+      if (t == 0) sm[warp * PA_ROWS + row] = m[i], sl[warp * PA_ROWS + row] = l[i];
+      float* w = so + (warp * PA_ROWS + row) * S::O_STRIDE;
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j) {  // tile (c, j % 8) has columns 64 c + 16 t + j % 8 and 8 more
-      const int d = (j / 8) * 64 + 16 * t + (j & 7);
-      w[d] = o[j][2 * i];
-      w[d + 8] = o[j][2 * i + 1];
+      for (int j = 0; j < DP / 8; j += 4) {  // tile (c, j % 8) has columns 64 c + 16 t + j % 8 and 8 more
+        const int d = (j / 8) * 64 + 16 * t + (j & 7);
+        *reinterpret_cast<float4*>(w + d) = make_float4(o[j][2 * i], o[j + 1][2 * i], o[j + 2][2 * i], o[j + 3][2 * i]);
+        *reinterpret_cast<float4*>(w + d + 8) = make_float4(o[j][2 * i + 1], o[j + 1][2 * i + 1], o[j + 2][2 * i + 1], o[j + 3][2 * i + 1]);
+      }
     }
-  }
-  __syncthreads();
-  // this CTA's rows: (max, sum, O) into warp 0's place
-  for (int i = threadIdx.x; i < PA_ROWS * DP; i += PA_THREADS) {
-    const int row = i / DP, d = i - row * DP;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, sm[w * PA_ROWS + row]);
-    float sum = 0.0f;
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) sum = fmaf(so[(w * PA_ROWS + row) * S::O_STRIDE + d], exp2f(sm[w * PA_ROWS + row] - base), sum);
-    so[row * S::O_STRIDE + d] = sum;
-  }
-  __syncthreads();
-  if (threadIdx.x < PA_ROWS) {
-    const int row = threadIdx.x;
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, sm[w * PA_ROWS + row]);
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) sum = fmaf(sl[w * PA_ROWS + row], exp2f(sm[w * PA_ROWS + row] - base), sum);
-    sm[row] = top, sl[row] = sum;
   }
   if (a.cluster > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -443,31 +461,39 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   } else {
     __syncthreads();
   }
-  // each CTA finishes its share of the rows
-  for (int row = rank; row < r_end - r0; row += a.cluster) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int c = 0; c < a.cluster; ++c) top = fmaxf(top, a.cluster > 1 ? ld_cluster(sm + row, c) : sm[row]);
+  // four columns of a row a thread, over all of the cluster's threads
+  const int quads = p.head_dim / 4;
+  for (int i = rank * PA_THREADS + threadIdx.x; i < rows * quads; i += a.cluster * PA_THREADS) {
+    const int row = i / quads, d = 4 * (i - row * quads);
+    float top = -INFINITY;
+    for (int c = 0; c < a.cluster; ++c)
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, ld_cluster(sm + w * PA_ROWS + row, c));
     const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int c = 0; c < a.cluster; ++c) {
-      const float mc = a.cluster > 1 ? ld_cluster(sm + row, c) : sm[row], lc = a.cluster > 1 ? ld_cluster(sl + row, c) : sl[row];
-      sum = fmaf(lc, exp2f(mc - base), sum);
-    }
-    for (int d = threadIdx.x; d < p.head_dim; d += PA_THREADS) {
-      float v = 0.0f;
-      for (int c = 0; c < a.cluster; ++c) {
-        const float mc = a.cluster > 1 ? ld_cluster(sm + row, c) : sm[row];
-        const float oc = a.cluster > 1 ? ld_cluster(so + row * S::O_STRIDE + d, c) : so[row * S::O_STRIDE + d];
-        v = fmaf(oc, exp2f(mc - base), v);
+      float4 part[PA_WARPS];
+      float f[PA_WARPS], s4[PA_WARPS];
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) {
+        f[w] = ld_cluster(sm + w * PA_ROWS + row, c);
+        s4[w] = ld_cluster(sl + w * PA_ROWS + row, c);
+        part[w] = ld_cluster4(so + (w * PA_ROWS + row) * S::O_STRIDE + d, c);
       }
-      if (a.splits > 1) {
-        a.part_o[(static_cast<long long>(part) * PA_ROWS + row) * p.head_dim + d] = v;
-      } else {
-        store_out(a, q.row0, r0 + row, head, d, sum == 0.0f ? 0.0f : v / sum);
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) {
+        const float e = ex2f(f[w] - base);
+        sum = fmaf(s4[w], e, sum);
+        v[0] = fmaf(part[w].x, e, v[0]), v[1] = fmaf(part[w].y, e, v[1]), v[2] = fmaf(part[w].z, e, v[2]), v[3] = fmaf(part[w].w, e, v[3]);
       }
     }
-    if (threadIdx.x == 0) {
-      if (a.splits > 1) a.part_ml[static_cast<long long>(part) * PA_ROWS + row] = make_float2(top, sum);
-      else store_lse(a, q.row0, r0 + row, head, top, sum);
+    if (a.splits > 1) {
+      *reinterpret_cast<float4*>(a.part_o + (static_cast<long long>(part) * PA_ROWS + row) * p.head_dim + d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) a.part_ml[static_cast<long long>(part) * PA_ROWS + row] = make_float2(top, sum);
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      store_out4(a, q.row0, r0 + row, head, d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+      if (d == 0) store_lse(a, q.row0, r0 + row, head, top, sum);
     }
   }
   if (a.cluster > 1) {  // no CTA leaves while others read its shared memory
@@ -534,18 +560,18 @@ Share share_out(const AttendLaunch& a) {
   r.tiles = static_cast<int>((few + PA_ROWS - 1) / PA_ROWS);
   r.units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tiles;
   const long long slots = 2LL * ctx().sm_count;
-  while (r.cluster < 8 && r.units * r.cluster < 4 * slots && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
+  while (r.cluster < 8 && r.units * r.cluster < 3 * slots && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
   while (r.units * r.cluster * r.splits < slots && keys >= 512 * 2 * r.cluster * r.splits) r.splits *= 2;
   if (r.splits > 1) r.bytes = static_cast<size_t>(r.units) * r.splits * PA_ROWS * row_bytes;
   return r;
 }
 
-template <int CT, int NQ, int DP>
+template <int CT, int NQ, int NP, int DP>
 int launch_rows_as(const AttendArgs& a, long long grid, cudaStream_t st) {
-  using S = PagedShape<CT, NQ, DP>;
+  using S = PagedShape<CT, NQ, NP, DP>;
   static PerDeviceOnce once;
   MB_TRY(once.run([]() -> int {
-    MB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<CT, NQ, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    MB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<CT, NQ, NP, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     return MIMIR_B200_OK;
   }));
   cudaLaunchConfig_t cfg = {};
@@ -562,15 +588,22 @@ int launch_rows_as(const AttendArgs& a, long long grid, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  MB_CUDA(cudaLaunchKernelEx(&cfg, paged_attention_kernel<CT, NQ, DP>, a));
+  MB_CUDA(cudaLaunchKernelEx(&cfg, paged_attention_kernel<CT, NQ, NP, DP>, a));
   count_launch();
   return MIMIR_B200_OK;
 }
-template <int CT, int NQ>
+template <int CT, int NQ, int NP>
 int launch_rows_dim(const AttendArgs& a, long long grid, cudaStream_t st) {
-  if (a.p.head_dim <= 64) return launch_rows_as<CT, NQ, 64>(a, grid, st);
-  if (a.p.head_dim <= 128) return launch_rows_as<CT, NQ, 128>(a, grid, st);
-  return launch_rows_as<CT, NQ, 256>(a, grid, st);
+  if (a.p.head_dim <= 64) return launch_rows_as<CT, NQ, NP, 64>(a, grid, st);
+  if (a.p.head_dim <= 128) return launch_rows_as<CT, NQ, NP, 128>(a, grid, st);
+  return launch_rows_as<CT, NQ, NP, 256>(a, grid, st);
+}
+// Queries of fp32 are two terms; probabilities two for results of fp32 or half, one (11 bits) for bfloat16's 8.
+template <int CT>
+int launch_rows_type(const AttendArgs& a, long long grid, cudaStream_t st) {
+  if (a.type == MIMIR_B200_T_F32) return launch_rows_dim<CT, 2, 2>(a, grid, st);
+  if (a.type == MIMIR_B200_T_F16) return launch_rows_dim<CT, 1, 2>(a, grid, st);
+  return launch_rows_dim<CT, 1, 1>(a, grid, st);
 }
 
 }  // namespace
@@ -618,13 +651,12 @@ int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
   if (!r.rows) return MIMIR_B200_OK;
   a.tiles = r.tiles, a.cluster = r.cluster, a.last_first = 0;
   parts(0, r.units, r.splits, PA_ROWS);
-  const bool two = l.type == MIMIR_B200_T_F32;
   switch (l.cache_type) {
-    case MIMIR_B200_T_F32: MB_TRY((launch_rows_dim<MIMIR_B200_T_F32, 2>(a, grid, st))); break;
-    case MIMIR_B200_T_BF16: MB_TRY((launch_rows_dim<MIMIR_B200_T_BF16, 1>(a, grid, st))); break;
-    case MIMIR_B200_T_F16: MB_TRY((two ? launch_rows_dim<MIMIR_B200_T_F16, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_F16, 1>(a, grid, st))); break;
-    case MIMIR_B200_T_I8: MB_TRY((two ? launch_rows_dim<MIMIR_B200_T_I8, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_I8, 1>(a, grid, st))); break;
-    default: MB_TRY((two ? launch_rows_dim<MIMIR_B200_T_E4M3, 2>(a, grid, st) : launch_rows_dim<MIMIR_B200_T_E4M3, 1>(a, grid, st))); break;
+    case MIMIR_B200_T_F32: MB_TRY((launch_rows_dim<MIMIR_B200_T_F32, 2, 2>(a, grid, st))); break;
+    case MIMIR_B200_T_BF16: MB_TRY((launch_rows_dim<MIMIR_B200_T_BF16, 1, 2>(a, grid, st))); break;
+    case MIMIR_B200_T_F16: MB_TRY(launch_rows_type<MIMIR_B200_T_F16>(a, grid, st)); break;
+    case MIMIR_B200_T_I8: MB_TRY(launch_rows_type<MIMIR_B200_T_I8>(a, grid, st)); break;
+    default: MB_TRY(launch_rows_type<MIMIR_B200_T_E4M3>(a, grid, st)); break;
   }
   if (r.splits > 1) MB_TRY(launch_merge(a, r.units, st));
   return MIMIR_B200_OK;

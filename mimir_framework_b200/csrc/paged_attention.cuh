@@ -27,6 +27,11 @@ int launch_paged_attention_tc(const AttendArgs& a, int cache_type, cudaStream_t 
 
 namespace {
 
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
   if constexpr (BF) {
@@ -66,14 +71,10 @@ __device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4], u
       hi[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   } else if constexpr (CT == MIMIR_B200_T_E4M3) {
-    // sign, exponent and mantissa moved to a half's places: the value times 2^-8 (the exponents' biases are 7 and 15), subnormals too;
-    // the codes 0x7f and 0xff (not a number) would be 480
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w = __byte_perm(r.w[i / 2], 0, (i & 1) ? 0x3424 : 0x1404);  // the code in the high byte of each half
-      uint32_t h = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
-      const uint32_t nan = __vcmpeq2(w & 0x7f007f00u, 0x7f007f00u);
-      hi[i] = h | (nan & 0x7e007e00u);
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(r.w[i / 2] >> (16 * (i & 1))), __NV_E4M3);
+      hi[i] = static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
     }
   } else {
 #pragma unroll
@@ -87,6 +88,14 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, int row0, int r, 
   if (a.type == MIMIR_B200_T_F32) static_cast<float*>(a.out)[at] = v;
   else if (a.type == MIMIR_B200_T_F16) static_cast<__half*>(a.out)[at] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+}
+// columns d .. d + 3
+__device__ __forceinline__ void store_out4(const AttendArgs& a, int row0, int r, int kv_head, int d, float v0, float v1, float v2, float v3) {
+  const int tok = r / a.group, h = kv_head * a.group + r - tok * a.group;
+  const long long at = (row0 + tok) * a.o_row + h * a.o_head + d;
+  if (a.type == MIMIR_B200_T_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(v0, v1, v2, v3);
+  else if (a.type == MIMIR_B200_T_F16) *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at) = make_uint2(pack2<false>(v0, v1), pack2<false>(v2, v3));
+  else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = make_uint2(pack2<true>(v0, v1), pack2<true>(v2, v3));
 }
 // top is in base two; a row that saw no key has -infinity
 __device__ __forceinline__ void store_lse(const AttendArgs& a, int row0, int r, int kv_head, float top, float sum) {

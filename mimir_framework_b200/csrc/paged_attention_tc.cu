@@ -39,11 +39,6 @@ struct TcShape {
   static constexpr int THREADS = NT * 128 + 128;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -153,7 +148,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
       up = __uint_as_float(static_cast<uint32_t>(e2) << 23);
       down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
     }
-    c2 = fabsf(a.scale) * LOG2E * up * (CT == MIMIR_B200_T_E4M3 ? 256.0f : 1.0f);
+    c2 = fabsf(a.scale) * LOG2E * up;
     if (a.scale < 0.0f) down = -down;  // (the largest product is then the smallest score's)
     for (int c = 0; c < DP / 8; ++c) {
       float f[8];
@@ -423,7 +418,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
       const bool raise = mx > base + 8.0f || (CODED && grow > v_unit);
       if (__any_sync(0xffffffffu, raise)) {
         const float nb = fmaxf(base, mx);
-        float f = base == -INFINITY ? 0.0f : ex2(base - nb);
+        float f = base == -INFINITY ? 0.0f : ex2f(base - nb);
         sum *= f;
         base = nb;
         if constexpr (CODED) {
@@ -455,7 +450,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
           float e[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            e[n] = ex2(fmaf(__uint_as_float(w[c][i + n]), c2, -sub));
+            e[n] = ex2f(fmaf(__uint_as_float(w[c][i + n]), c2, -sub));
             part[n] += e[n];
           }
           if constexpr (CODED) {
@@ -477,7 +472,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
     if (alive) {
       tcgen05_fence_after();
       const bool there = r < r_end;
-      const float unit_v = (CODED ? v_unit : 1.0f) * (CT == MIMIR_B200_T_E4M3 ? 256.0f : 1.0f);
+      const float unit_v = (CODED ? v_unit : 1.0f);
       const float inv = a.splits > 1 ? unit_v : sum == 0.0f ? 0.0f : unit_v / sum;
       const int h = head * a.group + r - tok * a.group;
       const long long part_row = static_cast<long long>(blockIdx.x) * (NT * TC_ROWS) + t * TC_ROWS + r_local;

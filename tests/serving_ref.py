@@ -126,7 +126,7 @@ def attention(pages, q, scale, causal, window):
     return out, lse, weight, reach
 
 
-def attention_bounds(out, weight, reach, dim, keys, type_, chunk=False):
+def attention_bounds(out, weight, reach, dim, keys, type_, chunk=False, one_half=False):
     """How far a result may be: |d out| and |d lse|.
 
     Score: a term of 22 bits a factor (2^-22 each of two), head_dim / 16 steps of up to three tensor instructions whose truncating sums
@@ -135,12 +135,14 @@ def attention_bounds(out, weight, reach, dim, keys, type_, chunk=False):
     for each block of 16 keys of a warp and each of up to 64 parts that meet (2^-24 each), the sum of probabilities likewise, the division.
     The result's type rounds once.  bfloat16 probabilities are hi + lo, 16 bits: 2^-17.  In chunks of many rows of 16 bits (`chunk`) a
     probability is one number of the cache's 16-bit type (half for 8-bit caches): it is off by half a step of its own, and so is each p |v|.
-    There a bfloat16 query may become a half times its row's largest: 2^-25 of that, less than the terms' 2^-21 of the reach."""
+    So is it by half's, 2^-11, where a bfloat16 result comes from a cache of half or 8 bits (`one_half`).  There a bfloat16 query may become a half times its row's largest: 2^-25 of that, less than the terms' 2^-21 of the reach."""
     score = reach * (2.0**-21 + 3 * math.ceil(dim / 16) * 2.0**-22 + 2.0**-23) * 1.5
     sums = (keys / 16 + 80) * 2.0**-24
     value = (2.0**-17 if type_ == abi.T_BF16 else 2.0**-22) + 6 * 2.0**-22 + 2.0**-21
     if chunk:
         value += half_step(type_)
+    if one_half:
+        value += 2.0**-11
     inner = weight * (2 * score + 2 * sums + value)
     return inner + (np.abs(out) + inner) * half_step(type_) + (2.0**-24 if type_ == abi.T_F16 else 0.0), score[..., 0] + sums + 2.0**-21
 

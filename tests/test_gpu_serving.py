@@ -162,7 +162,8 @@ def check_attention(p, q, out, lse, type_, causal, window):
     want, want_lse, weight, reach = attention(p, q[:n, :, : p.dim].double().cpu().numpy(), 1 / math.sqrt(p.dim), causal, window)
     # bf16 and e4m3 / i8 tensors meet bf16 or half terms; the bound goes by the result's type
     chunk = type_ != F32 and q.shape[1] // p.heads * max(p.rows, default=0) > 64
-    bound, lse_bound = attention_bounds(want, weight, reach, p.dim, max(p.kv, default=0), BF16 if p.type == BF16 else type_, chunk)
+    bound, lse_bound = attention_bounds(want, weight, reach, p.dim, max(p.kv, default=0), BF16 if p.type == BF16 else type_, chunk,
+                                         type_ == BF16 and p.type != BF16)
     err = np.abs(out[:n, :, : p.dim].double().cpu().numpy() - want)
     assert np.all(err <= bound), f"{np.max(err / np.maximum(bound, 1e-300))} of the bound"
     got = lse[:n].double().cpu().numpy()
