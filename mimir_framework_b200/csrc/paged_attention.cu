@@ -169,100 +169,145 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-  // ---- pages of a block's groups of eight keys (a page holds a multiple of eight) ----------------------------------------------------
-  int page_next[NG], slot_next[NG];
-  bool whole_next = false;  // every key of the block is there
-  auto fetch_pages = [&](int b) {
-    whole_next = b * KB >= k_begin && b * KB + KB <= k_end;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      const int key = b * KB + 8 * j;
+  // ---- pages of groups of eight keys (a page holds a multiple of eight): a lane looks one up, 32 of them ahead of their blocks -----------
+  int ahead_page, ahead_slot;  // of this lane's group of the next 32
+  int window = b0 * NG;        // first group of the present 32
+  auto look_up = [&](int first_group) {
+    const int key = (first_group + lane) * 8;
+    ahead_page = -2;  // no key of it is wanted
+    if (first_group + lane < b1 * NG && key < k_end && key + 7 >= k_begin) {
       const int pi = p.by_page.div(key);
-      slot_next[j] = key - pi * p.page_size;
-      page_next[j] = (b < b1 && key < k_end && key + 7 >= k_begin) ? paged_page(p, s, pi) : -1;
+      ahead_slot = key - pi * p.page_size;
+      ahead_page = __ldg(p.table + s * p.table_stride + pi);
     }
   };
-  long long off[NG];   // of a group's first key in the pages, -1: none
-  long long soff[NG];  // and in the scales
-  bool whole = false;
-  auto place_pages = [&]() {
-    whole = whole_next;
+  long long g_off, g_soff;  // where this lane's group begins in the pages and in the scales, -1: nowhere
+  unsigned g_there;         // lanes whose group is somewhere
+  auto take_window = [&]() {
+    g_off = -1;
+    if (static_cast<unsigned>(ahead_page) < static_cast<unsigned>(p.n_pages)) {
+      g_off = ahead_page * p.page_stride + ahead_slot * p.slot_stride + head * p.head_stride;
+      g_soff = (static_cast<long long>(ahead_page) * p.kv_heads + head) * p.page_size + ahead_slot;
+    } else if (ahead_page != -2) {
+      atomicOr(p.flags, PAGED_BAD_PAGE);
+    }
+    g_there = __ballot_sync(0xffffffffu, g_off >= 0);
+    look_up(window + 32);
+  };
+  long long off[NG], soff[NG];
+  unsigned there = 0;   // groups of the block that are somewhere
+  bool whole = false;   // every key of the block is there
+  auto place_pages = [&](int b) {
+    int at = b * NG - window;
+    if (at >= 32) {
+      window += 32, at -= 32;
+      take_window();
+    }
+    there = (g_there >> at) & ((1u << NG) - 1);
+    whole = there == (1u << NG) - 1 && b * KB >= k_begin && b * KB + KB <= k_end;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      whole = whole && page_next[j] >= 0;
-      off[j] = page_next[j] < 0 ? -1 : page_next[j] * p.page_stride + slot_next[j] * p.slot_stride + head * p.head_stride;
-      if constexpr (CODED) soff[j] = (static_cast<long long>(page_next[j]) * p.kv_heads + head) * p.page_size + slot_next[j] + 2 * t;
+      off[j] = __shfl_sync(0xffffffffu, g_off, at + j);
+      if constexpr (CODED) soff[j] = __shfl_sync(0xffffffffu, g_soff, at + j) + 2 * t;
+    }
+    if (at + 3 * NG <= 32) {  // the rows of the block after next, a line a lane
+      constexpr int LINES = DP * type_bytes(CT) > 128 ? DP * type_bytes(CT) / 128 : 1;  // of a row
+#pragma unroll
+      for (int n = 0; n < 2 * KB * LINES / 32; ++n) {
+        const int i = n * 32 + lane, line = i % LINES, key = (i / LINES) % KB, is_v = i / (LINES * KB);
+        const long long row = __shfl_sync(0xffffffffu, g_off, at + 2 * NG + key / 8);
+        const char* src = static_cast<const char*>(is_v ? p.v : p.k) + (row + (key & 7) * p.slot_stride) * type_bytes(CT) + 128 * line;
+        if (row >= 0 && 128 * line < p.head_dim * type_bytes(CT)) asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+      }
     }
   };
   Raw8<CT> kr[NG][UD / 32], vr[KB / 16][4][(UD + 63) / 64];
   float2 ks[NG], vs[NG];
   const long long k_lane = (g * p.slot_stride + 8 * t) * type_bytes(CT), v_lane = (2 * t * p.slot_stride + 8 * g) * type_bytes(CT), row_bytes = p.slot_stride * type_bytes(CT);
+  const bool full_dim = p.head_dim == DP;
   auto load_k = [&](int b, int u) {
+    if (whole && full_dim) {  // (most blocks: nothing to test)
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const char* base = static_cast<const char*>(p.k) + off[j] * type_bytes(CT) + k_lane;
+#pragma unroll
+        for (int c = 0; c < UD / 32; ++c) kr[j][c] = load8<CT>(base + (u * UD + 32 * c) * type_bytes(CT));
+        if (CODED && u == 0) ks[j] = __ldg(reinterpret_cast<const float2*>(p.k_scale + soff[j]));
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const int key = b * KB + 8 * j + g;
-      const bool go = whole || (off[j] >= 0 && key < k_end);
-      const char* base = static_cast<const char*>(p.k) + off[j] * type_bytes(CT) + k_lane + u * UD * type_bytes(CT);
+      const bool go = ((there >> j) & 1) && b * KB + 8 * j + g < k_end;
+      const char* base = static_cast<const char*>(p.k) + off[j] * type_bytes(CT) + k_lane;
 #pragma unroll
       for (int c = 0; c < UD / 32; ++c) {
-        if (go && u * UD + 32 * c + 8 * t < p.head_dim) kr[j][c] = load8<CT>(base + 32 * c * type_bytes(CT));
+        if (go && u * UD + 32 * c + 8 * t < p.head_dim) kr[j][c] = load8<CT>(base + (u * UD + 32 * c) * type_bytes(CT));
         else
 #pragma unroll
           for (uint32_t& w : kr[j][c].w) w = 0;
       }
       if (CODED && u == 0) {
         ks[j] = make_float2(0.0f, 0.0f);
-        if (off[j] >= 0) ks[j] = __ldg(reinterpret_cast<const float2*>(p.k_scale + soff[j]));
+        if ((there >> j) & 1) ks[j] = __ldg(reinterpret_cast<const float2*>(p.k_scale + soff[j]));
       }
     }
   };
   auto load_v = [&](int b, int u) {
-#pragma unroll
-    for (int k16 = 0; k16 < KB / 16; ++k16)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        const int j = 2 * k16 + (i >> 1), key = b * KB + 8 * j + 2 * t + (i & 1);
-        const bool go = whole || (off[j] >= 0 && key < k_end && key >= k_begin);  // (a key that no row sees is zero whatever its slot holds)
-        const char* base = static_cast<const char*>(p.v) + off[j] * type_bytes(CT) + v_lane + ((i & 1) ? row_bytes : 0) + u * UD * type_bytes(CT);
-#pragma unroll
-        for (int c = 0; c < (UD + 63) / 64; ++c) {
-          if (go && u * UD + 64 * c + 8 * g < p.head_dim) vr[k16][i][c] = load8<CT>(base + 64 * c * type_bytes(CT));
-          else
-#pragma unroll
-            for (uint32_t& w : vr[k16][i][c].w) w = 0;
-        }
-      }
-    if (CODED && u == 0) {
+    if (whole && full_dim) {
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const int key = b * KB + 8 * j + 2 * t;
-        vs[j] = make_float2(0.0f, 0.0f);
-        if (off[j] >= 0) vs[j] = __ldg(reinterpret_cast<const float2*>(p.v_scale + soff[j]));
-        if (!whole) {
-          if (key >= k_end || key < k_begin) vs[j].x = 0.0f;
-          if (key + 1 >= k_end || key + 1 < k_begin) vs[j].y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // keys 2 t, 2 t + 1 of the group
+          const char* base = static_cast<const char*>(p.v) + off[j] * type_bytes(CT) + v_lane + (i ? row_bytes : 0);
+#pragma unroll
+          for (int c = 0; c < (UD + 63) / 64; ++c) vr[j / 2][2 * (j & 1) + i][c] = load8<CT>(base + (u * UD + 64 * c) * type_bytes(CT));
         }
+        if (CODED && u == 0) vs[j] = __ldg(reinterpret_cast<const float2*>(p.v_scale + soff[j]));
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int key = b * KB + 8 * j + 2 * t;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool go = ((there >> j) & 1) && key + i < k_end && key + i >= k_begin;  // (a key that no row sees is zero whatever its slot holds)
+        const char* base = static_cast<const char*>(p.v) + off[j] * type_bytes(CT) + v_lane + (i ? row_bytes : 0);
+#pragma unroll
+        for (int c = 0; c < (UD + 63) / 64; ++c) {
+          Raw8<CT>& to = vr[j / 2][2 * (j & 1) + i][c];
+          if (go && u * UD + 64 * c + 8 * g < p.head_dim) to = load8<CT>(base + (u * UD + 64 * c) * type_bytes(CT));
+          else
+#pragma unroll
+            for (uint32_t& w : to.w) w = 0;
+        }
+      }
+      if (CODED && u == 0) {
+        vs[j] = make_float2(0.0f, 0.0f);
+        if ((there >> j) & 1) vs[j] = __ldg(reinterpret_cast<const float2*>(p.v_scale + soff[j]));
+        if (key >= k_end || key < k_begin) vs[j].x = 0.0f;
+        if (key + 1 >= k_end || key + 1 < k_begin) vs[j].y = 0.0f;
       }
     }
   };
 
   float v_unit = 0.0f;  // codes: the power of two that O's values are in
   if (b0 < b1) {
-    fetch_pages(b0);
-    place_pages();
+    look_up(window);
+    take_window();
+    place_pages(b0);
     load_k(b0, 0);
     load_v(b0, 0);
-    fetch_pages(b0 + 1);
   }
   for (int b = b0; b < b1; ++b) {
     // ---- scores ----------------------------------------------------------------------------------------------------------------
     float sc[NG][4];
-    bool there[NG];
+    const unsigned here = there;
     const bool full = whole && b * KB >= all_lo && b * KB + KB <= all_hi;
     float2 ks_now[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      there[j] = off[j] >= 0;
       if constexpr (CODED) ks_now[j] = ks[j];
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
@@ -295,9 +340,8 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     // the next block's keys are on their way while this one's values are used
     if constexpr (NU == 1) {
       if (b + 1 < b1) {
-        place_pages();
+        place_pages(b + 1);
         load_k(b + 1, 0);
-        fetch_pages(b + 2);
       }
     }
     // ---- running maximum and sum -----------------------------------------------------------------------------------------------------
@@ -310,7 +354,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
         if constexpr (CODED) v *= (i & 1) ? ks_now[j].y : ks_now[j].x;
         if (!full) {
           const int key = b * KB + 8 * j + 2 * t + (i & 1);
-          if (!(there[j] && key < lim_hi[i >> 1] && key >= lim_lo[i >> 1])) v = -INFINITY;
+          if (!(((here >> j) & 1) && key < lim_hi[i >> 1] && key >= lim_lo[i >> 1])) v = -INFINITY;
         }
         sc[j][i] = v;
         mx[i >> 1] = fmaxf(mx[i >> 1], v);
@@ -422,9 +466,8 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     }
     if constexpr (NU > 1) {
       if (b + 1 < b1) {
-        place_pages();
+        place_pages(b + 1);
         load_k(b + 1, 0);
-        fetch_pages(b + 2);
       }
     }
     if (b + 1 < b1) load_v(b + 1, 0);

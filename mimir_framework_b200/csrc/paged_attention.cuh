@@ -72,10 +72,8 @@ __device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4], u
     }
   } else if constexpr (CT == MIMIR_B200_T_E4M3) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(r.w[i / 2] >> (16 * (i & 1))), __NV_E4M3);
-      hi[i] = static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-    }
+    for (int i = 0; i < 2; ++i)
+      asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(hi[2 * i]), "=r"(hi[2 * i + 1]) : "r"(r.w[i]));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) hi[i] = r.w[i];
