@@ -82,7 +82,8 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   float* sl = sm + PA_WARPS * PA_ROWS;
   float* sscale = sl + PA_WARPS * PA_ROWS;                           // [16]
   const PagedView& p = a.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // (known to be the same in all lanes: uniform branches)
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = static_cast<int>(blockIdx.x) % a.cluster;
   const int part = static_cast<int>(blockIdx.x) / a.cluster;
   const int split = part % a.splits, unit = part / a.splits;
@@ -210,14 +211,14 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       off[j] = __shfl_sync(0xffffffffu, g_off, at + j);
       if constexpr (CODED) soff[j] = __shfl_sync(0xffffffffu, g_soff, at + j) + 2 * t;
     }
-    if (at + 3 * NG <= 32) {  // the rows of the block after next, a line a lane
+    if (at + 2 * NG <= 32) {  // the next block's rows, a line a lane
       constexpr int LINES = DP * type_bytes(CT) > 128 ? DP * type_bytes(CT) / 128 : 1;  // of a row
 #pragma unroll
       for (int n = 0; n < 2 * KB * LINES / 32; ++n) {
         const int i = n * 32 + lane, line = i % LINES, key = (i / LINES) % KB, is_v = i / (LINES * KB);
-        const long long row = __shfl_sync(0xffffffffu, g_off, at + 2 * NG + key / 8);
+        const long long row = __shfl_sync(0xffffffffu, g_off, at + NG + key / 8);
         const char* src = static_cast<const char*>(is_v ? p.v : p.k) + (row + (key & 7) * p.slot_stride) * type_bytes(CT) + 128 * line;
-        if (row >= 0 && 128 * line < p.head_dim * type_bytes(CT)) asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(row >= 0 && 128 * line < p.head_dim * type_bytes(CT) ? src : static_cast<const char*>(p.k)));
       }
     }
   };
