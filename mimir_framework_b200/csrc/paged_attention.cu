@@ -69,7 +69,7 @@ struct PagedShape {
 };
 
 template <int CT, int NQ, int NP, int DP>
-__global__ void __launch_bounds__(PA_THREADS, (DP > 128 || CT == MIMIR_B200_T_F32 || (DP > 64 && type_bytes(CT) == 1)) ? 2 : 3)
+__global__ void __launch_bounds__(PA_THREADS, DP > 64 ? 2 : 3)
 paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   using S = PagedShape<CT, NQ, NP, DP>;
   constexpr bool BF = S::BF, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3, WIDE = CT == MIMIR_B200_T_F32;
