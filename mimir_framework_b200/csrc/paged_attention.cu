@@ -61,7 +61,7 @@ template <int CT, int NQ, int NP, int DP>  // terms of a query and of a probabil
 struct PagedShape {
   static constexpr bool BF = CT == MIMIR_B200_T_BF16;
   static constexpr bool FRESH = NQ == 2;                                // P V of a block apart from O
-  static constexpr int KB = type_bytes(CT) == 1 ? 32 : 16;              // keys of a block
+  static constexpr int KB = type_bytes(CT) == 1 || (type_bytes(CT) == 2 && DP <= 128) ? 32 : 16;  // keys of a block
   static constexpr int UD = CT == MIMIR_B200_T_F32 ? 64 : DP < 128 ? DP : 128;  // head elements loaded at a time
   static constexpr int Q_BYTES = NQ * (DP / 16) * 32 * 16;
   static constexpr int O_STRIDE = DP + 4;
