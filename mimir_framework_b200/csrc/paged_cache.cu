@@ -35,6 +35,7 @@ struct CacheMove {
   void* v;
   long long row_stride, head_stride;
   int per_cta, group;  // rows of a CTA; lanes of a vector, a power of two
+  FastDiv by_row;      // vectors of a row
 };
 
 template <int CT, int T, bool WRITE>
@@ -76,51 +77,63 @@ __global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_con
   __syncthreads();
   const int lane = threadIdx.x & (a.group - 1), d = lane * 8;
   const bool mine = d < p.head_dim;
-  const int groups = PC_THREADS / a.group, vectors = rows * 2 * p.kv_heads;
-  // (whole warps stay in the loop for the shuffles)
-  for (int i0 = 0; i0 < vectors; i0 += groups) {
-    const int i = i0 + threadIdx.x / a.group;
-    const bool there = i < vectors;
-    const int row = there ? i / (2 * p.kv_heads) : 0, j = there ? i - row * 2 * p.kv_heads : 0;
-    const bool is_v = j >= p.kv_heads;
-    const int head = is_v ? j - p.kv_heads : j;
-    const bool go = there && mine && at[row] >= 0;
-    const long long user = (row0 + row) * a.row_stride + head * a.head_stride + d, slot = at[row] + head * p.head_stride + d;
-    char* mem = static_cast<char*>(is_v ? a.v : a.k) + user * type_bytes(T);
-    char* pool = static_cast<char*>(is_v ? p.v : p.k) + slot * type_bytes(CT);
-    float* scales = is_v ? p.v_scale : p.k_scale;
-    const long long si = scale_at[row] + static_cast<long long>(head) * p.page_size;
-    float f[8];
-    if constexpr (WRITE) {
+  const int groups = PC_THREADS / a.group, per_row = 2 * p.kv_heads, vectors = rows * per_row;
+  // (whole warps stay in the loop for the shuffles; U vectors of a group are on their way together)
+  constexpr int U = 4;
+  for (int i0 = 0; i0 < vectors; i0 += U * groups) {
+    Raw8<WRITE ? T : CT> raw[U];
+    char* to[U];
+    float* scale_of[U];
+    bool go[U];
+    float scale[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-      if (go) unpack8<T>(load8<T>(mem), f);
-      if constexpr (CODED) {
-        float amax = 0.0f;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * groups + threadIdx.x / a.group;
+      const bool there = i < vectors;
+      const int row = there ? a.by_row.div(i) : 0, j = there ? i - row * per_row : 0;
+      const bool is_v = j >= p.kv_heads;
+      const int head = is_v ? j - p.kv_heads : j;
+      go[u] = there && mine && at[row] >= 0;
+      char* mem = static_cast<char*>(is_v ? a.v : a.k) + ((row0 + row) * a.row_stride + head * a.head_stride + d) * type_bytes(T);
+      char* pool = static_cast<char*>(is_v ? p.v : p.k) + (at[row] + head * p.head_stride + d) * type_bytes(CT);
+      scale_of[u] = (is_v ? p.v_scale : p.k_scale) + scale_at[row] + static_cast<long long>(head) * p.page_size;
+      to[u] = WRITE ? pool : mem;
+      if (go[u]) raw[u] = load8<WRITE ? T : CT>(WRITE ? mem : pool);
+      else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = fabsf(f[e]);
-          if (v < INFINITY) amax = fmaxf(amax, v);
+        for (uint32_t& w : raw[u].w) w = 0;
+      if constexpr (!WRITE && CODED) scale[u] = go[u] ? *scale_of[u] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[8];
+      unpack8<WRITE ? T : CT>(raw[u], f);
+      if constexpr (WRITE) {
+        if constexpr (CODED) {
+          float amax = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = fabsf(f[e]);
+            if (v < INFINITY) amax = fmaxf(amax, v);
+          }
+          for (int o = a.group >> 1; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          const float s = __fmul_rn(amax, PART);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            // (a scale of zero: nothing but zeros, infinities and magnitudes whose scale is below fp32's smallest)
+            const float v = s > 0.0f ? __fdiv_rn(f[e], s) : 0.0f;
+            f[e] = CT != MIMIR_B200_T_I8 ? v : v == v ? fmaxf(-TOP, fminf(TOP, v)) : 0.0f;
+          }
+          if (go[u] && lane == 0) *scale_of[u] = s;
         }
-        for (int o = a.group >> 1; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float scale = __fmul_rn(amax, PART);
+        if (go[u]) store8<CT>(to[u], pack8<CT>(f));
+      } else {
+        if constexpr (CODED) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // (a scale of zero: nothing but zeros, infinities and magnitudes whose scale is below fp32's smallest)
-          const float v = scale > 0.0f ? __fdiv_rn(f[e], scale) : 0.0f;
-          f[e] = CT != MIMIR_B200_T_I8 ? v : v == v ? fmaxf(-TOP, fminf(TOP, v)) : 0.0f;
+          for (int e = 0; e < 8; ++e) f[e] *= scale[u];
         }
-        if (go && lane == 0) scales[si] = scale;
+        if (go[u]) store8<T>(to[u], pack8<T>(f));
       }
-      if (go) store8<CT>(pool, pack8<CT>(f));
-    } else if (go) {
-      unpack8<CT>(load8<CT>(pool), f);
-      if constexpr (CODED) {
-        const float scale = scales[si];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= scale;
-      }
-      store8<T>(mem, pack8<T>(f));
     }
   }
 }
@@ -140,6 +153,7 @@ template <bool WRITE>
 int launch_move(CacheMove a, int cache_type, int type, cudaStream_t st) {
   a.group = 1;
   while (a.group * 8 < a.p.head_dim) a.group *= 2;
+  a.by_row = FastDiv(static_cast<uint32_t>(2 * a.p.kv_heads));
   // rows of a CTA: enough for a pass of its threads, and no fewer CTAs than SMs for that
   a.per_cta = 1;
   while (a.per_cta < PC_ROWS && a.rows >= 8LL * ctx().sm_count * a.per_cta) a.per_cta *= 2;

@@ -38,7 +38,18 @@ __device__ __forceinline__ void from_f(float v, float* p) { *p = v; }
 __device__ __forceinline__ void from_f(float v, __half* p) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 
-// A CTA turns `per_cta` rows: their cosines and sines first (one pair serves every head), then all heads.
+// cosines and sines of `rows` rows from row0 on (one pair serves every head)
+__device__ __forceinline__ void angles(const RopeLaunch& r, long long row0, int rows, float2* cs) {
+  const int pairs = r.plan.rot_dim / 2;
+  for (int i = threadIdx.x; i < rows * pairs; i += RO_THREADS) {
+    const int row = i / pairs, pr = i - row * pairs;
+    const float2 v = turn_cos_sin(r.plan.step[pr] * static_cast<uint64_t>(static_cast<long long>(__ldg(r.positions + row0 + row))));
+    cs[i] = make_float2(v.x * r.plan.magnitude, v.y * r.plan.magnitude);
+  }
+  __syncthreads();
+}
+
+// Any sizes, strides and alignment: an element pair, or an element that passes, a thread.
 template <int T>
 __global__ void __launch_bounds__(RO_THREADS) rope_kernel(const __grid_constant__ RopeLaunch r, int per_cta) {
   using E = typename RopeElem<T>::type;
@@ -46,12 +57,7 @@ __global__ void __launch_bounds__(RO_THREADS) rope_kernel(const __grid_constant_
   const int pairs = r.plan.rot_dim / 2;
   const long long row0 = static_cast<long long>(blockIdx.x) * per_cta;
   const int rows = static_cast<int>(min(static_cast<long long>(per_cta), r.rows - row0));
-  for (int i = threadIdx.x; i < rows * pairs; i += RO_THREADS) {
-    const int row = i / pairs, pr = i - row * pairs;
-    float2 v = turn_cos_sin(r.plan.step[pr] * static_cast<uint64_t>(static_cast<long long>(__ldg(r.positions + row0 + row))));
-    cs[i] = make_float2(v.x * r.plan.magnitude, v.y * r.plan.magnitude);
-  }
-  __syncthreads();
+  angles(r, row0, rows, cs);
   const int rest = r.x == r.y ? 0 : r.dim - r.plan.rot_dim;  // elements that pass as they are
   const int per_head = pairs + rest, per_row = per_head * r.heads;
   for (int i = threadIdx.x; i < rows * per_row; i += RO_THREADS) {
@@ -71,20 +77,97 @@ __global__ void __launch_bounds__(RO_THREADS) rope_kernel(const __grid_constant_
   }
 }
 
-}  // namespace
-
-int launch_rope(const RopeLaunch& r, cudaStream_t st) {
+// Eight elements at a time (two loads of fp32): heads, strides and the turned part whole multiples of them, pointers 16-byte aligned.  An
+// item is eight elements: of both halves (INTER false), or eight neighbours (INTER true); or eight that pass.  The bytes bound it, each
+// read and written once; RO_ITEMS items a thread are on their way together, which one at a time did not cover.
+constexpr int RO_ITEMS = 2;
+template <int T, bool INTER>
+__global__ void __launch_bounds__(RO_THREADS) rope_vector_kernel(const __grid_constant__ RopeLaunch r, int per_cta, FastDiv by_row, FastDiv by_head) {
+  extern __shared__ float2 cs[];
   const int pairs = r.plan.rot_dim / 2;
+  const long long row0 = static_cast<long long>(blockIdx.x) * per_cta;
+  const int rows = static_cast<int>(min(static_cast<long long>(per_cta), r.rows - row0));
+  angles(r, row0, rows, cs);
+  const int turned = INTER ? r.plan.rot_dim / 8 : pairs / 8, per_head = static_cast<int>(by_head.d), per_row = static_cast<int>(by_row.d);
+  constexpr int SIZE = type_bytes(T);
+  for (int i0 = threadIdx.x; i0 < rows * per_row; i0 += RO_ITEMS * RO_THREADS) {
+    Raw8<T> a[RO_ITEMS], b[RO_ITEMS];
+    long long at[RO_ITEMS];
+    int angle[RO_ITEMS];
+#pragma unroll
+    for (int u = 0; u < RO_ITEMS; ++u) {
+      const int i = i0 + u * RO_THREADS;
+      angle[u] = -2;
+      if (i >= rows * per_row) continue;
+      const int row = by_row.div(i), j = i - row * per_row, head = by_head.div(j), e = j - head * per_head;
+      const bool pass = e >= turned;
+      const int d = pass ? r.plan.rot_dim + 8 * (e - turned) : 8 * e;
+      const char* x = static_cast<const char*>(r.x) + ((row0 + row) * r.x_row + head * r.x_head + d) * SIZE;
+      at[u] = ((row0 + row) * r.y_row + head * r.y_head + d) * SIZE;
+      angle[u] = pass ? -1 : row * pairs + (INTER ? 4 * e : 8 * e);
+      a[u] = load8<T>(x);
+      if (!INTER && !pass) b[u] = load8<T>(x + pairs * SIZE);
+    }
+#pragma unroll
+    for (int u = 0; u < RO_ITEMS; ++u) {
+      if (angle[u] == -2) continue;
+      char* y = static_cast<char*>(r.y) + at[u];
+      if (angle[u] >= 0) {
+        float f[8], g[8];
+        unpack8<T>(a[u], f);
+        if constexpr (INTER) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 t = cs[angle[u] + e];
+            g[2 * e] = f[2 * e] * t.x - f[2 * e + 1] * t.y;
+            g[2 * e + 1] = f[2 * e] * t.y + f[2 * e + 1] * t.x;
+          }
+          a[u] = pack8<T>(g);
+        } else {
+          unpack8<T>(b[u], g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 t = cs[angle[u] + e];
+            const float p = f[e] * t.x - g[e] * t.y;
+            g[e] = f[e] * t.y + g[e] * t.x;
+            f[e] = p;
+          }
+          a[u] = pack8<T>(f);
+          store8<T>(y + pairs * SIZE, pack8<T>(g));
+        }
+      }
+      store8<T>(y, a[u]);
+    }
+  }
+}
+
+template <int T>
+int launch_rope_as(const RopeLaunch& r, cudaStream_t st) {
+  const int pairs = r.plan.rot_dim / 2, rest = r.x == r.y ? 0 : r.dim - r.plan.rot_dim;
+  const bool inter = r.plan.interleaved != 0;
+  auto whole = [](long long v) { return v % 8 == 0; };
+  const bool vector = whole(inter ? r.plan.rot_dim : pairs) && whole(rest) && whole(r.plan.rot_dim) && whole(r.x_row) && whole(r.x_head) && whole(r.y_row) &&
+                      whole(r.y_head) && reinterpret_cast<uintptr_t>(r.x) % 16 == 0 && reinterpret_cast<uintptr_t>(r.y) % 16 == 0;
+  const int per_row = r.heads * (vector ? (inter ? r.plan.rot_dim : pairs) / 8 + rest / 8 : pairs + rest);
+  // rows of a CTA: for a few items a thread, and no fewer CTAs than fill the SMs
   int per_cta = 1;
-  while (per_cta < 4 && r.rows >= 4LL * ctx().sm_count * per_cta) per_cta *= 2;
-  const long long grid = (r.rows + per_cta - 1) / per_cta;
+  while (per_cta < 8 && r.rows >= 8LL * ctx().sm_count * per_cta && per_cta * per_row < 4 * RO_THREADS) per_cta *= 2;
+  const unsigned grid = static_cast<unsigned>((r.rows + per_cta - 1) / per_cta);
   const size_t smem = static_cast<size_t>(per_cta) * pairs * sizeof(float2);
-  if (r.type == MIMIR_B200_T_F32) rope_kernel<MIMIR_B200_T_F32><<<static_cast<unsigned>(grid), RO_THREADS, smem, st>>>(r, per_cta);
-  else if (r.type == MIMIR_B200_T_F16) rope_kernel<MIMIR_B200_T_F16><<<static_cast<unsigned>(grid), RO_THREADS, smem, st>>>(r, per_cta);
-  else rope_kernel<MIMIR_B200_T_BF16><<<static_cast<unsigned>(grid), RO_THREADS, smem, st>>>(r, per_cta);
+  if (!vector) rope_kernel<T><<<grid, RO_THREADS, smem, st>>>(r, per_cta);
+  else if (inter) rope_vector_kernel<T, true><<<grid, RO_THREADS, smem, st>>>(r, per_cta, FastDiv(per_row), FastDiv(per_row / r.heads));
+  else rope_vector_kernel<T, false><<<grid, RO_THREADS, smem, st>>>(r, per_cta, FastDiv(per_row), FastDiv(per_row / r.heads));
   MB_CUDA(cudaGetLastError());
   count_launch();
   return MIMIR_B200_OK;
+}
+
+}  // namespace
+
+int launch_rope(const RopeLaunch& r, cudaStream_t st) {
+  if (r.type == MIMIR_B200_T_F32) return launch_rope_as<MIMIR_B200_T_F32>(r, st);
+  if (r.type == MIMIR_B200_T_F16) return launch_rope_as<MIMIR_B200_T_F16>(r, st);
+  return launch_rope_as<MIMIR_B200_T_BF16>(r, st);
 }
 
 }  // namespace mb
