@@ -15,6 +15,7 @@ namespace {
 constexpr int PC_THREADS = 256;
 constexpr int PC_ROWS = 32;     // most rows a CTA looks up
 constexpr int PC_STARTS = 1024;  // sequence starts kept in shared memory
+constexpr int PC_HEADS = 32;     // heads of a CTA
 
 // the last s of 0 .. n with start[s] <= row, -1 if none (starts ascend; entries that do not are found out by the caller)
 __device__ __forceinline__ int last_start(const int* start, int n, int row) {
@@ -35,8 +36,19 @@ struct CacheMove {
   void* v;
   long long row_stride, head_stride;
   int per_cta, group;  // rows of a CTA; lanes of a vector, a power of two
-  FastDiv by_row;      // vectors of a row
+  FastDiv by_full, by_rest;  // vectors of a row of PC_HEADS heads, and of the last ones'
 };
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Codes of f / s, correctly rounded quotients by one reciprocal for all of them: with r = 1 / s rounded to nearest, q = f r and
 // q + (f - q s) r with fused multiply-adds is the IEEE quotient (Markstein, IBM J. Res. Dev. 34, 1990), where nothing under- or overflows:
@@ -68,10 +80,14 @@ __global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_con
   constexpr bool CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3;
   constexpr float TOP = CT == MIMIR_B200_T_I8 ? 127.0f : 448.0f, PART = 1.0f / TOP;
   __shared__ int starts[PC_STARTS];
-  __shared__ long long at[PC_ROWS];     // of a row's slot in the pages, -1: the row is none of a sequence
-  __shared__ long long scale_at[PC_ROWS];
+  // in bytes: a row's slot in the pages (-1: the row is none of a sequence) and in the scales, and where it begins in the tensors; then the
+  // same of a head, keys before values, from the pointers on (64-bit products a vector took a third of the instructions)
+  __shared__ long long at[PC_ROWS], scale_at[PC_ROWS], row_at[PC_ROWS];
+  __shared__ char *pool_of[2 * PC_HEADS], *mem_of[2 * PC_HEADS];
+  __shared__ float* scales_of[2 * PC_HEADS];
   const PagedView& p = a.p;
   const int row0 = blockIdx.x * a.per_cta, rows = min(a.per_cta, a.rows - row0);
+  const int head0 = blockIdx.y * PC_HEADS, heads = min(PC_HEADS, p.kv_heads - head0), per_row = 2 * heads;
   const bool kept = p.n_seqs < PC_STARTS;
   if (kept) {
     for (int i = threadIdx.x; i <= p.n_seqs; i += PC_THREADS) starts[i] = __ldg(a.start + i);
@@ -91,18 +107,27 @@ __global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_con
       } else if (pos >= 0 && pos < kv) {
         const int pi = p.by_page.div(pos), slot = pos - pi * p.page_size, page = paged_page(p, s, pi);
         if (page >= 0) {
-          where = page * p.page_stride + slot * p.slot_stride;
+          where = (page * p.page_stride + slot * p.slot_stride) * type_bytes(CT);
           sc = static_cast<long long>(page) * p.kv_heads * p.page_size + slot;
         }
       }
     }
     at[threadIdx.x] = where;
     scale_at[threadIdx.x] = sc;
+    row_at[threadIdx.x] = row * a.row_stride * type_bytes(T);
+  } else if (threadIdx.x >= 64 && static_cast<int>(threadIdx.x) - 64 < per_row) {
+    const int j = threadIdx.x - 64;
+    const bool is_v = j >= heads;
+    const long long head = head0 + (is_v ? j - heads : j);
+    pool_of[j] = static_cast<char*>(is_v ? p.v : p.k) + head * p.head_stride * type_bytes(CT);
+    mem_of[j] = static_cast<char*>(is_v ? a.v : a.k) + head * a.head_stride * type_bytes(T);
+    if constexpr (CODED) scales_of[j] = (is_v ? p.v_scale : p.k_scale) + head * p.page_size;
   }
   __syncthreads();
   const int lane = threadIdx.x & (a.group - 1), d = lane * 8;
   const bool mine = d < p.head_dim;
-  const int groups = PC_THREADS / a.group, per_row = 2 * p.kv_heads, vectors = rows * per_row;
+  const int groups = PC_THREADS / a.group, vectors = rows * per_row;
+  const FastDiv by_row = heads == PC_HEADS ? a.by_full : a.by_rest;
   // (whole warps stay in the loop for the shuffles; U vectors of a group are on their way together)
   constexpr int U = 4;
   for (int i0 = 0; i0 < vectors; i0 += U * groups) {
@@ -115,13 +140,12 @@ __global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_con
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * groups + threadIdx.x / a.group;
       const bool there = i < vectors;
-      const int row = there ? a.by_row.div(i) : 0, j = there ? i - row * per_row : 0;
-      const bool is_v = j >= p.kv_heads;
-      const int head = is_v ? j - p.kv_heads : j;
-      go[u] = there && mine && at[row] >= 0;
-      char* mem = static_cast<char*>(is_v ? a.v : a.k) + ((row0 + row) * a.row_stride + head * a.head_stride + d) * type_bytes(T);
-      char* pool = static_cast<char*>(is_v ? p.v : p.k) + (at[row] + head * p.head_stride + d) * type_bytes(CT);
-      scale_of[u] = (is_v ? p.v_scale : p.k_scale) + scale_at[row] + static_cast<long long>(head) * p.page_size;
+      const int row = there ? by_row.div(i) : 0, j = there ? i - row * per_row : 0;
+      const long long slot = at[row];
+      go[u] = there && mine && slot >= 0;
+      char* mem = mem_of[j] + row_at[row] + d * type_bytes(T);
+      char* pool = pool_of[j] + slot + d * type_bytes(CT);
+      if constexpr (CODED) scale_of[u] = scales_of[j] + scale_at[row];
       to[u] = WRITE ? pool : mem;
       if (go[u]) raw[u] = load8<WRITE ? T : CT>(WRITE ? mem : pool);
       else
@@ -135,10 +159,10 @@ __global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_con
       unpack8<WRITE ? T : CT>(raw[u], f);
       if constexpr (WRITE) {
         if constexpr (CODED) {
-          float amax = 0.0f, odd = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e])), odd = fmaf(f[e], 0.0f, odd);
-          const bool finite = !__any_sync(0xffffffffu, odd != 0.0f);  // (not a number: an infinity or none is there)
+          // (a maximum of not a number is one)
+          float amax = fmaxf(max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max3_nan(f[6], f[7], f[7])),
+                             -min3_nan(min3_nan(f[0], f[1], f[2]), min3_nan(f[3], f[4], f[5]), min3_nan(f[6], f[7], f[7])));
+          const bool finite = !__any_sync(0xffffffffu, !(amax < INFINITY));
           if (!finite) {
             amax = 0.0f;
 #pragma unroll
@@ -177,7 +201,7 @@ __global__ void __launch_bounds__(PC_THREADS) cache_move_kernel(const __grid_con
 
 template <bool WRITE, int CT>
 int launch_move_as(const CacheMove& a, int type, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>((a.rows + a.per_cta - 1) / a.per_cta);
+  const dim3 grid(static_cast<unsigned>((a.rows + a.per_cta - 1) / a.per_cta), static_cast<unsigned>((a.p.kv_heads + PC_HEADS - 1) / PC_HEADS));
   if (type == MIMIR_B200_T_F32) cache_move_kernel<CT, MIMIR_B200_T_F32, WRITE><<<grid, PC_THREADS, 0, st>>>(a);
   else if (type == MIMIR_B200_T_F16) cache_move_kernel<CT, MIMIR_B200_T_F16, WRITE><<<grid, PC_THREADS, 0, st>>>(a);
   else cache_move_kernel<CT, MIMIR_B200_T_BF16, WRITE><<<grid, PC_THREADS, 0, st>>>(a);
@@ -190,7 +214,8 @@ template <bool WRITE>
 int launch_move(CacheMove a, int cache_type, int type, cudaStream_t st) {
   a.group = 1;
   while (a.group * 8 < a.p.head_dim) a.group *= 2;
-  a.by_row = FastDiv(static_cast<uint32_t>(2 * a.p.kv_heads));
+  a.by_full = FastDiv(2 * PC_HEADS);
+  a.by_rest = FastDiv(static_cast<uint32_t>(2 * ((a.p.kv_heads - 1) % PC_HEADS + 1)));
   // rows of a CTA: enough for a pass of its threads, and no fewer CTAs than SMs for that
   a.per_cta = 1;
   while (a.per_cta < PC_ROWS && a.rows >= 8LL * ctx().sm_count * a.per_cta) a.per_cta *= 2;
