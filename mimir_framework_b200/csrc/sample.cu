@@ -391,7 +391,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       cluster.sync();
       return sh.found;
     };
-    auto sort = [&](int size) {  // sh.list, descending
+    // sh.list, descending; by the first warp alone (of 64) where `few` says so: a block's barrier a step is most of a short sort
+    auto sort = [&](int size, bool few) {
       for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
           for (int i = tid; i < size / 2; i += SA_THREADS) {
@@ -399,11 +400,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
             const u64 a0 = sh.list[p], a1 = sh.list[p | j];
             if ((a0 < a1) == ((p & k) == 0)) sh.list[p] = a1, sh.list[p | j] = a0;
           }
-          __syncthreads();
+          if (few) __syncwarp();
+          else __syncthreads();
         }
     };
-    // what `pick` says yes to into the first CTA's list; true there, whose list is filled up with zeros to a power of two
-    int size = 32;
+    // what `pick` says yes to into the first CTA's list, filled up there with zeros to a power of two from 64 on; the number, elsewhere -1
+    int size = 64;
     auto collect = [&](auto&& pick) {
       SampleShared* home = cluster.map_shared_rank(&sh, 0);
       for (int i = tid; i < vecs; i += SA_THREADS) {
@@ -418,15 +420,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         }
       }
       cluster.sync();
-      if (rank != 0) return false;
+      if (rank != 0) return -1;
       const int have = static_cast<int>(min(sh.list_n, static_cast<uint32_t>(SA_LIST)));
       while (size < have) size *= 2;
       for (int i = tid; i < SA_LIST; i += SA_THREADS)
         if (i >= have) sh.list[i] = 0;
       __syncthreads();
       if (tid == 0) sh.list_n = 0;
-      sort(size);
-      return true;
+      return have;
     };
 
     // The border among the logits of orders range_lo .. range_hi, and of the interval f.bin where `number` says so (f: what lies ahead of
@@ -460,7 +461,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         x_lo = value_of(range_lo), x_hi = value_of(range_hi);
       }
       if (f.in_n <= SA_LIST && shift != 0) {
-        if (collect(member)) {
+        if (collect(member) >= 0) {
+          sort(size, false);
           // a thread has two neighbours of the sorted list
           const uint32_t o0 = static_cast<uint32_t>(sh.list[2 * tid] >> 32), o1 = static_cast<uint32_t>(sh.list[2 * tid + 1] >> 32);
           const u64 w0 = o0 ? weigh(value_of(o0)) : 0, w1 = o1 ? weigh(value_of(o1)) : 0;
@@ -498,13 +500,22 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     };
     // The few down to top_k's interval, in the first CTA: top_k, top_p and min_p in the sorted list, then u in index order.
     auto finish = [&](int last) {
-      if (!collect([&](float v) { return v > -INFINITY && interval(v) <= last; })) return;
+      const int have = collect([&](float v) { return v > -INFINITY && interval(v) <= last; });
+      const bool few = have <= 64;
+      if (have < 0 || (few && warp)) return;
+      auto scan = [&](u64 v, u64* total) {
+        if (!few) return block_scan(v, sh.scan64, total);
+        const u64 inc = warp_scan(v, lane);
+        *total = __shfl_sync(0xffffffffu, inc, 31);
+        return inc - v;
+      };
+      sort(size, few);
       const u64 e0 = sh.list[2 * tid], e1 = sh.list[2 * tid + 1];
       const uint32_t o0 = static_cast<uint32_t>(e0 >> 32), o1 = static_cast<uint32_t>(e1 >> 32);
       const uint32_t most = static_cast<uint32_t>(top_k);
       const u64 w0 = o0 && 2u * tid < most ? weigh(value_of(o0)) : 0, w1 = o1 && 2u * tid + 1 < most ? weigh(value_of(o1)) : 0;
       u64 all, limit = ~0ull;
-      const u64 b0 = block_scan(w0 + w1, sh.scan64, &all);
+      const u64 b0 = scan(w0 + w1, &all);
       if (by_mass) {
         const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all));
         limit = part >= 1.0 ? static_cast<u64>(part) : 1ull;
@@ -513,11 +524,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       // index order: the kept ones by their index's complement, descending
       sh.list[2 * tid] = k0 ? (e0 << 32) | o0 : 0;
       sh.list[2 * tid + 1] = k1 ? (e1 << 32) | o1 : 0;
-      __syncthreads();
-      sort(size);
+      if (few) __syncwarp();
+      else __syncthreads();
+      sort(size, few);
       const u64 i0 = sh.list[2 * tid], i1 = sh.list[2 * tid + 1];
       const u64 x0 = i0 ? weigh(value_of(static_cast<uint32_t>(i0))) : 0, x1 = i1 ? weigh(value_of(static_cast<uint32_t>(i1))) : 0;
-      const u64 at = block_scan(x0 + x1, sh.scan64, &all);
+      const u64 at = scan(x0 + x1, &all);
       u64 until = static_cast<u64>(floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(all)));
       if (until >= all) until = all - 1;
       auto take = [&](u64 item, u64 from, u64 w) {
