@@ -93,12 +93,12 @@ struct SampleShared {
   double table[64];
   uint32_t count[SA_BINS], mass_lo[SA_BINS], mass_hi[SA_BINS];  // of this CTA's slice
   u64 list[SA_LIST];  // order in the high half; below it the index's complement where indices matter
+  u64 weight[256];
   uint32_t list_n;
   u64 scan64[33];
   uint32_t scan32[33];
   // read by the cluster's other CTAs
   int first;
-  uint32_t total_n;
   u64 total;
   Found found;
   Border border;
@@ -173,6 +173,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   __shared__ SampleShared sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  auto meet = [&]() {  // all threads of the row
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+  };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n;
   const long long row = blockIdx.x / ranks;
   const char* x = static_cast<const char*>(a.x) + row * a.row_stride * type_bytes(T);
@@ -263,26 +267,31 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     if (mm > -INFINITY) s = s * ex2f(fmaxf((m - mm) * s2, -200.0f)) + os * ex2f(fmaxf((om - mm) * s2, -200.0f));
     m = mm;
   };
+  auto join_warp = [&]() {
+    if (sum_now) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, rough, o);
-    join(top, rough, om, os);
-  }
+      for (int o = 16; o; o >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, rough, o);
+        join(top, rough, om, os);
+      }
+    } else {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  };
+  join_warp();
   if (tid < 64) sh.table[tid] = powers.v[tid];
   if (tid == 0) sh.list_n = 0;
   if (lane == 0) sh.warp_top[warp] = top, sh.warp_sum[warp] = rough;
-  cluster.sync();
+  meet();
   {  // every warp joins the parts of all
     top = -INFINITY, rough = 0.0f;
     for (int i = lane; i < ranks * SA_WARPS; i += 32) {
       const SampleShared* s = cluster.map_shared_rank(&sh, i / SA_WARPS);
-      join(top, rough, s->warp_top[i % SA_WARPS], s->warp_sum[i % SA_WARPS]);
+      if (sum_now) join(top, rough, s->warp_top[i % SA_WARPS], s->warp_sum[i % SA_WARPS]);
+      else top = fmaxf(top, s->warp_top[i % SA_WARPS]);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, rough, o);
-      join(top, rough, om, os);
-    }
+    join_warp();
   }
 
   if (top == -INFINITY || top == INFINITY || !(t > 0.0f)) {  // the largest's first index, or none
@@ -300,13 +309,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     if (tid == 0) sh.first = 0x7fffffff;
     __syncthreads();
     if (lane == 0) atomicMin(&sh.first, at);
-    cluster.sync();
+    meet();
     if (rank == 0 && tid == 0) {
       for (int c = 0; c < ranks; ++c) at = min(at, *cluster.map_shared_rank(&sh.first, c));
       a.ids[row] = top == -INFINITY ? -1 : at;
       if (a.logprob) a.logprob[row] = top == -INFINITY ? -INFINITY : 0.0f;
     }
-    cluster.sync();  // (no CTA leaves while others read its shared memory)
+    meet();  // (no CTA leaves while others read its shared memory)
     return;
   }
   int room = 0;  // n <= 2^room
@@ -316,9 +325,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   weigh.scale = sh.scale;
   weigh.one = static_cast<double>(1ull << min(62 - room, 51));
   {
-    // 600 powers of two down; where that is no smaller float, every other logit is further down than that
-    float low = static_cast<float>(fmax(static_cast<double>(top) - 415.888 * static_cast<double>(t), -3.4028234e38));
-    if ((static_cast<double>(top) - low) * weigh.scale > 900.0 || low >= top) {
+    // some 600 powers of two down; where no float is about there, every other logit is further down than that
+    float low = fmaxf(top - 415.888f * t, -3.4028234e38f);
+    const float down = (top - low) * s2;
+    if (!(down < 900.0f) || low >= top) {
       low = fmaxf(value_of(order_of(top) - 1), -3.4028235e38f);
       weigh.scale = fmin(weigh.scale, 600.0 / (static_cast<double>(top) - low));
     }
@@ -333,7 +343,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   Border border = {0, 0, 0};
   if (by_count || by_mass) {
     const float width = static_cast<float>(32.0 * weigh.scale);  // of (max - x), in intervals
-    const int share = SA_BINS / ranks;                           // intervals that this CTA adds up
     // rounded in the low bits of 2^23 + it; what is not a number is in the last one
     auto interval = [&](float v) { return static_cast<int>(__float_as_uint(fminf((top - v) * width, SA_BINS - 1.0f) + 8388608.0f) & (2 * SA_BINS - 1)); };
     auto add_mass = [&](int bin, u64 w) {
@@ -341,8 +350,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + lo < old ? 1u : 0u);
       if (hi) atomicAdd(&sh.mass_hi[bin], hi);
     };
+    bool cleared = false;
     auto clear = [&]() {
-      __syncthreads();
+      if (cleared) meet();  // (others have read what is cleared)
+      else __syncthreads();
+      cleared = true;
       for (int i = tid; i < SA_BINS; i += SA_THREADS) sh.count[i] = sh.mass_lo[i] = sh.mass_hi[i] = 0;
       if (tid == 0) sh.found.bin = -1, sh.window[0] = sh.window[1] = SA_BINS - 1;
       __syncthreads();
@@ -350,49 +362,34 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     // the interval in which the candidates reach want_n in number, or `want` in mass, counted from (above_n, above)
     u64 want = 0;
     auto find = [&](bool number, uint32_t want_n, uint32_t above_n, u64 above) {
-      cluster.sync();
+      meet();
       u64 m[2] = {0, 0};
       uint32_t c[2] = {0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = 2 * tid + h;
-        if (i >= share) continue;
-        for (int q = 0; q < ranks; ++q) {
-          const SampleShared* s = cluster.map_shared_rank(&sh, q);
-          c[h] += s->count[rank * share + i];
-          if (!number) m[h] += (static_cast<u64>(s->mass_hi[rank * share + i]) << 32) + s->mass_lo[rank * share + i];
+      for (int q = 0; q < ranks; ++q) {
+        const SampleShared* s = cluster.map_shared_rank(&sh, q);
+        const uint2 n2 = *reinterpret_cast<const uint2*>(s->count + 2 * tid);
+        c[0] += n2.x, c[1] += n2.y;
+        if (!number) {
+          const uint2 lo = *reinterpret_cast<const uint2*>(s->mass_lo + 2 * tid), hi = *reinterpret_cast<const uint2*>(s->mass_hi + 2 * tid);
+          m[0] += (static_cast<u64>(hi.x) << 32) + lo.x, m[1] += (static_cast<u64>(hi.y) << 32) + lo.y;
         }
       }
       u64 all = 0, mb = 0;
       uint32_t all_n;
       if (!number) mb = block_scan(m[0] + m[1], sh.scan64, &all);
       uint32_t cb = block_scan(c[0] + c[1], sh.scan32, &all_n);
-      if (tid == 0) sh.total = all, sh.total_n = all_n;
-      cluster.sync();
-      for (int q = 0; q < rank; ++q) {
-        const SampleShared* s = cluster.map_shared_rank(&sh, q);
-        mb += s->total, cb += s->total_n;
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int i = 2 * tid + h;
-        if (i < share && c[h] > 0) {
-          const u64 ahead = above + mb;
-          const uint32_t ahead_n = above_n + cb;
-          if (number ? ahead_n < want_n && ahead_n + c[h] >= want_n : ahead < want && ahead + m[h] >= want) {
-            Found f;
-            f.bin = rank * share + i;
-            f.above = ahead, f.above_n = ahead_n, f.in = m[h], f.in_n = c[h];
-            for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->found = f;
-          }
-        }
+        const u64 ahead = above + mb;
+        const uint32_t ahead_n = above_n + cb;
+        if (c[h] > 0 && (number ? ahead_n < want_n && ahead_n + c[h] >= want_n : ahead < want && ahead + m[h] >= want))
+          sh.found = {2 * tid + h, ahead_n, c[h], ahead, m[h]};
         mb += m[h], cb += c[h];
       }
-      cluster.sync();
+      __syncthreads();
       return sh.found;
     };
-    // sh.list, descending; by the first warp alone (of 64) where `few` says so: a block's barrier a step is most of a short sort
-    auto sort = [&](int size, bool few) {
+    auto sort = [&](int size) {  // sh.list, descending
       for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
           for (int i = tid; i < size / 2; i += SA_THREADS) {
@@ -400,8 +397,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
             const u64 a0 = sh.list[p], a1 = sh.list[p | j];
             if ((a0 < a1) == ((p & k) == 0)) sh.list[p] = a1, sh.list[p | j] = a0;
           }
-          if (few) __syncwarp();
-          else __syncthreads();
+          __syncthreads();
         }
     };
     // what `pick` says yes to into the first CTA's list, filled up there with zeros to a power of two from 64 on; the number, elsewhere -1
@@ -419,7 +415,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
           }
         }
       }
-      cluster.sync();
+      meet();
       if (rank != 0) return -1;
       const int have = static_cast<int>(min(sh.list_n, static_cast<uint32_t>(SA_LIST)));
       while (size < have) size *= 2;
@@ -462,7 +458,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       }
       if (f.in_n <= SA_LIST && shift != 0) {
         if (collect(member) >= 0) {
-          sort(size, false);
+          sort(size);
           // a thread has two neighbours of the sorted list
           const uint32_t o0 = static_cast<uint32_t>(sh.list[2 * tid] >> 32), o1 = static_cast<uint32_t>(sh.list[2 * tid + 1] >> 32);
           const u64 w0 = o0 ? weigh(value_of(o0)) : 0, w1 = o1 ? weigh(value_of(o1)) : 0;
@@ -483,7 +479,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
           test(2 * tid, b0, n0, w0);
           test(2 * tid + 1, b0 + w0, n0 + 1, w1);
         }
-        cluster.sync();
+        meet();
         border = *cluster.map_shared_rank(&sh.border, 0);
       } else {
         // one order alone
@@ -501,37 +497,69 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
     // The few down to top_k's interval, in the first CTA: top_k, top_p and min_p in the sorted list, then u in index order.
     auto finish = [&](int last) {
       const int have = collect([&](float v) { return v > -INFINITY && interval(v) <= last; });
-      const bool few = have <= 64;
-      if (have < 0 || (few && warp)) return;
-      auto scan = [&](u64 v, u64* total) {
-        if (!few) return block_scan(v, sh.scan64, total);
-        const u64 inc = warp_scan(v, lane);
-        *total = __shfl_sync(0xffffffffu, inc, 31);
-        return inc - v;
+      if (have < 0) return;
+      const uint32_t most = static_cast<uint32_t>(top_k);
+      auto limit_of = [&](u64 all) {
+        if (!by_mass) return ~0ull;
+        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all));
+        return part >= 1.0 ? static_cast<u64>(part) : 1ull;
       };
-      sort(size, few);
+      auto until_of = [&](u64 all) {
+        const u64 until = static_cast<u64>(floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(all)));
+        return until >= all ? all - 1 : until;
+      };
+      if (size <= 256) {
+        // each with each, several threads a logit: how many and how much are ahead of it, then how much is before it by index (a sort
+        // by one warp took 5000 cycles for 64)
+        const int parts = SA_THREADS / size, item = tid / parts, part = tid % parts, per = size / parts;
+        if (tid < size) sh.weight[tid] = sh.list[tid] ? weigh(value_of(static_cast<uint32_t>(sh.list[tid] >> 32))) : 0;
+        __syncthreads();
+        const u64 mine_l = sh.list[item], w = sh.weight[item];
+        u64 ahead = 0;
+        uint32_t rank_l = 0;
+        for (int j = 0; j < per; ++j) {
+          const int i = j * parts + part;
+          if (sh.list[i] > mine_l) ++rank_l, ahead += sh.weight[i];
+        }
+        for (int o = parts >> 1; o; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o), rank_l += __shfl_xor_sync(0xffffffffu, rank_l, o);
+        const uint32_t last_rank = min(most, static_cast<uint32_t>(have)) - 1;
+        if (mine_l && rank_l == last_rank && part == 0) sh.above = ahead + w;
+        __syncthreads();
+        const u64 kept = mine_l && rank_l <= last_rank && ahead < limit_of(sh.above) && w >= least ? w : 0;
+        if (part == 0) sh.weight[item] = kept;
+        __syncthreads();
+        u64 before = 0, all = 0;
+        for (int j = 0; j < per; ++j) {
+          const int i = j * parts + part;
+          const u64 o = sh.weight[i];
+          all += o;
+          if (static_cast<uint32_t>(sh.list[i]) > static_cast<uint32_t>(mine_l)) before += o;  // (the index's complement)
+        }
+        for (int o = parts >> 1; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o), before += __shfl_xor_sync(0xffffffffu, before, o);
+        const u64 until = until_of(all);
+        if (part == 0 && before <= until && until < before + kept) {
+          a.ids[row] = static_cast<int>(~static_cast<uint32_t>(mine_l));
+          if (a.logprob) a.logprob[row] = log_share(kept, all);
+        }
+        return;
+      }
+      sort(size);
       const u64 e0 = sh.list[2 * tid], e1 = sh.list[2 * tid + 1];
       const uint32_t o0 = static_cast<uint32_t>(e0 >> 32), o1 = static_cast<uint32_t>(e1 >> 32);
-      const uint32_t most = static_cast<uint32_t>(top_k);
       const u64 w0 = o0 && 2u * tid < most ? weigh(value_of(o0)) : 0, w1 = o1 && 2u * tid + 1 < most ? weigh(value_of(o1)) : 0;
-      u64 all, limit = ~0ull;
-      const u64 b0 = scan(w0 + w1, &all);
-      if (by_mass) {
-        const double part = ceil(fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(all));
-        limit = part >= 1.0 ? static_cast<u64>(part) : 1ull;
-      }
+      u64 all;
+      const u64 b0 = block_scan(w0 + w1, sh.scan64, &all);
+      const u64 limit = limit_of(all);
       const bool k0 = o0 && 2u * tid < most && b0 < limit && w0 >= least, k1 = o1 && 2u * tid + 1 < most && b0 + w0 < limit && w1 >= least;
       // index order: the kept ones by their index's complement, descending
       sh.list[2 * tid] = k0 ? (e0 << 32) | o0 : 0;
       sh.list[2 * tid + 1] = k1 ? (e1 << 32) | o1 : 0;
-      if (few) __syncwarp();
-      else __syncthreads();
-      sort(size, few);
+      __syncthreads();
+      sort(size);
       const u64 i0 = sh.list[2 * tid], i1 = sh.list[2 * tid + 1];
       const u64 x0 = i0 ? weigh(value_of(static_cast<uint32_t>(i0))) : 0, x1 = i1 ? weigh(value_of(static_cast<uint32_t>(i1))) : 0;
-      const u64 at = scan(x0 + x1, &all);
-      u64 until = static_cast<u64>(floor(fmin(fmax(static_cast<double>(u), 0.0), 1.0) * static_cast<double>(all)));
-      if (until >= all) until = all - 1;
+      const u64 at = block_scan(x0 + x1, sh.scan64, &all);
+      const u64 until = until_of(all);
       auto take = [&](u64 item, u64 from, u64 w) {
         if (!(from <= until && until < from + w)) return;
         a.ids[row] = static_cast<int>(~static_cast<uint32_t>(item >> 32));
@@ -568,7 +596,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
 #pragma unroll
         for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == 0) sh.warp_sum[warp] = v;
-        cluster.sync();
+        meet();
         v = 0.0f;
         for (int i = lane; i < ranks * SA_WARPS; i += 32) v += cluster.map_shared_rank(&sh, i / SA_WARPS)->warp_sum[i % SA_WARPS];
 #pragma unroll
@@ -602,34 +630,25 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
           if (bin < cut && v[e] >= from) atomicAdd(&sh.mass_lo[bin], w);
         }
       }
-      cluster.sync();
+      meet();
       {
         u64 m[2] = {0, 0}, all;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int i = 2 * tid + h;
-          if (i >= share) continue;
-          for (int q = 0; q < ranks; ++q) m[h] += cluster.map_shared_rank(&sh, q)->mass_lo[rank * share + i];
+        for (int q = 0; q < ranks; ++q) {
+          const uint2 lo = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sh, q)->mass_lo + 2 * tid);
+          m[0] += lo.x, m[1] += lo.y;
         }
         u64 ahead = block_scan(m[0] + m[1], sh.scan64, &all);
-        if (tid == 0) sh.total = all;
-        cluster.sync();
-        for (int q = 0; q < rank; ++q) ahead += cluster.map_shared_rank(&sh, q)->total;
         const double near = static_cast<double>(top_p) * 0x1p30;
         const double low = near - 0x1p20, high = near + 0x1p20;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = 2 * tid + h;
           const double b = static_cast<double>(ahead), e = static_cast<double>(ahead + m[h]);
-          if (i < share) {
-            if (rank * share + i == 0 ? e >= low : b < low && e >= low)
-              for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->window[0] = rank * share + i;
-            if (b < high && e >= high)
-              for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&sh, q)->window[1] = rank * share + i;
-          }
+          if (i == 0 ? e >= low : b < low && e >= low) sh.window[0] = i;
+          if (b < high && e >= high) sh.window[1] = i;
           ahead += m[h];
         }
-        cluster.sync();
+        __syncthreads();
       }
       const int bin0 = sh.window[0], bin1 = sh.window[1];
       // min_p ends before top_p does: top_p takes nothing away
@@ -661,7 +680,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         if (tid == 0) sh.above = sh.inside = sh.total = 0, sh.inside_n = 0;
         __syncthreads();
         if (lane == 0) atomicAdd(&sh.above, ahead), atomicAdd(&sh.inside, in), atomicAdd(&sh.total, all), atomicAdd(&sh.inside_n, in_n);
-        cluster.sync();
+        meet();
         Found f = {0, 0, 0, 0, 0};
         all = 0;
         for (int q = 0; q < ranks; ++q) {
@@ -682,7 +701,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       }
     }
     if (done) {
-      cluster.sync();  // (no CTA leaves while others read its shared memory)
+      meet();  // (no CTA leaves while others read its shared memory)
       return;
     }
   }
@@ -720,7 +739,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
   const u64 mass_inc = warp_scan(mass, lane);
   const uint32_t ties_inc = warp_scan(ties, lane);
   if (lane == 31) sh.warp_mass[warp] = mass_inc, sh.warp_ties[warp] = ties_inc;
-  cluster.sync();
+  meet();
   u64 tie_w = border.order ? weigh(value_of(border.order)) : 0;
   if (tie_w < least) tie_w = 0;
   const uint32_t allowed = border.ties;
@@ -778,7 +797,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       if (run > until) break;
     }
   }
-  cluster.sync();
+  meet();
 }
 
 template <int T, bool KEPT>
