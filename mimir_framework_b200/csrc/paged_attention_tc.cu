@@ -7,7 +7,8 @@
 //   warps 0-3, 4-7   softmax of row tile 0 and 1: a thread has a row, reads its 128 scores from tensor memory and writes the probabilities
 //                    back over them as 16-bit pairs, from where P V reads them (A operand in tensor memory)
 //   warp 8           issues the tensor instructions: per key tile P_0 V, Q_0 K', P_1 V, Q_1 K' (K' the next tile)
-//   warps 9-11       bring K and V tiles out of the pages into a ring, rows found through the page table, 8-bit codes as halves
+//   warps 9-11       bring K and V tiles out of the pages into a ring: by TMA, a box of a page's slots a lane (copies a thread each took 6300
+//                    cycles a key tile, twice what everything else did); 8-bit codes through registers, as halves
 // Heads of over 128 elements have one tile of 128 rows (O takes 256 columns of tensor memory) and two score tiles that alternate.
 // K and V tiles lie in the same layout, [64 elements][key] rows of 128 swizzled bytes: K-major for Q K^T, MN-major for P V.
 // The running maximum is raised only when a score outgrows it by 2^8, so O in tensor memory is rescaled a few times a row.
@@ -44,12 +45,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {  // zeros where there is nothing
-  const int n = there ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// (64 elements, slots, head, page)
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // MN-major operand of 64-element columns `column` bytes apart, 16 keys (two groups of eight 128-byte rows) an instruction
 __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t column) {
@@ -57,9 +58,15 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t column) {
          (1ull << 46) | (2ull << 61);
 }
 
+// Tensor maps of the pages for 16-bit caches: boxes of `slots` slots, a power of two that divides a page, and of one.
+struct PageMaps {
+  CUtensorMap k, v, v_row;
+  int slots;
+};
+
 template <int DP, int CT>
 __global__ void __launch_bounds__(TcShape<DP, CT>::THREADS, 1)
-paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
+paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ PageMaps maps) {
   using S = TcShape<DP, CT>;
   constexpr bool BF = S::BF, CODED = S::CODED;
   constexpr int NT = S::NT, NS = S::NS, TILE = S::TILE, SUB = S::SUB;
@@ -98,7 +105,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(kv_full + i, TC_LOADERS);
+      mbar_init(kv_full + i, CODED ? TC_LOADERS : 1);
       mbar_init(kv_empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -170,98 +177,130 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
     // ---- loaders -----------------------------------------------------------------------------------------------------------------------------
     const int id = static_cast<int>(threadIdx.x) - (NT * 128 + 32);
     const uint32_t ring_at = smem_u32(ring);
-    bool ok = true, pending = false;
-    for (int j = 0; j < n_kt; ++j) {  // (a thread whose wait gave up keeps coming to the barrier)
-      const int key0 = (kt0 + j) * TC_KEYS;
-      long long* at = offs + (j & 1) * TC_KEYS;
-      float* sc = scales + (j % (NS / 2)) * 2 * TC_KEYS;
-      long long scale_at[2] = {-1, -1};
+    if constexpr (!CODED) {
+      // one warp brings keys, one values; box x of a tile is (slots of a page, 64 elements)
+      const int kv = warp - (NT * 4 + 1), boxes = TC_KEYS / maps.slots;
+      int issued = 0;
+      for (int j = 0; j < n_kt && kv < 2; ++j) {
+        const int i = 2 * j + kv, st = i % NS, key0 = (kt0 + j) * TC_KEYS;
+        constexpr int ROUNDS = SUB > 2 ? SUB / 2 : 1;  // (boxes * SUB <= 16 * SUB)
+        int page[ROUNDS], slot[ROUNDS];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int k = id + i * TC_LOADERS, key = key0 + k;
-        if (k < TC_KEYS) {
-          long long where = -1;
-          if (key >= k_begin && key < k_end) {
-            const int pi = p.by_page.div(key), slot = key - pi * p.page_size, page = paged_page(p, s, pi);
-            if (page >= 0) {
-              where = page * p.page_stride + slot * p.slot_stride + head * p.head_stride;
-              scale_at[i] = (static_cast<long long>(page) * p.kv_heads + head) * p.page_size + slot;
-            } else {
-              *missing = 1;
-            }
+        for (int n = 0; n < ROUNDS; ++n) {
+          const int x = n * 32 + lane, key = key0 + x % boxes * maps.slots;
+          page[n] = p.n_pages, slot[n] = 0;  // (outside the map: zeros)
+          if (x < boxes * SUB && key < k_end && key + maps.slots > k_begin) {
+            const int pi = p.by_page.div(key), found = paged_page(p, s, pi);
+            slot[n] = key - pi * p.page_size;
+            if (found >= 0) page[n] = found;
+            else *missing = 1;
           }
-          at[k] = where;
         }
+        if (!mbar_wait_warp(kv_empty + st, static_cast<uint32_t>((i / NS) & 1) ^ 1, abort_flag, a.err_word, 61)) break;
+        if (lane == 0) mbar_expect_tx(kv_full + st, TILE);
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < ROUNDS; ++n) {
+          const int x = n * 32 + lane, bx = x % boxes, sub = x / boxes, key = key0 + bx * maps.slots;
+          if (x >= boxes * SUB) continue;
+          const uint32_t dst = ring_at + st * TILE + sub * (TC_KEYS * 128) + bx * maps.slots * 128;
+          if (kv == 0) {
+            tma_load_4d(dst, &maps.k, kv_full + st, 64 * sub, slot[n], head, page[n]);
+          } else if (page[n] == p.n_pages || (key >= k_begin && key + maps.slots <= k_end)) {
+            tma_load_4d(dst, &maps.v, kv_full + st, 64 * sub, slot[n], head, page[n]);
+          } else {  // (a value that no row sees must be zero whatever its slot holds)
+            for (int r = 0; r < maps.slots; ++r)
+              tma_load_4d(dst + r * 128, &maps.v_row, kv_full + st, 64 * sub, slot[n] + r, head, key + r >= k_begin && key + r < k_end ? page[n] : p.n_pages);
+          }
+        }
+        __syncwarp();
+        issued = j + 1;
       }
-      __syncwarp();
-      asm volatile("barrier.sync 1, 96;" ::: "memory");
+      if (*abort_flag && kv < 2) {  // a wait gave up: nothing may still be on its way into shared memory when the block ends
+        int still = 0;
+        for (int j = max(0, issued - NS / 2); j < issued; ++j)
+          mbar_wait_warp(kv_full + (2 * j + kv) % NS, static_cast<uint32_t>(((2 * j + kv) / NS) & 1), &still, a.err_word, 61);
+      }
+    } else {
+      // a tile's codes are on their way in registers while the one before it becomes halves
+      constexpr int N = (TC_KEYS * (DP / 8) + TC_LOADERS - 1) / TC_LOADERS;
+      Raw8<CT> raw[N];
+      long long scale_at[2] = {-1, -1};
+      auto find_rows = [&](int j) {
+        const int key0 = (kt0 + j) * TC_KEYS;
+        long long* at = offs + (j & 1) * TC_KEYS;
 #pragma unroll
-      for (int kv = 0; kv < 2 && ok; ++kv) {
-        const int i = 2 * j + kv, st = i % NS;
-        const uint32_t round = static_cast<uint32_t>((i / NS) & 1) ^ 1;
-        if (!CODED && pending && !mbar_test(kv_empty + st, round)) {
-          // no stage free: the tile on its way is handed over first (what frees a stage may be waiting for it)
-          copies_wait<0>();
-          fence_proxy_async_smem();
-          mbar_arrive(kv_full + (i - 1) % NS);
-          pending = false;
-        }
-        if (!mbar_wait(kv_empty + st, round, abort_flag, a.err_word, 61)) { ok = false; break; }
-        const uint32_t dst = ring_at + st * TILE;
-        const char* src = static_cast<const char*>(kv ? p.v : p.k);
-        if constexpr (!CODED) {
-          // the copies of one tile are on their way while the next one's are issued; a tile is handed over when its own are there
-#pragma unroll 4
-          for (int x = id; x < TC_KEYS * (DP / 8); x += TC_LOADERS) {
-            const int k = x / (DP / 8), c = x % (DP / 8);
-            const bool there = at[k] >= 0 && 8 * c < p.head_dim;
-            copy16(dst + (c >> 3) * (TC_KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), there ? src + (at[k] + 8 * c) * 2 : src, there);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          if (pending) {
-            copies_wait<1>();
-            fence_proxy_async_smem();
-            mbar_arrive(kv_full + (i - 1) % NS);
-          }
-          pending = true;
-        } else {
-          constexpr int U = 4;
-          for (int x0 = id; x0 < TC_KEYS * (DP / 8); x0 += U * TC_LOADERS) {
-            Raw8<CT> raw[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int x = x0 + u * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
-              raw[u].w[0] = raw[u].w[1] = 0;
-              if (k < TC_KEYS && at[k] >= 0 && 8 * c < p.head_dim) raw[u] = load8<CT>(src + at[k] + 8 * c);
+        for (int i = 0; i < 2; ++i) {
+          const int k = id + i * TC_LOADERS, key = key0 + k;
+          scale_at[i] = -1;
+          if (k < TC_KEYS) {
+            long long where = -1;
+            if (key >= k_begin && key < k_end) {
+              const int pi = p.by_page.div(key), slot = key - pi * p.page_size, page = paged_page(p, s, pi);
+              if (page >= 0) {
+                where = page * p.page_stride + slot * p.slot_stride + head * p.head_stride;
+                scale_at[i] = (static_cast<long long>(page) * p.kv_heads + head) * p.page_size + slot;
+              } else {
+                *missing = 1;
+              }
             }
+            at[k] = where;
+          }
+        }
+        __syncwarp();
+        asm volatile("barrier.sync 1, 96;" ::: "memory");
+      };
+      auto fetch = [&](int j, int kv) {
+        const long long* at = offs + (j & 1) * TC_KEYS;
+        const char* src = static_cast<const char*>(kv ? p.v : p.k);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int x = x0 + u * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
+        for (int n = 0; n < N; ++n) {
+          const int x = id + n * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
+          raw[n].w[0] = raw[n].w[1] = 0;
+          if (k < TC_KEYS && at[k] >= 0 && 8 * c < p.head_dim) raw[n] = load8<CT>(src + at[k] + 8 * c);
+        }
+      };
+      bool ok = true;
+      if (n_kt > 0) {
+        find_rows(0);
+        fetch(0, 0);
+      }
+      for (int j = 0; j < n_kt; ++j) {  // (a thread whose wait gave up keeps coming to the barrier)
+        float* sc = scales + (j % (NS / 2)) * 2 * TC_KEYS;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int i = 2 * j + kv, st = i % NS;
+          if (ok) ok = mbar_wait(kv_empty + st, static_cast<uint32_t>((i / NS) & 1) ^ 1, abort_flag, a.err_word, 61);
+          if (ok) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              const int x = id + n * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
               uint32_t hi[4], lo[4];
-              to_pairs<CT>(raw[u], hi, lo);
+              to_pairs<CT>(raw[n], hi, lo);
               if (k < TC_KEYS)
                 *reinterpret_cast<uint4*>(ring + st * TILE + (c >> 3) * (TC_KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             }
-          }
-          if (kv) {  // both scales with the values, whose stage is let go of last
+            if (kv) {  // both scales with the values, whose stage is let go of last
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const int k = id + n * TC_LOADERS;
-              if (k < TC_KEYS) {
-                sc[k] = scale_at[n] >= 0 ? __ldg(p.k_scale + scale_at[n]) : 0.0f;
-                sc[TC_KEYS + k] = scale_at[n] >= 0 ? __ldg(p.v_scale + scale_at[n]) : 0.0f;
+              for (int n = 0; n < 2; ++n) {
+                const int k = id + n * TC_LOADERS;
+                if (k < TC_KEYS) {
+                  sc[k] = scale_at[n] >= 0 ? __ldg(p.k_scale + scale_at[n]) : 0.0f;
+                  sc[TC_KEYS + k] = scale_at[n] >= 0 ? __ldg(p.v_scale + scale_at[n]) : 0.0f;
+                }
               }
             }
+            fence_proxy_async_smem();
+            mbar_arrive(kv_full + st);
           }
-          fence_proxy_async_smem();
-          mbar_arrive(kv_full + st);
+          if (kv == 0) {
+            fetch(j, 1);
+          } else if (j + 1 < n_kt) {
+            find_rows(j + 1);
+            fetch(j + 1, 0);
+          }
         }
       }
-    }
-    if constexpr (!CODED) {
-      copies_wait<0>();
-      fence_proxy_async_smem();
-      if (ok && pending) mbar_arrive(kv_full + (2 * n_kt - 1) % NS);
     }
   } else if (warp == NT * 4) {
     // ---- tensor instructions -------------------------------------------------------------------------------------------------------------------
@@ -517,6 +556,28 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a) {
   }
 }
 
+// 4-D map over the pages of a 16-bit cache: (element, slot, head, page), boxes of 64 elements and `slots` slots, 128-byte swizzle
+int make_page_map(CUtensorMap* map, const PagedView& p, const void* base, int slots) {
+  using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  if (!fn) return fail(MIMIR_B200_E_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  auto bytes = [](int extent, long long stride) { return static_cast<cuuint64_t>(extent > 1 ? stride * 2 : 16); };  // (one of a kind has no stride)
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.head_dim), static_cast<cuuint64_t>(p.page_size), static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.n_pages)};
+  cuuint64_t strides[3] = {bytes(p.page_size, p.slot_stride), bytes(p.kv_heads, p.head_stride), bytes(p.n_pages, p.page_stride)};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(slots), 1, 1};
+  cuuint32_t step[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MIMIR_B200_E_UNSUPPORTED, "paged_attention: no tensor map over these pages (%d)", static_cast<int>(r));
+  return MIMIR_B200_OK;
+}
+
 template <int DP, int CT>
 int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
   using S = TcShape<DP, CT>;
@@ -526,7 +587,15 @@ int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
     return MIMIR_B200_OK;
   }));
   const long long grid = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * a.tiles * a.splits;
-  paged_attention_tc_kernel<DP, CT><<<static_cast<unsigned>(grid), S::THREADS, S::SMEM, st>>>(a);
+  PageMaps maps = {};
+  if constexpr (!S::CODED) {
+    maps.slots = 8;
+    while (maps.slots < TC_KEYS && a.p.page_size % (2 * maps.slots) == 0) maps.slots *= 2;
+    MB_TRY(make_page_map(&maps.k, a.p, a.p.k, maps.slots));
+    MB_TRY(make_page_map(&maps.v, a.p, a.p.v, maps.slots));
+    MB_TRY(make_page_map(&maps.v_row, a.p, a.p.v, 1));
+  }
+  paged_attention_tc_kernel<DP, CT><<<static_cast<unsigned>(grid), S::THREADS, S::SMEM, st>>>(a, maps);
   MB_CUDA(cudaGetLastError());
   count_launch();
   return MIMIR_B200_OK;

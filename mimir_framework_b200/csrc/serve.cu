@@ -49,6 +49,9 @@ int check_sizes(const char* what, const MimirPagedCache* c, const MimirPagedBatc
   if (c->head_dim % 8 || c->head_dim > 256) return fail(MIMIR_B200_E_UNSUPPORTED, "%s: head_dim %d is not a multiple of 8 up to 256", what, c->head_dim);
   if (c->page_stride % 8 || c->slot_stride % 8 || c->head_stride % 8 || c->page_stride < 0 || c->slot_stride < 0 || c->head_stride < 0)
     return fail(MIMIR_B200_E_UNSUPPORTED, "%s: cache strides are multiples of 8 elements", what);
+  if ((c->page_size > 1 && c->slot_stride == 0) || (c->kv_heads > 1 && c->head_stride == 0) || (c->n_pages > 1 && c->page_stride == 0) ||
+      c->page_stride >= (1LL << 38) || c->slot_stride >= (1LL << 38) || c->head_stride >= (1LL << 38))
+    return fail(MIMIR_B200_E_UNSUPPORTED, "%s: cache strides are positive and below 2^38 elements", what);
   if (b->n_seqs < 0 || b->n_rows < 0 || b->max_rows < 0 || b->max_kv < 0 || b->table_stride < 0)
     return fail(MIMIR_B200_E_INVALID, "%s: a negative size in the batch", what);
   return MIMIR_B200_OK;
