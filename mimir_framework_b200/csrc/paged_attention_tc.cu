@@ -15,6 +15,7 @@
 // Probabilities of a bfloat16 cache are rounded to bfloat16 (8 bits, relative to each probability), else to half (11 bits); their sum is
 // of the unrounded ones, in fp32.  Scores, maxima, sums and O are fp32.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "launch.cuh"
@@ -52,6 +53,37 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                : "memory");
 }
 
+// pairs of fp32 in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// 2^x on the FMA lanes, for x of at most 127 (below -126: 2^-126): x = n + f, |f| <= 1/2, and the polynomial of fourth degree in f whose
+// largest relative error is least (2.6e-6, by Remez' exchange); n goes into the exponent.  A share of the exponentials done so leaves the
+// special-function lanes, 16 a cycle and SM, less to do.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // (-126; what is not a number stays so)
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float2 m = add2(x, make_float2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: n in the low bits
+  const float2 n = add2(m, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 p = fma2(f, make_float2(9.5701021e-3f, 9.5701021e-3f), make_float2(5.5917859e-2f, 5.5917859e-2f));
+  p = fma2(p, f, make_float2(0.24024744f, 0.24024744f));
+  p = fma2(p, f, make_float2(0.69312179f, 0.69312179f));
+  p = fma2(p, f, make_float2(0.99999928f, 0.99999928f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(m.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(m.y) << 23)));
+}
+
 // MN-major operand of 64-element columns `column` bytes apart, 16 keys (two groups of eight 128-byte rows) an instruction
 __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t column) {
   return static_cast<uint64_t>((saddr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(column >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
@@ -81,8 +113,9 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   float* scales = reinterpret_cast<float*>(ring + NS * TILE);
   long long* offs = reinterpret_cast<long long*>(ring + NS * TILE + S::SCALES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * TILE + S::SCALES + S::OFFS);
-  uint64_t *kv_full = bars, *kv_empty = bars + NS, *s_full = bars + 2 * NS /*[2]*/, *p_full = s_full + 2 /*[2]*/, *pv_done = s_full + 4 /*[2]*/, *drained = s_full + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 7);
+  uint64_t *kv_full = bars, *kv_empty = bars + NS, *s_full = bars + 2 * NS /*[2]*/, *p_full = s_full + 2 /*[2]*/, *p_half = s_full + 4 /*[2]*/,
+           *pv_done = s_full + 6 /*[2]*/, *drained = s_full + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 9);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* missing = abort_flag + 1;  // the loaders met a page outside the cache
 
@@ -111,6 +144,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 4);
+      mbar_init(p_half + i, 4);
       mbar_init(pv_done + i, 1);
     }
     mbar_init(drained, 1);
@@ -318,12 +352,15 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       }
       __syncwarp();
     };
-    auto values = [&](int tt, int j) {  // O_tt (+)= P V_j
+    auto values = [&](int tt, int j, int half) {  // O_tt (+)= P V_j, 64 keys
       const uint32_t v_at = ring_at + ((2 * j + 1) % NS) * TILE, pa = tmem + (NT == 2 ? tt : (j & 1)) * TC_KEYS, d = tmem_o + tt * DP;
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < TC_KEYS / 16; ++k) umma_f16_ts(d, pa + 8 * k, desc_mn(v_at + k * 2048, TC_KEYS * 128), idesc_o, (j | k) != 0 ? 1u : 0u);
-        umma_commit(pv_done + tt);
+        for (int n = 0; n < TC_KEYS / 32; ++n) {
+          const int k = half * (TC_KEYS / 32) + n;
+          umma_f16_ts(d, pa + 8 * k, desc_mn(v_at + k * 2048, TC_KEYS * 128), idesc_o, (j | k) != 0 ? 1u : 0u);
+        }
+        if (half) umma_commit(pv_done + tt);
       }
       __syncwarp();
     };
@@ -336,8 +373,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       tcgen05_fence_after();
       return ok;
     };
-    auto ready = [&](int tt, int j) {
-      const bool ok = mbar_wait_warp(p_full + (NT == 2 ? tt : (j & 1)), static_cast<uint32_t>((NT == 2 ? j : j >> 1) & 1), abort_flag, a.err_word, 64);
+    auto ready = [&](int tt, int j, uint64_t* bar) {
+      const bool ok = mbar_wait_warp(bar + (NT == 2 ? tt : (j & 1)), static_cast<uint32_t>((NT == 2 ? j : j >> 1) & 1), abort_flag, a.err_word, 64);
       tcgen05_fence_after();
       return ok;
     };
@@ -350,10 +387,13 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       const bool more = j + 1 < n_kt;
       if constexpr (NT == 2) {
         for (int tt = 0; tt < tiles_here && ok; ++tt) {
-          ok = ready(tt, j);
+          ok = ready(tt, j, p_half);
           if (ok && tt == 0) ok = full(2 * j + 1, 63);
           if (!ok) break;
-          values(tt, j);
+          values(tt, j, 0);
+          ok = ready(tt, j, p_full);
+          if (!ok) break;
+          values(tt, j, 1);
           if (tt == tiles_here - 1) release(2 * j + 1);
           if (more) {
             if (tt == 0) ok = full(2 * j + 2, 62);
@@ -369,9 +409,12 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           scores(0, j + 1);
           release(2 * j + 2);
         }
-        ok = ready(0, j) && full(2 * j + 1, 63);
+        ok = ready(0, j, p_half) && full(2 * j + 1, 63);
         if (!ok) break;
-        values(0, j);
+        values(0, j, 0);
+        ok = ready(0, j, p_full);
+        if (!ok) break;
+        values(0, j, 1);
         release(2 * j + 1);
       }
     }
@@ -417,6 +460,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
             w[c][i + 3] = __float_as_uint(__uint_as_float(w[c][i + 3]) * k4.w);
           }
       }
+      const bool masked = key0 < all_lo || key0 + TC_KEYS > all_hi || *missing;
       if (key0 < all_lo || key0 + TC_KEYS > all_hi) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -438,12 +482,12 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
             }
           }
       }
-      float mx = -INFINITY;
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int i = 0; i < 32; i += 2)
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) mx = max3(mx, __uint_as_float(w[c][i]), __uint_as_float(w[c][i + 1]));
-      mx *= c2;
+        for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(w[c][i]), __uint_as_float(w[c][i + 1]));
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2;
       float grow = 0.0f;
       if constexpr (CODED) {
         float top = 0.0f;
@@ -480,33 +524,44 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         }
       }
       const float sub = base == -INFINITY ? 0.0f : base, inv_unit = CODED ? 1.0f / v_unit : 1.0f;
-      float part[4] = {};
+      float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      const float2 cc = make_float2(c2, c2), ss = make_float2(-sub, -sub);
+      // the probabilities, half of the keys at a time: P V of the first half runs while the second is computed
+      auto weigh_keys = [&](auto few_special) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float e[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            e[n] = ex2f(fmaf(__uint_as_float(w[c][i + n]), c2, -sub));
-            part[n] += e[n];
+          for (int i = 0; i < 32; i += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(w[c][i]), __uint_as_float(w[c][i + 1])), cc, ss);
+            // (keys behind a mask need an exact zero: they take the special function)
+            float2 e = decltype(few_special)::value && (i & 7) == 6 ? exp2_poly(x) : make_float2(ex2f(x.x), ex2f(x.y));
+            part[(i >> 1) & 1] = add2(part[(i >> 1) & 1], e);
+            if constexpr (CODED) {
+              const float2 v2 = *reinterpret_cast<const float2*>(sc + TC_KEYS + 32 * c + i);
+              e.x *= v2.x * inv_unit, e.y *= v2.y * inv_unit;
+            }
+            pk[i / 2] = pack2<BF>(e.x, e.y);
           }
-          if constexpr (CODED) {
-            const float4 v4 = *reinterpret_cast<const float4*>(sc + TC_KEYS + 32 * c + i);
-            e[0] *= v4.x * inv_unit, e[1] *= v4.y * inv_unit, e[2] *= v4.z * inv_unit, e[3] *= v4.w * inv_unit;
+          tmem_st_32x16(ts + 16 * c, pk);
+          if (c == 1) {
+            tmem_wait_st();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_half + buf);
           }
-          pk[i / 2] = pack2<BF>(e[0], e[1]);
-          pk[i / 2 + 1] = pack2<BF>(e[2], e[3]);
         }
-        tmem_st_32x16(ts + 16 * c, pk);
-      }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      };
+      if (masked) weigh_keys(std::false_type());
+      else weigh_keys(std::true_type());
+      sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + buf);
     }
+    // the last P V, and with two score tiles the one before it first (a barrier two phases behind looks complete)
+    if (NT == 1 && alive && n_kt > 1) alive = mbar_wait_warp(pv_done, static_cast<uint32_t>(n_kt - 2) & 1, abort_flag, a.err_word, 69);
     if (alive && n_kt > 0) alive = mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(n_kt - 1) & 1, abort_flag, a.err_word, 69);
     if (alive) {
       tcgen05_fence_after();
