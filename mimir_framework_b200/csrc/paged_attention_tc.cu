@@ -27,6 +27,7 @@ namespace mb {
 namespace {
 
 constexpr int TC_LOADERS = 96, TC_TMEM = 512;
+constexpr int TC_POLY = 6;  // of eight exponentials the last two go to the FMA lanes (none: 2 % more time, of four the last two: 9 %)
 
 template <int DP, int CT>
 struct TcShape {
@@ -113,9 +114,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   float* scales = reinterpret_cast<float*>(ring + NS * TILE);
   long long* offs = reinterpret_cast<long long*>(ring + NS * TILE + S::SCALES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * TILE + S::SCALES + S::OFFS);
-  uint64_t *kv_full = bars, *kv_empty = bars + NS, *s_full = bars + 2 * NS /*[2]*/, *p_full = s_full + 2 /*[2]*/, *p_half = s_full + 4 /*[2]*/,
-           *pv_done = s_full + 6 /*[2]*/, *drained = s_full + 8;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 9);
+  uint64_t *kv_full = bars, *kv_empty = bars + NS, *s_full = bars + 2 * NS /*[2]*/, *p_full = s_full + 2 /*[2]*/, *pv_done = s_full + 4 /*[2]*/, *drained = s_full + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 7);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* missing = abort_flag + 1;  // the loaders met a page outside the cache
 
@@ -144,7 +144,6 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 4);
-      mbar_init(p_half + i, 4);
       mbar_init(pv_done + i, 1);
     }
     mbar_init(drained, 1);
@@ -342,25 +341,24 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     const uint32_t q_at = smem_u32(sq), ring_at = smem_u32(ring);
     auto scores = [&](int tt, int j) {  // S = Q_tt K_j^T
       const uint32_t k_at = ring_at + ((2 * j) % NS) * TILE, d = tmem + (NT == 2 ? tt : (j & 1)) * TC_KEYS;
+      const uint64_t q_desc = make_smem_desc(q_at + tt * TILE, 128), k_desc = make_smem_desc(k_at, 128);
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t o = (k >> 2) * (TC_KEYS * 128) + (k & 3) * 32;
-          umma_bf16(d, make_smem_desc(q_at + tt * TILE + o, 128), make_smem_desc(k_at + o, 128), idesc_s, k != 0 ? 1u : 0u);
+          const uint64_t o = ((k >> 2) * (TC_KEYS * 128) + (k & 3) * 32) >> 4;
+          umma_bf16(d, q_desc + o, k_desc + o, idesc_s, k != 0 ? 1u : 0u);
         }
         umma_commit(s_full + (NT == 2 ? tt : (j & 1)));
       }
       __syncwarp();
     };
-    auto values = [&](int tt, int j, int half) {  // O_tt (+)= P V_j, 64 keys
+    auto values = [&](int tt, int j) {  // O_tt (+)= P V_j
       const uint32_t v_at = ring_at + ((2 * j + 1) % NS) * TILE, pa = tmem + (NT == 2 ? tt : (j & 1)) * TC_KEYS, d = tmem_o + tt * DP;
+      const uint64_t v_desc = desc_mn(v_at, TC_KEYS * 128);
       if (elect_one()) {
 #pragma unroll
-        for (int n = 0; n < TC_KEYS / 32; ++n) {
-          const int k = half * (TC_KEYS / 32) + n;
-          umma_f16_ts(d, pa + 8 * k, desc_mn(v_at + k * 2048, TC_KEYS * 128), idesc_o, (j | k) != 0 ? 1u : 0u);
-        }
-        if (half) umma_commit(pv_done + tt);
+        for (int k = 0; k < TC_KEYS / 16; ++k) umma_f16_ts(d, pa + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+        umma_commit(pv_done + tt);
       }
       __syncwarp();
     };
@@ -373,8 +371,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       tcgen05_fence_after();
       return ok;
     };
-    auto ready = [&](int tt, int j, uint64_t* bar) {
-      const bool ok = mbar_wait_warp(bar + (NT == 2 ? tt : (j & 1)), static_cast<uint32_t>((NT == 2 ? j : j >> 1) & 1), abort_flag, a.err_word, 64);
+    auto ready = [&](int tt, int j) {
+      const bool ok = mbar_wait_warp(p_full + (NT == 2 ? tt : (j & 1)), static_cast<uint32_t>((NT == 2 ? j : j >> 1) & 1), abort_flag, a.err_word, 64);
       tcgen05_fence_after();
       return ok;
     };
@@ -387,13 +385,9 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       const bool more = j + 1 < n_kt;
       if constexpr (NT == 2) {
         for (int tt = 0; tt < tiles_here && ok; ++tt) {
-          ok = ready(tt, j, p_half);
-          if (ok && tt == 0) ok = full(2 * j + 1, 63);
+          ok = (tt > 0 || full(2 * j + 1, 63)) && ready(tt, j);
           if (!ok) break;
-          values(tt, j, 0);
-          ok = ready(tt, j, p_full);
-          if (!ok) break;
-          values(tt, j, 1);
+          values(tt, j);
           if (tt == tiles_here - 1) release(2 * j + 1);
           if (more) {
             if (tt == 0) ok = full(2 * j + 2, 62);
@@ -409,12 +403,9 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           scores(0, j + 1);
           release(2 * j + 2);
         }
-        ok = ready(0, j, p_half) && full(2 * j + 1, 63);
+        ok = full(2 * j + 1, 63) && ready(0, j);
         if (!ok) break;
-        values(0, j, 0);
-        ok = ready(0, j, p_full);
-        if (!ok) break;
-        values(0, j, 1);
+        values(0, j);
         release(2 * j + 1);
       }
     }
@@ -442,52 +433,45 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       if (CODED && alive) alive = mbar_wait_warp(kv_full + (2 * j + 1) % NS, static_cast<uint32_t>(((2 * j + 1) / NS) & 1), abort_flag, a.err_word, 67);
       if (!alive) break;
       tcgen05_fence_after();
-      uint32_t w[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32_nowait(ts + 32 * c, w[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld_regs(w[c]);
       const int key0 = (kt0 + j) * TC_KEYS;
-      if constexpr (CODED) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
+      const bool masked = key0 < all_lo || key0 + TC_KEYS > all_hi || *missing;
+      // 32 scores of the row, times their keys' scales, with what the row does not see at -infinity
+      auto read_scores = [&](int c, uint32_t (&w)[32]) {
+        tmem_ld_32x32_nowait(ts + 32 * c, w);
+        tmem_wait_ld_regs(w);
+        if constexpr (CODED) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             const float4 k4 = *reinterpret_cast<const float4*>(sc + 32 * c + i);
-            w[c][i] = __float_as_uint(__uint_as_float(w[c][i]) * k4.x);
-            w[c][i + 1] = __float_as_uint(__uint_as_float(w[c][i + 1]) * k4.y);
-            w[c][i + 2] = __float_as_uint(__uint_as_float(w[c][i + 2]) * k4.z);
-            w[c][i + 3] = __float_as_uint(__uint_as_float(w[c][i + 3]) * k4.w);
+            w[i] = __float_as_uint(__uint_as_float(w[i]) * k4.x);
+            w[i + 1] = __float_as_uint(__uint_as_float(w[i + 1]) * k4.y);
+            w[i + 2] = __float_as_uint(__uint_as_float(w[i + 2]) * k4.z);
+            w[i + 3] = __float_as_uint(__uint_as_float(w[i + 3]) * k4.w);
           }
-      }
-      const bool masked = key0 < all_lo || key0 + TC_KEYS > all_hi || *missing;
-      if (key0 < all_lo || key0 + TC_KEYS > all_hi) {
+        }
+        if (masked) {
+          const int lo = lim_lo - key0 - 32 * c, hi = lim_hi - key0 - 32 * c;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+          for (int i = 0; i < 32; ++i)
+            if (i < lo || i >= hi) w[i] = 0xff800000u;
+          if (*missing) {  // a page of this sequence is none of the cache's: which keys are out is looked up again
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int key = key0 + 32 * c + i;
-            if (key < lim_lo || key >= lim_hi) w[c][i] = 0xff800000u;
-          }
-      }
-      if (*missing) {  // a page of this sequence is none of the cache's: which keys are out is looked up again
+            for (int i = 0; i < 32; i += 8) {
+              const int key = key0 + 32 * c + i;
+              if (key + 7 >= k_begin && key < k_end && paged_page(p, s, p.by_page.div(key)) < 0) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            const int key = key0 + 32 * c + i;
-            if (key + 7 >= k_begin && key < k_end && paged_page(p, s, p.by_page.div(key)) < 0) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) w[c][i + e] = 0xff800000u;
+                for (int e = 0; e < 8; ++e) w[i + e] = 0xff800000u;
+              }
             }
           }
-      }
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        }
+      };
+      auto largest = [&](const uint32_t (&w)[32], float m) {
+        float m4[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 32; i += 2)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(w[c][i]), __uint_as_float(w[c][i + 1]));
-      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2;
+        for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+        return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      };
       float grow = 0.0f;
       if constexpr (CODED) {
         float top = 0.0f;
@@ -498,8 +482,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         const int e2 = min(240, max(14, static_cast<int>(__float_as_uint(top) >> 23)));
         grow = __uint_as_float(static_cast<uint32_t>(e2) << 23);
       }
-      const bool raise = mx > base + 8.0f || (CODED && grow > v_unit);
-      if (__any_sync(0xffffffffu, raise)) {
+      // another maximum, and O with it
+      auto rescale = [&](float mx) {
         const float nb = fmaxf(base, mx);
         float f = base == -INFINITY ? 0.0f : ex2f(base - nb);
         sum *= f;
@@ -509,52 +493,68 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           f *= v_unit / nu;
           v_unit = nu;
         }
-        if (j > 0) {
-          if (!mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(j - 1) & 1, abort_flag, a.err_word, 68)) { alive = false; break; }
-          tcgen05_fence_after();
+        if (j == 0) return true;
+        if (!mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(j - 1) & 1, abort_flag, a.err_word, 68)) return false;
+        tcgen05_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32_nowait(tmem_o + t * DP + lanes + 32 * c, o);
-            tmem_wait_ld_regs(o);
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32_nowait(tmem_o + t * DP + lanes + 32 * c, o);
+          tmem_wait_ld_regs(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st_32x32(tmem_o + t * DP + lanes + 32 * c, o);
-          }
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          tmem_st_32x32(tmem_o + t * DP + lanes + 32 * c, o);
         }
-      }
-      const float sub = base == -INFINITY ? 0.0f : base, inv_unit = CODED ? 1.0f / v_unit : 1.0f;
-      float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-      const float2 cc = make_float2(c2, c2), ss = make_float2(-sub, -sub);
-      // the probabilities, half of the keys at a time: P V of the first half runs while the second is computed
+        return true;
+      };
+      uint32_t pk[4][16];
+      float2 part[2];
+      // the probabilities by the present maximum, packed; the largest score on the way
       auto weigh_keys = [&](auto few_special) {
+        const float sub = base == -INFINITY ? 0.0f : base, inv_unit = CODED ? 1.0f / v_unit : 1.0f;
+        const float2 cc = make_float2(c2, c2), ss = make_float2(-sub, -sub);
+        part[0] = part[1] = make_float2(0.0f, 0.0f);
+        float mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+          uint32_t w[32];
+          read_scores(c, w);
+          mx = largest(w, mx);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float2 x = fma2(make_float2(__uint_as_float(w[c][i]), __uint_as_float(w[c][i + 1])), cc, ss);
+            const float2 x = fma2(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), cc, ss);
             // (keys behind a mask need an exact zero: they take the special function)
-            float2 e = decltype(few_special)::value && (i & 7) == 6 ? exp2_poly(x) : make_float2(ex2f(x.x), ex2f(x.y));
+            float2 e = decltype(few_special)::value && (i & TC_POLY) == TC_POLY ? exp2_poly(x) : make_float2(ex2f(x.x), ex2f(x.y));
             part[(i >> 1) & 1] = add2(part[(i >> 1) & 1], e);
             if constexpr (CODED) {
               const float2 v2 = *reinterpret_cast<const float2*>(sc + TC_KEYS + 32 * c + i);
               e.x *= v2.x * inv_unit, e.y *= v2.y * inv_unit;
             }
-            pk[i / 2] = pack2<BF>(e.x, e.y);
-          }
-          tmem_st_32x16(ts + 16 * c, pk);
-          if (c == 1) {
-            tmem_wait_st();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_half + buf);
+            pk[c][i / 2] = pack2<BF>(e.x, e.y);
           }
         }
+        return mx * c2;
       };
-      if (masked) weigh_keys(std::false_type());
-      else weigh_keys(std::true_type());
+      // a first maximum where a row of the warp has none yet; after that the present one is used at once, and only where a score outgrows it
+      // by more than 2^8 (a few times a row) are the tile's probabilities computed again by a new one
+      if (__any_sync(0xffffffffu, base == -INFINITY) || (CODED && grow > v_unit)) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[32];
+          read_scores(c, w);
+          mx = largest(w, mx);
+        }
+        if (!rescale(mx * c2)) { alive = false; break; }
+      }
+      const float mx = masked ? weigh_keys(std::false_type()) : weigh_keys(std::true_type());
+      if (__any_sync(0xffffffffu, mx > base + 8.0f)) {
+        if (!rescale(mx)) { alive = false; break; }
+        weigh_keys(std::false_type());
+      }
       sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_st_32x16(ts + 16 * c, pk[c]);
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
