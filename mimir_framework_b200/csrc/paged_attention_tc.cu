@@ -8,7 +8,7 @@
 //                    back over them as 16-bit pairs, from where P V reads them (A operand in tensor memory)
 //   warp 8           issues the tensor instructions: per key tile P_0 V, Q_0 K', P_1 V, Q_1 K' (K' the next tile)
 //   warps 9-11       bring K and V tiles out of the pages into a ring: by TMA, a box of a page's slots a lane (copies a thread each took 6300
-//                    cycles a key tile, twice what everything else did); 8-bit codes through registers, as halves
+//                    cycles a key tile, twice what everything else did); 8-bit codes through the registers of seven warps, as halves
 // Heads of over 128 elements have one tile of 128 rows (O takes 256 columns of tensor memory) and two score tiles that alternate.
 // K and V tiles lie in the same layout, [64 elements][key] rows of 128 swizzled bytes: K-major for Q K^T, MN-major for P V.
 // The running maximum is raised only when a score outgrows it by 2^8, so O in tensor memory is rescaled a few times a row.
@@ -26,7 +26,7 @@
 namespace mb {
 namespace {
 
-constexpr int TC_LOADERS = 96, TC_TMEM = 512;
+constexpr int TC_TMEM = 512;
 constexpr int TC_POLY = 6;  // of eight exponentials the last two go to the FMA lanes (none: 2 % more time, of four the last two: 9 %)
 
 template <int DP, int CT>
@@ -39,7 +39,11 @@ struct TcShape {
   static constexpr int SCALES = CODED ? NS / 2 * 2 * TC_KEYS * 4 : 0;  // [V stage][key, value][key]
   static constexpr int OFFS = 2 * TC_KEYS * 8;         // where the rows of a key tile lie, two tiles
   static constexpr int SMEM = NT * TILE + NS * TILE + SCALES + OFFS + 512;
-  static constexpr int THREADS = NT * 128 + 128;
+  static constexpr int LOADERS = CODED ? 224 : 96;     // threads that bring tiles
+  static constexpr int THREADS = NT * 128 + 32 + LOADERS;
+  // 8-bit codes take seven loader warps, which leave registers to the softmax warps: the shares add up to the launch's
+  static constexpr int SOFT_REGS = NT == 2 ? 168 : 232, LOAD_REGS = NT == 2 ? 88 : 136, LAUNCH_REGS = NT == 2 ? 128 : 168;
+  static_assert(!CODED || NT * 128 * SOFT_REGS + 256 * LOAD_REGS == THREADS * LAUNCH_REGS, "register shares");
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -138,7 +142,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(kv_full + i, CODED ? TC_LOADERS : 1);
+      mbar_init(kv_full + i, CODED ? S::LOADERS : 1);
       mbar_init(kv_empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -206,6 +210,10 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + 2 * TC_KEYS;  // tile t at + t * DP
 
+  if constexpr (CODED) {
+    if (warp < NT * 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFT_REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::LOAD_REGS));
+  }
   if (warp > NT * 4) {
     // ---- loaders -----------------------------------------------------------------------------------------------------------------------------
     const int id = static_cast<int>(threadIdx.x) - (NT * 128 + 32);
@@ -256,7 +264,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       }
     } else {
       // a tile's codes are on their way in registers while the one before it becomes halves
-      constexpr int N = (TC_KEYS * (DP / 8) + TC_LOADERS - 1) / TC_LOADERS;
+      constexpr int N = (TC_KEYS * (DP / 8) + S::LOADERS - 1) / S::LOADERS;
       Raw8<CT> raw[N];
       long long scale_at[2] = {-1, -1};
       auto find_rows = [&](int j) {
@@ -264,7 +272,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         long long* at = offs + (j & 1) * TC_KEYS;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int k = id + i * TC_LOADERS, key = key0 + k;
+          const int k = id + i * S::LOADERS, key = key0 + k;
           scale_at[i] = -1;
           if (k < TC_KEYS) {
             long long where = -1;
@@ -281,14 +289,14 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           }
         }
         __syncwarp();
-        asm volatile("barrier.sync 1, 96;" ::: "memory");
+        asm volatile("barrier.sync 1, %0;" ::"n"(S::LOADERS) : "memory");
       };
       auto fetch = [&](int j, int kv) {
         const long long* at = offs + (j & 1) * TC_KEYS;
         const char* src = static_cast<const char*>(kv ? p.v : p.k);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          const int x = id + n * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
+          const int x = id + n * S::LOADERS, k = x / (DP / 8), c = x % (DP / 8);
           raw[n].w[0] = raw[n].w[1] = 0;
           if (k < TC_KEYS && at[k] >= 0 && 8 * c < p.head_dim) raw[n] = load8<CT>(src + at[k] + 8 * c);
         }
@@ -307,7 +315,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           if (ok) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-              const int x = id + n * TC_LOADERS, k = x / (DP / 8), c = x % (DP / 8);
+              const int x = id + n * S::LOADERS, k = x / (DP / 8), c = x % (DP / 8);
               uint32_t hi[4], lo[4];
               to_pairs<CT>(raw[n], hi, lo);
               if (k < TC_KEYS)
@@ -316,7 +324,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
             if (kv) {  // both scales with the values, whose stage is let go of last
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
-                const int k = id + n * TC_LOADERS;
+                const int k = id + n * S::LOADERS;
                 if (k < TC_KEYS) {
                   sc[k] = scale_at[n] >= 0 ? __ldg(p.k_scale + scale_at[n]) : 0.0f;
                   sc[TC_KEYS + k] = scale_at[n] >= 0 ? __ldg(p.v_scale + scale_at[n]) : 0.0f;
