@@ -565,11 +565,15 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       for (int c = 0; c < 4; ++c) tmem_st_32x16(ts + 16 * c, pk[c]);
       tmem_wait_st();
       tcgen05_fence_before();
+      // With two score tiles the last product's wait, below, comes while the one before it may still run, and a barrier two phases behind looks
+      // complete.  So that one is waited for first; here, where the last cannot be through yet: two phases ahead looks incomplete for good.
+      if (NT == 1 && j > 0 && j + 1 == n_kt) {
+        alive = mbar_wait_warp(pv_done, static_cast<uint32_t>(j - 1) & 1, abort_flag, a.err_word, 69);
+        if (!alive) break;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + buf);
     }
-    // the last P V, and with two score tiles the one before it first (a barrier two phases behind looks complete)
-    if (NT == 1 && alive && n_kt > 1) alive = mbar_wait_warp(pv_done, static_cast<uint32_t>(n_kt - 2) & 1, abort_flag, a.err_word, 69);
     if (alive && n_kt > 0) alive = mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(n_kt - 1) & 1, abort_flag, a.err_word, 69);
     if (alive) {
       tcgen05_fence_after();

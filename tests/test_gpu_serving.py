@@ -213,6 +213,21 @@ def test_attention_of_chunks(backend, rows, kv, kv_heads, group, dim, page, caus
     check_attention(p, q, out, lse, type_, causal, window)
 
 
+@pytest.mark.parametrize("cache,type_,dim", [(BF16, BF16, 256), (I8, F16, 256)])
+def test_chunks_whose_score_tiles_alternate_many_times_over(backend, cache, type_, dim):
+    """Many blocks' ends: none may wait for a product that is through already."""
+    p = Pages([512] * 8, [2048] * 8, 4, dim, 64, cache, seed=5)
+    p.fill()
+    outs = []
+    q, out, lse = attend(backend, p, 8, type_)
+    outs.append(out.clone())
+    a = backend.paged_attention(q.data_ptr(), out.data_ptr(), type_, 8, 8 * dim, dim, 8 * dim, dim, 1 / math.sqrt(dim), lse=lse.data_ptr())
+    for _ in range(100):
+        backend.dev_paged_attention(p.cache(), p.batch(), a)
+    backend.check_device()
+    assert torch.equal(outs[0], out)
+
+
 @pytest.mark.parametrize("cache,type_", [(BF16, BF16), (E4M3, F16), (F16, BF16)])
 def test_chunks_with_a_negative_scale_a_bad_page_and_large_scores(backend, cache, type_):
     p = Pages([150, 70], [400, 90], 2, 64, 16, cache, seed=2)
