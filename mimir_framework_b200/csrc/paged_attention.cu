@@ -60,6 +60,8 @@ __device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
 template <int CT, int NQ, int NP, int DP>  // terms of a query and of a probability
 struct PagedShape {
   static constexpr bool BF = CT == MIMIR_B200_T_BF16;
+  // halves: probabilities of up to 2^14 (times a code's scale 2^15) are exact to 2^-39 of the largest where 2^-25 would be
+  static constexpr float ROOM = BF ? 0.0f : 14.0f;
   static constexpr bool FRESH = NQ == 2;                                // P V of a block apart from O
   static constexpr int KB = type_bytes(CT) == 1 || (type_bytes(CT) == 2 && DP <= 128) ? 32 : 16;  // keys of a block
   static constexpr int UD = CT == MIMIR_B200_T_F32 ? 64 : DP < 128 ? DP : 128;  // head elements loaded at a time
@@ -366,7 +368,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      const float mn = fmaxf(m[i], mx[i]);
+      const float mn = fmaxf(m[i], mx[i] - S::ROOM);
       raise = raise || mn > m[i];
       base[i] = mn == -INFINITY ? 0.0f : mn;  // (a row that has seen nothing yet)
       alpha[i] = ex2f(m[i] - base[i]);
@@ -578,20 +580,21 @@ struct Share {
   long long units = 0, tc_units = 0;
   size_t bytes = 0, tc_bytes = 0;
 };
-// Queries of 16 bits and more rows than a tile of the tensor cores is worth.
-constexpr int TC_FEW = 64;
+// Up to how many rows of a head go to the row kernel.  Up to 4 x 8 K keys, 8 key heads of 128, here and by tcgen05: 32 rows 57 and 53 us in
+// bfloat16, 47 and 78 over int8, 76 and 49 for fp32; 64 rows 111 and 54 us in bfloat16.
+constexpr int TC_FEW = 32;
 Share share_out(const AttendLaunch& a) {
   Share r;
   const int group = a.heads / a.p.kv_heads;
   const long long most = static_cast<long long>(a.p.max_rows) * group;
   const int keys = a.window > 0 && a.window < a.p.max_kv ? a.window : a.p.max_kv;  // (of a row; a chunk sees a little more)
   const size_t row_bytes = a.p.head_dim * sizeof(float) + sizeof(float2);
-  if (a.type != MIMIR_B200_T_F32 && most > TC_FEW) {
+  if (tc_takes(a.cache_type, a.type, a.p.head_dim) && most > TC_FEW) {
     r.chunks = true;
     // (one sequence: its rows are many; of several, some may have few)
     r.rows = a.p.n_seqs > 1;
     r.few = r.rows ? TC_FEW : 0;
-    const int per = tc_tile_rows(a.p.head_dim);
+    const int per = tc_tile_rows(a.type, a.p.head_dim);
     r.tc_tiles = static_cast<int>((most + per - 1) / per);
     r.tc_units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tc_tiles;
     while (r.tc_units * r.tc_splits * 2 <= ctx().sm_count && keys >= 1024 * r.tc_splits) r.tc_splits *= 2;
@@ -688,7 +691,7 @@ int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
   };
   if (r.chunks) {
     a.tiles = r.tc_tiles, a.last_first = 1;
-    parts(r.bytes, r.tc_units, r.tc_splits, tc_tile_rows(l.p.head_dim));
+    parts(r.bytes, r.tc_units, r.tc_splits, tc_tile_rows(l.type, l.p.head_dim));
     MB_TRY(launch_paged_attention_tc(a, l.cache_type, st));
     if (r.tc_splits > 1) MB_TRY(launch_merge(a, r.tc_units, st));
   }

@@ -20,9 +20,10 @@ struct AttendArgs {
   float2* part_ml;
   int* err_word;
 };
-// paged_attention_tc.cu: chunks of many rows; queries of 16 bits
+// paged_attention_tc.cu: chunks of many rows; not fp32 caches, nor fp32 queries of heads over 128
 constexpr int TC_KEYS = 128, TC_ROWS = 128;
-inline int tc_tile_rows(int head_dim) { return head_dim <= 128 ? 2 * TC_ROWS : TC_ROWS; }
+inline bool tc_takes(int cache_type, int type, int head_dim) { return cache_type != MIMIR_B200_T_F32 && (type != MIMIR_B200_T_F32 || head_dim <= 128); }
+inline int tc_tile_rows(int type, int head_dim) { return head_dim <= 128 && type != MIMIR_B200_T_F32 ? 2 * TC_ROWS : TC_ROWS; }
 int launch_paged_attention_tc(const AttendArgs& a, int cache_type, cudaStream_t st);
 
 namespace {

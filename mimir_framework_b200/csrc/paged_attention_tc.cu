@@ -9,7 +9,8 @@
 //   warp 8           issues the tensor instructions: per key tile P_0 V, Q_0 K', P_1 V, Q_1 K' (K' the next tile)
 //   warps 9-11       bring K and V tiles out of the pages into a ring: by TMA, a box of a page's slots a lane (copies a thread each took 6300
 //                    cycles a key tile, twice what everything else did); 8-bit codes through the registers of seven warps, as halves
-// Heads of over 128 elements have one tile of 128 rows (O takes 256 columns of tensor memory) and two score tiles that alternate.
+// Heads of over 128 elements have one tile of 128 rows (O takes 256 columns of tensor memory) and two score tiles that alternate.  So have
+// queries of fp32, which are two halves a value (22 bits) and whose probabilities are, over all 128 columns of the scores.
 // K and V tiles lie in the same layout, [64 elements][key] rows of 128 swizzled bytes: K-major for Q K^T, MN-major for P V.
 // The running maximum is raised only when a score outgrows it by 2^8, so O in tensor memory is rescaled a few times a row.
 // Probabilities of a bfloat16 cache are rounded to bfloat16 (8 bits, relative to each probability), else to half (11 bits); their sum is
@@ -29,16 +30,18 @@ namespace {
 constexpr int TC_TMEM = 512;
 constexpr int TC_POLY = 6;  // of eight exponentials the last two go to the FMA lanes (none: 2 % more time, of four the last two: 9 %)
 
-template <int DP, int CT>
+template <int DP, int CT, int NQ>  // NQ: terms of a query and of a probability
 struct TcShape {
   static constexpr bool BF = CT == MIMIR_B200_T_BF16, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3;
-  static constexpr int NT = DP <= 128 ? 2 : 1;         // row tiles
+  static constexpr int NT = DP <= 128 && NQ == 1 ? 2 : 1;  // row tiles
   static constexpr int SUB = DP / 64;                  // 64-element columns of a tile
   static constexpr int TILE = SUB * TC_KEYS * 128;     // bytes of a K or V tile, and of a Q tile
   static constexpr int NS = DP == 64 ? 6 : DP == 128 ? 4 : 2;
   static constexpr int SCALES = CODED ? NS / 2 * 2 * TC_KEYS * 4 : 0;  // [V stage][key, value][key]
   static constexpr int OFFS = 2 * TC_KEYS * 8;         // where the rows of a key tile lie, two tiles
-  static constexpr int SMEM = NT * TILE + NS * TILE + SCALES + OFFS + 512;
+  static constexpr int SMEM = NT * NQ * TILE + NS * TILE + SCALES + OFFS + 512;
+  // halves: probabilities of up to 2^6, by the maximum that may be 2^8 too low 2^14, are exact to 2^-31 of the largest where 2^-25 would be
+  static constexpr float ROOM = BF ? 0.0f : 6.0f;
   static constexpr int LOADERS = CODED ? 224 : 96;     // threads that bring tiles
   static constexpr int THREADS = NT * 128 + 32 + LOADERS;
   // 8-bit codes take seven loader warps, which leave registers to the softmax warps: the shares add up to the launch's
@@ -101,10 +104,10 @@ struct PageMaps {
   int slots;
 };
 
-template <int DP, int CT>
-__global__ void __launch_bounds__(TcShape<DP, CT>::THREADS, 1)
+template <int DP, int CT, int NQ>
+__global__ void __launch_bounds__(TcShape<DP, CT, NQ>::THREADS, 1)
 paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ PageMaps maps) {
-  using S = TcShape<DP, CT>;
+  using S = TcShape<DP, CT, NQ>;
   constexpr bool BF = S::BF, CODED = S::CODED;
   constexpr int NT = S::NT, NS = S::NS, TILE = S::TILE, SUB = S::SUB;
   constexpr float LOG2E = 1.4426950408889634f;
@@ -114,7 +117,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     return;
   }
   uint8_t* sq = smem;
-  uint8_t* ring = sq + NT * TILE;
+  uint8_t* ring = sq + NT * NQ * TILE;  // (after the queries' terms)
   float* scales = reinterpret_cast<float*>(ring + NS * TILE);
   long long* offs = reinterpret_cast<long long*>(ring + NS * TILE + S::SCALES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * TILE + S::SCALES + S::OFFS);
@@ -168,19 +171,20 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   if (t < NT) {
     const int h = head * a.group + r - tok * a.group;
     const bool there = r < r_end;
-    const char* src = static_cast<const char*>(a.q) + ((seq.row0 + tok) * a.q_row + h * a.q_head) * 2;
-    const bool from_bf = a.type == MIMIR_B200_T_BF16;
+    const char* src = static_cast<const char*>(a.q) + ((seq.row0 + tok) * a.q_row + h * a.q_head) * (NQ == 2 ? 4 : 2);
+    const bool from_bf = a.type == MIMIR_B200_T_BF16, scaled = NQ == 2 || (!BF && from_bf);
     auto read = [&](int c, float (&f)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = 0.0f;
       if (there && 8 * c < p.head_dim) {
-        if (from_bf) unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(src + 16 * c), f);
+        if constexpr (NQ == 2) unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(src + 32 * c), f);
+        else if (from_bf) unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(src + 16 * c), f);
         else unpack8<MIMIR_B200_T_F16>(load8<MIMIR_B200_T_F16>(src + 16 * c), f);
       }
     };
-    // bfloat16 as half: the row times a power of two that brings its largest to [1, 2) (bits below 2^-24 of that are lost)
+    // bfloat16 and fp32 as halves: the row times a power of two that brings its largest to [1, 2) (bits below 2^-24 of that are lost)
     float up = 1.0f, down = 1.0f;
-    if (!BF && from_bf) {
+    if (scaled) {
       float top = 0.0f;
       for (int c = 0; c < DP / 8; ++c) {
         float f[8];
@@ -192,15 +196,18 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       up = __uint_as_float(static_cast<uint32_t>(e2) << 23);
       down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
     }
-    c2 = fabsf(a.scale) * LOG2E * up;
+    // (fp32: the tensor core's sums are low by 1.5e-8 of their value an instruction)
+    c2 = fabsf(a.scale) * LOG2E * up * (NQ == 2 ? 1.0f + 1.5e-8f * (DP / 8) : 1.0f);
     if (a.scale < 0.0f) down = -down;  // (the largest product is then the smallest score's)
     for (int c = 0; c < DP / 8; ++c) {
       float f[8];
       read(c, f);
-      uint32_t w[4];
+      uint32_t w[4], l[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pack2<BF>(f[2 * e] * down, f[2 * e + 1] * down);
-      *reinterpret_cast<uint4*>(sq + t * TILE + (c >> 3) * (TC_ROWS * 128) + r_local * 128 + (((c & 7) ^ (r_local & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int e = 0; e < 4; ++e) split2<BF>(f[2 * e] * down, f[2 * e + 1] * down, w[e], l[e]);
+      uint8_t* to = sq + t * TILE + (c >> 3) * (TC_ROWS * 128) + r_local * 128 + (((c & 7) ^ (r_local & 7)) << 4);
+      *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+      if constexpr (NQ == 2) *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
     }
     fence_proxy_async_smem();
   }
@@ -355,6 +362,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         for (int k = 0; k < DP / 16; ++k) {
           const uint64_t o = ((k >> 2) * (TC_KEYS * 128) + (k & 3) * 32) >> 4;
           umma_bf16(d, q_desc + o, k_desc + o, idesc_s, k != 0 ? 1u : 0u);
+          if constexpr (NQ == 2) umma_bf16(d, q_desc + (TILE >> 4) + o, k_desc + o, idesc_s, 1u);
         }
         umma_commit(s_full + (NT == 2 ? tt : (j & 1)));
       }
@@ -365,7 +373,10 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       const uint64_t v_desc = desc_mn(v_at, TC_KEYS * 128);
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < TC_KEYS / 16; ++k) umma_f16_ts(d, pa + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < TC_KEYS / 16; ++k) {
+          umma_f16_ts(d, pa + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+          if constexpr (NQ == 2) umma_f16_ts(d, pa + TC_KEYS / 2 + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, 1u);
+        }
         umma_commit(pv_done + tt);
       }
       __syncwarp();
@@ -492,7 +503,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
       }
       // another maximum, and O with it
       auto rescale = [&](float mx) {
-        const float nb = fmaxf(base, mx);
+        const float nb = fmaxf(base, mx - S::ROOM);
         float f = base == -INFINITY ? 0.0f : ex2f(base - nb);
         sum *= f;
         base = nb;
@@ -515,7 +526,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         }
         return true;
       };
-      uint32_t pk[4][16];
+      uint32_t pk[4][16], pl[4][16];  // (pl: what the rounding leaves, for fp32)
       float2 part[2];
       // the probabilities by the present maximum, packed; the largest score on the way
       auto weigh_keys = [&](auto few_special) {
@@ -538,7 +549,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
               const float2 v2 = *reinterpret_cast<const float2*>(sc + TC_KEYS + 32 * c + i);
               e.x *= v2.x * inv_unit, e.y *= v2.y * inv_unit;
             }
-            pk[c][i / 2] = pack2<BF>(e.x, e.y);
+            if constexpr (NQ == 2) split2<BF>(e.x, e.y, pk[c][i / 2], pl[c][i / 2]);
+            else pk[c][i / 2] = pack2<BF>(e.x, e.y);
           }
         }
         return mx * c2;
@@ -555,14 +567,17 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         }
         if (!rescale(mx * c2)) { alive = false; break; }
       }
-      const float mx = masked ? weigh_keys(std::false_type()) : weigh_keys(std::true_type());
-      if (__any_sync(0xffffffffu, mx > base + 8.0f)) {
+      const float mx = masked ? weigh_keys(std::false_type()) : weigh_keys(std::integral_constant<bool, NQ == 1>());
+      if (__any_sync(0xffffffffu, mx > base + (8.0f + S::ROOM))) {
         if (!rescale(mx)) { alive = false; break; }
         weigh_keys(std::false_type());
       }
       sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_st_32x16(ts + 16 * c, pk[c]);
+      for (int c = 0; c < 4; ++c) {
+        tmem_st_32x16(ts + 16 * c, pk[c]);
+        if constexpr (NQ == 2) tmem_st_32x16(ts + TC_KEYS / 2 + 16 * c, pl[c]);
+      }
       tmem_wait_st();
       tcgen05_fence_before();
       // With two score tiles the last product's wait, below, comes while the one before it may still run, and a barrier two phases behind looks
@@ -578,11 +593,13 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     if (alive) {
       tcgen05_fence_after();
       const bool there = r < r_end;
-      const float unit_v = (CODED ? v_unit : 1.0f);
+      // fp32: two instructions for 16 keys that the row sees, each of which lost 1.5e-8
+      const int keys_seen = max(0, min(lim_hi, (kt0 + n_kt) * TC_KEYS) - max(lim_lo, kt0 * TC_KEYS));
+      const float unit_v = (CODED ? v_unit : 1.0f) * (NQ == 2 ? 1.0f + 1.5e-8f * (keys_seen / 8) : 1.0f);
       const float inv = a.splits > 1 ? unit_v : sum == 0.0f ? 0.0f : unit_v / sum;
       const int h = head * a.group + r - tok * a.group;
       const long long part_row = static_cast<long long>(blockIdx.x) * (NT * TC_ROWS) + t * TC_ROWS + r_local;
-      char* dst = static_cast<char*>(a.out) + ((seq.row0 + tok) * a.o_row + h * a.o_head) * 2;
+      char* dst = static_cast<char*>(a.out) + ((seq.row0 + tok) * a.o_row + h * a.o_head) * (NQ == 2 ? 4 : 2);
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
@@ -601,6 +618,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[i + e]) * inv;
           if (a.splits > 1) {
             store8<MIMIR_B200_T_F32>(a.part_o + part_row * p.head_dim + d, pack8<MIMIR_B200_T_F32>(f));
+          } else if constexpr (NQ == 2) {
+            store8<MIMIR_B200_T_F32>(dst + 4 * d, pack8<MIMIR_B200_T_F32>(f));
           } else if (a.type == MIMIR_B200_T_BF16) {
             store8<MIMIR_B200_T_BF16>(dst + 2 * d, pack8<MIMIR_B200_T_BF16>(f));
           } else {
@@ -645,12 +664,12 @@ int make_page_map(CUtensorMap* map, const PagedView& p, const void* base, int sl
   return MIMIR_B200_OK;
 }
 
-template <int DP, int CT>
+template <int DP, int CT, int NQ>
 int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
-  using S = TcShape<DP, CT>;
+  using S = TcShape<DP, CT, NQ>;
   static PerDeviceOnce once;
   MB_TRY(once.run([]() -> int {
-    MB_CUDA(cudaFuncSetAttribute(paged_attention_tc_kernel<DP, CT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    MB_CUDA(cudaFuncSetAttribute(paged_attention_tc_kernel<DP, CT, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     return MIMIR_B200_OK;
   }));
   const long long grid = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * a.tiles * a.splits;
@@ -662,16 +681,19 @@ int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
     MB_TRY(make_page_map(&maps.v, a.p, a.p.v, maps.slots));
     MB_TRY(make_page_map(&maps.v_row, a.p, a.p.v, 1));
   }
-  paged_attention_tc_kernel<DP, CT><<<static_cast<unsigned>(grid), S::THREADS, S::SMEM, st>>>(a, maps);
+  paged_attention_tc_kernel<DP, CT, NQ><<<static_cast<unsigned>(grid), S::THREADS, S::SMEM, st>>>(a, maps);
   MB_CUDA(cudaGetLastError());
   count_launch();
   return MIMIR_B200_OK;
 }
 template <int CT>
 int launch_tc_dim(const AttendArgs& a, cudaStream_t st) {
-  if (a.p.head_dim <= 64) return launch_tc_as<64, CT>(a, st);
-  if (a.p.head_dim <= 128) return launch_tc_as<128, CT>(a, st);
-  return launch_tc_as<256, CT>(a, st);
+  if constexpr (CT != MIMIR_B200_T_BF16) {
+    if (a.type == MIMIR_B200_T_F32) return a.p.head_dim <= 64 ? launch_tc_as<64, CT, 2>(a, st) : launch_tc_as<128, CT, 2>(a, st);
+  }
+  if (a.p.head_dim <= 64) return launch_tc_as<64, CT, 1>(a, st);
+  if (a.p.head_dim <= 128) return launch_tc_as<128, CT, 1>(a, st);
+  return launch_tc_as<256, CT, 1>(a, st);
 }
 
 }  // namespace
