@@ -17,6 +17,7 @@
 #include <cmath>
 
 #include "common.h"
+#include "launch.cuh"
 #include "paged.cuh"
 #include "paged_attention.cuh"
 
@@ -92,7 +93,12 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   const int tile = unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
   const PagedSeq q = paged_seq(p, s);
   const int r0 = tile * PA_ROWS, n_rows = q.rows * a.group;
-  if (r0 >= n_rows || n_rows > a.few) return;  // (the whole cluster)
+  // Launched behind chunks it runs beside their last blocks, of which it reads nothing; one block of it ends after them, and so does the launch.
+  const bool last = blockIdx.x + 1 == gridDim.x;
+  if (r0 >= n_rows || n_rows > a.few) {  // (the whole cluster)
+    if (last) pdl_wait();
+    return;
+  }
   const int r_end = min(r0 + PA_ROWS, n_rows);
   const int pos0 = q.kv - q.rows;  // of the sequence's first new token
   const int pos_first = pos0 + r0 / a.group, pos_last = pos0 + (r_end - 1) / a.group;
@@ -546,6 +552,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
+  if (last) pdl_wait();
 }
 
 // The parts of a tile that several CTAs or clusters computed, in order.
@@ -626,14 +633,19 @@ int launch_rows_as(const AttendArgs& a, long long grid, cudaStream_t st) {
   cfg.blockDim = dim3(PA_THREADS);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (a.cluster > 1) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(a.cluster);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
     cfg.numAttrs = 1;
+  }
+  if (a.behind_chunks) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
   }
   MB_CUDA(cudaLaunchKernelEx(&cfg, paged_attention_kernel<CT, NQ, NP, DP>, a));
   count_launch();
@@ -689,14 +701,15 @@ int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(l.ws) + offset);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(units) * splits * rows * l.p.head_dim);
   };
+  AttendArgs chunks = a;
   if (r.chunks) {
     a.tiles = r.tc_tiles, a.last_first = 1;
     parts(r.bytes, r.tc_units, r.tc_splits, tc_tile_rows(l.type, l.p.head_dim));
+    chunks = a;
     MB_TRY(launch_paged_attention_tc(a, l.cache_type, st));
-    if (r.tc_splits > 1) MB_TRY(launch_merge(a, r.tc_units, st));
   }
-  if (!r.rows) return MIMIR_B200_OK;
-  a.tiles = r.tiles, a.cluster = r.cluster, a.last_first = 0;
+  if (!r.rows) return r.tc_splits > 1 ? launch_merge(chunks, r.tc_units, st) : MIMIR_B200_OK;
+  a.tiles = r.tiles, a.cluster = r.cluster, a.last_first = 0, a.behind_chunks = r.chunks;
   parts(0, r.units, r.splits, PA_ROWS);
   switch (l.cache_type) {
     case MIMIR_B200_T_F32: MB_TRY((launch_rows_dim<MIMIR_B200_T_F32, 2, 2>(a, grid, st))); break;
@@ -705,6 +718,7 @@ int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
     case MIMIR_B200_T_I8: MB_TRY(launch_rows_type<MIMIR_B200_T_I8>(a, grid, st)); break;
     default: MB_TRY(launch_rows_type<MIMIR_B200_T_E4M3>(a, grid, st)); break;
   }
+  if (r.tc_splits > 1) MB_TRY(launch_merge(chunks, r.tc_units, st));
   if (r.splits > 1) MB_TRY(launch_merge(a, r.units, st));
   return MIMIR_B200_OK;
 }

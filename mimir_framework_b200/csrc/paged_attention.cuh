@@ -16,6 +16,7 @@ struct AttendArgs {
   int few;                                 // (token, head) rows of a sequence and key head: up to so many are the row kernel's
   int tiles, cluster, splits;              // of the rows of a sequence; CTAs and clusters that share a tile's keys
   int part_rows, last_first;               // rows of a tile; tiles are numbered from the last
+  int behind_chunks;                       // the row kernel: launched behind the chunks' kernel, with which it shares nothing
   float* part_o;                           // [unit][split][part_rows][head_dim], [unit][split][part_rows] (max, sum): splits > 1
   float2* part_ml;
   int* err_word;

@@ -214,6 +214,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  pdl_launch_dependents();  // sequences of few rows, another kernel's, may start on SMs that come free
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + 2 * TC_KEYS;  // tile t at + t * DP
 
