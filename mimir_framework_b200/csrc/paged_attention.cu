@@ -555,27 +555,35 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   if (last) pdl_wait();
 }
 
-// The parts of a tile that several CTAs or clusters computed, in order.
+// The parts of a tile that several CTAs or clusters computed, in order; a warp a row (a block a row: 16 us more for 16 K rows of two parts).
 __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ AttendArgs a) {
   const PagedView& p = a.p;
-  const int unit = blockIdx.x / a.part_rows, row = blockIdx.x % a.part_rows;
-  const int at = unit % a.tiles, tile = a.last_first ? a.tiles - 1 - at : at, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
-  const PagedSeq q = paged_seq(p, s);
+  const int at = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 5), unit = at / a.part_rows, row = at % a.part_rows, lane = threadIdx.x & 31;
+  int tile, head;
+  PagedSeq q;
+  if (a.chunks) {
+    const ChunkUnit u = chunk_unit(a, unit);
+    q = u.seq, tile = u.tile, head = u.head;
+  } else {
+    const int sh = unit / a.tiles;
+    tile = unit % a.tiles, head = sh % p.kv_heads;
+    q = paged_seq(p, sh / p.kv_heads);
+  }
   const int r = tile * a.part_rows + row, n_rows = q.rows * a.group;
-  if (r >= n_rows || (a.last_first ? n_rows <= a.few : n_rows > a.few)) return;
+  if (r >= n_rows || (!a.chunks && n_rows > a.few)) return;
   const float2* ml = a.part_ml + static_cast<long long>(unit) * a.splits * a.part_rows + row;
   const float* po = a.part_o + (static_cast<long long>(unit) * a.splits * a.part_rows + row) * p.head_dim;
   float top = -INFINITY, sum = 0.0f;
   for (int c = 0; c < a.splits; ++c) top = fmaxf(top, ml[c * a.part_rows].x);
   const float base = top == -INFINITY ? 0.0f : top;
   for (int c = 0; c < a.splits; ++c) sum = fmaf(ml[c * a.part_rows].y, exp2f(ml[c * a.part_rows].x - base), sum);
-  for (int d = threadIdx.x; d < p.head_dim; d += 128) {
+  for (int d = lane; d < p.head_dim; d += 32) {
     float v = 0.0f;
     for (int c = 0; c < a.splits; ++c)
       v = fmaf(po[static_cast<long long>(c) * a.part_rows * p.head_dim + d], exp2f(ml[c * a.part_rows].x - base), v);
     store_out(a, q.row0, r, head, d, sum == 0.0f ? 0.0f : v / sum);
   }
-  if (threadIdx.x == 0) store_lse(a, q.row0, r, head, top, sum);
+  if (lane == 0) store_lse(a, q.row0, r, head, top, sum);
 }
 
 // How a call is shared out between the two kernels, and each one's tiles over CTAs.
@@ -583,7 +591,7 @@ struct Share {
   bool rows = true, chunks = false;  // which kernels run
   int few = 0x7fffffff;
   int tiles = 1, cluster = 1, splits = 1;   // row kernel
-  int tc_tiles = 1, tc_splits = 1;
+  int tc_splits = 1;
   long long units = 0, tc_units = 0;
   size_t bytes = 0, tc_bytes = 0;
 };
@@ -602,8 +610,10 @@ Share share_out(const AttendLaunch& a) {
     r.rows = a.p.n_seqs > 1;
     r.few = r.rows ? TC_FEW : 0;
     const int per = tc_tile_rows(a.type, a.p.head_dim);
-    r.tc_tiles = static_cast<int>((most + per - 1) / per);
-    r.tc_units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tc_tiles;
+    // at most so many tiles: full ones, and one of each sequence of more than `few` rows that is not
+    const long long all = static_cast<long long>(a.p.n_rows) * group, chunks = all / (r.few + 1) < a.p.n_seqs ? all / (r.few + 1) : a.p.n_seqs;
+    const long long longest = a.p.n_seqs * ((most + per - 1) / per);
+    r.tc_units = a.p.kv_heads * (all / per + chunks < longest ? all / per + chunks : longest);
     while (r.tc_units * r.tc_splits * 2 <= ctx().sm_count && keys >= 1024 * r.tc_splits) r.tc_splits *= 2;
     if (r.tc_splits > 1) r.tc_bytes = static_cast<size_t>(r.tc_units) * r.tc_splits * per * row_bytes;
   }
@@ -674,7 +684,7 @@ size_t paged_attention_ws_bytes(const AttendLaunch& a) {
 
 namespace {
 int launch_merge(const AttendArgs& a, long long units, cudaStream_t st) {
-  paged_merge_kernel<<<static_cast<unsigned>(units * a.part_rows), 128, 0, st>>>(a);
+  paged_merge_kernel<<<static_cast<unsigned>(units * a.part_rows / 4), 128, 0, st>>>(a);
   MB_CUDA(cudaGetLastError());
   count_launch();
   return MIMIR_B200_OK;
@@ -703,13 +713,13 @@ int launch_paged_attention(const AttendLaunch& l, cudaStream_t st) {
   };
   AttendArgs chunks = a;
   if (r.chunks) {
-    a.tiles = r.tc_tiles, a.last_first = 1;
+    a.chunks = 1;
     parts(r.bytes, r.tc_units, r.tc_splits, tc_tile_rows(l.type, l.p.head_dim));
     chunks = a;
-    MB_TRY(launch_paged_attention_tc(a, l.cache_type, st));
+    MB_TRY(launch_paged_attention_tc(a, l.cache_type, r.tc_units * r.tc_splits, st));
   }
   if (!r.rows) return r.tc_splits > 1 ? launch_merge(chunks, r.tc_units, st) : MIMIR_B200_OK;
-  a.tiles = r.tiles, a.cluster = r.cluster, a.last_first = 0, a.behind_chunks = r.chunks;
+  a.tiles = r.tiles, a.cluster = r.cluster, a.chunks = 0, a.behind_chunks = r.chunks;
   parts(0, r.units, r.splits, PA_ROWS);
   switch (l.cache_type) {
     case MIMIR_B200_T_F32: MB_TRY((launch_rows_dim<MIMIR_B200_T_F32, 2, 2>(a, grid, st))); break;

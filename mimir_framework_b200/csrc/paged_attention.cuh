@@ -15,7 +15,8 @@ struct AttendArgs {
   float scale;
   int few;                                 // (token, head) rows of a sequence and key head: up to so many are the row kernel's
   int tiles, cluster, splits;              // of the rows of a sequence; CTAs and clusters that share a tile's keys
-  int part_rows, last_first;               // rows of a tile; tiles are numbered from the last
+  int part_rows;                           // rows of a tile
+  int chunks;                              // tiles of the sequences with more than `few` rows only, numbered by chunk_unit()
   int behind_chunks;                       // the row kernel: launched behind the chunks' kernel, with which it shares nothing
   float* part_o;                           // [unit][split][part_rows][head_dim], [unit][split][part_rows] (max, sum): splits > 1
   float2* part_ml;
@@ -25,9 +26,42 @@ struct AttendArgs {
 constexpr int TC_KEYS = 128, TC_ROWS = 128;
 inline bool tc_takes(int cache_type, int type, int head_dim) { return cache_type != MIMIR_B200_T_F32 && (type != MIMIR_B200_T_F32 || head_dim <= 128); }
 inline int tc_tile_rows(int type, int head_dim) { return head_dim <= 128 && type != MIMIR_B200_T_F32 ? 2 * TC_ROWS : TC_ROWS; }
-int launch_paged_attention_tc(const AttendArgs& a, int cache_type, cudaStream_t st);
+int launch_paged_attention_tc(const AttendArgs& a, int cache_type, long long grid, cudaStream_t st);
 
 namespace {
+// The `unit`-th tile of the sequences that have more than `few` rows, by a whole warp: their tiles of the first key head, the last first (its
+// rows see the most keys), then the next head's, then the next sequence's.  A grid over sequences x the longest one's tiles had mostly empty
+// blocks in a batch of one chunk and many single tokens (2048 new tokens and 31 single ones: 8192 blocks, 306 us in all; so numbered 512, 248).
+struct ChunkUnit {
+  PagedSeq seq;
+  int s = -1, head = 0, tile = 0;
+};
+__device__ __forceinline__ ChunkUnit chunk_unit(const AttendArgs& a, int unit) {
+  ChunkUnit u;
+  const int lane = threadIdx.x & 31;
+  for (int first = 0; first < a.p.n_seqs; first += 32) {
+    PagedSeq q;
+    if (first + lane < a.p.n_seqs) q = paged_seq(a.p, first + lane);
+    const int rows = q.rows * a.group, tiles = rows > a.few ? (rows + a.part_rows - 1) / a.part_rows : 0;
+    int sum = tiles * a.p.kv_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const uint32_t behind = __ballot_sync(0xffffffffu, unit < sum);
+    if (behind) {
+      const int at = __ffs(behind) - 1, n = __shfl_sync(0xffffffffu, tiles, at), rest = unit - __shfl_sync(0xffffffffu, sum, at) + n * a.p.kv_heads;
+      u.seq.row0 = __shfl_sync(0xffffffffu, q.row0, at);
+      u.seq.rows = __shfl_sync(0xffffffffu, q.rows, at);
+      u.seq.kv = __shfl_sync(0xffffffffu, q.kv, at);
+      u.s = first + at, u.head = rest / n, u.tile = n - 1 - rest % n;
+      return u;
+    }
+    unit -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return u;
+}
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;

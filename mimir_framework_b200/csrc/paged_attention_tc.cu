@@ -129,11 +129,10 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   const PagedView& p = a.p;
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int split = static_cast<int>(blockIdx.x) % a.splits, unit = static_cast<int>(blockIdx.x) / a.splits;
-  // (the last rows see the most keys: their CTAs start first)
-  const int tile = a.tiles - 1 - unit % a.tiles, sh = unit / a.tiles, head = sh % p.kv_heads, s = sh / p.kv_heads;
-  const PagedSeq seq = paged_seq(p, s);
-  const int n_rows = seq.rows * a.group, r0 = tile * NT * TC_ROWS;
-  if (n_rows <= a.few || r0 >= n_rows) return;
+  const ChunkUnit mine = chunk_unit(a, unit);
+  if (mine.s < 0) return;
+  const PagedSeq seq = mine.seq;
+  const int s = mine.s, head = mine.head, n_rows = seq.rows * a.group, r0 = mine.tile * NT * TC_ROWS;
   const int r_end = min(r0 + NT * TC_ROWS, n_rows), tiles_here = (r_end - r0 + TC_ROWS - 1) / TC_ROWS;
   const int pos0 = seq.kv - seq.rows;
   const int pos_first = pos0 + r0 / a.group, pos_last = pos0 + (r_end - 1) / a.group;
@@ -666,14 +665,13 @@ int make_page_map(CUtensorMap* map, const PagedView& p, const void* base, int sl
 }
 
 template <int DP, int CT, int NQ>
-int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
+int launch_tc_as(const AttendArgs& a, long long grid, cudaStream_t st) {
   using S = TcShape<DP, CT, NQ>;
   static PerDeviceOnce once;
   MB_TRY(once.run([]() -> int {
     MB_CUDA(cudaFuncSetAttribute(paged_attention_tc_kernel<DP, CT, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     return MIMIR_B200_OK;
   }));
-  const long long grid = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * a.tiles * a.splits;
   PageMaps maps = {};
   if constexpr (!S::CODED) {
     maps.slots = 8;
@@ -688,23 +686,23 @@ int launch_tc_as(const AttendArgs& a, cudaStream_t st) {
   return MIMIR_B200_OK;
 }
 template <int CT>
-int launch_tc_dim(const AttendArgs& a, cudaStream_t st) {
+int launch_tc_dim(const AttendArgs& a, long long grid, cudaStream_t st) {
   if constexpr (CT != MIMIR_B200_T_BF16) {
-    if (a.type == MIMIR_B200_T_F32) return a.p.head_dim <= 64 ? launch_tc_as<64, CT, 2>(a, st) : launch_tc_as<128, CT, 2>(a, st);
+    if (a.type == MIMIR_B200_T_F32) return a.p.head_dim <= 64 ? launch_tc_as<64, CT, 2>(a, grid, st) : launch_tc_as<128, CT, 2>(a, grid, st);
   }
-  if (a.p.head_dim <= 64) return launch_tc_as<64, CT, 1>(a, st);
-  if (a.p.head_dim <= 128) return launch_tc_as<128, CT, 1>(a, st);
-  return launch_tc_as<256, CT, 1>(a, st);
+  if (a.p.head_dim <= 64) return launch_tc_as<64, CT, 1>(a, grid, st);
+  if (a.p.head_dim <= 128) return launch_tc_as<128, CT, 1>(a, grid, st);
+  return launch_tc_as<256, CT, 1>(a, grid, st);
 }
 
 }  // namespace
 
-int launch_paged_attention_tc(const AttendArgs& a, int cache_type, cudaStream_t st) {
+int launch_paged_attention_tc(const AttendArgs& a, int cache_type, long long grid, cudaStream_t st) {
   switch (cache_type) {
-    case MIMIR_B200_T_F16: return launch_tc_dim<MIMIR_B200_T_F16>(a, st);
-    case MIMIR_B200_T_BF16: return launch_tc_dim<MIMIR_B200_T_BF16>(a, st);
-    case MIMIR_B200_T_I8: return launch_tc_dim<MIMIR_B200_T_I8>(a, st);
-    default: return launch_tc_dim<MIMIR_B200_T_E4M3>(a, st);
+    case MIMIR_B200_T_F16: return launch_tc_dim<MIMIR_B200_T_F16>(a, grid, st);
+    case MIMIR_B200_T_BF16: return launch_tc_dim<MIMIR_B200_T_BF16>(a, grid, st);
+    case MIMIR_B200_T_I8: return launch_tc_dim<MIMIR_B200_T_I8>(a, grid, st);
+    default: return launch_tc_dim<MIMIR_B200_T_E4M3>(a, grid, st);
   }
 }
 
