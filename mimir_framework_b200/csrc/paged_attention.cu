@@ -606,8 +606,8 @@ Share share_out(const AttendLaunch& a) {
   const size_t row_bytes = a.p.head_dim * sizeof(float) + sizeof(float2);
   if (tc_takes(a.cache_type, a.type, a.p.head_dim) && most > TC_FEW) {
     r.chunks = true;
-    // (one sequence: its rows are many; of several, some may have few)
-    r.rows = a.p.n_seqs > 1;
+    // (one sequence: its rows are many, and so are those of one token of a large group; of several sequences some may have few)
+    r.rows = a.p.n_seqs > 1 && group <= TC_FEW;
     r.few = r.rows ? TC_FEW : 0;
     const int per = tc_tile_rows(a.type, a.p.head_dim);
     // at most so many tiles: full ones, and one of each sequence of more than `few` rows that is not

@@ -38,6 +38,12 @@ int check_device_pointer(const char* what, const char* name, const void* p) {
     return fail(MIMIR_B200_E_INVALID, "%s: %s is on device %d, the current device is %d", what, name, at.device, ctx().device);
   return MIMIR_B200_OK;
 }
+// ... of 4-byte words
+int check_device_words(const char* what, const char* name, const void* p) {
+  MB_TRY(check_device_pointer(what, name, p));
+  if (reinterpret_cast<uintptr_t>(p) & 3) return fail(MIMIR_B200_E_INVALID, "%s: %s is not 4-byte aligned", what, name);
+  return MIMIR_B200_OK;
+}
 
 // the sizes of a cache and a batch (no pointers)
 int check_sizes(const char* what, const MimirPagedCache* c, const MimirPagedBatch* b) {
@@ -62,14 +68,14 @@ int check_pointers(const char* what, const MimirPagedCache* c, const MimirPagedB
   MB_TRY(check_device_pointer(what, "the cache's v", c->v));
   const bool coded = c->type == MIMIR_B200_T_I8 || c->type == MIMIR_B200_T_E4M3;
   if (coded) {
-    MB_TRY(check_device_pointer(what, "the cache's k_scale", c->k_scale));
-    MB_TRY(check_device_pointer(what, "the cache's v_scale", c->v_scale));
+    MB_TRY(check_device_words(what, "the cache's k_scale", c->k_scale));
+    MB_TRY(check_device_words(what, "the cache's v_scale", c->v_scale));
   }
   if (!aligned16(c->k) || !aligned16(c->v) || (coded && (!aligned16(c->k_scale) || !aligned16(c->v_scale))))
     return fail(MIMIR_B200_E_UNSUPPORTED, "%s: the cache's pointers are not 16-byte aligned", what);
-  if (rows) MB_TRY(check_device_pointer(what, "row_start", b->row_start));
-  MB_TRY(check_device_pointer(what, "kv_len", b->kv_len));
-  if (b->table_stride > 0) MB_TRY(check_device_pointer(what, "page_table", b->page_table));
+  if (rows) MB_TRY(check_device_words(what, "row_start", b->row_start));
+  MB_TRY(check_device_words(what, "kv_len", b->kv_len));
+  if (b->table_stride > 0) MB_TRY(check_device_words(what, "page_table", b->page_table));
   v->k = c->k, v->v = c->v, v->k_scale = c->k_scale, v->v_scale = c->v_scale;
   v->page_stride = c->page_stride, v->slot_stride = c->slot_stride, v->head_stride = c->head_stride;
   v->n_pages = c->n_pages, v->page_size = c->page_size, v->kv_heads = c->kv_heads, v->head_dim = c->head_dim;
@@ -104,7 +110,11 @@ int check_attention(const char* what, const MimirPagedCache* c, const MimirPaged
     return fail(MIMIR_B200_E_UNSUPPORTED, "%s: strides of q and out are multiples of 8 elements", what);
   l->p.n_seqs = b->n_seqs, l->p.n_rows = b->n_rows, l->p.max_rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows, l->p.max_kv = b->max_kv;
   l->p.kv_heads = c->kv_heads, l->p.head_dim = c->head_dim, l->p.page_size = c->page_size;
-  l->cache_type = c->type, l->type = at->type, l->heads = at->heads, l->causal = at->causal != 0, l->window = at->window, l->scale = at->scale;
+  if (static_cast<long long>(l->p.max_rows) * at->heads > 0x7fffffffLL) return fail(MIMIR_B200_E_INVALID, "%s: too many rows and heads for one call", what);
+  if (l->p.max_kv > (1 << 30)) l->p.max_kv = 1 << 30;  // (key numbers leave room to round up; a longer sequence is reported as one that does not fit)
+  // a window that no sequence fills is none
+  l->cache_type = c->type, l->type = at->type, l->heads = at->heads, l->causal = at->causal != 0, l->scale = at->scale;
+  l->window = at->window < l->p.max_kv ? at->window : 0;
   l->q = at->q, l->out = at->out, l->lse = at->lse, l->ws = at->workspace, l->ws_bytes = at->workspace_bytes;
   l->q_row = at->row_stride, l->q_head = at->head_stride, l->o_row = at->out_row_stride, l->o_head = at->out_head_stride;
   return MIMIR_B200_OK;
@@ -130,7 +140,7 @@ int mimir_b200_dev_rope(const MimirRopePlan* plan, const int32_t* positions, con
   if (x == y && (x_row_stride != y_row_stride || x_head_stride != y_head_stride)) return fail(MIMIR_B200_E_INVALID, "rope: in place with two sets of strides");
   MB_REQUIRE_INIT();
   if (rows == 0 || heads == 0) return MIMIR_B200_OK;
-  MB_TRY(check_device_pointer("rope", "positions", positions));
+  MB_TRY(check_device_words("rope", "positions", positions));
   MB_TRY(check_device_pointer("rope", "x", x));
   MB_TRY(check_device_pointer("rope", "y", y));
   const uintptr_t size = static_cast<uintptr_t>(type_bytes(type));
@@ -163,7 +173,7 @@ int mimir_b200_dev_cache_read(const MimirPagedCache* cache, const MimirPagedBatc
   PagedView p = {};
   MB_TRY(check_row_tensors("cache_read", k, v, type, row_stride, head_stride));
   MB_TRY(check_pointers("cache_read", cache, batch, &p, false));
-  MB_TRY(check_device_pointer("cache_read", "out_start", out_start));
+  MB_TRY(check_device_words("cache_read", "out_start", out_start));
   return launch_cache_read(p, cache->type, out_start, out_rows, k, v, type, row_stride, head_stride, static_cast<cudaStream_t>(stream));
 }
 
@@ -182,15 +192,15 @@ int mimir_b200_dev_paged_attention(const MimirPagedCache* cache, const MimirPage
   MB_TRY(check_attention("paged_attention", cache, batch, attention, &l));
   MB_REQUIRE_INIT();
   if (l.p.n_seqs == 0 || l.p.n_rows == 0 || l.p.max_rows == 0) return MIMIR_B200_OK;
-  const int max_rows = l.p.max_rows;
+  const int max_rows = l.p.max_rows, max_kv = l.p.max_kv;
   MB_TRY(check_device_pointer("paged_attention", "q", l.q));
   MB_TRY(check_device_pointer("paged_attention", "out", l.out));
-  if (l.lse) MB_TRY(check_device_pointer("paged_attention", "lse", l.lse));
+  if (l.lse) MB_TRY(check_device_words("paged_attention", "lse", l.lse));
   if (l.ws) MB_TRY(check_device_pointer("paged_attention", "workspace", l.ws));
-  if (!aligned16(l.q) || !aligned16(l.out) || !aligned16(l.ws) || (reinterpret_cast<uintptr_t>(l.lse) & 3))
+  if (!aligned16(l.q) || !aligned16(l.out) || !aligned16(l.ws))
     return fail(MIMIR_B200_E_UNSUPPORTED, "paged_attention: q, out and workspace start on 16 bytes");
   MB_TRY(check_pointers("paged_attention", cache, batch, &l.p, true));
-  l.p.max_rows = max_rows;
+  l.p.max_rows = max_rows, l.p.max_kv = max_kv;
   return launch_paged_attention(l, static_cast<cudaStream_t>(stream));
 }
 
@@ -203,13 +213,13 @@ int mimir_b200_dev_sample_rows(const void* logits, int type, long long rows, int
   MB_REQUIRE_INIT();
   if (rows == 0) return MIMIR_B200_OK;
   MB_TRY(check_device_pointer("sample_rows", "logits", logits));
-  MB_TRY(check_device_pointer("sample_rows", "uniform", uniform));
-  MB_TRY(check_device_pointer("sample_rows", "ids", ids));
-  if (temperature) MB_TRY(check_device_pointer("sample_rows", "temperature", temperature));
-  if (top_k) MB_TRY(check_device_pointer("sample_rows", "top_k", top_k));
-  if (top_p) MB_TRY(check_device_pointer("sample_rows", "top_p", top_p));
-  if (min_p) MB_TRY(check_device_pointer("sample_rows", "min_p", min_p));
-  if (logprob) MB_TRY(check_device_pointer("sample_rows", "logprob", logprob));
+  MB_TRY(check_device_words("sample_rows", "uniform", uniform));
+  MB_TRY(check_device_words("sample_rows", "ids", ids));
+  if (temperature) MB_TRY(check_device_words("sample_rows", "temperature", temperature));
+  if (top_k) MB_TRY(check_device_words("sample_rows", "top_k", top_k));
+  if (top_p) MB_TRY(check_device_words("sample_rows", "top_p", top_p));
+  if (min_p) MB_TRY(check_device_words("sample_rows", "min_p", min_p));
+  if (logprob) MB_TRY(check_device_words("sample_rows", "logprob", logprob));
   if (reinterpret_cast<uintptr_t>(logits) % static_cast<uintptr_t>(type_bytes(type))) return fail(MIMIR_B200_E_INVALID, "sample_rows: misaligned logits");
   SampleLaunch s = {};
   s.x = logits, s.rows = rows, s.row_stride = row_stride, s.n = n, s.type = type;

@@ -119,6 +119,35 @@ def test_cache_write_and_read(backend, cache, type_, order):
             assert (got[which][-1] == -7.0).all()
 
 
+@pytest.mark.parametrize("cache,type_", [(F16, F16), (E4M3, BF16)])
+def test_cache_of_many_heads_and_sequences(backend, cache, type_):
+    """More heads than a block moves at once, more sequences than it keeps the starts of."""
+    rng = np.random.default_rng(1)
+    for n_seqs, heads, dim in ((3, 70, 64), (1100, 2, 16)):
+        rows = [int(v) for v in rng.integers(0, 3, n_seqs)]
+        kv = [n + int(v) for n, v in zip(rows, rng.integers(0, 9, n_seqs))]
+        p, q = (Pages(rows, kv, heads, dim, 8, cache, seed=2) for _ in range(2))
+        k, v = (normal(p.n_rows, heads, dim, seed=s, dtype=TORCH[type_]) for s in (1, 2))
+        backend.dev_cache_write(p.cache(), p.batch(), k.data_ptr(), v.data_ptr(), type_, heads * dim, dim)
+        for s in range(n_seqs):
+            if rows[s]:
+                for which, x in ((0, k), (1, v)):
+                    q.put(which, s, np.arange(kv[s] - rows[s], kv[s]), x[q.starts[s] : q.starts[s + 1]])
+        for a, b in zip(p.pool + p.scale, q.pool + q.scale):
+            if a is not None:
+                a, b = a.float(), b.float()
+                assert ((a == b) | (a.isnan() & b.isnan())).all()
+        p.fill(seed=4)
+        starts = np.concatenate([[0], np.cumsum(kv)]).astype(np.int32)
+        o = torch.from_numpy(starts).cuda()
+        got = [torch.full((int(starts[-1]), heads, dim), -7.0, dtype=TORCH[type_], device="cuda") for _ in range(2)]
+        backend.dev_cache_read(p.cache(), p.batch(), o.data_ptr(), int(starts[-1]), got[0].data_ptr(), got[1].data_ptr(), type_, heads * dim, dim)
+        backend.check_device()
+        for which in range(2):
+            want = np.concatenate([p.get(which, s) for s in range(n_seqs)])
+            assert torch.equal(got[which].cpu(), torch.from_numpy(want).float().to(TORCH[type_]))
+
+
 @pytest.mark.parametrize("cache", [I8, E4M3])
 def test_codes_of_values_that_are_not_finite(backend, cache):
     p = Pages([4], [4], 1, 8, 8, cache)
@@ -228,6 +257,98 @@ def test_chunks_whose_score_tiles_alternate_many_times_over(backend, cache, type
         backend.dev_paged_attention(p.cache(), p.batch(), a)
     backend.check_device()
     assert torch.equal(outs[0], out)
+
+
+@pytest.mark.parametrize("cache,type_", [(BF16, BF16), (F16, F32), (I8, F16)])
+def test_attention_of_many_sequences(backend, cache, type_):
+    """More sequences than a warp has lanes, of no, few and many rows in no order; rows behind the last one stay."""
+    rng = np.random.default_rng(4)
+    rows = [int(rng.choice([0, 1, 1, 1, 16, 17, 40, 150])) for _ in range(83)] + [0, 0, 133]
+    kv = [int(max(0, r + rng.integers(-3, 90))) for r in rows]
+    p = Pages(rows, kv, 2, 64, 16, cache, seed=8)
+    p.fill()
+    q, out, lse = attend(backend, p, 4, type_, window=50, extra_rows=5)
+    backend.check_device()
+    check_attention(p, q, out, lse, type_, True, 50)
+
+
+@pytest.mark.parametrize("cache,type_", [(BF16, BF16), (F16, F32), (I8, F16), (F32, F32)])
+@pytest.mark.parametrize("rows,group", [([1, 1, 0, 1], 48), ([1], 71), ([2, 1], 40)])
+def test_attention_of_one_key_head_for_many(backend, rows, group, cache, type_):
+    """A single token's heads alone are more rows than a tile of few."""
+    p = Pages(rows, [900, 33, 5, 1][: len(rows)], 1, 64, 16, cache, seed=8)
+    p.fill()
+    q, out, lse = attend(backend, p, group, type_)
+    backend.check_device()
+    check_attention(p, q, out, lse, type_, True, 0)
+
+
+def test_attention_with_the_largest_window_and_limits(backend):
+    """Numbers at the end of their range: a window that nothing fills is none, limits are limits."""
+    most = 2**31 - 1
+    for rows in ([3, 1], [60, 2]):
+        p = Pages(rows, [50, 40], 1, 64, 16, F16, seed=8)
+        p.fill()
+        q, out, lse = attend(backend, p, 2, F16, window=most)
+        check_attention(p, q, out, lse, F16, True, 0)
+        got = out.clone()
+        q, out, lse = attend(backend, p, 2, F16, window=most, max_kv=most, max_rows=most)
+        backend.check_device()
+        check_attention(p, q, out, lse, F16, True, 0)
+
+
+@pytest.mark.parametrize("rows", [[1, 2], [140, 3]])
+@pytest.mark.parametrize("cache,type_", [(BF16, BF16), (F16, F16), (E4M3, BF16), (I8, F32)])
+def test_attention_over_large_pages(backend, rows, cache, type_):
+    for page, order in ((256, "head"), (1000, "slot")):
+        p = Pages(rows, [1300, 999], 1, 128, page, cache, order, seed=3)
+        p.fill()
+        q, out, lse = attend(backend, p, 2, type_)
+        backend.check_device()
+        check_attention(p, q, out, lse, type_, True, 0)
+
+
+@pytest.mark.parametrize("rows,kv", [([2, 1], [15000, 2]), ([90, 1, 3], [6000, 4000, 70]), ([300, 40], [310, 7000])])
+def test_attention_on_two_streams_and_captured(backend, rows, kv):
+    """Two batches at once, each with its workspace, and a captured call that is replayed over other lengths and pages."""
+    ps = [Pages(rows, kv, 1, 64, 16, F16, seed=s) for s in (1, 2)]
+    calls, keep = [], []
+    for i, p in enumerate(ps):
+        p.fill(seed=i)
+        q = normal(p.n_rows, 2, 64, seed=i, dtype=torch.float16)
+        out, lse = torch.full_like(q, -7.0), torch.full((p.n_rows, 2), -7.0, device="cuda")
+        a = backend.paged_attention(q.data_ptr(), out.data_ptr(), F16, 2, 128, 64, 128, 64, 0.125, lse=lse.data_ptr())
+        ws = torch.full((backend.paged_attention_workspace(p.cache(), p.batch(), a) + 16,), 255, dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        calls.append(a)
+        keep.append((q, out, lse, ws))
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for p, a, s in zip(ps, calls, streams):
+            backend.dev_paged_attention(p.cache(), p.batch(), a, s.cuda_stream)
+    torch.cuda.synchronize()
+    backend.check_device()
+    for p, (q, out, lse, _) in zip(ps, keep):
+        check_attention(p, q, out, lse, F16, True, 0)
+    p, a, (q, out, lse, _) = ps[0], calls[0], keep[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        backend.dev_paged_attention(p.cache(), p.batch(), a, streams[0].cuda_stream)
+    # fewer rows in each sequence, in other places: the rest of the rows stay
+    r = Pages([(n + 1) // 2 for n in rows], [n - 1 for n in kv], 1, 64, 16, F16, seed=5, spare=0)
+    r.table = np.where(r.table >= 0, r.table + 1, r.table)[:, : p.width]
+    r.n_pages, r.pool, r.width = p.n_pages, p.pool, p.width
+    r.table = np.pad(r.table, ((0, 0), (0, p.width - r.table.shape[1])), constant_values=-77)
+    r.fill(seed=9)
+    for here, new in zip(p.dev, (r.starts, r.kv, r.table)):
+        here.copy_(torch.from_numpy(np.asarray(new, np.int32)))
+    out.fill_(-7.0)
+    lse.fill_(-7.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    backend.check_device()
+    check_attention(r, q, out, lse, F16, True, 0)
 
 
 @pytest.mark.parametrize("cache,type_", [(BF16, BF16), (E4M3, F16), (F16, BF16)])
@@ -390,6 +511,27 @@ def test_refusals_of_pointers(backend):
     backend.check_device()
 
 
+def test_refusals_of_words_off_their_boundary(backend):
+    p = Pages([1], [40], 2, 64, 16, I8, seed=9)
+    x = normal(1, 4, 64, dtype=torch.float16)
+    room = torch.zeros(64, dtype=torch.int32, device="cuda")
+    odd, ok = room.data_ptr() + 2, room.data_ptr()
+    att = backend.paged_attention(x.data_ptr(), x.data_ptr(), F16, 4, 256, 64, 256, 64, 0.125)
+    lse = backend.paged_attention(x.data_ptr(), x.data_ptr(), F16, 4, 256, 64, 256, 64, 0.125, lse=odd)
+    for f in (lambda: backend.dev_paged_attention(p.cache(), p.batch(row_start=odd), att), lambda: backend.dev_paged_attention(p.cache(), p.batch(kv_len=odd), att),
+              lambda: backend.dev_paged_attention(p.cache(), p.batch(page_table=odd), att), lambda: backend.dev_paged_attention(p.cache(), p.batch(), lse),
+              lambda: backend.dev_cache_write(p.cache(), p.batch(kv_len=odd), x.data_ptr(), x.data_ptr(), F16, 128, 64),
+              lambda: backend.dev_cache_read(p.cache(), p.batch(), odd, 1, x.data_ptr(), x.data_ptr(), F16, 128, 64),
+              lambda: backend.dev_rope(backend.rope_plan(64), odd, x.data_ptr(), x.data_ptr(), 1, 4, 64, (256, 64), (256, 64), F16),
+              lambda: backend.dev_sample_rows(x.data_ptr(), F16, 1, 256, 256, None, None, None, None, odd, ok),
+              lambda: backend.dev_sample_rows(x.data_ptr(), F16, 1, 256, 256, None, odd, None, None, ok, ok),
+              lambda: backend.dev_sample_rows(x.data_ptr(), F16, 1, 256, 256, None, None, None, None, ok, odd)):
+        with pytest.raises(backend.MimirB200Error, match="aligned") as e:
+            f()
+        assert e.value.status == abi.E_INVALID
+    backend.check_device()
+
+
 # ---- sampling -------------------------------------------------------------------------------------------------------------------------
 def draw(backend, x, t=None, k=None, p=None, m=None, u=None, type_=F32, stride=None):
     rows, n = x.shape
@@ -428,6 +570,31 @@ def test_sampling(backend, rows, n, type_):
         check_sample(x, t, kk, pp, mm, u, ids, logp)
     ids, logp = draw(backend, x, None, None, None, None, u, type_)
     check_sample(x, None, None, None, None, u, ids, logp)
+
+
+@pytest.mark.parametrize("n,type_", [(400_003, F32), (1_500_001, BF16)])
+def test_sampling_of_rows_beyond_shared_memory(backend, n, type_):
+    x = normal(2, n, seed=n, scale=3.0, dtype=TORCH[type_])
+    g = np.random.default_rng(n)
+    for k, p, m in [(0, 1.0, 0.0), (40, 0.9, 0.0), (5000, 0.8, 0.0), (0, 0.95, 0.02), (0, 0.5, 0.0), (n - 7, 0.999, 0.0)]:
+        u = torch.from_numpy(g.random(2).astype(np.float32)).cuda()
+        kk, pp, mm = torch.full((2,), k, dtype=torch.int32, device="cuda"), torch.full((2,), p, device="cuda"), torch.full((2,), m, device="cuda")
+        ids, logp = draw(backend, x, None, kk, pp, mm, u, type_)
+        check_sample(x, None, kk, pp, mm, u, ids, logp)
+
+
+def test_sampling_with_parameters_that_are_no_numbers(backend):
+    """Not a number: the largest logit (temperature), all (top_p, min_p), the first that stays (uniform)."""
+    x = normal(6, 2000, seed=3, scale=2.0)
+    u, ones = torch.full((6,), 0.4, device="cuda"), torch.ones(6, device="cuda")
+    nan = torch.full((6,), float("nan"), device="cuda")
+    ids, _ = draw(backend, x, nan, None, None, None, u)
+    assert np.array_equal(ids, x.argmax(1).cpu().numpy())
+    want = draw(backend, x, ones, None, None, None, u)
+    for got in (draw(backend, x, ones, None, nan, None, u), draw(backend, x, ones, None, None, nan, u)):
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    ids, _ = draw(backend, x, ones, torch.full((6,), 3, dtype=torch.int32, device="cuda"), None, None, nan)
+    assert np.array_equal(ids, x.topk(3, 1).indices.min(1).values.cpu().numpy())
 
 
 def test_sampling_of_equal_and_absent_logits(backend):

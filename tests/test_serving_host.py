@@ -125,6 +125,19 @@ def test_attention_refuses(name, value, status):
         assert e.value.status == status
 
 
+@pytest.mark.parametrize("name,value", [("c_slot_stride", 0), ("c_head_stride", 0), ("c_page_stride", 0), ("c_page_stride", 1 << 38), ("c_slot_stride", 1 << 38)])
+def test_cache_strides_that_fold_or_run_away_are_refused(name, value):
+    test_cache_calls_refuse_sizes(name, value, abi.E_UNSUPPORTED)
+
+
+def test_more_rows_and_heads_than_32_bits_are_refused():
+    cache, batch, att = call(b_n_rows=1 << 29, b_max_rows=1 << 29, a_heads=4)
+    for f in (lambda: rt.dev_paged_attention(cache, batch, att), lambda: rt.paged_attention_workspace(cache, batch, att)):
+        with pytest.raises(rt.MimirB200Error, match="too many rows") as e:
+            f()
+        assert e.value.status == abi.E_INVALID
+
+
 def test_row_types_and_sizes_are_refused():
     cache, batch, _ = call()
     plan = rt.rope_plan(64)
