@@ -583,6 +583,21 @@ def test_sampling_of_rows_beyond_shared_memory(backend, n, type_):
         check_sample(x, None, kk, pp, mm, u, ids, logp)
 
 
+@pytest.mark.parametrize("rows,n,type_", [(200, 1000, F32), (96, 32000, BF16), (40, 151936, F16)])
+def test_sampling_by_mass_and_by_least_share(backend, rows, n, type_):
+    """min_p leaves a few or many, and top_p takes some of them or none; shares that meet the border exactly."""
+    x = normal(rows, n, seed=n + 1, scale=2.5, dtype=TORCH[type_])
+    x[::7] = x[::7].round() / 2  # (many equals)
+    x[1] = 0.0
+    x[2, 3:] = -20.0
+    g = np.random.default_rng(n)
+    for _ in range(4):
+        u, t, p, m = (torch.from_numpy(v.astype(np.float32)).cuda() for v in (g.random(rows), g.uniform(0.3, 2.0, rows), 1 - 10 ** g.uniform(-3, -0.2, rows), 10 ** g.uniform(-4, -0.2, rows)))
+        p[1], p[2], p[3] = 0.5, 0.25, 0.0
+        ids, logp = draw(backend, x, t, None, p, m, u, type_)
+        check_sample(x, t, None, p, m, u, ids, logp)
+
+
 def test_sampling_with_parameters_that_are_no_numbers(backend):
     """Not a number: the largest logit (temperature), all (top_p, min_p), the first that stays (uniform)."""
     x = normal(6, 2000, seed=3, scale=2.0)
