@@ -619,12 +619,14 @@ Share share_out(const AttendLaunch& a) {
   }
   if (!r.rows) return r;
   // A cluster of up to eight CTAs meets through shared memory at no extra launch; beyond that (few tiles, long sequences) clusters
-  // leave parts in the workspace for a second launch.
+  // leave parts in the workspace for a second launch.  Clusters until there are as many CTAs as SMs: blocks cost a few us to start and meet.
+  // 8 key heads of 128, 16 sequences of up to 4 K keys 61 us (up to three CTAs a slot: 78), of up to 1 K 18 (25), 32 of up to 4 K 90 (101), one of
+  // 4 K 9.1 (single CTAs: 15).
   const long long few = r.chunks ? TC_FEW : most;
   r.tiles = static_cast<int>((few + PA_ROWS - 1) / PA_ROWS);
   r.units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tiles;
   const long long slots = 2LL * ctx().sm_count;
-  while (r.cluster < 8 && r.units * r.cluster < 3 * slots && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
+  while (r.cluster < 8 && r.units * r.cluster < ctx().sm_count && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
   while (r.units * r.cluster * r.splits < slots && keys >= 512 * 2 * r.cluster * r.splits) r.splits *= 2;
   if (r.splits > 1) r.bytes = static_cast<size_t>(r.units) * r.splits * PA_ROWS * row_bytes;
   return r;
