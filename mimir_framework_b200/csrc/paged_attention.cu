@@ -14,6 +14,8 @@
 // largest to [1, 2).  Probabilities are two terms for bfloat16 caches too (16 bits), one half (11 bits) where only the result is bfloat16.
 // Codes of eight bits are exact in half; their scales multiply scores and probabilities.  For fp32 results each block's P V starts from
 // zero and is added in fp32, because the tensor core's accumulation truncates (1.5e-8 of the value an instruction).
+// 64 sequences of up to 4 K bfloat16 keys, 8 key heads of 128: 163 us, 0.76 of the copy rate (bytes in flight: eight warps an SM, whose registers
+// hold them).  4 of up to 128 K e4m3 keys: 209 us, 0.69 of it (codes become halves on the ordinary lanes).
 #include <cmath>
 
 #include "common.h"
@@ -614,7 +616,13 @@ Share share_out(const AttendLaunch& a) {
     const long long all = static_cast<long long>(a.p.n_rows) * group, chunks = all / (r.few + 1) < a.p.n_seqs ? all / (r.few + 1) : a.p.n_seqs;
     const long long longest = a.p.n_seqs * ((most + per - 1) / per);
     r.tc_units = a.p.kv_heads * (all / per + chunks < longest ? all / per + chunks : longest);
-    while (r.tc_units * r.tc_splits * 2 <= ctx().sm_count && keys >= 1024 * r.tc_splits) r.tc_splits *= 2;
+    // Keys are split while SMs are idle and it pays: 1.25 us a key tile (of 128 elements), against a second launch and the parts written and read
+    // at 3 TB/s.  512 tokens of 32 heads over 1 K keys 28 us whole, 44 in two; over 8 K 127 and 95; 64 tokens over 8 K 124 and, in eight, 34.
+    auto time = [&](int splits) {
+      const double tiles = static_cast<double>((keys + TC_KEYS - 1) / TC_KEYS) / splits;
+      return 1.25 * tiles * a.p.head_dim / 128 + (splits > 1 ? 3.0 + 2e-6 / 3 * static_cast<double>(r.tc_units) * splits * per * row_bytes : 0.0);
+    };
+    while (r.tc_units * r.tc_splits * 2 <= ctx().sm_count && keys >= 2 * TC_KEYS * r.tc_splits && time(2 * r.tc_splits) < time(r.tc_splits)) r.tc_splits *= 2;
     if (r.tc_splits > 1) r.tc_bytes = static_cast<size_t>(r.tc_units) * r.tc_splits * per * row_bytes;
   }
   if (!r.rows) return r;
@@ -627,7 +635,11 @@ Share share_out(const AttendLaunch& a) {
   r.units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tiles;
   const long long slots = 2LL * ctx().sm_count;
   while (r.cluster < 8 && r.units * r.cluster < ctx().sm_count && keys >= 128 * 2 * r.cluster) r.cluster *= 2;
-  while (r.units * r.cluster * r.splits < slots && keys >= 512 * 2 * r.cluster * r.splits) r.splits *= 2;
+  // Parts: 512 keys a CTA or more while all CTAs find room at once, 2048 or more where that takes a second round (8 of 4 K keys 29 us in one, 41 in
+  // two; 4 of 128 K e4m3 keys 243 and 206).
+  while (r.units * r.cluster * r.splits < slots &&
+         keys >= (r.units * r.cluster * r.splits * 2 <= slots ? 512 : 2048) * 2LL * r.cluster * r.splits)
+    r.splits *= 2;
   if (r.splits > 1) r.bytes = static_cast<size_t>(r.units) * r.splits * PA_ROWS * row_bytes;
   return r;
 }

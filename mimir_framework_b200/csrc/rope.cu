@@ -5,6 +5,7 @@
 // fraction itself, exact in the integer product; what is off is step_i's rounding alone, position * 2^-65 turns.  (In fp32 the
 // angle of position 100 000 would be off by up to 0.004.)  The quadrant comes off in integers, and the rest, at most an eighth of
 // a turn, becomes fp32 with its full 24 bits.
+// Bound by its bytes: 8192 rows of 40 heads of 128 in fp32, 64 of them turned, 54 us, 0.95 of the rate of a plain copy.
 #include <cmath>
 
 #include "common.h"
