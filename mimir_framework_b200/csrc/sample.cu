@@ -886,10 +886,12 @@ int launch_as(const SampleLaunch& s, int cluster, int slice, cudaStream_t st) {
 template <int T>
 int launch_t(const SampleLaunch& s, cudaStream_t st) {
   constexpr int STEP = 32 * Vec<T>::N;  // a warp's vectors
-  // as few CTAs as hold the row two to an SM, more while SMs would be idle and each keeps a few thousand logits
-  const int fits = static_cast<int>(SA_SLICE) / type_bytes(T);
+  // As few CTAs as hold the row two to an SM, and one to an SM rather than eight (clusters of eight start late and leave SMs idle): 128 rows of
+  // 128 K fp32 logits 57 us in four, 71 in eight.  More while half the SMs are idle and each keeps a few thousand logits: 64 rows of 32 K
+  // 12 us in one, 26 in eight; one of 128 K 13 in eight.
   int cluster = 1;
-  while (cluster < 8 && (static_cast<long long>(cluster) * fits < s.n || (s.rows * cluster < 2LL * ctx().sm_count && s.n / cluster >= 4096))) cluster *= 2;
+  auto holds = [&](int n) { return static_cast<long long>(n) * static_cast<long long>((n < 4 ? SA_SLICE : SA_LARGE) / type_bytes(T)) >= s.n; };
+  while (cluster < 8 && (!holds(cluster) || (2 * s.rows * cluster < ctx().sm_count && s.n / cluster >= 4096))) cluster *= 2;
   const long long each = (s.n + cluster - 1) / cluster;
   const int slice = static_cast<int>((each + STEP - 1) / STEP * STEP);
   if (s.rows * cluster > 0x7fffffffLL) return fail(MIMIR_B200_E_INVALID, "sample_rows: too many rows for one call");
