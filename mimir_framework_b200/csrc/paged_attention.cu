@@ -598,19 +598,25 @@ struct Share {
   size_t bytes = 0, tc_bytes = 0;
 };
 // Up to how many rows of a head go to the row kernel.  Up to 4 x 8 K keys, 8 key heads of 128, here and by tcgen05: 32 rows 57 and 53 us in
-// bfloat16, 47 and 78 over int8, 76 and 49 for fp32; 64 rows 111 and 54 us in bfloat16.
-constexpr int TC_FEW = 32;
+// bfloat16, 47 and 78 over int8, 76 and 49 for fp32; 64 rows 111 and 54 us in bfloat16.  Codes cost tcgen05 a pass through registers and shared
+// memory: 64 rows of 4 x up to 128 K e4m3 keys 686 and 1006 us, 64 x up to 4 K 348 and 416, 128 rows 620 and 443; not so heads over 128 (int8, 64
+// rows 824 and 614) or fp32 queries (456 and 436), whose share here grows as well.
+int few_rows(const AttendLaunch& a) {
+  const bool codes = a.cache_type == MIMIR_B200_T_I8 || a.cache_type == MIMIR_B200_T_E4M3;
+  return codes && a.type != MIMIR_B200_T_F32 && a.p.head_dim <= 128 ? 64 : 32;
+}
 Share share_out(const AttendLaunch& a) {
   Share r;
   const int group = a.heads / a.p.kv_heads;
   const long long most = static_cast<long long>(a.p.max_rows) * group;
+  const int most_few = few_rows(a);
   const int keys = a.window > 0 && a.window < a.p.max_kv ? a.window : a.p.max_kv;  // (of a row; a chunk sees a little more)
   const size_t row_bytes = a.p.head_dim * sizeof(float) + sizeof(float2);
-  if (tc_takes(a.cache_type, a.type, a.p.head_dim) && most > TC_FEW) {
+  if (tc_takes(a.cache_type, a.type, a.p.head_dim) && most > most_few) {
     r.chunks = true;
     // (one sequence: its rows are many, and so are those of one token of a large group; of several sequences some may have few)
-    r.rows = a.p.n_seqs > 1 && group <= TC_FEW;
-    r.few = r.rows ? TC_FEW : 0;
+    r.rows = a.p.n_seqs > 1 && group <= most_few;
+    r.few = r.rows ? most_few : 0;
     const int per = tc_tile_rows(a.type, a.p.head_dim);
     // at most so many tiles: full ones, and one of each sequence of more than `few` rows that is not
     const long long all = static_cast<long long>(a.p.n_rows) * group, chunks = all / (r.few + 1) < a.p.n_seqs ? all / (r.few + 1) : a.p.n_seqs;
@@ -630,7 +636,7 @@ Share share_out(const AttendLaunch& a) {
   // leave parts in the workspace for a second launch.  Clusters until there are as many CTAs as SMs: blocks cost a few us to start and meet.
   // 8 key heads of 128, 16 sequences of up to 4 K keys 61 us (up to three CTAs a slot: 78), of up to 1 K 18 (25), 32 of up to 4 K 90 (101), one of
   // 4 K 9.1 (single CTAs: 15).
-  const long long few = r.chunks ? TC_FEW : most;
+  const long long few = r.chunks ? most_few : most;
   r.tiles = static_cast<int>((few + PA_ROWS - 1) / PA_ROWS);
   r.units = static_cast<long long>(a.p.n_seqs) * a.p.kv_heads * r.tiles;
   const long long slots = 2LL * ctx().sm_count;
