@@ -198,6 +198,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     }
     // (fp32: the tensor core's sums are low by 1.5e-8 of their value an instruction)
     c2 = fabsf(a.scale) * LOG2E * up * (NQ == 2 ? 1.0f + 1.5e-8f * (DP / 8) : 1.0f);
+    c2 = fmaxf(c2, 0x1p-149f);  // (masked scores are -infinity before they are multiplied: a scale of zero would make them no numbers)
     if (a.scale < 0.0f) down = -down;  // (the largest product is then the smallest score's)
     for (int c = 0; c < DP / 8; ++c) {
       float f[8];

@@ -1,0 +1,60 @@
+"""Serving calls at the ends of what they accept."""
+import numpy as np
+import pytest
+import torch
+
+from mimir_framework_b200 import abi
+from serving_ref import TORCH, Pages, attention, attention_bounds
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16, I8, E4M3 = abi.T_F32, abi.T_F16, abi.T_BF16, abi.T_I8, abi.T_E4M3
+
+
+def normal(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def attend(backend, p, q, type_, scale, causal=True, window=0, **batch):
+    """out and lse of q [rows][heads][dim] over the pages."""
+    rows, heads, dim = q.shape
+    out, lse = torch.full_like(q, -7.0), torch.full((rows, heads), -7.0, device="cuda")
+    b = p.batch(**batch)
+    a = backend.paged_attention(q.data_ptr(), out.data_ptr(), type_, heads, heads * dim, dim, heads * dim, dim, scale, causal, window, lse.data_ptr())
+    size = backend.paged_attention_workspace(p.cache(), b, a)
+    ws = torch.full((size + 16,), 255, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), size
+    backend.dev_paged_attention(p.cache(), b, a)
+    torch.cuda.synchronize()
+    backend.check_device()
+    return out, lse
+
+
+def held(p, q, out, lse, type_, scale, causal, window, chunk):
+    want, want_lse, weight, reach = attention(p, q.double().cpu().numpy(), scale, causal, window)
+    bound, lse_bound = attention_bounds(want, weight, reach, p.dim, max(p.kv), BF16 if p.type == BF16 else type_, chunk and type_ != F32,
+                                        type_ == BF16 and p.type != BF16)
+    err = np.abs(out.double().cpu().numpy() - want)
+    assert np.all(err <= bound), f"{np.max(err / np.maximum(bound, 1e-300))} of the bound"
+    got, some = lse.double().cpu().numpy(), ~np.isneginf(want_lse)
+    assert np.array_equal(~np.isneginf(got), some)
+    got, want_lse, lse_bound = got[some], want_lse[some], lse_bound[some]
+    assert np.all(np.abs(got - want_lse) <= lse_bound + np.abs(want_lse) * 2.0**-22)
+
+
+# ---- scores --------------------------------------------------------------------------------------------------------------------------
+PAIRS = [(BF16, BF16), (F16, F16), (F16, BF16), (F16, F32), (I8, F16), (I8, BF16), (I8, F32), (E4M3, F16), (E4M3, BF16), (E4M3, F32), (F32, F32)]
+
+
+@pytest.mark.parametrize("cache,type_", PAIRS)
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-30, -1e-30])
+@pytest.mark.parametrize("rows,kv,dim,causal,window", [([150, 3], [400, 130], 64, True, 0), ([140, 70], [300, 50], 64, True, 33), ([160], [333], 128, False, 0)])
+def test_a_scale_of_zero_or_next_to_it_is_the_mean(backend, rows, kv, dim, causal, window, scale, cache, type_):
+    """Many rows and few; some queries are all zeros, whose products vanish with the scale."""
+    p = Pages(rows, kv, 1, dim, 16, cache, seed=dim)
+    p.fill()
+    q = normal(p.n_rows, 2, dim, seed=3, dtype=TORCH[type_])
+    q[::5] = 0.0
+    out, lse = attend(backend, p, q, type_, scale, causal, window)
+    held(p, q, out, lse, type_, scale, causal, window, True)
