@@ -50,9 +50,10 @@ struct TcShape {
   static_assert(!CODED || NT * 128 * SOFT_REGS + 256 * LOAD_REGS == THREADS * LAUNCH_REGS, "register shares");
 };
 
+// (not a number where one of them is: it decides which exponentials a tile gets)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // (64 elements, slots, head, page)
@@ -79,10 +80,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 // 2^x on the FMA lanes, for x of at most 127 (below -126: 2^-126): x = n + f, |f| <= 1/2, and the polynomial of fourth degree in f whose
 // largest relative error is least (2.6e-6, by Remez' exchange); n goes into the exponent.  A share of the exponentials done so leaves the
-// special-function lanes, 16 a cycle and SM, less to do.
+// special-function lanes, 16 a cycle and SM, less to do.  What is not a number may come out as one: callers do without it then.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // (-126; what is not a number stays so)
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
   const float2 m = add2(x, make_float2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: n in the low bits
   const float2 n = add2(m, make_float2(-12582912.0f, -12582912.0f));
   const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
@@ -491,7 +491,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         float m4[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(w[i]), __uint_as_float(w[i + 1]));
-        return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        return max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]);
       };
       float grow = 0.0f;
       if constexpr (CODED) {
@@ -558,7 +558,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         return mx * c2;
       };
       // a first maximum where a row of the warp has none yet; after that the present one is used at once, and only where a score outgrows it
-      // by more than 2^8 (a few times a row) are the tile's probabilities computed again by a new one
+      // by more than 2^8 (a few times a row), or is not a number, are the tile's probabilities computed again by a new one and without polynomials
       if (__any_sync(0xffffffffu, base == -INFINITY) || (CODED && grow > v_unit)) {
         float mx = -INFINITY;
 #pragma unroll
@@ -570,7 +570,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         if (!rescale(mx * c2)) { alive = false; break; }
       }
       const float mx = masked ? weigh_keys(std::false_type()) : weigh_keys(std::integral_constant<bool, NQ == 1>());
-      if (__any_sync(0xffffffffu, mx > base + (8.0f + S::ROOM))) {
+      if (__any_sync(0xffffffffu, !(mx <= base + (8.0f + S::ROOM)))) {
         if (!rescale(mx)) { alive = false; break; }
         weigh_keys(std::false_type());
       }

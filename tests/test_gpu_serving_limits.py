@@ -58,3 +58,27 @@ def test_a_scale_of_zero_or_next_to_it_is_the_mean(backend, rows, kv, dim, causa
     q[::5] = 0.0
     out, lse = attend(backend, p, q, type_, scale, causal, window)
     held(p, q, out, lse, type_, scale, causal, window, True)
+
+
+@pytest.mark.parametrize("cache,type_", [(BF16, BF16), (F16, F16), (F16, BF16), (F16, F32), (F32, F32)])
+@pytest.mark.parametrize("rows,causal", [(150, False), (150, True), (2, False)])
+@pytest.mark.parametrize("at", [0, 6, 7, 14, 29, 127])
+def test_a_key_that_is_no_number_makes_every_row_that_sees_it_none(backend, rows, causal, at, cache, type_):
+    """In any column of a tile without masks and in one with them; rows before it and other heads go on."""
+    kv = 384
+    p = Pages([rows], [kv], 2, 64, 16, cache, seed=2)
+    p.fill()
+    q = normal(rows, 4, 64, seed=3, dtype=TORCH[type_])
+    clean, clean_lse = attend(backend, p, q, type_, 0.125, causal)
+    held(p, q, clean, clean_lse, type_, 0.125, causal, 0, True)
+    for key in (at, 256 + at):
+        page, slot = p.slots(0, 0, [key])
+        where = (int(page[0]), int(slot[0]), 1)
+        kept = p.pool[0][where].clone()
+        p.pool[0][where] = float("nan")
+        out, lse = attend(backend, p, q, type_, 0.125, causal)
+        p.pool[0][where] = kept
+        sees = torch.arange(kv - rows, kv, device="cuda") >= key if causal else torch.ones(rows, dtype=torch.bool, device="cuda")
+        assert out[sees][:, 2:].isnan().all() and lse[sees][:, 2:].isnan().all()
+        out[sees, 2:], lse[sees, 2:] = clean[sees, 2:], clean_lse[sees, 2:]
+        held(p, q, out, lse, type_, 0.125, causal, 0, True)
