@@ -9,8 +9,8 @@
 //   2. top_k: counts of 1024 intervals of (max - x) / T and the interval in which the border lies.  Up to 1024 logits down to that
 //      are gathered, sorted and finished in one CTA; else the border itself is found among the interval's
 //      top_p: rough masses of the intervals (one 32-bit addition in shared memory a logit) say between which two the border lies, a
-//      part in 2^10 of the mass to either side.  Where min_p ends before them, top_p takes nothing away.  Else every weight is taken
-//      exactly, what lies between the two is listed, and the border found among it.
+//      part in 2^10 of the mass to either side, and what n roundings to units of 2^-30 may add.  Where min_p ends before them, top_p
+//      takes nothing away.  Else every weight is taken exactly, what lies between the two is listed, and the border found among it.
 //      min_p and top_p: what min_p leaves is summed roughly first, and mostly that is enough
 //      A border among logits: up to 1024 are sorted in one CTA; more are divided by their bits until they are fewer or all the same
 //   3. masses of the warps' stretches of the row in index order; the stretch in which u falls is walked
@@ -693,7 +693,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         }
         u64 ahead = block_scan(m[0] + m[1], sh.scan64, &all);
         const double near = static_cast<double>(top_p) * 0x1p30;
-        const double low = near - 0x1p20, high = near + 0x1p20;
+        // (each of n logits is rounded to a unit: up to half of one off, all the same way where they are alike)
+        const double slack = 0x1p20 + 0.5 * n, low = near - slack, high = near + slack;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = 2 * tid + h;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from mimir_framework_b200 import abi
-from serving_ref import TORCH, Pages, attention, attention_bounds
+from serving_ref import TORCH, Pages, attention, attention_bounds, sample
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16, I8, E4M3 = abi.T_F32, abi.T_F16, abi.T_BF16, abi.T_I8, abi.T_E4M3
@@ -82,3 +82,25 @@ def test_a_key_that_is_no_number_makes_every_row_that_sees_it_none(backend, rows
         assert out[sees][:, 2:].isnan().all() and lse[sees][:, 2:].isnan().all()
         out[sees, 2:], lse[sees, 2:] = clean[sees, 2:], clean_lse[sees, 2:]
         held(p, q, out, lse, type_, 0.125, causal, 0, True)
+
+
+# ---- sampling ----------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,top_p,min_p,type_", [("many small", 0.998, 0.0015, F32), ("many small", 0.998, 0.0015, BF16), ("equals", 0.995, 0.5, BF16), ("equals", 0.6, 0.5, F16)])
+def test_sampling_by_mass_and_least_share_of_the_most_logits(backend, kind, top_p, min_p, type_):
+    """Shares that are less than a rough sum resolves, or all off the same way."""
+    n = 1 << 24
+    if kind == "many small":  # a quarter at one, the rest at about two thousandths
+        x = torch.full((1, n), -6.25, device="cuda")
+        x[:, ::4] = 0.0
+    else:  # each one's share is nearly half a unit of 2^-30 off
+        x = torch.zeros(1, n, device="cuda")
+        x[:, : n - round(2**30 / 66.49)] = -float("inf")
+    x = x.to(TORCH[type_])
+    u, p, m = (torch.full((1,), v, device="cuda") for v in (0.5 if kind == "many small" else 0.9999, top_p, min_p))
+    ids, logp = torch.full((1,), -7, dtype=torch.int32, device="cuda"), torch.zeros(1, device="cuda")
+    backend.dev_sample_rows(x.data_ptr(), type_, 1, n, n, None, None, p.data_ptr(), m.data_ptr(), u.data_ptr(), ids.data_ptr(), logp.data_ptr())
+    torch.cuda.synchronize()
+    want, lp, _ = sample(x[0].double().cpu().numpy(), 1.0, 0, float(p[0]), float(m[0]), float(u[0]))
+    # the reference adds 2^24 numbers up one after the other: off by up to 2^-29 of 2^22 or so, which is four of the small ones
+    assert abs(int(ids[0]) - want) <= (5 if kind == "many small" else 0)
+    assert abs(float(logp[0]) - lp) <= 2.0**-22 * max(1.0, abs(lp))
