@@ -89,7 +89,7 @@ struct Context {
   std::atomic<uint64_t> launches{0};
   // One device word that kernels with bounded waits set when a wait gives up, read by the calls through an ErrorWatch (ops.h).
   int* dev_error_word = nullptr;
-  std::mutex error_mu;                     // held while the word is looked at on the host and cleared
+  std::mutex error_mu;                     // held while the word, or the findings behind it, are looked at on the host and cleared
   std::vector<int*> error_words;           // page-locked words that no call uses at the moment
   bool host_words = false;                 // these and the blocks exist
   std::vector<uint8_t*> stage_blocks;      // page-locked blocks of STAGE_BYTES, likewise (StageBlock, ops.h)

@@ -6,15 +6,28 @@
 
 namespace mb {
 
+// words[2] = words[1], which is left at zero, in one step: what another stream finds meanwhile is in the one or in the other
+__global__ void take_findings_kernel(int* words) { words[2] = atomicExch(words + 1, 0); }
+
 int paged_flags_read(cudaStream_t st) {
   Context& c = ctx();
   if (!c.paged_used.load()) return MIMIR_B200_OK;
   int flags = 0;
-  MB_CUDA(cudaMemcpyAsync(&flags, c.dev_error_word + 1, sizeof(int), cudaMemcpyDeviceToHost, st));
-  MB_CUDA(cudaStreamSynchronize(st));
+  auto look = [&](int word) -> int {
+    MB_CUDA(cudaMemcpyAsync(&flags, c.dev_error_word + word, sizeof(int), cudaMemcpyDeviceToHost, st));
+    MB_CUDA(cudaStreamSynchronize(st));
+    return MIMIR_B200_OK;
+  };
+  MB_TRY(look(1));
   if (!flags) return MIMIR_B200_OK;
-  MB_CUDA(cudaMemsetAsync(c.dev_error_word + 1, 0, sizeof(int), st));
-  MB_CUDA(cudaStreamSynchronize(st));
+  {
+    std::lock_guard<std::mutex> lk(c.error_mu);  // (words[2] is one call's at a time)
+    take_findings_kernel<<<1, 1, 0, st>>>(c.dev_error_word);
+    MB_CUDA(cudaGetLastError());
+    count_launch();
+    MB_TRY(look(2));
+  }
+  if (!flags) return MIMIR_B200_OK;  // (another thread has them)
   return fail(MIMIR_B200_E_INVALID, "paged batch:%s%s%s", (flags & PAGED_BAD_ROWS) ? " row ranges that do not fit the tensors;" : "",
               (flags & PAGED_BAD_LEN) ? " a key count that does not fit max_kv or the page table;" : "",
               (flags & PAGED_BAD_PAGE) ? " a page number outside the cache;" : "");

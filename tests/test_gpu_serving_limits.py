@@ -1,4 +1,7 @@
 """Serving calls at the ends of what they accept."""
+import threading
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -104,3 +107,54 @@ def test_sampling_by_mass_and_least_share_of_the_most_logits(backend, kind, top_
     # the reference adds 2^24 numbers up one after the other: off by up to 2^-29 of 2^22 or so, which is four of the small ones
     assert abs(int(ids[0]) - want) <= (5 if kind == "many small" else 0)
     assert abs(float(logp[0]) - lp) <= 2.0**-22 * max(1.0, abs(lp))
+
+
+# ---- findings ------------------------------------------------------------------------------------------------------------------------------
+def test_findings_are_reported_once_whoever_asks(backend):
+    """One thread makes bad calls of changing kinds and asks after each; another asks all the time, of another stream.  Every finding reaches one
+    of them, and is gone then."""
+    p = Pages([1], [40], 1, 64, 16, F16, seed=9)
+    p.fill()
+    x = normal(1, 1, 64, dtype=torch.float16)
+    bad_rows, bad_len = torch.tensor([0, 5], dtype=torch.int32, device="cuda"), torch.tensor([99], dtype=torch.int32, device="cuda")
+    bad_page = torch.full_like(p.dev[2], -1)
+    torch.cuda.synchronize()
+    kinds = [("row ranges", p.batch(row_start=bad_rows.data_ptr())), ("key count", p.batch(kv_len=bad_len.data_ptr())), ("page number", p.batch(page_table=bad_page.data_ptr()))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    seen, rounds, stop, trouble = [], [0], threading.Event(), []
+
+    def ask(stream):
+        try:
+            backend.check_device(stream.cuda_stream)
+        except backend.MimirB200Error as e:
+            seen.append(str(e))
+
+    def other():
+        try:
+            torch.cuda.set_device(0)
+            while not stop.is_set():
+                ask(streams[1])
+                rounds[0] += 1
+        except Exception as e:  # (the first thread must not wait for good)
+            trouble.append(e)
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    lost = []
+    try:
+        for i in range(999):
+            what, batch = kinds[i % 3]
+            before = len(seen)
+            backend.dev_cache_write(p.cache(), batch, x.data_ptr(), x.data_ptr(), F16, 64, 64, streams[0].cuda_stream)
+            ask(streams[0])
+            now = rounds[0]
+            # (a finding that the other has taken it has told two rounds later)
+            while not any(what in s for s in seen[before:]) and rounds[0] < now + 2 and not trouble:
+                time.sleep(0)
+            if not any(what in s for s in seen[before:]):
+                lost.append(i)
+    finally:
+        stop.set()
+        thread.join()
+    assert not trouble and not lost, (trouble, len(lost))
+    assert [sum(what in s for s in seen) for what, _ in kinds] == [333, 333, 333]
