@@ -615,8 +615,8 @@ int mimir_b200_dev_cache_read(const MimirPagedCache* cache, const MimirPagedBatc
  * kv_len - rows + i; causal: it sees keys up to its position; window > 0: keys above position - window.  A row that sees no key is
  * zero and its lse -infinity.  Keys and values that no row of the sequence's call sees are not used whatever they hold; a value that some
  * row sees meets the others' zeros and has to be finite.  A sequence has up to 2^30 keys.
- * type (of q and out): F32, F16 or BF16 on caches of type F16, I8, E4M3; BF16 on BF16; F32 on F32 (whose keys and values have the
- * range of the default operand planes, +-65504).  Scores, sums and results are kept in fp32. */
+ * type (of q and out): F32, F16 or BF16 on caches of type F16, I8, E4M3; BF16 on BF16; F32 on F32.  Scores, sums and
+ * results are kept in fp32. */
 typedef struct MimirPagedAttention {
   const void* q;                              /* [n_rows][heads][head_dim], strides in elements, multiples of 8, 16-byte aligned */
   void* out;                                  /* the same shape */

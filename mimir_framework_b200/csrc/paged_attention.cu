@@ -10,8 +10,10 @@
 //            meet in (distributed) shared memory in a fixed order
 //   K        lane (g, t) holds elements 8 t .. 8 t + 7 of each 32 of key g:  two contraction steps
 //   V        lane (g, t) holds elements 8 g .. 8 g + 7 of each 64 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: eight column tiles
-// fp32 queries and probabilities are two IEEE-half terms (hi + lo, 22 bits): queries after a power of two per row has brought their
-// largest to [1, 2).  Probabilities are two terms for bfloat16 caches too (16 bits), one half (11 bits) where only the result is bfloat16.
+// fp32 caches, and what meets them, are two terms of 11 bits with fp32's exponents (hi + lo, m16n8k8): an element keeps 22 bits by itself, whatever
+// is beside it.  Halves would take half the tensor instructions (64 sequences of up to 4 K keys 368 us, 445 so; heads of 64 199 and 218) but cannot
+// hold what is far from one.  Over other caches fp32 queries and probabilities are two IEEE-half terms (22 bits): queries after a power of two per row has brought
+// their largest to [1, 2).  Probabilities are two terms for bfloat16 caches too (16 bits), one half (11 bits) where only the result is bfloat16.
 // Codes of eight bits are exact in half; their scales multiply scores and probabilities.  For fp32 results each block's P V starts from
 // zero and is added in fp32, because the tensor core's accumulation truncates (1.5e-8 of the value an instruction).
 // 64 sequences of up to 4 K bfloat16 keys, 8 key heads of 128: 163 us, 0.76 of the copy rate (bytes in flight: eight warps an SM, whose registers
@@ -38,6 +40,18 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint4& a, uint32_t
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+// m16n8k8 of fp32 numbers with 11 bits: lane (g, t) has rows g and g + 8 of A in columns t (x, y) and t + 4 (z, w), rows t and t + 4 of column g of B
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// a number of fp32 as two of 11 bits each, off by 2^-22 of it whatever its size (the first is cut off, not rounded: an instruction less, and
+// the largest numbers stay finite)
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
 template <bool BF>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   if constexpr (BF) mma_bf16(c, a, b0, b1);
@@ -62,26 +76,27 @@ __device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
 
 template <int CT, int NQ, int NP, int DP>  // terms of a query and of a probability
 struct PagedShape {
-  static constexpr bool BF = CT == MIMIR_B200_T_BF16;
+  static constexpr bool BF = CT == MIMIR_B200_T_BF16, WIDE = CT == MIMIR_B200_T_F32;
   // halves: probabilities of up to 2^14 (times a code's scale 2^15) are exact to 2^-39 of the largest where 2^-25 would be
-  static constexpr float ROOM = BF ? 0.0f : 14.0f;
+  static constexpr float ROOM = BF || WIDE ? 0.0f : 14.0f;
   static constexpr bool FRESH = NQ == 2;                                // P V of a block apart from O
   static constexpr int KB = type_bytes(CT) == 1 || (type_bytes(CT) == 2 && DP <= 128) ? 32 : 16;  // keys of a block
   static constexpr int UD = CT == MIMIR_B200_T_F32 ? 64 : DP < 128 ? DP : 128;  // head elements loaded at a time
-  static constexpr int Q_BYTES = NQ * (DP / 16) * 32 * 16;
+  static constexpr int Q_STEPS = DP / (WIDE ? 8 : 16), Q_BYTES = NQ * Q_STEPS * 32 * 16;  // of the contraction
   static constexpr int O_STRIDE = DP + 4;
   static constexpr int SMEM = Q_BYTES + PA_WARPS * PA_ROWS * (O_STRIDE + 2) * 4 + 2 * PA_ROWS * 4;
 };
 
+// (three CTAs to an SM where that spills little; fp32 caches, heads of 64, 64 sequences of up to 4 K keys: 285 us in three, 218 in two)
 template <int CT, int NQ, int NP, int DP>
-__global__ void __launch_bounds__(PA_THREADS, DP > 64 ? 2 : 3)
+__global__ void __launch_bounds__(PA_THREADS, DP > 64 || CT == MIMIR_B200_T_F32 ? 2 : 3)
 paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   using S = PagedShape<CT, NQ, NP, DP>;
-  constexpr bool BF = S::BF, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3, WIDE = CT == MIMIR_B200_T_F32;
+  constexpr bool BF = S::BF, CODED = CT == MIMIR_B200_T_I8 || CT == MIMIR_B200_T_E4M3, WIDE = S::WIDE;
   constexpr int KB = S::KB, NG = KB / 8, UD = S::UD, NU = DP / UD;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint4* sq = reinterpret_cast<uint4*>(smem);                        // [NQ][DP / 16][32 lanes]
+  uint4* sq = reinterpret_cast<uint4*>(smem);                        // [NQ][Q_STEPS][32 lanes]
   float* so = reinterpret_cast<float*>(smem + S::Q_BYTES);           // [warp][16][O_STRIDE]
   float* sm = so + PA_WARPS * PA_ROWS * S::O_STRIDE;                 // [warp][16] maxima, then [warp][16] sums
   float* sl = sm + PA_WARPS * PA_ROWS;
@@ -127,7 +142,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       else unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(src), f);
     }
     float scale = 1.0f;
-    if (!BF && a.type != MIMIR_B200_T_F16) {
+    if (!BF && !WIDE && a.type != MIMIR_B200_T_F16) {
       float top = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
@@ -141,7 +156,17 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       for (int e = 0; e < 8; ++e) f[e] *= inv;
     }
     if (lane == 0) sscale[row] = scale;
-    if (d < DP) {
+    if (WIDE && d < DP) {
+      // elements 8 c + 2 i and + 1 belong to lane (row % 8, c % 4) of step 4 (c / 4) + i: registers row / 8 and row / 8 + 2
+      const int c = lane, to = (row & 7) * 4 + (c & 3), reg = row >> 3;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t hi, lo;
+        split_tf32(f[e], hi, lo);
+        uint32_t* w = reinterpret_cast<uint32_t*>(sq + (4 * (c / 4) + e / 2) * 32 + to) + reg + 2 * (e & 1);
+        w[0] = hi, w[S::Q_STEPS * 32 * 4] = lo;
+      }
+    } else if (d < DP) {
       // elements 8 c .. 8 c + 7 belong to lane (row % 8, c % 4) of steps 2 (c / 4) and 2 (c / 4) + 1: registers row / 8 and row / 8 + 2
       const int c = lane;
 #pragma unroll
@@ -153,7 +178,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
         uint32_t* w = reinterpret_cast<uint32_t*>(sq + step * 32 + to);
         w[reg] = hi0, w[reg + 2] = hi1;
         if constexpr (NQ == 2) {
-          w = reinterpret_cast<uint32_t*>(sq + (DP / 16 + step) * 32 + to);
+          w = reinterpret_cast<uint32_t*>(sq + (S::Q_STEPS + step) * 32 + to);
           w[reg] = lo0, w[reg + 2] = lo1;
         }
       }
@@ -313,7 +338,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
   }
   for (int b = b0; b < b1; ++b) {
     // ---- scores ----------------------------------------------------------------------------------------------------------------
-    float sc[NG][4];
+    float sc[NG][4], sc_q[WIDE ? NG : 1][4], sc_k[WIDE ? NG : 1][4];  // (fp32: sums of the smaller products apart, for shorter chains of instructions)
     const unsigned here = there;
     const bool full = whole && b * KB >= all_lo && b * KB + KB <= all_hi;
     float2 ks_now[NG];
@@ -322,27 +347,47 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
       if constexpr (CODED) ks_now[j] = ks[j];
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc_q[j][i] = sc_k[j][i] = 0.0f;
+      }
     }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
       for (int c = 0; c < UD / 32; ++c) {
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int step = (u * UD + 32 * c) / 8 + h;
+            const uint4 qa = sq[step * 32 + lane], ql = sq[(S::Q_STEPS + step) * 32 + lane];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+              uint32_t hi[2], lo[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) split_tf32(__uint_as_float(kr[j][c].w[2 * h + i]), hi[i], lo[i]);
+              mma_tf32(sc[j], qa, hi[0], hi[1]);
+              mma_tf32(sc_q[j], ql, hi[0], hi[1]);
+              mma_tf32(sc_k[j], qa, lo[0], lo[1]);
+            }
+          }
+          continue;
+        }
         uint4 qa[2], ql[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int step = (u * UD + 32 * c) / 16 + h;
           qa[h] = sq[step * 32 + lane];
-          if constexpr (NQ == 2) ql[h] = sq[(DP / 16 + step) * 32 + lane];
+          if constexpr (NQ == 2) ql[h] = sq[(S::Q_STEPS + step) * 32 + lane];
         }
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          uint32_t hi[4], lo[4];
-          to_pairs<CT>(kr[j][c], hi, lo);
+          uint32_t hi[4];
+          to_pairs<CT>(kr[j][c], hi);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             mma16<BF>(sc[j], qa[h], hi[2 * h], hi[2 * h + 1]);
             if constexpr (NQ == 2) mma16<BF>(sc[j], ql[h], hi[2 * h], hi[2 * h + 1]);
-            if constexpr (WIDE) mma16<BF>(sc[j], qa[h], lo[2 * h], lo[2 * h + 1]);
           }
         }
       }
@@ -361,7 +406,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
     for (int j = 0; j < NG; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float v = sc[j][i] * c2[i >> 1];
+        float v = (WIDE ? sc[j][i] + (sc_q[j][i] + sc_k[j][i]) : sc[j][i]) * c2[i >> 1];
         if constexpr (CODED) v *= (i & 1) ? ks_now[j].y : ks_now[j].x;
         if (!full) {
           const int key = b * KB + 8 * j + 2 * t + (i & 1);
@@ -409,7 +454,7 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[j][i] *= alpha[i >> 1];
     }
-    uint4 ph[KB / 16], pl[KB / 16];
+    uint4 ph[KB / (WIDE ? 8 : 16)], pl[KB / (WIDE ? 8 : 16)];
 #pragma unroll
     for (int k16 = 0; k16 < KB / 16; ++k16) {
       uint32_t hi[2][2], lo[2][2];  // [group of eight keys][row]
@@ -423,7 +468,9 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
           l[i >> 1] += e[i];
           if constexpr (CODED) e[i] *= (i & 1) ? vf[j].y : vf[j].x;
         }
-        if constexpr (NP == 2) {
+        if constexpr (WIDE) {  // (keys 2 t and 2 t + 1 of the group are columns t and t + 4)
+          split_tf32(e[0], ph[j].x, pl[j].x), split_tf32(e[2], ph[j].y, pl[j].y), split_tf32(e[1], ph[j].z, pl[j].z), split_tf32(e[3], ph[j].w, pl[j].w);
+        } else if constexpr (NP == 2) {
           split2<BF>(e[0], e[1], hi[x][0], lo[x][0]);
           split2<BF>(e[2], e[3], hi[x][1], lo[x][1]);
         } else {
@@ -431,8 +478,8 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
           hi[x][1] = pack2<BF>(e[2], e[3]);
         }
       }
-      ph[k16] = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
-      if constexpr (NP == 2) pl[k16] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
+      if constexpr (!WIDE) ph[k16] = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
+      if constexpr (!WIDE && NP == 2) pl[k16] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
     }
     // ---- values ------------------------------------------------------------------------------------------------------------------------
 #pragma unroll
@@ -448,9 +495,24 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
         }
 #pragma unroll
         for (int k16 = 0; k16 < KB / 16; ++k16) {
-          uint32_t h4[4][4], l4[4][4];  // [this lane's four keys][pair of columns]
+          if constexpr (WIDE) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) to_pairs<CT>(vr[k16][i][c], h4[i], l4[i]);
+            for (int x = 0; x < 2; ++x) {  // groups of eight keys
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) split_tf32(__uint_as_float(vr[k16][2 * x + i][c].w[n]), hi[i], lo[i]);
+                mma_tf32(acc[n], ph[2 * k16 + x], hi[0], hi[1]);
+                mma_tf32(acc[n], pl[2 * k16 + x], hi[0], hi[1]);
+                mma_tf32(acc[n], ph[2 * k16 + x], lo[0], lo[1]);
+              }
+            }
+            continue;
+          }
+          uint32_t h4[4][4];  // [this lane's four keys][pair of columns]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to_pairs<CT>(vr[k16][i][c], h4[i]);
 #pragma unroll
           for (int n = 0; n < 8; ++n) {  // column tiles
             float(&to)[4] = S::FRESH ? acc[n] : o[(u * UD + 64 * c) / 8 + n];
@@ -458,7 +520,6 @@ paged_attention_kernel(const __grid_constant__ AttendArgs a) {
             const uint32_t w0 = __byte_perm(h4[0][n / 2], h4[1][n / 2], sel), w1 = __byte_perm(h4[2][n / 2], h4[3][n / 2], sel);
             mma16<BF>(to, ph[k16], w0, w1);
             if constexpr (NP == 2) mma16<BF>(to, pl[k16], w0, w1);
-            if constexpr (WIDE) mma16<BF>(to, ph[k16], __byte_perm(l4[0][n / 2], l4[1][n / 2], sel), __byte_perm(l4[2][n / 2], l4[3][n / 2], sel));
           }
         }
         if constexpr (S::FRESH) {

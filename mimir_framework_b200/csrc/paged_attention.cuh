@@ -90,13 +90,10 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2<BF>(x - h.x, y - h.y);
 }
 
-// eight elements of a cache type as four pairs in the tensor type (and, of fp32, what those leave in a second four)
+// eight elements of a cache of 16 or 8 bits as four pairs in the tensor type
 template <int CT>
-__device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-  if constexpr (CT == MIMIR_B200_T_F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) split2<false>(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]), hi[i], lo[i]);
-  } else if constexpr (CT == MIMIR_B200_T_I8) {
+__device__ __forceinline__ void to_pairs(const Raw8<CT>& r, uint32_t (&hi)[4]) {
+  if constexpr (CT == MIMIR_B200_T_I8) {
     // 0x6400 | (code + 128) is 1024 + 128 + code as a half
     const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
 #pragma unroll

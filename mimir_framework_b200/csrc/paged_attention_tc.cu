@@ -325,8 +325,8 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
 #pragma unroll
             for (int n = 0; n < N; ++n) {
               const int x = id + n * S::LOADERS, k = x / (DP / 8), c = x % (DP / 8);
-              uint32_t hi[4], lo[4];
-              to_pairs<CT>(raw[n], hi, lo);
+              uint32_t hi[4];
+              to_pairs<CT>(raw[n], hi);
               if (k < TC_KEYS)
                 *reinterpret_cast<uint4*>(ring + st * TILE + (c >> 3) * (TC_KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             }

@@ -1,4 +1,5 @@
 """Serving calls at the ends of what they accept."""
+import math
 import threading
 import time
 
@@ -107,6 +108,28 @@ def test_sampling_by_mass_and_least_share_of_the_most_logits(backend, kind, top_
     # the reference adds 2^24 numbers up one after the other: off by up to 2^-29 of 2^22 or so, which is four of the small ones
     assert abs(int(ids[0]) - want) <= (5 if kind == "many small" else 0)
     assert abs(float(logp[0]) - lp) <= 2.0**-22 * max(1.0, abs(lp))
+
+
+# ---- values -------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,kv,dim,group", [([1, 2], [33, 300], 64, 4), ([40], [170], 128, 2), ([3, 17], [90, 20], 256, 1), ([1], [5], 8, 1)])
+@pytest.mark.parametrize("size", [1e6, 1e-3, 1e-6, 1e-20, "mixed"])
+def test_fp32_caches_of_any_size(backend, size, rows, kv, dim, group):
+    """Keys and values of an fp32 cache keep their bits whatever they are near, each by itself."""
+    p = Pages(rows, kv, 2, dim, 8, F32, seed=4)
+    p.fill()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    for which in range(2):
+        if size == "mixed":  # values over 2^60, keys over 2^20, from element to element
+            span = 30.0 if which else 10.0
+            f = torch.exp2(torch.rand(p.pool[which].shape, generator=g, device="cuda") * 2 * span - span)
+        else:
+            f = size
+        p.pool[which].mul_(f)
+    scale = 2.0**-8 if size == "mixed" else 1 / (size * math.sqrt(dim))
+    q = normal(p.n_rows, 2 * group, dim, seed=3)
+    out, lse = attend(backend, p, q, F32, scale)
+    held(p, q, out, lse, F32, scale, True, 0, False)
 
 
 # ---- findings ------------------------------------------------------------------------------------------------------------------------------
