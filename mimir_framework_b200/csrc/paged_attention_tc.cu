@@ -10,7 +10,9 @@
 //   warps 9-11       bring K and V tiles out of the pages into a ring: by TMA, a box of a page's slots a lane (copies a thread each took 6300
 //                    cycles a key tile, twice what everything else did); 8-bit codes through the registers of seven warps, as halves
 // Heads of over 128 elements have one tile of 128 rows (O takes 256 columns of tensor memory) and two score tiles that alternate.  So have
-// queries of fp32, which are two halves a value (22 bits) and whose probabilities are, over all 128 columns of the scores.
+// queries of fp32, which are two halves a value (22 bits) and whose probabilities are, over all 128 columns of the scores.  For them O holds the
+// products of two key tiles only, and what these come to is added in fp32 to a sum in the rest of tensor memory: the tensor core's accumulation
+// truncates, which over 16 K keys came to 2.3e-4 of rows whose probability was on the first 64.
 // K and V tiles lie in the same layout, [64 elements][key] rows of 128 swizzled bytes: K-major for Q K^T, MN-major for P V.
 // The running maximum is raised only when a score outgrows it by 2^8, so O in tensor memory is rescaled a few times a row.
 // Probabilities of a bfloat16 cache are rounded to bfloat16 (8 bits, relative to each probability), else to half (11 bits); their sum is
@@ -39,6 +41,11 @@ struct TcShape {
   static constexpr int TILE = SUB * TC_KEYS * 128;     // bytes of a K or V tile, and of a Q tile
   static constexpr int NS = DP == 64 ? 6 : DP == 128 ? 4 : 2;
   static constexpr int SCALES = CODED ? NS / 2 * 2 * TC_KEYS * 4 : 0;  // [V stage][key, value][key]
+  // fp32 results: key tiles whose products the tensor core adds up, truncating; what they come to is added to a sum beside them, rounded.  Four
+  // chunks of 1.6 to 2 K tokens behind up to 8 K keys of half, heads of 128: 1078 us without, 1124 by two (1175 by one, 1083 by four); heads of 64
+  // over e4m3 1350 and 1487.
+  static constexpr int GROUP = NQ == 2 ? 2 : 0;
+  static_assert((GROUP & (GROUP - 1)) == 0 && (GROUP == 0 || 2 * TC_KEYS + 2 * DP <= TC_TMEM), "tensor memory");
   static constexpr int OFFS = 2 * TC_KEYS * 8;         // where the rows of a key tile lie, two tiles
   static constexpr int SMEM = NT * NQ * TILE + NS * TILE + SCALES + OFFS + 512;
   // halves: probabilities of up to 2^6, by the maximum that may be 2^8 too low 2^14, are exact to 2^-31 of the largest where 2^-25 would be
@@ -110,7 +117,7 @@ __global__ void __launch_bounds__(TcShape<DP, CT, NQ>::THREADS, 1)
 paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ PageMaps maps) {
   using S = TcShape<DP, CT, NQ>;
   constexpr bool BF = S::BF, CODED = S::CODED;
-  constexpr int NT = S::NT, NS = S::NS, TILE = S::TILE, SUB = S::SUB;
+  constexpr int NT = S::NT, NS = S::NS, TILE = S::TILE, SUB = S::SUB, GROUP = S::GROUP;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it
@@ -218,6 +225,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
   pdl_launch_dependents();  // sequences of few rows, another kernel's, may start on SMs that come free
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + 2 * TC_KEYS;  // tile t at + t * DP
+  const uint32_t tmem_sum = tmem_o + DP;       // GROUP > 0: of the groups of key tiles before the present one
 
   if constexpr (CODED) {
     if (warp < NT * 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFT_REGS));
@@ -373,10 +381,11 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     auto values = [&](int tt, int j) {  // O_tt (+)= P V_j
       const uint32_t v_at = ring_at + ((2 * j + 1) % NS) * TILE, pa = tmem + (NT == 2 ? tt : (j & 1)) * TC_KEYS, d = tmem_o + tt * DP;
       const uint64_t v_desc = desc_mn(v_at, TC_KEYS * 128);
+      const int first = GROUP > 0 ? j & (GROUP - 1) : j;
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < TC_KEYS / 16; ++k) {
-          umma_f16_ts(d, pa + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, (j | k) != 0 ? 1u : 0u);
+          umma_f16_ts(d, pa + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, (first | k) != 0 ? 1u : 0u);
           if constexpr (NQ == 2) umma_f16_ts(d, pa + TC_KEYS / 2 + 8 * k, v_desc + ((k * 2048) >> 4), idesc_o, 1u);
         }
         umma_commit(pv_done + tt);
@@ -444,7 +453,16 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     const int w_first = __shfl_sync(0xffffffffu, pos, 0), w_last = __shfl_sync(0xffffffffu, pos, 31);
     const int all_hi = a.causal ? min(seq.kv, w_first + 1) : seq.kv, all_lo = a.window > 0 ? max(0, w_last - a.window + 1) : 0;
     float base = -INFINITY, sum = 0.0f;
+    float sum_f = 1.0f, o_f = 1.0f;  // GROUP > 0: what the sum of the earlier groups, and O where it is complete, are still to be multiplied by
     float v_unit = 0.0f;  // codes: the power of two that O's values are in
+    if constexpr (GROUP > 0) {  // (a sum that starts from zero has one form of addition; with a first one of its own 1 to 6 % more time)
+      uint32_t none[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) none[i] = 0;
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) tmem_st_32x32(tmem_sum + lanes + 32 * c, none);
+      tmem_wait_st();
+    }
     bool alive = true;
     for (int j = 0; j < n_kt; ++j) {
       const int buf = NT == 2 ? t : (j & 1);
@@ -503,6 +521,7 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         const int e2 = min(240, max(14, static_cast<int>(__float_as_uint(top) >> 23)));
         grow = __uint_as_float(static_cast<uint32_t>(e2) << 23);
       }
+      const bool complete = GROUP > 0 && j > 0 && (j & (GROUP - 1)) == 0;  // O is a group's: the next product starts another
       // another maximum, and O with it
       auto rescale = [&](float mx) {
         const float nb = fmaxf(base, mx - S::ROOM);
@@ -514,7 +533,9 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
           f *= v_unit / nu;
           v_unit = nu;
         }
-        if (j == 0) return true;
+        sum_f *= f;
+        if (complete) o_f *= f;
+        if (j == 0 || complete) return true;
         if (!mbar_wait_warp(pv_done + (NT == 2 ? t : 0), static_cast<uint32_t>(j - 1) & 1, abort_flag, a.err_word, 68)) return false;
         tcgen05_fence_after();
 #pragma unroll 1
@@ -580,6 +601,26 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         tmem_st_32x16(ts + 16 * c, pk[c]);
         if constexpr (NQ == 2) tmem_st_32x16(ts + TC_KEYS / 2 + 16 * c, pl[c]);
       }
+      if (GROUP > 0 && complete) {
+        alive = mbar_wait_warp(pv_done, static_cast<uint32_t>(j - 1) & 1, abort_flag, a.err_word, 70);
+        if (!alive) break;
+        tcgen05_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32], old[32];
+          tmem_ld_32x32_nowait(tmem_o + lanes + 32 * c, o);
+          tmem_ld_32x32_nowait(tmem_sum + lanes + 32 * c, old);
+          tmem_wait_ld_regs(o);
+          tmem_wait_ld_regs(old);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float v = __uint_as_float(o[i]) * o_f;
+            o[i] = __float_as_uint(fmaf(__uint_as_float(old[i]), sum_f, v));
+          }
+          tmem_st_32x32(tmem_sum + lanes + 32 * c, o);
+        }
+        sum_f = o_f = 1.0f;
+      }
       tmem_wait_st();
       tcgen05_fence_before();
       // With two score tiles the last product's wait, below, comes while the one before it may still run, and a barrier two phases behind looks
@@ -595,9 +636,10 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
     if (alive) {
       tcgen05_fence_after();
       const bool there = r < r_end;
-      // fp32: two instructions for 16 keys that the row sees, each of which lost 1.5e-8
+      // fp32: a group's products, two instructions for 16 keys that the row sees, are low by 1.5e-8 an instruction where these weigh alike, by
+      // nothing or twice that where the last or the first have all the weight
       const int keys_seen = max(0, min(lim_hi, (kt0 + n_kt) * TC_KEYS) - max(lim_lo, kt0 * TC_KEYS));
-      const float unit_v = (CODED ? v_unit : 1.0f) * (NQ == 2 ? 1.0f + 1.5e-8f * (keys_seen / 8) : 1.0f);
+      const float unit_v = (CODED ? v_unit : 1.0f) * (GROUP > 0 ? 1.0f + 1.5e-8f * (min(keys_seen, GROUP * TC_KEYS) / 8) : 1.0f);
       const float inv = a.splits > 1 ? unit_v : sum == 0.0f ? 0.0f : unit_v / sum;
       const int h = head * a.group + r - tok * a.group;
       const long long part_row = static_cast<long long>(blockIdx.x) * (NT * TC_ROWS) + t * TC_ROWS + r_local;
@@ -610,6 +652,13 @@ paged_attention_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_con
         if (n_kt > 0) {
           tmem_ld_32x32_nowait(tmem_o + t * DP + lanes + 32 * c, o);
           tmem_wait_ld_regs(o);
+          if (GROUP > 0 && n_kt > GROUP) {
+            uint32_t old[32];
+            tmem_ld_32x32_nowait(tmem_sum + lanes + 32 * c, old);
+            tmem_wait_ld_regs(old);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(old[i]), sum_f, __uint_as_float(o[i])));
+          }
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {

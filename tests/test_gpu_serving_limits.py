@@ -132,6 +132,39 @@ def test_fp32_caches_of_any_size(backend, size, rows, kv, dim, group):
     held(p, q, out, lse, F32, scale, True, 0, False)
 
 
+@pytest.mark.parametrize("cache", [F16, I8, E4M3])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lead", [40.0, 12.0])
+@pytest.mark.parametrize("first", [0, 64, 8064, 16320])
+def test_fp32_results_of_chunks_do_not_drift_with_the_keys(backend, first, lead, dim, cache):
+    """Nearly all of the probability on 64 of 16 K keys, at the beginning, in the middle or at the end.  80 sequences share the pages, so that
+    none of them is divided among blocks."""
+    n, rows, seqs = 16384, 40, 80
+    p = Pages([rows], [n], 1, dim, 64, cache, seed=1)
+    keys = torch.zeros(n, 1, dim, device="cuda")
+    keys[first : first + 64, :, 0] = lead
+    p.put(0, 0, np.arange(n), torch.where(keys == 0, 1e-30, keys) if cache in (I8, E4M3) else keys)
+    values = normal(n, 1, dim, seed=2).abs() + 0.5  # (of one sign: nothing cancels)
+    p.put(1, 0, np.arange(n), values)
+    q = torch.zeros(rows, 1, dim, device="cuda")
+    q[..., 0] = 1.0
+    many = q.repeat(seqs, 1, 1)
+    starts = torch.arange(0, rows * seqs + 1, rows, dtype=torch.int32, device="cuda")
+    lens, table = p.dev[1].repeat(seqs), p.dev[2].repeat(seqs, 1).contiguous()
+    out, lse = attend(backend, p, many, F32, 1.0, False, row_start=starts.data_ptr(), kv_len=lens.data_ptr(), page_table=table.data_ptr(), n_seqs=seqs,
+                      n_rows=rows * seqs, max_rows=rows)
+    assert torch.equal(out, out[:1].expand_as(out)) and torch.equal(lse, lse[:1].expand_as(lse))
+    want, want_lse, weight, _ = attention(p, q.double().cpu().numpy(), 1.0, False, 0)
+    # The 64 keys' scores are one product each and alike, so what they are off by cancels.  A probability is two halves (2^-22).  The sum of
+    # probabilities has half a unit (2^-24) each of up to 96 additions within a tile, and sum and products one for each tile added to them, where
+    # the others' probabilities are not zero (64 and 128 keys do not meet a border: one tile has nearly all).  Two tiles' products are 32 instructions
+    # that truncate, by a unit (2^-23) at most.  The others' share is under 1e-3, and their scores' 2^-21 * 12 count for that.
+    tiles = 128 if lead < 20 else 1
+    bound = 2.0**-22 + (96 + 2 * tiles) * 2.0**-24 + 32 * 2.0**-23 + 12 * 2.0**-21 * 1e-3 + 2.0**-23
+    err = np.abs(out[:rows].double().cpu().numpy() - want)
+    assert np.all(err <= bound * weight), f"{np.max(err / weight)}, bound {bound}"
+
+
 # ---- findings ------------------------------------------------------------------------------------------------------------------------------
 def test_findings_are_reported_once_whoever_asks(backend):
     """One thread makes bad calls of changing kinds and asks after each; another asks all the time, of another stream.  Every finding reaches one
