@@ -721,6 +721,11 @@ int launch_tc_as(const AttendArgs& a, long long grid, cudaStream_t st) {
   static PerDeviceOnce once;
   MB_TRY(once.run([]() -> int {
     MB_CUDA(cudaFuncSetAttribute(paged_attention_tc_kernel<DP, CT, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    if (S::CODED) {  // (setmaxnreg waits for registers of the launch's own: with fewer than the shares add up to it would wait for good)
+      cudaFuncAttributes at;
+      MB_CUDA(cudaFuncGetAttributes(&at, paged_attention_tc_kernel<DP, CT, NQ>));
+      if (at.numRegs < S::LAUNCH_REGS) return fail(MIMIR_B200_E_UNSUPPORTED, "paged_attention: compiled with %d registers a thread, %d are shared out", at.numRegs, S::LAUNCH_REGS);
+    }
     return MIMIR_B200_OK;
   }));
   PageMaps maps = {};
