@@ -165,6 +165,24 @@ def test_fp32_results_of_chunks_do_not_drift_with_the_keys(backend, first, lead,
     assert np.all(err <= bound * weight), f"{np.max(err / weight)}, bound {bound}"
 
 
+@pytest.mark.parametrize("cache,type_,few", [(BF16, BF16, 32), (F16, F16, 32), (F16, BF16, 32), (F16, F32, 32), (I8, F16, 64), (I8, BF16, 64), (E4M3, F16, 64), (E4M3, F32, 32)])
+@pytest.mark.parametrize("dim,window", [(64, 0), (128, 90)])
+def test_few_rows_beside_chunks_keep_their_terms(backend, dim, window, cache, type_, few):
+    """A sequence of few rows is as exact in a batch with chunks as alone: its probabilities have two terms."""
+    rows, kv = [200, 1, few, few - 3, 150], [300, 777, 100, few - 9, 400]
+    p = Pages(rows, kv, 2, dim, 16, cache, seed=5)
+    p.fill()
+    q = normal(p.n_rows, 2, dim, seed=3, dtype=TORCH[type_])
+    out, lse = attend(backend, p, q, type_, dim**-0.5, True, window)
+    held(p, q, out, lse, type_, dim**-0.5, True, window, True)
+    want, _, weight, reach = attention(p, q.double().cpu().numpy(), dim**-0.5, True, window)
+    bound, _ = attention_bounds(want, weight, reach, dim, max(kv), BF16 if cache == BF16 else type_, False, type_ == BF16 and cache != BF16)
+    err = np.abs(out.double().cpu().numpy() - want)
+    for s in (1, 2, 3):
+        at = slice(p.starts[s], p.starts[s + 1])
+        assert np.all(err[at] <= bound[at]), f"{np.max(err[at] / np.maximum(bound[at], 1e-300))} of the bound"
+
+
 # ---- findings ------------------------------------------------------------------------------------------------------------------------------
 def test_findings_are_reported_once_whoever_asks(backend):
     """One thread makes bad calls of changing kinds and asks after each; another asks all the time, of another stream.  Every finding reaches one
