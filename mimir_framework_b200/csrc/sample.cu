@@ -120,6 +120,7 @@ struct Weigh {
   double one;         // what a weight of 1 is as an integer
   float least_x;      // w is zero there and below
   const double* table;
+  __device__ __forceinline__ double power(float x) const { return (static_cast<double>(x) - top) * scale; }  // of two, before w is rounded to an integer
   __device__ __forceinline__ u64 operator()(float x) const {
     const double y = (static_cast<double>(fmaxf(x, least_x)) - top) * scale;
     const double s = y + 105553116266496.0;  // 1.5 * 2^46: y rounded to 64ths in the low bits
@@ -135,10 +136,11 @@ struct Weigh {
   }
 };
 
-// the logarithm of w / total, to fp32's last bits near one too
-__device__ __forceinline__ float log_share(u64 w, u64 total) {
+// the logarithm of x's share, w of total: near one from the integers, else from the logit, of which a small w keeps few bits
+__device__ __forceinline__ float log_share(const Weigh& weigh, float x, u64 w, u64 total) {
   const u64 left = total - w;
-  return left < w ? log1pf(-(static_cast<float>(left) / static_cast<float>(total))) : logf(static_cast<float>(w) / static_cast<float>(total));
+  if (left < w) return log1pf(-(static_cast<float>(left) / static_cast<float>(total)));
+  return static_cast<float>(weigh.power(x) * 0.69314718055994531) - logf(static_cast<float>(total) * (1.0f / static_cast<float>(weigh.one)));
 }
 
 template <class V>
@@ -548,7 +550,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
         const u64 until = until_of(all);
         if (part == 0 && before <= until && until < before + kept) {
           a.ids[row] = static_cast<int>(~static_cast<uint32_t>(mine_l));
-          if (a.logprob) a.logprob[row] = log_share(kept, all);
+          if (a.logprob) a.logprob[row] = log_share(weigh, value_of(static_cast<uint32_t>(mine_l >> 32)), kept, all);
         }
         return true;
       }
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       auto take = [&](u64 item, u64 from, u64 w) {
         if (!(from <= until && until < from + w)) return;
         a.ids[row] = static_cast<int>(~static_cast<uint32_t>(item >> 32));
-        if (a.logprob) a.logprob[row] = log_share(w, all);
+        if (a.logprob) a.logprob[row] = log_share(weigh, value_of(static_cast<uint32_t>(item)), w, all);
       };
       take(i0, at, x0);
       take(i1, at + x0, x1);
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows_kernel(const __grid
       const u64 inc = warp_scan(w, lane);
       if (run + inc - w <= until && until < run + inc) {
         a.ids[row] = first + e + lane;
-        if (a.logprob) a.logprob[row] = log_share(w, total);
+        if (a.logprob) a.logprob[row] = log_share(weigh, v, w, total);
       }
       run += __shfl_sync(0xffffffffu, inc, 31);
       seen += __popc(equal);

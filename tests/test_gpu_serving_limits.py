@@ -110,6 +110,26 @@ def test_sampling_by_mass_and_least_share_of_the_most_logits(backend, kind, top_
     assert abs(float(logp[0]) - lp) <= 2.0**-22 * max(1.0, abs(lp))
 
 
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (0, 1.0 - 2.0**-20), (3000, 1.0), (200, 1.0), (900, 1.0)])
+@pytest.mark.parametrize("down", [3.0, 15.0, 22.0, 27.0, 30.0])
+def test_the_logarithm_of_a_small_share_keeps_its_bits(backend, down, top_k, top_p):
+    """The first index is taken (uniform 0), whose share is e^-down or less."""
+    n = 70000
+    x = normal(2, n, seed=4, scale=1.0) - 45.0
+    x[:, 0] = -down + 0.123
+    x[1, : top_k // 2] = -down + 0.123
+    x[:, 7000:7100] = normal(2, 100, seed=5, scale=0.1).clamp(max=0.4)
+    x[:, 7050] = 0.5
+    u, k, p = torch.zeros(2, device="cuda"), torch.full((2,), top_k, dtype=torch.int32, device="cuda"), torch.full((2,), top_p, device="cuda")
+    ids, logp = torch.full((2,), -7, dtype=torch.int32, device="cuda"), torch.zeros(2, device="cuda")
+    backend.dev_sample_rows(x.data_ptr(), F32, 2, n, n, None, k.data_ptr(), p.data_ptr(), None, u.data_ptr(), ids.data_ptr(), logp.data_ptr())
+    torch.cuda.synchronize()
+    for r in range(2):
+        want, lp, _ = sample(x[r].double().cpu().numpy(), 1.0, top_k, float(p[r]), 0.0, 0.0)
+        # two logarithms of fp32 that do not cancel, their difference, and a sum's rounding: under four units of 2^-24 of it; a share over one half is not among them
+        assert int(ids[r]) == want and abs(float(logp[r]) - lp) <= 2.0**-22 * abs(lp), (float(logp[r]), lp)
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("rows,kv,dim,group", [([1, 2], [33, 300], 64, 4), ([40], [170], 128, 2), ([3, 17], [90, 20], 256, 1), ([1], [5], 8, 1)])
 @pytest.mark.parametrize("size", [1e6, 1e-3, 1e-6, 1e-20, "mixed"])
