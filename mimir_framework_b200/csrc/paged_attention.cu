@@ -15,9 +15,9 @@
 // hold what is far from one.  Over other caches fp32 queries and probabilities are two IEEE-half terms (22 bits): queries after a power of two per row has brought
 // their largest to [1, 2).  Probabilities are two terms for bfloat16 caches too (16 bits), one half (11 bits) where only the result is bfloat16.
 // Codes of eight bits are exact in half; their scales multiply scores and probabilities.  For fp32 results each block's P V starts from
-// zero and is added in fp32, because the tensor core's accumulation truncates (1.5e-8 of the value an instruction).
-// 64 sequences of up to 4 K bfloat16 keys, 8 key heads of 128: 163 us, 0.76 of the copy rate (bytes in flight: eight warps an SM, whose registers
-// hold them).  4 of up to 128 K e4m3 keys: 209 us, 0.69 of it (codes become halves on the ordinary lanes).
+// zero and is added in fp32, because the tensor core's accumulation truncates (1.5e-8 of the value an instruction, up to 2^-23).
+// 64 sequences of up to 4 K bfloat16 keys, 8 key heads of 128: 165 us, 0.75 of the copy rate (bytes in flight: eight warps an SM, whose registers
+// hold them; CTAs of unequal length).  4 of up to 128 K e4m3 keys: 210 us, 0.69 of it (the loads' latency again, and codes that become halves).
 #include <cmath>
 
 #include "common.h"

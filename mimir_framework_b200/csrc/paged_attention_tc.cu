@@ -17,7 +17,7 @@
 // The running maximum is raised only when a score outgrows it by 2^8, so O in tensor memory is rescaled a few times a row.
 // Probabilities of a bfloat16 cache are rounded to bfloat16 (8 bits, relative to each probability), else to half (11 bits); their sum is
 // of the unrounded ones, in fp32.  Scores, maxima, sums and O are fp32.
-// Four chunks of 1.6 to 2 K tokens behind up to 8 K keys, 32 heads of 128 over 8 key heads, bfloat16: 605 us, 1.19 PFLOP/s; the products alone 465.
+// Four chunks of 1.6 to 2 K tokens behind up to 8 K keys, 32 heads of 128 over 8 key heads, bfloat16: 606 us, 1.19 PFLOP/s; the products alone 465.
 #include <cmath>
 #include <type_traits>
 

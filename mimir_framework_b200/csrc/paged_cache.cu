@@ -6,8 +6,8 @@
 //   I8:   scale = amax * (1 / 127), code = x / scale to nearest (ties to even)      E4M3: scale = amax * (1 / 448), likewise
 // amax is over the finite elements; 1 / 127 and 1 / 448 are fp32 constants and the division is the IEEE one, so that codes are what any
 // fp32 program gets that computes them so.
-// Writing codes is bound by instruction issue (two thirds of it the quotients): 27 K tokens, 8 key heads of 128, bfloat16 to int8 48 us, 2.0 times
-// its bytes' time at the copy rate.  Reading is bound by its bytes: 16 sequences of up to 8 K int8 keys to bfloat16 95 us, the copy rate.
+// Writing codes is bound by instruction issue (160 instructions for a warp's 256 elements, some 50 of them the quotients): 27 K tokens, 8 key heads of
+// 128, bfloat16 to int8 46 us, 1.9 times its bytes' time at the copy rate.  Reading is bound by its bytes: 16 sequences of up to 8 K int8 keys to bfloat16 95 us, the copy rate.
 #include "common.h"
 #include "paged.cuh"
 
