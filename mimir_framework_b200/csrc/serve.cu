@@ -1,5 +1,7 @@
 // serve.cu — the C calls of the serving group: what the host can see of their arguments is checked here, what lies in device memory by
 // the kernels (paged.cuh).
+#include <cmath>
+
 #include "common.h"
 #include "host_call.h"
 #include "paged.cuh"
@@ -115,7 +117,7 @@ int check_attention(const char* what, const MimirPagedCache* c, const MimirPaged
   if (!row_type(at->type)) return fail(MIMIR_B200_E_INVALID, "%s: q and out are F32, F16 or BF16, not type %d", what, at->type);
   if (at->heads <= 0 || at->heads % c->kv_heads) return fail(MIMIR_B200_E_INVALID, "%s: %d heads are no multiple of %d key heads", what, at->heads, c->kv_heads);
   if (at->window < 0) return fail(MIMIR_B200_E_INVALID, "%s: negative window", what);
-  if (!(at->scale == at->scale)) return fail(MIMIR_B200_E_INVALID, "%s: the scale is not a number", what);
+  if (!std::isfinite(at->scale)) return fail(MIMIR_B200_E_INVALID, "%s: the scale is not finite", what);
   if ((c->type == MIMIR_B200_T_F32 && at->type != MIMIR_B200_T_F32) || (c->type == MIMIR_B200_T_BF16 && at->type != MIMIR_B200_T_BF16))
     return fail(MIMIR_B200_E_UNSUPPORTED, "%s: a cache of type F32 or BF16 takes queries of its own type", what);
   if (at->row_stride % 8 || at->head_stride % 8 || at->out_row_stride % 8 || at->out_head_stride % 8 || at->row_stride < 0 || at->head_stride < 0 ||
