@@ -615,11 +615,12 @@ int mimir_b200_dev_cache_read(const MimirPagedCache* cache, const MimirPagedBatc
  * kv_len - rows + i; causal: it sees keys up to its position; window > 0: keys above position - window.  A row that sees no key is
  * zero and its lse -infinity.  Keys and values that no row of the sequence's call sees are not used whatever they hold; a value that some
  * row sees meets the others' zeros and has to be finite.  A sequence has up to 2^30 keys.
- * type (of q and out): F32, F16 or BF16 on caches of type F16, I8, E4M3; BF16 on BF16; F32 on F32.  Scores, sums and
- * results are kept in fp32.  For the product with the values a probability is rounded: to 22 bits for F32 results; to 11 for BF16 results over F16, I8
- * and E4M3; else to 22 (over BF16: 16) in sequences of few rows and to 11 (8) where more of them go together, which begins at 33 (token, head) rows of
- * a key head, over I8 and E4M3 for F16 and BF16 and heads up to 128 at 65, and in a batch of one sequence, or of larger groups, goes by max_rows.  Results of F16 and BF16
- * lose up to 2^-23 of their size for each 16 of a sequence's keys to the tensor cores' sums. */
+ * type (of q and out): F32, F16 or BF16 on caches of type F16, I8, E4M3; BF16 on BF16; F32 on F32. The scale is finite. Scores,
+ * sums and results are kept in fp32. For the product with the values a probability is rounded: to 22 bits for F32 results; to 11
+ * for BF16 results over F16, I8 and E4M3; else to 22 (over BF16: 16) in sequences of few rows and to 11 (8) where more of them go
+ * together, which begins at 33 (token, head) rows of a key head, over I8 and E4M3 for F16 and BF16 and heads up to 128 at 65, and
+ * in a batch of one sequence, or of larger groups, goes by max_rows. Results of F16 and BF16 lose up to 2^-23 of their size for
+ * each 16 of a sequence's keys to the tensor cores' sums. */
 typedef struct MimirPagedAttention {
   const void* q;                              /* [n_rows][heads][head_dim], strides in elements, multiples of 8, 16-byte aligned */
   void* out;                                  /* the same shape */
