@@ -186,7 +186,7 @@ extern "C" int mimir_b200_rope_plan(const MimirRopeSpec* spec, MimirRopePlan* pl
   const bool ranged = spec->scaling == MIMIR_B200_ROPE_BANDS || spec->scaling == MIMIR_B200_ROPE_RAMP;
   if (ranged && !(spec->low > 0.0 && spec->high > spec->low && std::isfinite(spec->high) && spec->original_len > 0.0 && std::isfinite(spec->original_len)))
     return fail(MIMIR_B200_E_INVALID, "rope_plan: 0 < low < high and original_len > 0 are needed");
-  if (!std::isfinite(spec->magnitude) || spec->magnitude < 0.0) return fail(MIMIR_B200_E_INVALID, "rope_plan: magnitude must be finite and not negative");
+  if (!std::isfinite(static_cast<float>(spec->magnitude)) || spec->magnitude < 0.0) return fail(MIMIR_B200_E_INVALID, "rope_plan: magnitude must be finite in fp32 and not negative");
   const long double two_pi = 6.283185307179586476925286766559L, base = spec->base, factor = spec->factor;
   int first = 0, last = 0;
   if (spec->scaling == MIMIR_B200_ROPE_RAMP) {

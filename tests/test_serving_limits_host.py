@@ -13,3 +13,10 @@ def test_a_scale_that_is_not_finite_is_refused(scale):
         with pytest.raises(rt.MimirB200Error, match="scale") as e:
             f()
         assert e.value.status == abi.E_INVALID
+
+
+@pytest.mark.parametrize("magnitude", [1e39, 1e300, float("inf")])
+def test_a_rotary_magnitude_beyond_fp32_is_refused(magnitude):
+    with pytest.raises(rt.MimirB200Error, match="magnitude") as e:
+        rt.rope_plan(64, magnitude=magnitude)
+    assert e.value.status == abi.E_INVALID
