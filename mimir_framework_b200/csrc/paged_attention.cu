@@ -661,7 +661,7 @@ struct Share {
 // Up to how many rows of a head go to the row kernel.  Up to 4 x 8 K keys, 8 key heads of 128, here and by tcgen05: 32 rows 57 and 53 us in
 // bfloat16, 47 and 78 over int8, 76 and 49 for fp32; 64 rows 111 and 54 us in bfloat16.  Codes cost tcgen05 a pass through registers and shared
 // memory: 64 rows of 4 x up to 128 K e4m3 keys 686 and 1006 us, 64 x up to 4 K 348 and 416, 128 rows 620 and 443; not so heads over 128 (int8, 64
-// rows 824 and 614) or fp32 queries (456 and 436), whose share here grows as well.
+// rows 824 and 614) or fp32 queries (456 and 441), whose share here grows as well.
 int few_rows(const AttendLaunch& a) {
   const bool codes = a.cache_type == MIMIR_B200_T_I8 || a.cache_type == MIMIR_B200_T_E4M3;
   return codes && a.type != MIMIR_B200_T_F32 && a.p.head_dim <= 128 ? 64 : 32;
