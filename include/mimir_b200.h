@@ -13,7 +13,7 @@
  *   3. whole-graph calls                    (mirror of Model::forwardPassView itself: the
  *      layer list is translated once, weights are uploaded once, activations stay in HBM)
  *   4. serving calls with DEVICE pointers   (rotary positions, a paged key / value cache, attention
- *      over it, sampling)
+ *      over it, sampling; the norms and products of a layer between them)
  *
  * Layout conventions are the reference's: every activation is a flat row-major fp32 vector for
  * one sample (images CHW, sequences [seq, dim]); `batch` is a leading dimension added by this
@@ -515,7 +515,7 @@ int mimir_b200_dev_eltwise(int op, const float* a, const float* b, float* y, int
                            long long nb, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
- * 4. Serving: rotary positions, a paged key / value cache, attention over it, a token from logits
+ * 4. Serving: rotary positions, a paged key / value cache, attention over it, a token from logits, a layer's norms and products
  *
  * What a host that generates text for many users at once needs next to the layer ops; no counterpart in the reference, whose
  * generation re-runs the prefix.  Device pointers, asynchronous on `stream` (a cudaStream_t of the calling thread's current
@@ -650,6 +650,51 @@ int mimir_b200_dev_paged_attention(const MimirPagedCache* cache, const MimirPage
 int mimir_b200_dev_sample_rows(const void* logits, int type, long long rows, int n, long long row_stride, const float* temperature,
                                const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* ids,
                                float* logprob, void* stream);
+
+/* Rows between a layer's products.  s = x + residual (x alone where residual is NULL), in fp32; sum receives s in x's type.  With norm
+ * != 0, v = s / sqrt(mean(s^2) + eps) * gamma over the n elements of the row, s before its rounding to sum; else v = s.  y receives v in
+ * y_type: F32, F16, BF16, or E4M3 codes with one scale a row, y_scale = (largest magnitude of v) * (1 / 448 in fp32), codes as dev_cache_write
+ * makes them.  A row's own numbers decide about it alone: one that holds an infinity or what is not a number leaves the others as they are.
+ * sum may be x or residual, and y may be x or residual, with their stride and type; other overlaps are not allowed.  n up to 32 768. */
+typedef struct MimirNormRows {
+  const void* x;        /* [rows][n], rows x_stride elements apart */
+  const void* residual; /* the same type, or NULL */
+  void* sum;            /* the same type, or NULL */
+  const float* gamma;   /* [n], or NULL (ones); only with norm */
+  void* y;              /* [rows][n] of y_type */
+  float* y_scale;       /* [rows], E4M3 only */
+  int64_t x_stride, residual_stride, sum_stride, y_stride;
+  int32_t type, y_type; /* type: F32, F16 or BF16 */
+  int32_t rows, n, norm;
+  float eps;
+} MimirNormRows;
+int mimir_b200_dev_norm_rows(const MimirNormRows* norm, void* stream);
+
+/* Products of rows with a weight matrix: z = x w^T (with E4M3 operands times x_scale of the row and w_scale of the feature) + bias,
+ *   dev_linear:       out = act(z) + residual
+ *   dev_gated_linear: out = act(z) * z', z' likewise from up, up_scale and up_bias
+ * x, w and up have one type, F16, BF16 or E4M3; their rows start on 16 bytes and have strides of multiples of 16 bytes; any n_in, n_out and
+ * rows.  out (and residual, of its type) has any alignment of its elements and any stride.  Products are exact and summed in fp32, the result is rounded
+ * once: the tensor cores' sums lose up to 2^-23 of their size for each 16 (E4M3: 32) of n_in; for results of type F32 they are taken out every
+ * 256 and added rounded.  activation: -1 (none), MIMIR_B200_ELT_GELU, _SILU, _RELU, _TANH or _SIGMOID.  residual may be out, with its
+ * stride; other overlaps of out are not allowed. */
+typedef struct MimirLinear {
+  const void* x;         /* [rows][n_in] */
+  const void* w;         /* [n_out][n_in]; of a gated pair the one that the activation follows */
+  const void* up;        /* [n_out][n_in], dev_gated_linear only */
+  const float* x_scale;  /* [rows], E4M3 only */
+  const float* w_scale;  /* [n_out], E4M3 only */
+  const float* up_scale; /* [n_out], E4M3 only, dev_gated_linear only */
+  const float* bias;     /* [n_out], or NULL */
+  const float* up_bias;  /* [n_out], or NULL, dev_gated_linear only */
+  const void* residual;  /* [rows][n_out] of out_type, or NULL; dev_linear only */
+  void* out;             /* [rows][n_out] */
+  int64_t x_stride, w_stride, up_stride, residual_stride, out_stride; /* elements */
+  int32_t type, out_type; /* out_type: F32, F16 or BF16 */
+  int32_t rows, n_in, n_out, activation;
+} MimirLinear;
+int mimir_b200_dev_linear(const MimirLinear* linear, void* stream);
+int mimir_b200_dev_gated_linear(const MimirLinear* linear, void* stream);
 
 #ifdef __cplusplus
 }

@@ -127,6 +127,18 @@ class MimirPagedAttention(C.Structure):
         (n, C.c_int32) for n in ("type", "heads", "causal", "window")] + [("scale", C.c_float), ("reserved", C.c_int32)]
 
 
+class MimirNormRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "sum", "gamma", "y", "y_scale")] + [
+        (n, C.c_int64) for n in ("x_stride", "residual_stride", "sum_stride", "y_stride")] + [
+        (n, C.c_int32) for n in ("type", "y_type", "rows", "n", "norm")] + [("eps", C.c_float)]
+
+
+class MimirLinear(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "up", "x_scale", "w_scale", "up_scale", "bias", "up_bias", "residual", "out")] + [
+        (n, C.c_int64) for n in ("x_stride", "w_stride", "up_stride", "residual_stride", "out_stride")] + [
+        (n, C.c_int32) for n in ("type", "out_type", "rows", "n_in", "n_out", "activation")]
+
+
 # Defaults of the reference's `struct Layer` (Layers.hpp:86-219) for the fields the descriptor
 # carries, after the accessor resolution the shim performs (kernel 3, stride 1, padding 0).
 LAYER_DEFAULTS = dict(

@@ -4,6 +4,7 @@
 
 #include "common.h"
 #include "host_call.h"
+#include "layer.cuh"
 #include "paged.cuh"
 
 namespace mb {
@@ -135,6 +136,86 @@ int check_attention(const char* what, const MimirPagedCache* c, const MimirPaged
   return MIMIR_B200_OK;
 }
 
+// ---- a layer's norms and products ---------------------------------------------------------------------------------------------------
+bool on_boundary(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0; }
+// rows of `wide` elements, `stride` apart, that do not run into one another
+int check_row_stride(const char* what, const char* name, long long stride, long long rows, long long wide) {
+  if (stride < 0 || (rows > 1 && stride < wide) || stride >= (1LL << 36))
+    return fail(MIMIR_B200_E_INVALID, "%s: %s has rows of %lld elements, %lld apart", what, name, wide, stride);
+  return MIMIR_B200_OK;
+}
+
+int check_norm_rows(const MimirNormRows* a) {
+  const char* what = "norm_rows";
+  if (!a) return fail(MIMIR_B200_E_INVALID, "%s: null argument", what);
+  if (!row_type(a->type)) return fail(MIMIR_B200_E_INVALID, "%s: x is F32, F16 or BF16, not type %d", what, a->type);
+  if (!row_type(a->y_type) && a->y_type != MIMIR_B200_T_E4M3)
+    return fail(a->y_type == MIMIR_B200_T_I8 ? MIMIR_B200_E_UNSUPPORTED : MIMIR_B200_E_INVALID, "%s: y is F32, F16, BF16 or E4M3, not type %d", what, a->y_type);
+  if (a->rows < 0 || a->n <= 0) return fail(MIMIR_B200_E_INVALID, "%s: %d rows of %d", what, a->rows, a->n);
+  if (a->n > 32768) return fail(MIMIR_B200_E_UNSUPPORTED, "%s: rows of %d elements (32 768 at most)", what, a->n);
+  if (a->norm && !(a->eps >= 0.0f && std::isfinite(a->eps))) return fail(MIMIR_B200_E_INVALID, "%s: eps is negative or not finite", what);
+  if (!a->norm && a->gamma) return fail(MIMIR_B200_E_INVALID, "%s: gamma without the norm", what);
+  if ((a->y_type == MIMIR_B200_T_E4M3) != (a->y_scale != nullptr)) return fail(MIMIR_B200_E_INVALID, "%s: y_scale belongs to a y of type E4M3", what);
+  MB_TRY(check_row_stride(what, "x", a->x_stride, a->rows, a->n));
+  if (a->residual) MB_TRY(check_row_stride(what, "residual", a->residual_stride, a->rows, a->n));
+  if (a->sum) MB_TRY(check_row_stride(what, "sum", a->sum_stride, a->rows, a->n));
+  MB_TRY(check_row_stride(what, "y", a->y_stride, a->rows, a->n));
+  if (a->y == a->sum && a->y) return fail(MIMIR_B200_E_INVALID, "%s: sum and y are one tensor", what);
+  if ((a->sum && ((a->sum == a->x && a->sum_stride != a->x_stride) || (a->sum == a->residual && a->sum_stride != a->residual_stride))) ||
+      (a->y && ((a->y == a->x && (a->y_stride != a->x_stride || a->y_type != a->type)) ||
+                (a->y == a->residual && (a->y_stride != a->residual_stride || a->y_type != a->type)))))
+    return fail(MIMIR_B200_E_INVALID, "%s: in place with another stride or type", what);
+  return MIMIR_B200_OK;
+}
+
+int check_linear(const char* what, const MimirLinear* a, bool gated) {
+  if (!a) return fail(MIMIR_B200_E_INVALID, "%s: null argument", what);
+  if (a->type == MIMIR_B200_T_F32 || a->type == MIMIR_B200_T_I8) return fail(MIMIR_B200_E_UNSUPPORTED, "%s: operands are F16, BF16 or E4M3, not type %d", what, a->type);
+  if (a->type != MIMIR_B200_T_F16 && a->type != MIMIR_B200_T_BF16 && a->type != MIMIR_B200_T_E4M3)
+    return fail(MIMIR_B200_E_INVALID, "%s: unknown operand type %d", what, a->type);
+  if (!row_type(a->out_type)) return fail(MIMIR_B200_E_INVALID, "%s: out is F32, F16 or BF16, not type %d", what, a->out_type);
+  if (a->rows < 0 || a->n_in <= 0 || a->n_out <= 0) return fail(MIMIR_B200_E_INVALID, "%s: %d rows, %d in, %d out", what, a->rows, a->n_in, a->n_out);
+  if (static_cast<long long>(a->rows) * a->n_out > (1LL << 40) || a->n_in > (1 << 24) || a->n_out > (1 << 24) || a->rows > (1 << 24))
+    return fail(MIMIR_B200_E_INVALID, "%s: too many rows, inputs or features for one call", what);
+  if (a->activation != -1 && (a->activation < MIMIR_B200_ELT_GELU || a->activation > MIMIR_B200_ELT_SIGMOID))
+    return fail(MIMIR_B200_E_UNSUPPORTED, "%s: activation %d is none of a product's", what, a->activation);
+  const bool coded = a->type == MIMIR_B200_T_E4M3;
+  if (coded != (a->x_scale != nullptr) || coded != (a->w_scale != nullptr) || (coded && gated) != (a->up_scale != nullptr))
+    return fail(MIMIR_B200_E_INVALID, "%s: scales belong to operands of type E4M3, each its own", what);
+  if (!gated && (a->up || a->up_bias)) return fail(MIMIR_B200_E_INVALID, "%s: up belongs to gated_linear", what);
+  if (gated && a->residual) return fail(MIMIR_B200_E_INVALID, "%s: a residual belongs to linear", what);
+  const long long unit = 16 / type_bytes(a->type);
+  MB_TRY(check_row_stride(what, "x", a->x_stride, a->rows, a->n_in));
+  MB_TRY(check_row_stride(what, "w", a->w_stride, a->n_out, a->n_in));
+  if (gated) MB_TRY(check_row_stride(what, "up", a->up_stride, a->n_out, a->n_in));
+  if (a->residual) MB_TRY(check_row_stride(what, "residual", a->residual_stride, a->rows, a->n_out));
+  MB_TRY(check_row_stride(what, "out", a->out_stride, a->rows, a->n_out));
+  if (a->x_stride % unit || a->w_stride % unit || (gated && a->up_stride % unit))
+    return fail(MIMIR_B200_E_UNSUPPORTED, "%s: strides of operands are multiples of 16 bytes", what);
+  if (a->residual && a->residual == a->out && a->residual_stride != a->out_stride) return fail(MIMIR_B200_E_INVALID, "%s: in place with two strides", what);
+  return MIMIR_B200_OK;
+}
+
+int run_linear(const char* what, const MimirLinear* a, bool gated, void* stream) {
+  MB_TRY(check_linear(what, a, gated));
+  MB_REQUIRE_INIT();
+  if (a->rows == 0) return MIMIR_B200_OK;
+  MB_TRY(check_device_pointer(what, "x", a->x));
+  MB_TRY(check_device_pointer(what, "w", a->w));
+  if (gated) MB_TRY(check_device_pointer(what, "up", a->up));
+  if (!aligned16(a->x) || !aligned16(a->w) || (gated && !aligned16(a->up))) return fail(MIMIR_B200_E_UNSUPPORTED, "%s: operands start on 16 bytes", what);
+  if (a->x_scale) MB_TRY(check_device_words(what, "x_scale", a->x_scale));
+  if (a->w_scale) MB_TRY(check_device_words(what, "w_scale", a->w_scale));
+  if (a->up_scale) MB_TRY(check_device_words(what, "up_scale", a->up_scale));
+  if (a->bias) MB_TRY(check_device_words(what, "bias", a->bias));
+  if (a->up_bias) MB_TRY(check_device_words(what, "up_bias", a->up_bias));
+  if (a->residual) MB_TRY(check_device_pointer(what, "residual", a->residual));
+  MB_TRY(check_device_pointer(what, "out", a->out));
+  const int size = type_bytes(a->out_type);
+  if (!on_boundary(a->out, size) || !on_boundary(a->residual, size)) return fail(MIMIR_B200_E_INVALID, "%s: misaligned pointer", what);
+  return launch_linear(*a, gated, static_cast<cudaStream_t>(stream));
+}
+
 }  // namespace
 }  // namespace mb
 
@@ -241,5 +322,24 @@ int mimir_b200_dev_sample_rows(const void* logits, int type, long long rows, int
   s.temperature = temperature, s.top_k = top_k, s.top_p = top_p, s.min_p = min_p, s.uniform = uniform, s.ids = ids, s.logprob = logprob;
   return launch_sample_rows(s, static_cast<cudaStream_t>(stream));
 }
+
+int mimir_b200_dev_norm_rows(const MimirNormRows* norm, void* stream) {
+  MB_TRY(check_norm_rows(norm));
+  MB_REQUIRE_INIT();
+  if (norm->rows == 0) return MIMIR_B200_OK;
+  MB_TRY(check_device_pointer("norm_rows", "x", norm->x));
+  MB_TRY(check_device_pointer("norm_rows", "y", norm->y));
+  if (norm->residual) MB_TRY(check_device_pointer("norm_rows", "residual", norm->residual));
+  if (norm->sum) MB_TRY(check_device_pointer("norm_rows", "sum", norm->sum));
+  if (norm->gamma) MB_TRY(check_device_words("norm_rows", "gamma", norm->gamma));
+  if (norm->y_scale) MB_TRY(check_device_words("norm_rows", "y_scale", norm->y_scale));
+  const int size = type_bytes(norm->type);
+  if (!on_boundary(norm->x, size) || !on_boundary(norm->residual, size) || !on_boundary(norm->sum, size) || !on_boundary(norm->y, type_bytes(norm->y_type)))
+    return fail(MIMIR_B200_E_INVALID, "norm_rows: misaligned pointer");
+  return launch_norm_rows(*norm, static_cast<cudaStream_t>(stream));
+}
+
+int mimir_b200_dev_linear(const MimirLinear* linear, void* stream) { return run_linear("linear", linear, false, stream); }
+int mimir_b200_dev_gated_linear(const MimirLinear* linear, void* stream) { return run_linear("gated_linear", linear, true, stream); }
 
 }  // extern "C"

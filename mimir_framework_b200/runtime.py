@@ -125,6 +125,9 @@ _SIGS = {
     "mimir_b200_paged_attention_workspace": [_P, _P, _P, _P],
     "mimir_b200_dev_paged_attention": [_P, _P, _P, _P],
     "mimir_b200_dev_sample_rows": [_P, C.c_int, C.c_longlong, C.c_int, C.c_longlong] + [_P] * 8,
+    "mimir_b200_dev_norm_rows": [_P, _P],
+    "mimir_b200_dev_linear": [_P, _P],
+    "mimir_b200_dev_gated_linear": [_P, _P],
 }
 
 EXPORTED_SYMBOLS = sorted(list(_SIGS) + ["mimir_b200_last_error"])
@@ -637,6 +640,30 @@ def dev_paged_attention(cache, batch, attention, stream: int = 0):
 def dev_sample_rows(logits, type, rows, n, row_stride, temperature, top_k, top_p, min_p, uniform, ids, logprob=None, stream: int = 0):
     """temperature, top_k, top_p, min_p and logprob may be None."""
     check(lib().mimir_b200_dev_sample_rows(logits, type, rows, n, row_stride, temperature, top_k, top_p, min_p, uniform, ids, logprob, stream))
+
+
+def norm_rows(x, y, rows, n, type, y_type, x_stride, y_stride, gamma=None, residual=None, residual_stride=0, sum=None, sum_stride=0, y_scale=None,
+              norm=True, eps=1e-5):
+    return abi.MimirNormRows(x, residual, sum, gamma, y, y_scale, x_stride, residual_stride, sum_stride, y_stride, type, y_type, rows, n, int(norm), eps)
+
+
+def dev_norm_rows(norm, stream: int = 0):
+    check(lib().mimir_b200_dev_norm_rows(C.byref(norm), stream))
+
+
+def linear(x, w, out, rows, n_in, n_out, type, out_type, x_stride, w_stride, out_stride, x_scale=None, w_scale=None, bias=None, activation=-1,
+           residual=None, residual_stride=0, up=None, up_stride=0, up_scale=None, up_bias=None):
+    """up and what belongs to it: of a gated pair (dev_gated_linear)."""
+    return abi.MimirLinear(x, w, up, x_scale, w_scale, up_scale, bias, up_bias, residual, out, x_stride, w_stride, up_stride, residual_stride, out_stride,
+                           type, out_type, rows, n_in, n_out, activation)
+
+
+def dev_linear(linear, stream: int = 0):
+    check(lib().mimir_b200_dev_linear(C.byref(linear), stream))
+
+
+def dev_gated_linear(linear, stream: int = 0):
+    check(lib().mimir_b200_dev_gated_linear(C.byref(linear), stream))
 
 
 class Replicas:
