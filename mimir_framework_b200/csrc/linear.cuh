@@ -1,0 +1,123 @@
+// linear.cuh — what the two kernels of the serving group's products share: rows times a weight matrix on tcgen05 with both operands K-major,
+// as they lie in memory.
+//
+//   z[m][n] = sum_k x[m][k] w[n][k]  (times x_scale[m] w_scale[n] for E4M3)  + bias[n],    out = act(z) + residual,  or  act(z) * z_up
+//
+// A K block is 128 bytes of every operand row (64 values of 16 bits, 128 of 8), the span of the shared-memory swizzle; four instructions of 32
+// bytes each take it.  What differs between the operand types is the instruction's kind and format alone.
+#pragma once
+
+#include "common.h"
+#include "epilogue.cuh"
+#include "layer.cuh"
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace mb {
+
+constexpr int LIN_BLOCK = 128;   // bytes of a row in a K block
+constexpr int LIN_W_BOX = 64;    // weight rows of a TMA box
+constexpr int LIN_CHUNK = 256;   // inputs that results of F32 add up in the tensor core before they are taken out
+
+struct LinearParams {
+  const float* x_scale;
+  const float* w_scale;
+  const float* up_scale;
+  const float* bias;
+  const float* up_bias;
+  const char* residual;
+  char* out;
+  long long residual_row, out_row;  // bytes
+  int rows, n_out, out_type, act;
+  int kblocks, chunk;               // K blocks of a product, and of an accumulation in tensor memory
+  uint32_t formats;                 // instruction descriptor: operand formats
+  int vec_out, vec_res;             // result, residual: rows on 32 bytes
+  int vec_cols;                     // bias and weight scales on 16 bytes
+  int* err_word;
+};
+
+// linear_tiles.cu (many rows): tiles of 256 rows x 256 features; linear_rows.cu (few): 128 features and up to 256 rows
+double linear_tiles_cycles(const MimirLinear& a, bool gated);
+int launch_linear_tiles(const MimirLinear& a, const LinearParams& p, bool gated, cudaStream_t st);
+double linear_rows_cycles(const MimirLinear& a, bool gated);
+int launch_linear_rows(const MimirLinear& a, const LinearParams& p, bool gated, cudaStream_t st);
+// tensor map of an operand: boxes of 128 bytes x `box_rows` rows, 128-byte swizzle, zeros beyond its rows and inputs
+int make_operand_map(CUtensorMap* map, const void* base, int type, long long rows, int n_in, long long stride, int box_rows);
+
+namespace {
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+               : "memory");
+}
+// into this CTA's shared memory, counted on a barrier of the pair's
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1)
+               : "memory");
+}
+// 8-bit floats: 32 values of K an instruction
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// An instruction descriptor without its operand formats (LinearParams::formats): fp32 sums, both operands K-major
+__host__ __device__ constexpr uint32_t linear_idesc(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// not a number stays one
+__device__ __forceinline__ float relu_nan(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __noinline__ float act_slow(float v, int act) { return act == MIMIR_B200_ELT_TANH ? tanhf(v) : 1.0f / (1.0f + expf(-v)); }
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+  switch (act) {
+    case -1: break;
+    case MIMIR_B200_ELT_GELU:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = gelu_ref(v[j]);
+      break;
+    case MIMIR_B200_ELT_SILU:
+#pragma unroll
+      for (int j = 0; j < N; j += 2) silu2(v[j], v[j + 1]);
+      break;
+    case MIMIR_B200_ELT_RELU:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = relu_nan(v[j]);
+      break;
+    default:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = act_slow(v[j], act);
+  }
+}
+
+__device__ __forceinline__ float load_typed(const char* p, int type) {
+  if (type == MIMIR_B200_T_F32) return *reinterpret_cast<const float*>(p);
+  if (type == MIMIR_B200_T_F16) return __half2float(*reinterpret_cast<const __half*>(p));
+  return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
+}
+__device__ __forceinline__ void store_typed(char* p, int type, float v) {
+  if (type == MIMIR_B200_T_F32) *reinterpret_cast<float*>(p) = v;
+  else if (type == MIMIR_B200_T_F16) *reinterpret_cast<__half*>(p) = __float2half_rn(v);
+  else *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
+}
+
+}  // namespace
+}  // namespace mb

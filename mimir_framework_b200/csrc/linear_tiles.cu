@@ -1,0 +1,413 @@
+// linear_tiles.cu — products of many rows.
+//
+// Clusters of two CTAs on neighbouring SMs share a tile of 256 rows x 256 features (tcgen05 with cta_group::2): each loads its own 128 rows of x
+// and half of the weights' 256, so that a byte of operands in shared memory is used 256 times.  A gated pair's tile is 128 features of each matrix:
+// the leader's half of the N side is the gate's, the other's is up's, and a thread finds both of an output in its own row of
+// tensor memory.  The kernel is persistent, tensor memory holds two accumulators of 256 columns:
+//   warp 0     TMA into a ring of six stages of 32 KB a CTA
+//   warp 1     (the leader's) issues the instructions for both
+//   warps 2-9  results: two warps for each 32 rows, half of the columns each; 32 columns at a time through activation, gate and residual
+// Results of F32 are taken out every 256 inputs and added up in registers: the tensor core's additions truncate.
+#include "launch.cuh"
+#include "linear.cuh"
+
+namespace mb {
+namespace {
+
+constexpr int TM = 128, TN = 256;  // rows of a CTA, columns of an accumulator
+constexpr int STAGES = 6, A_BYTES = TM * LIN_BLOCK, W_BYTES = TN / 2 * LIN_BLOCK, STAGE = A_BYTES + W_BYTES;
+constexpr int THREADS = 320, EPI_WARPS = 8, TURN = 32 * 33 * 4;  // a warp's tile for results that are turned around
+constexpr int SMEM = STAGES * STAGE + EPI_WARPS * TURN + 256 + 1024;
+static_assert(SMEM <= 232448, "exceeds the 227 KB of shared memory a CTA may use");
+
+struct TileParams {
+  LinearParams l;
+  int tiles_m, tiles_n, group_n;
+  int full;  // tiles from this one on run as two of half the columns: the last round's, where it would leave half of the SMs idle
+};
+
+// Work item t: its tile and, of one that is cut, which half of the columns (else -1).  Groups of group_n column tiles, so that the tiles
+// at work at one time share rows and weights in L2.
+__device__ __forceinline__ int tile_of(const TileParams& p, int t, int& tm, int& tn) {
+  int cut = -1;
+  if (t >= p.full) {
+    cut = (t - p.full) & 1;
+    t = p.full + ((t - p.full) >> 1);
+  }
+  const int per = p.group_n * p.tiles_m, g = t / per, r = t - g * per, n0 = g * p.group_n, wide = min(p.group_n, p.tiles_n - n0);
+  tm = r / wide;
+  tn = n0 + r % wide;
+  return cut;
+}
+
+// scale and bias of 32 neighbouring features
+template <bool F8>
+__device__ __forceinline__ void scaled(const LinearParams& p, float (&v)[32], float sx, const float* scale, const float* bias, int col0) {
+  if (p.vec_cols && col0 + 32 <= p.n_out) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + col0 + j)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if constexpr (F8) {
+        const float4 s = __ldg(reinterpret_cast<const float4*>(scale + col0 + j));
+        v[j] = fmaf(v[j] * sx, s.x, b.x), v[j + 1] = fmaf(v[j + 1] * sx, s.y, b.y);
+        v[j + 2] = fmaf(v[j + 2] * sx, s.z, b.z), v[j + 3] = fmaf(v[j + 3] * sx, s.w, b.w);
+      } else if (bias) {
+        v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const bool there = col0 + j < p.n_out;
+    const float b = bias && there ? __ldg(bias + col0 + j) : 0.0f;
+    if constexpr (F8) v[j] = fmaf(v[j] * sx, there ? __ldg(scale + col0 + j) : 0.0f, b);
+    else v[j] += b;
+  }
+}
+
+// 32 results of this lane's row, columns col0 on, to where they belong
+__device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32], int row0, int col0, float* turn) {
+  const int lane = threadIdx.x & 31, row = row0 + lane;
+  const int size = p.out_type == MIMIR_B200_T_F32 ? 4 : 2;
+  const bool full = col0 + 32 <= p.n_out;
+  if (full && p.vec_out && (!p.residual || p.vec_res)) {
+    if (p.residual && row < p.rows) {
+      const char* r = p.residual + row * p.residual_row + static_cast<long long>(col0) * size;
+      if (size == 4) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          float q[8];
+          unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(r + j * 4), q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j + e] += q[e];
+        }
+      } else {
+        Raw8<MIMIR_B200_T_F16> raw[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw[j] = load8<MIMIR_B200_T_F16>(r + j * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float q[8];
+          if (p.out_type == MIMIR_B200_T_F16) {
+            unpack8<MIMIR_B200_T_F16>(raw[j], q);
+          } else {
+            Raw8<MIMIR_B200_T_BF16> b;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b.w[e] = raw[j].w[e];
+            unpack8<MIMIR_B200_T_BF16>(b, q);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[8 * j + e] += q[e];
+        }
+      }
+    }
+    char* o = p.out + row * p.out_row + static_cast<long long>(col0) * size;
+    if (row >= p.rows) {
+    } else if (size == 4) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) st_global_v8(reinterpret_cast<float*>(o) + j, &v[j]);
+    } else {
+      uint32_t w[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (p.out_type == MIMIR_B200_T_F16) {
+          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      st_global_v8_b32(o, &w[0]);
+      st_global_v8_b32(o + 32, &w[8]);
+    }
+    __syncwarp();
+    return;
+  }
+  // rows off their boundary, and the last columns: turned around, so that a warp's lanes write neighbours
+#pragma unroll
+  for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
+  __syncwarp();
+  const int col = col0 + lane, rows = min(32, p.rows - row0);
+  if (col < p.n_out) {
+    char* o = p.out + row0 * p.out_row + static_cast<long long>(col) * size;
+    const char* r = p.residual ? p.residual + row0 * p.residual_row + static_cast<long long>(col) * size : nullptr;
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) {
+      float z = turn[i * 33 + lane];
+      if (p.residual) z += load_typed(r + i * p.residual_row, p.out_type);
+      store_typed(o + i * p.out_row, p.out_type, z);
+    }
+  }
+  __syncwarp();
+}
+
+template <bool F8, bool GATED, bool F32>
+__global__ void __launch_bounds__(THREADS, 1)
+linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_up,
+                    const __grid_constant__ TileParams tp) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* turns = reinterpret_cast<float*>(smem + STAGES * STAGE);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + EPI_WARPS * TURN);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* acc_full = empty_bar + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const LinearParams& p = tp.l;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1, all = tp.tiles_m * tp.tiles_n, items = 2 * all - tp.full;
+  constexpr int OUT = GATED ? TN / 2 : TN;  // features of a tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * EPI_WARPS);  // (the leader's collects both CTAs' warps)
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the other's barriers are there
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    const bool one = elect_one();
+    const CUtensorMap* const wmap = GATED && rank ? &map_up : &map_w;
+    constexpr int per_block = F8 ? LIN_BLOCK : LIN_BLOCK / 2;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = first; t < items && ok; t += step) {
+      int tm, tn;
+      const int cut = tile_of(tp, t, tm, tn);
+      const int x_row = (2 * tm + rank) * TM;
+      int w_row = tn * OUT + (cut > 0 ? OUT / 2 : 0);
+      if (!GATED) w_row += rank * (cut >= 0 ? TN / 4 : TN / 2);
+      const uint32_t bytes = 2 * (A_BYTES + (cut >= 0 ? W_BYTES / 2 : W_BYTES));
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 101)) { ok = false; break; }
+        if (one) {
+          uint8_t* base = smem + stage * STAGE;
+          // the leader's barrier counts the bytes of both CTAs, whichever arrive first
+          if (rank == 0) mbar_expect_tx(&full_bar[stage], bytes);
+          const uint32_t fb = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          tma_load_2d_pair(base, &map_x, fb, kb * per_block, x_row);
+          tma_load_2d_pair(base + A_BYTES, wmap, fb, kb * per_block, w_row);
+          if (cut < 0) tma_load_2d_pair(base + A_BYTES + W_BYTES / 2, wmap, fb, kb * per_block, w_row + LIN_W_BOX);
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    // what was asked for has landed and been used (or the abort flag is up) before the CTA leaves
+    for (int s = 0; s < STAGES; ++s) {
+      if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 102)) break;
+      if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool one = elect_one();
+      const uint32_t id_full = linear_idesc(2 * TM, TN) | p.formats, id_cut = linear_idesc(2 * TM, TN / 2) | p.formats;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ready = false, ok = true;
+      for (int t = first; t < items && ok; t += step) {
+        const uint32_t idesc = t >= tp.full ? id_cut : id_full;
+        for (int kb = 0; kb < p.kblocks && ok;) {
+          if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.err_word, 103)) { ok = false; break; }
+          tcgen05_fence_after();
+          const uint32_t d = tmem + static_cast<uint32_t>(acc * TN);
+          const int from = kb, to = min(p.kblocks, kb + p.chunk);
+          for (; kb < to; ++kb) {
+            if (!__all_sync(0xffffffffu, ready) && !mbar_wait_warp(&full_bar[stage], phase, abort_flag, p.err_word, 104)) { ok = false; break; }
+            tcgen05_fence_after();
+            const uint32_t sa = smem_u32(smem + stage * STAGE);
+            const uint64_t da = make_smem_desc(sa, LIN_BLOCK), dw = make_smem_desc(sa + A_BYTES, LIN_BLOCK);
+            uint64_t* done = &empty_bar[stage];
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            ready = mbar_test(&full_bar[stage], phase);
+            if (one) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {  // 32 bytes further in a descriptor's address field: 2
+                const uint32_t add = (kb != from || k != 0) ? 1u : 0u;
+                if constexpr (F8) umma_f8_pair(d, da + 2 * k, dw + 2 * k, idesc, add);
+                else umma_bf16_pair(d, da + 2 * k, dw + 2 * k, idesc, add);
+              }
+              umma_commit_pair(mapa_shared(smem_u32(done), 0));
+              umma_commit_pair(mapa_shared(smem_u32(done), 1));
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (one) {
+            umma_commit_pair(mapa_shared(smem_u32(&acc_full[acc]), 0));
+            umma_commit_pair(mapa_shared(smem_u32(&acc_full[acc]), 1));
+          }
+          __syncwarp();
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    float* turn = turns + ew * (TURN / 4);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    auto take = [&]() -> uint32_t {
+      ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag, p.err_word, 105);
+      tcgen05_fence_after();
+      return tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * TN);
+    };
+    auto give_back = [&] {
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    };
+    for (int t = first; t < items && ok; t += step) {
+      int tm, tn;
+      const int cut = tile_of(tp, t, tm, tn);
+      const int row0 = (2 * tm + rank) * TM + quad * 32;
+      const int wide = cut >= 0 ? OUT / 2 : OUT;             // features of this item
+      const int mine = half * (wide / 2), nch = wide / 64;   // this warp's first, and how many times 32
+      const int col00 = tn * OUT + (cut > 0 ? OUT / 2 : 0) + mine;
+      float sx = 1.0f;
+      if (F8 && row0 + lane < p.rows) sx = __ldg(p.x_scale + row0 + lane);
+      auto finish = [&](float (&z)[32], float (&u)[32], int col0) {
+        scaled<F8>(p, z, sx, p.w_scale, p.bias, col0);
+        activate(z, p.act);
+        if constexpr (GATED) {
+          scaled<F8>(p, u, sx, p.up_scale, p.up_bias, col0);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] *= u[j];
+        }
+        write_out(p, z, row0, col0, turn);
+      };
+      if constexpr (F32) {
+        float v[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;
+        for (int kb = 0; kb < p.kblocks && ok; kb += p.chunk) {
+          const uint32_t at = take();
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // (of a gated pair: two of the one, two of the other)
+            const int n = GATED ? i & 1 : i;
+            if (n >= nch) continue;
+            float w[32];
+            tmem_ld_32x32(at + static_cast<uint32_t>(mine + n * 32 + (GATED && i >= 2 ? wide : 0)), w);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[i][j] += w[j];
+          }
+          give_back();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < (GATED ? 2 : 4); ++i)
+          if (i < nch && col00 + i * 32 < p.n_out) finish(v[i], v[GATED ? i + 2 : i], col00 + i * 32);
+      } else {
+        const uint32_t at = take();
+        if (!ok) break;
+#pragma unroll 1
+        for (int i = 0; i < nch; ++i) {
+          if (col00 + i * 32 >= p.n_out) break;
+          float z[32], u[32];
+          tmem_ld_32x32(at + static_cast<uint32_t>(mine + i * 32), z);
+          if constexpr (GATED) tmem_ld_32x32(at + static_cast<uint32_t>(mine + i * 32 + wide), u);
+          finish(z, u, col00 + i * 32);
+        }
+        give_back();
+      }
+    }
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither leaves, or frees tensor memory, while the other may still signal it
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+struct TileShape {
+  long long tiles_m, tiles_n;
+  int pairs;
+  long long full, items;
+};
+TileShape tile_shape(const MimirLinear& a, bool gated) {
+  TileShape s;
+  const int out = gated ? TN / 2 : TN;
+  s.tiles_m = (a.rows + 2 * TM - 1) / (2 * TM);
+  s.tiles_n = (a.n_out + out - 1) / out;
+  s.pairs = ctx().sm_count / 2;
+  const long long tiles = s.tiles_m * s.tiles_n, rest = tiles % s.pairs;
+  s.full = 2 * rest <= s.pairs ? tiles - rest : tiles;
+  s.items = 2 * tiles - s.full;
+  return s;
+}
+
+template <bool F8, bool GATED, bool F32>
+int launch_as(const CUtensorMap (&maps)[3], const TileParams& p, unsigned grid, cudaStream_t st) {
+  auto kern = linear_tiles_kernel<F8, GATED, F32>;
+  static PerDeviceOnce once;
+  MB_TRY(once.run([&]() -> int {
+    MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    return MIMIR_B200_OK;
+  }));
+  MB_TRY(launch_pdl(kern, dim3(grid), dim3(THREADS), SMEM, st, 2, maps[0], maps[1], maps[2], p));
+  count_launch();
+  return MIMIR_B200_OK;
+}
+
+}  // namespace
+
+double linear_tiles_cycles(const MimirLinear& a, bool gated) {
+  const TileShape s = tile_shape(a, gated);
+  if (s.items > 0x7fffffffLL / 4) return 1e30;
+  const double blocks = (static_cast<double>(a.n_in) * type_bytes(a.type) + LIN_BLOCK - 1) / LIN_BLOCK;
+  const long long rounds = (s.full + s.pairs - 1) / s.pairs;
+  return (rounds + (s.items > s.full ? 0.55 : 0.0)) * blocks * 4 * 128 + 4000.0;
+}
+
+int launch_linear_tiles(const MimirLinear& a, const LinearParams& l, bool gated, cudaStream_t st) {
+  const TileShape s = tile_shape(a, gated);
+  CUtensorMap maps[3];
+  MB_TRY(make_operand_map(&maps[0], a.x, a.type, a.rows, a.n_in, a.x_stride, TM));
+  MB_TRY(make_operand_map(&maps[1], a.w, a.type, a.n_out, a.n_in, a.w_stride, LIN_W_BOX));
+  maps[2] = maps[1];
+  if (gated) MB_TRY(make_operand_map(&maps[2], a.up, a.type, a.n_out, a.n_in, a.up_stride, LIN_W_BOX));
+  TileParams p = {};
+  p.l = l, p.tiles_m = static_cast<int>(s.tiles_m), p.tiles_n = static_cast<int>(s.tiles_n), p.full = static_cast<int>(s.full);
+  p.group_n = p.tiles_n < 8 ? p.tiles_n : 8;
+  const unsigned grid = static_cast<unsigned>(2 * (s.items < s.pairs ? s.items : s.pairs));
+  const bool f32 = a.out_type == MIMIR_B200_T_F32;
+  if (a.type == MIMIR_B200_T_E4M3)
+    return gated ? (f32 ? launch_as<true, true, true>(maps, p, grid, st) : launch_as<true, true, false>(maps, p, grid, st))
+                 : (f32 ? launch_as<true, false, true>(maps, p, grid, st) : launch_as<true, false, false>(maps, p, grid, st));
+  return gated ? (f32 ? launch_as<false, true, true>(maps, p, grid, st) : launch_as<false, true, false>(maps, p, grid, st))
+               : (f32 ? launch_as<false, false, true>(maps, p, grid, st) : launch_as<false, false, false>(maps, p, grid, st));
+}
+
+}  // namespace mb
