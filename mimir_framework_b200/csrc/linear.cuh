@@ -118,6 +118,28 @@ __device__ __forceinline__ void store_typed(char* p, int type, float v) {
   else if (type == MIMIR_B200_T_F16) *reinterpret_cast<__half*>(p) = __float2half_rn(v);
   else *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
 }
+// Eight neighbouring values, `left` of them there; vec: all, on 16 bytes
+__device__ __forceinline__ void load_eight(const char* p, int type, bool vec, int left, float (&v)[8]) {
+  if (vec) {
+    if (type == MIMIR_B200_T_F32) unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(p), v);
+    else if (type == MIMIR_B200_T_F16) unpack8<MIMIR_B200_T_F16>(load8<MIMIR_B200_T_F16>(p), v);
+    else unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(p), v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < left ? load_typed(p + j * type_bytes(type), type) : 0.0f;
+}
+__device__ __forceinline__ void store_eight(char* p, int type, bool vec, int left, const float (&v)[8]) {
+  if (vec) {
+    if (type == MIMIR_B200_T_F32) store8<MIMIR_B200_T_F32>(p, pack8<MIMIR_B200_T_F32>(v));
+    else if (type == MIMIR_B200_T_F16) store8<MIMIR_B200_T_F16>(p, pack8<MIMIR_B200_T_F16>(v));
+    else store8<MIMIR_B200_T_BF16>(p, pack8<MIMIR_B200_T_BF16>(v));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) store_typed(p + j * type_bytes(type), type, v[j]);
+}
 
 }  // namespace
 }  // namespace mb
