@@ -31,7 +31,7 @@ struct LinearParams {
   int rows, n_out, out_type, act;
   int kblocks, chunk;               // K blocks of a product, and of an accumulation in tensor memory
   uint32_t formats;                 // instruction descriptor: operand formats
-  int vec_out, vec_res;             // result, residual: rows on 32 bytes
+  int vec_out, vec_res;             // result, residual: all rows on 32 bytes, on 16, or neither (0)
   int vec_cols;                     // bias and weight scales on 16 bytes
   int* err_word;
 };
@@ -119,16 +119,6 @@ __device__ __forceinline__ void store_typed(char* p, int type, float v) {
   else *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
 }
 // Eight neighbouring values, `left` of them there; vec: all, on 16 bytes
-__device__ __forceinline__ void load_eight(const char* p, int type, bool vec, int left, float (&v)[8]) {
-  if (vec) {
-    if (type == MIMIR_B200_T_F32) unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(p), v);
-    else if (type == MIMIR_B200_T_F16) unpack8<MIMIR_B200_T_F16>(load8<MIMIR_B200_T_F16>(p), v);
-    else unpack8<MIMIR_B200_T_BF16>(load8<MIMIR_B200_T_BF16>(p), v);
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < left ? load_typed(p + j * type_bytes(type), type) : 0.0f;
-}
 __device__ __forceinline__ void store_eight(char* p, int type, bool vec, int left, const float (&v)[8]) {
   if (vec) {
     if (type == MIMIR_B200_T_F32) store8<MIMIR_B200_T_F32>(p, pack8<MIMIR_B200_T_F32>(v));

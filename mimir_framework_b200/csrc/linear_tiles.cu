@@ -71,7 +71,7 @@ __device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32],
   const int lane = threadIdx.x & 31, row = row0 + lane;
   const int size = p.out_type == MIMIR_B200_T_F32 ? 4 : 2;
   const bool full = col0 + 32 <= p.n_out;
-  if (full && p.vec_out && (!p.residual || p.vec_res)) {
+  if (full && p.vec_out == 32 && (!p.residual || p.vec_res)) {
     if (p.residual && row < p.rows) {
       const char* r = p.residual + row * p.residual_row + static_cast<long long>(col0) * size;
       if (size == 4) {
