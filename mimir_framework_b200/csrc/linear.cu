@@ -44,9 +44,8 @@ int launch_linear(const MimirLinear& a, bool gated, cudaStream_t st) {
   p.formats = a.type == MIMIR_B200_T_BF16 ? (1u << 7) | (1u << 10) : 0u;  // (half, E4M3: 0)
   p.vec_out = on(a.out, p.out_row, 32) ? 32 : on(a.out, p.out_row, 16) ? 16 : 0;
   p.vec_res = on(a.residual, p.residual_row, 32) ? 32 : on(a.residual, p.residual_row, 16) ? 16 : 0;
-  p.vec_cols = on(a.bias, 0, 16) && on(a.up_bias, 0, 16) && on(a.w_scale, 0, 16) && on(a.up_scale, 0, 16);
   p.err_word = ctx().dev_error_word;
-  return linear_rows_cycles(a, gated) <= linear_tiles_cycles(a, gated) ? launch_linear_rows(a, p, gated, st) : launch_linear_tiles(a, p, gated, st);
+  return linear_rows_us(a, gated) <= linear_tiles_us(a, gated) ? launch_linear_rows(a, p, gated, st) : launch_linear_tiles(a, p, gated, st);
 }
 
 }  // namespace mb

@@ -32,14 +32,13 @@ struct LinearParams {
   int kblocks, chunk;               // K blocks of a product, and of an accumulation in tensor memory
   uint32_t formats;                 // instruction descriptor: operand formats
   int vec_out, vec_res;             // result, residual: all rows on 32 bytes, on 16, or neither (0)
-  int vec_cols;                     // bias and weight scales on 16 bytes
   int* err_word;
 };
 
 // linear_tiles.cu (many rows): tiles of 256 rows x 256 features; linear_rows.cu (few): 128 features and up to 256 rows
-double linear_tiles_cycles(const MimirLinear& a, bool gated);
+double linear_tiles_us(const MimirLinear& a, bool gated);
 int launch_linear_tiles(const MimirLinear& a, const LinearParams& p, bool gated, cudaStream_t st);
-double linear_rows_cycles(const MimirLinear& a, bool gated);
+double linear_rows_us(const MimirLinear& a, bool gated);
 int launch_linear_rows(const MimirLinear& a, const LinearParams& p, bool gated, cudaStream_t st);
 // tensor map of an operand: boxes of 128 bytes x `box_rows` rows, 128-byte swizzle, zeros beyond its rows and inputs
 int make_operand_map(CUtensorMap* map, const void* base, int type, long long rows, int n_in, long long stride, int box_rows);

@@ -8,6 +8,9 @@
 //   warp 1     (the leader's) issues the instructions for both
 //   warps 2-9  results: two warps for each 32 rows, half of the columns each; 32 columns at a time through activation, gate and residual
 // Results of F32 are taken out every 256 inputs and added up in registers: the tensor core's additions truncate.
+#include <algorithm>
+#include <cmath>
+
 #include "launch.cuh"
 #include "linear.cuh"
 
@@ -16,8 +19,10 @@ namespace {
 
 constexpr int TM = 128, TN = 256;  // rows of a CTA, columns of an accumulator
 constexpr int STAGES = 6, A_BYTES = TM * LIN_BLOCK, W_BYTES = TN / 2 * LIN_BLOCK, STAGE = A_BYTES + W_BYTES;
-constexpr int THREADS = 320, EPI_WARPS = 8, TURN = 32 * 33 * 4;  // a warp's tile for results that are turned around
-constexpr int SMEM = STAGES * STAGE + EPI_WARPS * TURN + 256 + 1024;
+constexpr int THREADS = 320, EPI_WARPS = 8;
+constexpr int TURN = 32 * 17 * 4;     // a warp's tile for results that are turned around, 16 columns at a time
+constexpr int COLS = 256 * 4;         // scales and biases of a warp's columns
+constexpr int SMEM = STAGES * STAGE + EPI_WARPS * (TURN + COLS) + 256 + 1024;
 static_assert(SMEM <= 232448, "exceeds the 227 KB of shared memory a CTA may use");
 
 struct TileParams {
@@ -40,29 +45,19 @@ __device__ __forceinline__ int tile_of(const TileParams& p, int t, int& tm, int&
   return cut;
 }
 
-// scale and bias of 32 neighbouring features
+// scale and bias of 32 neighbouring features, from shared memory
 template <bool F8>
-__device__ __forceinline__ void scaled(const LinearParams& p, float (&v)[32], float sx, const float* scale, const float* bias, int col0) {
-  if (p.vec_cols && col0 + 32 <= p.n_out) {
+__device__ __forceinline__ void scaled(float (&v)[32], float sx, const float* scale, const float* bias) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + col0 + j)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if constexpr (F8) {
-        const float4 s = __ldg(reinterpret_cast<const float4*>(scale + col0 + j));
-        v[j] = fmaf(v[j] * sx, s.x, b.x), v[j + 1] = fmaf(v[j + 1] * sx, s.y, b.y);
-        v[j + 2] = fmaf(v[j + 2] * sx, s.z, b.z), v[j + 3] = fmaf(v[j + 3] * sx, s.w, b.w);
-      } else if (bias) {
-        v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
-      }
+  for (int j = 0; j < 32; j += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(bias + j);
+    if constexpr (F8) {
+      const float4 s = *reinterpret_cast<const float4*>(scale + j);
+      v[j] = fmaf(v[j] * sx, s.x, b.x), v[j + 1] = fmaf(v[j + 1] * sx, s.y, b.y);
+      v[j + 2] = fmaf(v[j + 2] * sx, s.z, b.z), v[j + 3] = fmaf(v[j + 3] * sx, s.w, b.w);
+    } else {
+      v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
     }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const bool there = col0 + j < p.n_out;
-    const float b = bias && there ? __ldg(bias + col0 + j) : 0.0f;
-    if constexpr (F8) v[j] = fmaf(v[j] * sx, there ? __ldg(scale + col0 + j) : 0.0f, b);
-    else v[j] += b;
   }
 }
 
@@ -125,22 +120,36 @@ __device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32],
     __syncwarp();
     return;
   }
-  // rows off their boundary, and the last columns: turned around, so that a warp's lanes write neighbours
+  // rows off their boundary, and the last columns: turned around, so that a warp's lanes write neighbours, 16 columns of two rows at a time
+  const int rows = min(32, p.rows - row0);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
-  __syncwarp();
-  const int col = col0 + lane, rows = min(32, p.rows - row0);
-  if (col < p.n_out) {
-    char* o = p.out + row0 * p.out_row + static_cast<long long>(col) * size;
-    const char* r = p.residual ? p.residual + row0 * p.residual_row + static_cast<long long>(col) * size : nullptr;
-#pragma unroll 8
-    for (int i = 0; i < rows; ++i) {
-      float z = turn[i * 33 + lane];
-      if (p.residual) z += load_typed(r + i * p.residual_row, p.out_type);
-      store_typed(o + i * p.out_row, p.out_type, z);
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = v[h * 16 + j];
+    __syncwarp();
+    const int at = lane & 15, col = col0 + h * 16 + at;
+    if (col < p.n_out) {
+      char* o = p.out + row0 * p.out_row + static_cast<long long>(col) * size;
+      const char* r = p.residual ? p.residual + row0 * p.residual_row + static_cast<long long>(col) * size : nullptr;
+#pragma unroll
+      for (int i0 = 0; i0 < 32; i0 += 16) {
+        float q[8];
+        if (p.residual) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int k = i0 + 2 * i + (lane >> 4);
+            q[i] = k < rows ? load_typed(r + k * p.residual_row, p.out_type) : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k = i0 + 2 * i + (lane >> 4);
+          if (k < rows) store_typed(o + k * p.out_row, p.out_type, p.residual ? turn[k * 17 + at] + q[i] : turn[k * 17 + at]);
+        }
+      }
     }
+    __syncwarp();
   }
-  __syncwarp();
 }
 
 template <bool F8, bool GATED, bool F32>
@@ -150,7 +159,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* turns = reinterpret_cast<float*>(smem + STAGES * STAGE);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + EPI_WARPS * TURN);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + EPI_WARPS * (TURN + COLS));
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* acc_full = empty_bar + STAGES;
   uint64_t* acc_empty = acc_full + 2;
@@ -267,7 +276,8 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
   } else {
     const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-    float* turn = turns + ew * (TURN / 4);
+    float* const turn = turns + ew * ((TURN + COLS) / 4);
+    float* const cols = turn + TURN / 4;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -291,11 +301,23 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const int col00 = tn * OUT + (cut > 0 ? OUT / 2 : 0) + mine;
       float sx = 1.0f;
       if (F8 && row0 + lane < p.rows) sx = __ldg(p.x_scale + row0 + lane);
+      // the columns' scales and biases while the sums are made: [bias][of up][scale][of up], as many as the warp has columns (a gated pair: 64, else 128)
+      constexpr int EACH = GATED ? 64 : 128;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int which = i * 32 / EACH, col = col00 + i * 32 % EACH + lane;
+        if (!F8 && which >= (GATED ? 2 : 1)) break;
+        const float* from = GATED ? (which == 0 ? p.bias : which == 1 ? p.up_bias : which == 2 ? p.w_scale : p.up_scale) : which == 0 ? p.bias : p.w_scale;
+        cols[i * 32 + lane] = from && col < p.n_out ? __ldg(from + col) : 0.0f;
+      }
+      __syncwarp();
+      const float* const my_cols = cols - col00;  // (+ column)
       auto finish = [&](float (&z)[32], float (&u)[32], int col0) {
-        scaled<F8>(p, z, sx, p.w_scale, p.bias, col0);
+        scaled<F8>(z, sx, my_cols + (GATED ? 2 : 1) * EACH + col0, my_cols + col0);
         activate(z, p.act);
         if constexpr (GATED) {
-          scaled<F8>(p, u, sx, p.up_scale, p.up_bias, col0);
+          scaled<F8>(u, sx, my_cols + 3 * EACH + col0, my_cols + EACH + col0);
 #pragma unroll
           for (int j = 0; j < 32; ++j) z[j] *= u[j];
         }
@@ -383,12 +405,13 @@ int launch_as(const CUtensorMap (&maps)[3], const TileParams& p, unsigned grid, 
 
 }  // namespace
 
-double linear_tiles_cycles(const MimirLinear& a, bool gated) {
+// An estimate in us (see row_shape): 0.376 for a block of a round of tiles, 0.233 for one of halves.
+double linear_tiles_us(const MimirLinear& a, bool gated) {
   const TileShape s = tile_shape(a, gated);
   if (s.items > 0x7fffffffLL / 4) return 1e30;
-  const double blocks = (static_cast<double>(a.n_in) * type_bytes(a.type) + LIN_BLOCK - 1) / LIN_BLOCK;
-  const long long rounds = (s.full + s.pairs - 1) / s.pairs;
-  return (rounds + (s.items > s.full ? 0.55 : 0.0)) * blocks * 4 * 128 + 4000.0;
+  const double blocks = std::ceil(static_cast<double>(a.n_in) * type_bytes(a.type) / LIN_BLOCK), rounds = std::ceil(static_cast<double>(s.full) / s.pairs);
+  const double hbm = blocks * LIN_BLOCK * (gated ? 2 : 1) * a.n_out / 6.55e6;
+  return std::max(blocks * (0.376 * rounds + (s.items > s.full ? 0.233 : 0.0)), hbm) + 6.5 + (a.type == MIMIR_B200_T_E4M3 ? 1.0 : 0.0);
 }
 
 int launch_linear_tiles(const MimirLinear& a, const LinearParams& l, bool gated, cudaStream_t st) {

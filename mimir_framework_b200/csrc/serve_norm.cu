@@ -5,15 +5,20 @@
 // One pass: a row lies in the registers of the threads that share it (eight elements at a time, so that loads and stores are 16 bytes), its
 // sum of squares and, for codes, its largest magnitude are each one meeting of these threads.  Statistics are fp32.  Codes are those
 // of an IEEE division by the scale, as in the cache.
+#include <algorithm>
+
 #include "common.h"
+#include "epilogue.cuh"
 #include "launch.cuh"
 #include "layer.cuh"
 #include "paged.cuh"
+#include "sm100_ptx.cuh"
 
 namespace mb {
 namespace {
 
 constexpr int NR_WARP_THREADS = 128;  // of a CTA whose warps have a row each
+constexpr int NR_MAX_STAGES = 8, NR_RING = 108 * 1024;  // rows ahead at most, bytes of them in a CTA
 
 struct NormParams {
   const char* x;
@@ -23,9 +28,10 @@ struct NormParams {
   char* y;
   float* y_scale;
   long long x_row, residual_row, sum_row, y_row;  // bytes
-  int rows, n, norm, early;
+  int rows, n, norm, early, stages;
   bool x_vec, residual_vec, sum_vec, gamma_vec, y_vec;  // rows start on 16 bytes
-  float eps;
+  float eps, inv_n;
+  int* err_word;
 };
 
 // Eight elements from column `col` on, those from n on zero.
@@ -60,7 +66,27 @@ __device__ __forceinline__ void row_store8(char* row, int col, int n, bool vec, 
   }
 }
 
-// A number of each thread of a row, joined; every thread has the result (`buf`: 32 words of the CTA's, of one meeting).
+// Two values in a register pair, for the instructions that work on both (epilogue.cuh); eight elements are four pairs.
+using Pair = unsigned long long;
+template <int T>
+__device__ __forceinline__ void to_pairs(const Raw8<T>& r, Pair (&f)[4]) {
+  float v[8];
+  unpack8<T>(r, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = pack2(v[2 * i], v[2 * i + 1]);
+}
+__device__ __forceinline__ void from_pairs(const Pair (&f)[4], float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(f[i], v[2 * i], v[2 * i + 1]);
+}
+// the larger of two magnitudes and a third number, not a number if one of them is none
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// A number of each thread of a row, joined; every thread has the result (`buf`: 24 words of the CTA's, of one meeting).
 template <bool WARP, bool MAX>
 __device__ __forceinline__ float meet(float v, float* buf) {
 #pragma unroll
@@ -69,128 +95,269 @@ __device__ __forceinline__ float meet(float v, float* buf) {
     v = MAX ? fmaxf(v, w) : v + w;
   }
   if constexpr (WARP) return v;
-  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
   if (warps == 1) return v;
-  if (lane == 0) buf[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = lane < warps ? buf[lane] : 0.0f;  // (sums and magnitudes: zero changes neither)
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, w) : v + w;
+  // (words of no warp are zero: neither sums nor magnitudes mind)
+  const float4* words = reinterpret_cast<const float4*>(buf);
+  auto four = [](float4 s) { return MAX ? fmaxf(fmaxf(s.x, s.y), fmaxf(s.z, s.w)) : (s.x + s.y) + (s.z + s.w); };
+  const float a = four(words[0]), b = four(words[1]);
+  v = MAX ? fmaxf(a, b) : a + b;
+  if (warps > 8) {
+    const float c = four(words[2]), d = four(words[3]);
+    v = MAX ? fmaxf(v, fmaxf(c, d)) : v + (c + d);
+    if (warps > 16) {
+      const float e = four(words[4]), g = four(words[5]);
+      v = MAX ? fmaxf(v, fmaxf(e, g)) : v + (e + g);
+    }
   }
   return v;
 }
+// 1 / sqrt(x), off by less than 1.5 units of 2^-24: the approximation (2^-22) and a Newton step
+__device__ __forceinline__ float root_reciprocal(float x) {
+  float r;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  const float e = fmaf(-x * r, r, 1.0f);
+  return fabsf(e) < 1.0f ? fmaf(0.5f * r, e, r) : r;  // (zero and infinity: as the approximation has them)
+}
 
-// V vectors of eight elements a thread; WARP: a row to a warp, else to the CTA.
+// A row from the sums s that its threads hold on: V vectors of eight elements each; WARP: a row to a warp, else to the CTA.  Instructions bound it
+// where memory does not, so two elements go through one wherever there is such a one (8 192 rows of 4 096 with residual to codes took 37 M
+// instructions and 47 us element by element, 42 so).  A row that is not `live` takes part in the meetings and leaves nothing.
 template <int TX, int TY, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? NR_WARP_THREADS : 1024) norm_rows_serve_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float buf[2][32];
-  pdl_early_if(p.early);
-  pdl_wait();
-  const int row = WARP ? blockIdx.x * (NR_WARP_THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
-  if (WARP && row >= p.rows) return;
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x, step = (WARP ? 32 : blockDim.x) * 8;
-  const char* x = p.x + row * p.x_row;
-  Raw8<TX> raw[V], res[V];
+__device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, Pair (&f)[V][4], float (&buf)[2][32]) {
+  if (p.sum && live) {
+    char* const sum = p.sum + row * p.sum_row;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int col = v * step + t * 8;
-    raw[v] = row_load8<TX>(x, col, p.n, p.x_vec);
-    if (p.residual) res[v] = row_load8<TX>(p.residual + row * p.residual_row, col, p.n, p.residual_vec);
-  }
-  float f[V][8];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    unpack8<TX>(raw[v], f[v]);
-    if (p.residual) {
-      float g[8];
-      unpack8<TX>(res[v], g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[v][e] += g[e];
+    for (int v = 0; v < V; ++v) {
+      float s[8];
+      from_pairs(f[v], s);
+      row_store8<TX>(sum, v * step + t * 8, p.n, p.sum_vec, pack8<TX>(s));
     }
   }
   if (p.norm) {
-    float q = 0.0f;
+    Pair q2 = pack2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float a = 0.0f, b = 0.0f;
+      Pair a = mul2(f[v][0], f[v][0]);
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) a = fmaf(f[v][e], f[v][e], a), b = fmaf(f[v][e + 1], f[v][e + 1], b);
-      q += a + b;
+      for (int i = 1; i < 4; ++i) a = fma2(f[v][i], f[v][i], a);
+      q2 = add2(q2, a);
     }
-    q = meet<WARP, false>(q, buf[0]);
-    if (p.sum) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) row_store8<TX>(p.sum + row * p.sum_row, v * step + t * 8, p.n, p.sum_vec, pack8<TX>(f[v]));
-    }
-    const float mean = __fdiv_rn(q, static_cast<float>(p.n)) + p.eps;
-    float r = __frsqrt_rn(mean);
+    float q0, q1;
+    unpack2(q2, q0, q1);
+    const float q = meet<WARP, false>(q0 + q1, buf[0]), mean = fmaf(q, p.inv_n, p.eps);
+    float r = root_reciprocal(mean);
     if (!(q < INFINITY) || mean < 0x1p-100f) {
       // squares beyond fp32's range (or below it, next to no eps): once more with the row's largest near one
       float top = 0.0f, rest = 0.0f;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
+      for (int v = 0; v < V; ++v) {
+        float s[8];
+        from_pairs(f[v], s);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fabsf(f[v][e]) > top || f[v][e] != f[v][e] ? fabsf(f[v][e]) : top;
+        for (int e = 0; e < 8; e += 2) top = max_abs3(s[e], s[e + 1], top);
+      }
       if (!(top < INFINITY)) top = INFINITY;  // (not a number is as good as infinite here)
       top = meet<WARP, true>(top, buf[1]);
       if (top > 0.0f && top < INFINITY) {
         const int k = max(-100, min(126, ilogbf(top)));
         const float down = scalbnf(1.0f, -k);
 #pragma unroll
-        for (int v = 0; v < V; ++v)
+        for (int v = 0; v < V; ++v) {
+          float s[8];
+          from_pairs(f[v], s);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            f[v][e] *= down;
-            rest = fmaf(f[v][e], f[v][e], rest);
+            s[e] *= down;
+            rest = fmaf(s[e], s[e], rest);
           }
-        r = __frsqrt_rn(__fdiv_rn(meet<WARP, false>(rest, buf[0]), static_cast<float>(p.n)) + p.eps * down * down);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[v][i] = pack2(s[2 * i], s[2 * i + 1]);
+        }
+        r = root_reciprocal(fmaf(meet<WARP, false>(rest, buf[0]), p.inv_n, p.eps * down * down));
       }
     }
+    const Pair r2 = pack2(r, r);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int col = v * step + t * 8;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[v][e] *= r;
       if (p.gamma) {
-        float g[8];
-        unpack8<MIMIR_B200_T_F32>(row_load8<MIMIR_B200_T_F32>(reinterpret_cast<const char*>(p.gamma), col, p.n, p.gamma_vec), g);
+        Pair g[4];
+        to_pairs<MIMIR_B200_T_F32>(row_load8<MIMIR_B200_T_F32>(reinterpret_cast<const char*>(p.gamma), col, p.n, p.gamma_vec), g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[v][e] = col + e < p.n ? f[v][e] * g[e] : 0.0f;
+        for (int i = 0; i < 4; ++i) f[v][i] = mul2(mul2(f[v][i], r2), g[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], r2);
       }
     }
-  } else if (p.sum) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) row_store8<TX>(p.sum + row * p.sum_row, v * step + t * 8, p.n, p.sum_vec, pack8<TX>(f[v]));
   }
-  float scale = 0.0f;
+  char* const y = p.y + row * p.y_row;
   if constexpr (TY == MIMIR_B200_T_E4M3) {
     float top = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < V; ++v) {
+      float s[8];
+      from_pairs(f[v], s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (fabsf(f[v][e]) < INFINITY) top = fmaxf(top, fabsf(f[v][e]));
-    scale = __fmul_rn(meet<WARP, true>(top, buf[1]), 1.0f / 448.0f);
-    if (t == 0) p.y_scale[row] = scale;
+      for (int e = 0; e < 8; e += 2) top = max_abs3(s[e], s[e + 1], top);
+    }
+    top = meet<WARP, true>(top < INFINITY ? top : INFINITY, buf[1]);  // (infinite, too, for what is not a number)
+    const bool finite = top < INFINITY;
+    if (!finite) {  // over the finite ones
+      top = 0.0f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float s[8];
+        from_pairs(f[v], s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (fabsf(s[e]) < INFINITY) top = fmaxf(top, fabsf(s[e]));
+      }
+      top = meet<WARP, true>(top, buf[0]);
+    }
+    const float scale = __fmul_rn(top, 1.0f / 448.0f);
+    if (t == 0 && live) p.y_scale[row] = scale;
+    // codes of the IEEE quotients by one reciprocal, as quotient_codes has them (a zero's sign aside)
+    const bool quick = finite && (scale == 0.0f || scale > 0x1p-80f);
+    const float inverse = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+    const Pair r2 = pack2(inverse, inverse), s2 = pack2(-scale, -scale);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int col = v * step + t * 8;
+      if (col >= p.n || !live) break;
+      float s[8];
+      if (quick) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Pair n = mul2(f[v][i], r2);
+          unpack2(fma2(fma2(n, s2, f[v][i]), r2, n), s[2 * i], s[2 * i + 1]);
+        }
+      } else {
+        from_pairs(f[v], s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = scale > 0.0f ? __fdiv_rn(s[e], scale) : 0.0f;
+      }
+      row_store8<TY>(y, col, p.n, p.y_vec, pack8<TY>(s));
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float s[8];
+      from_pairs(f[v], s);
+      if (live) row_store8<TY>(y, v * step + t * 8, p.n, p.y_vec, pack8<TY>(s));
+    }
+  }
+}
+
+// Threads of a CTA at most and CTAs to an SM at least, for the registers: rows of F32 have two vectors a thread up to 12 288 elements (2 048 rows of
+// them to bfloat16 with residual 59 us, with four 74), of 16 bits up to 8 192 (4 096 rows of 10 240 to codes 64 us, with four 54).
+template <int TX, bool WARP, int V>
+constexpr int norm_threads() { return WARP ? NR_WARP_THREADS : V == 2 && TX == MIMIR_B200_T_F32 ? 768 : 512; }
+template <int TX, bool WARP, int V>
+constexpr int norm_ctas() { return WARP ? (V == 4 ? 4 : 8) : V == 2 ? (TX == MIMIR_B200_T_F32 ? 2 : 3) : V == 4 ? 2 : 1; }
+
+template <int TX, int TY, int V, bool WARP>
+__global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WARP, V>()) norm_rows_serve_kernel(const __grid_constant__ NormParams p) {
+  __shared__ __align__(16) float buf[2][32];
+  pdl_early_if(p.early);
+  if (!WARP && threadIdx.x < 64) buf[threadIdx.x >> 5][threadIdx.x & 31] = 0.0f;
+  pdl_wait();
+  const int row = WARP ? blockIdx.x * (NR_WARP_THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= p.rows) return;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x, step = (WARP ? 32 : blockDim.x) * 8;
+  const char* const x = p.x + row * p.x_row;
+  Pair f[V][4];
+  Raw8<TX> raw[V], res[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    raw[v] = row_load8<TX>(x, v * step + t * 8, p.n, p.x_vec);
+    if (p.residual) res[v] = row_load8<TX>(p.residual + row * p.residual_row, v * step + t * 8, p.n, p.residual_vec);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int col = v * step + t * 8;
-    if (col >= p.n) break;
-    if constexpr (TY == MIMIR_B200_T_E4M3) {
+    to_pairs<TX>(raw[v], f[v]);
+    if (p.residual) {
+      Pair g[4];
+      to_pairs<TX>(res[v], g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[v][e] = scale > 0.0f ? __fdiv_rn(f[v][e], scale) : 0.0f;
+      for (int i = 0; i < 4; ++i) f[v][i] = add2(f[v][i], g[i]);
     }
-    row_store8<TY>(p.y + row * p.y_row, col, p.n, p.y_vec, pack8<TY>(f[v]));
+  }
+  if (!WARP) __syncthreads();  // (the words of no warp)
+  finish_row<TX, TY, V, WARP>(p, row, true, t, step, f, buf);
+}
+
+// The same for many long rows of 16 bits without a residual: few CTAs fit into the registers, so the rows come through a ring in shared memory by
+// bulk copies asked for several rows ahead, and what is on its way does not stand still while a row's threads meet.  5 003 rows of 12 288 halves
+// to codes 38 us, without it 46 (with a residual 65 against 54, and for rows that more CTAs hold 63 against 40: not there).
+template <int TX, int TY>
+__global__ void __launch_bounds__(512, 2) norm_rows_ring_kernel(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t bars[NR_MAX_STAGES];
+  __shared__ __align__(16) float buf[2][32];
+  __shared__ volatile int abort_word;
+  const int t = threadIdx.x, step = blockDim.x * 8, apart = gridDim.x;
+  const uint32_t bytes = static_cast<uint32_t>(p.n) * type_bytes(TX);
+  if (t < 64) buf[t >> 5][t & 31] = 0.0f;
+  if (t == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&bars[s], 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  pdl_wait();
+  auto ask = [&](int row, int s) {
+    mbar_expect_tx(&bars[s], bytes);
+    bulk_load_1d(ring + s * bytes, p.x + row * p.x_row, bytes, &bars[s]);
+  };
+  long long next = blockIdx.x;  // the row that is asked for next
+  if (t == 0)
+    for (int s = 0; s < p.stages && next < p.rows; ++s, next += apart) ask(static_cast<int>(next), s);
+  int stage = 0;
+  uint32_t phase = 0;
+#pragma unroll 1
+  for (long long row = blockIdx.x; row < p.rows; row += apart) {
+    // (a thread whose wait gives up stays for the others' meetings, leaves nothing and asks for nothing more)
+    const bool ok = mbar_wait(&bars[stage], phase, &abort_word, p.err_word, 121);
+    const char* x = reinterpret_cast<const char*>(ring + stage * bytes);
+    Pair f[4][4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) to_pairs<TX>(row_load8<TX>(x, v * step + t * 8, p.n, true), f[v]);
+    __syncthreads();
+    if (t == 0 && ok && next < p.rows) {
+      ask(static_cast<int>(next), stage);
+      next += apart;
+    }
+    finish_row<TX, TY, 4, false>(p, static_cast<int>(row), ok, t, step, f, buf);
+    if (++stage == p.stages) { stage = 0; phase ^= 1; }
   }
 }
 
 template <int TX, int TY, int V, bool WARP>
 int launch_as(const NormParams& p, int threads, cudaStream_t st) {
-  const unsigned grid = WARP ? (static_cast<unsigned>(p.rows) + NR_WARP_THREADS / 32 - 1) / (NR_WARP_THREADS / 32) : static_cast<unsigned>(p.rows);
+  constexpr int PER = WARP ? NR_WARP_THREADS / 32 : 1;
+  const unsigned grid = (static_cast<unsigned>(p.rows) + PER - 1) / PER;
   NormParams q = p;
+  if constexpr (!WARP && V == 4 && TX != MIMIR_B200_T_F32) {
+    const size_t row_bytes = static_cast<size_t>(p.n) * type_bytes(TX);
+    const unsigned at_once = static_cast<unsigned>(ctx().sm_count * 2);
+    if (p.x_vec && !p.residual && row_bytes % 16 == 0 && grid > 2 * at_once) {
+      auto kern = norm_rows_ring_kernel<TX, TY>;
+      static PerDeviceOnce once;
+      MB_TRY(once.run([&]() -> int {
+        MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NR_RING));
+        return MIMIR_B200_OK;
+      }));
+      q.stages = static_cast<int>(std::min<size_t>(NR_RING / row_bytes, NR_MAX_STAGES));  // (rows of up to 32 KB: three at least)
+      MB_TRY(launch_pdl(kern, dim3(at_once), dim3(static_cast<unsigned>(threads)), q.stages * row_bytes, st, 1, q));
+      count_launch();
+      return MIMIR_B200_OK;
+    }
+  }
   q.early = pdl_small_grid(grid);
   MB_TRY(launch_pdl(norm_rows_serve_kernel<TX, TY, V, WARP>, dim3(grid), dim3(static_cast<unsigned>(threads)), 0, st, 1, q));
   count_launch();
@@ -199,12 +366,13 @@ int launch_as(const NormParams& p, int threads, cudaStream_t st) {
 template <int TX, int TY>
 int launch_rows(const NormParams& p, cudaStream_t st) {
   const int vectors = (p.n + 7) / 8;
+  auto threads = [&](int v) { return round_up((vectors + v - 1) / v, 32); };
   if (vectors <= 32) return launch_as<TX, TY, 1, true>(p, NR_WARP_THREADS, st);
   if (vectors <= 64) return launch_as<TX, TY, 2, true>(p, NR_WARP_THREADS, st);
   if (vectors <= 128) return launch_as<TX, TY, 4, true>(p, NR_WARP_THREADS, st);
-  const int v = vectors <= 1024 ? 2 : 4;
-  const int threads = round_up((vectors + v - 1) / v, 32);
-  return v == 2 ? launch_as<TX, TY, 2, false>(p, threads, st) : launch_as<TX, TY, 4, false>(p, threads, st);
+  if (vectors <= norm_threads<TX, false, 2>() * 2) return launch_as<TX, TY, 2, false>(p, threads(2), st);
+  if (vectors <= 2048) return launch_as<TX, TY, 4, false>(p, threads(4), st);
+  return launch_as<TX, TY, 8, false>(p, threads(8), st);
 }
 template <int TX>
 int launch_to(const NormParams& p, int y_type, cudaStream_t st) {
@@ -228,7 +396,7 @@ int launch_norm_rows(const MimirNormRows& a, cudaStream_t st) {
   p.x = static_cast<const char*>(a.x), p.residual = static_cast<const char*>(a.residual), p.sum = static_cast<char*>(a.sum);
   p.gamma = a.gamma, p.y = static_cast<char*>(a.y), p.y_scale = a.y_scale;
   p.x_row = a.x_stride * xs, p.residual_row = a.residual_stride * xs, p.sum_row = a.sum_stride * xs, p.y_row = a.y_stride * ys;
-  p.rows = a.rows, p.n = a.n, p.norm = a.norm, p.eps = a.eps;
+  p.rows = a.rows, p.n = a.n, p.norm = a.norm, p.eps = a.eps, p.inv_n = 1.0f / static_cast<float>(a.n), p.err_word = ctx().dev_error_word;
   p.x_vec = vectors_at(p.x, p.x_row, 16), p.residual_vec = vectors_at(p.residual, p.residual_row, 16), p.sum_vec = vectors_at(p.sum, p.sum_row, 16);
   p.gamma_vec = vectors_at(p.gamma, 0, 16), p.y_vec = vectors_at(p.y, p.y_row, ys == 1 ? 8 : 16);
   switch (a.type) {

@@ -45,9 +45,9 @@ def e4m3_half_step(q):
     return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(q), 2.0**-6))) - 4)
 
 
-# A sum of squares is fma chains of 4, joined in at most 4 + 1 + 10 additions of positive numbers; with the squares' own relative error (twice s's
-# 2^-24) and the mean's division and eps 24 units of 2^-24, halved by the root; the root, s and two products: 16 units.
-NORM_UNITS = 16 * 2.0**-24
+# A sum of squares is a product and three fmas, joined in at most 8 + 1 + 5 + 4 additions of positive numbers; with the squares' own relative error (twice
+# s's 2^-24), 1 / n's and the fma with eps 26 units of 2^-24, halved by the root; the root (1.5), s (1) and two products (2): 17.5 units.
+NORM_UNITS = 17.5 * 2.0**-24
 
 
 # ---- products -------------------------------------------------------------------------------------------------------------------------

@@ -63,6 +63,31 @@ def test_norm_rows(backend, rows, n, y_type, type_):
             assert scale is None or scale[rows] == -7
 
 
+@pytest.mark.parametrize("type_", [F16, BF16])
+@pytest.mark.parametrize("y_type", [F32, BF16, E4M3])
+@pytest.mark.parametrize("rows,n", [(593, 8200), (2000, 12288), (1200, 16384)])
+def test_norm_of_many_long_rows(backend, rows, n, y_type, type_):
+    """More rows than the device holds at once: every CTA has several, the last of them fewer."""
+    x = normal(rows, n, seed=rows, scale=2.0, dtype=TORCH[type_])
+    x[rows // 2, 5] = float("nan")
+    for norm in (True, False):
+        y, scale = torch.full((rows + 1, n + 16), -7.0, device="cuda").to(TORCH[y_type]), torch.full((rows + 1,), -7.0, device="cuda")
+        call_norm(backend, x, y[:, :n], y_type, type_, scale=scale if y_type == E4M3 else None, norm=norm, rows=rows)
+        backend.check_device()
+        fine = [0, 1, rows // 2 - 1, rows // 2 + 1, rows - 2, rows - 1] + list(range(3, rows, 97))
+        part = y[:, :n].view(torch.uint8 if y_type == E4M3 else y.dtype)[fine].view(TORCH[y_type])
+        check_norm(x[fine], None, None, norm, 1e-5, type_, y_type, part, None, scale[fine])
+        rest = y.float()
+        assert rest[rows // 2, 5].isnan() and rest[rows // 2, :n].isnan().all() == norm
+        assert (rest[:, n:] == rest[rows, 0]).all() and (rest[rows] == rest[rows, 0]).all() and scale[rows] == -7
+        same = torch.empty_like(x)
+        if y_type == type_:
+            call_norm(backend, x.clone(), same, type_, type_, norm=norm)
+            z = x.clone()
+            call_norm(backend, z, z, type_, type_, norm=norm)
+            assert torch.equal(z.nan_to_num(3.0), same.nan_to_num(3.0))
+
+
 @pytest.mark.parametrize("type_", [F32, BF16])
 def test_norm_rows_in_place(backend, type_):
     x, r = normal(7, 768, seed=1, dtype=TORCH[type_]), normal(7, 768, seed=2, dtype=TORCH[type_])
