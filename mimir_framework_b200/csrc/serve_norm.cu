@@ -238,7 +238,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
       } else {
         from_pairs(f[v], s);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = scale > 0.0f ? __fdiv_rn(s[e], scale) : 0.0f;
+        for (int e = 0; e < 8; ++e) s[e] = scale > 0.0f ? __fdiv_rn(s[e], scale) : fabsf(s[e]) < INFINITY ? 0.0f : s[e];  // (no scale: a row with none finite but zeros)
       }
       row_store8<TY>(y, col, p.n, p.y_vec, pack8<TY>(s));
     }
