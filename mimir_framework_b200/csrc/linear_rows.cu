@@ -19,7 +19,7 @@ namespace mb {
 namespace {
 
 constexpr int RM = 128;  // rows of an instruction: features of a CTA at most
-constexpr int MAX_STAGES = 24;
+constexpr int MAX_STAGES = 24, EARLY = 4, AHEAD = 4;
 constexpr int MAX_CLUSTER = 8, UNIT = 16, TURN = 2 * UNIT * RM * 4;  // (two turns of a unit for four warps)
 constexpr int STATIC = 3072, DYNAMIC = 232448 - STATIC, DYNAMIC_TWO = (228 * 1024) / 2 - 1024 - STATIC;  // shared memory of a CTA, one or two to an SM
 // A CTA of a cluster waits for others that may still be asking for tensor memory.  So that none of them can be kept from it by a CTA that waits
@@ -103,10 +103,11 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
   const int feature0 = ft * rp.features, x_row0 = rt * n;
   const int b0 = share_begin(p.kblocks, rank, rp.cluster), b1 = share_begin(p.kblocks, rank + 1, rp.cluster);
 
-  // The producer starts on its own: barriers, and what the ring holds at once, before the others are through with their set-up.
+  // The producer starts on its own: barriers and the first few blocks, before the others are through with their set-up.  (Not all that the ring
+  // holds: asking for it takes as long as its bytes need, and the first instruction would wait for that.)
   constexpr int per_block = F8 ? LIN_BLOCK : LIN_BLOCK / 2;
   const int w_bytes = rp.features * LIN_BLOCK;
-  const int at_once = min(rp.stages, b1 - b0);
+  const int at_once = min(min(rp.stages, b1 - b0), EARLY);
   auto load_block = [&](int stage, int b) {
     uint8_t* base = smem + stage * rp.stage_bytes;
     uint64_t* bar = &full_bar[stage];
@@ -127,8 +128,16 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
     __syncwarp();
-    pdl_wait();
     const bool one = elect_one();
+    // the first weights into L2 while the kernel before this one finishes (what it may still write there is not lost: L2 is where both meet)
+    for (int i = 0; i < min(AHEAD, b1 - b0); ++i) {
+      if (one) {
+        tma_prefetch_2d(&map_w, (b0 + i) * per_block, feature0);
+        if constexpr (GATED) tma_prefetch_2d(&map_up, (b0 + i) * per_block, feature0);
+      }
+      __syncwarp();
+    }
+    pdl_wait();
     for (int i = 0; i < at_once; ++i) {
       if (one) load_block(i, b0 + i);
       __syncwarp();

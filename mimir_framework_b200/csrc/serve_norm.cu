@@ -136,6 +136,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
       row_store8<TX>(sum, v * step + t * 8, p.n, p.sum_vec, pack8<TX>(s));
     }
   }
+  float root = 1.0f;  // that the elements still lack
   if (p.norm) {
     Pair q2 = pack2(0.0f, 0.0f);
 #pragma unroll
@@ -179,18 +180,23 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
         r = root_reciprocal(fmaf(meet<WARP, false>(rest, buf[0]), p.inv_n, p.eps * down * down));
       }
     }
+    // For codes the root stays out of the elements, as it cancels in their quotients by the largest: a rounding less.  (Rows so large that s gamma
+    // might leave fp32's range take it in.)
+    const bool later = TY == MIMIR_B200_T_E4M3 && r > 0x1p-20f;
+    if (later) root = r;
     const Pair r2 = pack2(r, r);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int col = v * step + t * 8;
+      if (!later) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], r2);
+      }
       if (p.gamma) {
         Pair g[4];
         to_pairs<MIMIR_B200_T_F32>(row_load8<MIMIR_B200_T_F32>(reinterpret_cast<const char*>(p.gamma), col, p.n, p.gamma_vec), g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[v][i] = mul2(mul2(f[v][i], r2), g[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], r2);
+        for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], g[i]);
       }
     }
   }
@@ -218,12 +224,14 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
       }
       top = meet<WARP, true>(top, buf[0]);
     }
-    const float scale = __fmul_rn(top, 1.0f / 448.0f);
-    if (t == 0 && live) p.y_scale[row] = scale;
-    // codes of the IEEE quotients by one reciprocal, as quotient_codes has them (a zero's sign aside)
-    const bool quick = finite && (scale == 0.0f || scale > 0x1p-80f);
-    const float inverse = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
-    const Pair r2 = pack2(inverse, inverse), s2 = pack2(-scale, -scale);
+    const float part = __fmul_rn(top, 1.0f / 448.0f);
+    if (t == 0 && live) p.y_scale[row] = __fmul_rn(part, root);
+    // Without the norm codes of the IEEE quotients by one reciprocal, as quotient_codes has them (a zero's sign aside): those of 16-bit values are often
+    // just between two codes.  Of a norm's values products with 448 / largest (`again` is zero), which is nearer to the quotients by the
+    // largest itself: of 33 M codes 20 % fewer fall on the other side of a border than by the rounded scale.
+    const bool quick = finite && (part == 0.0f || part > 0x1p-80f);
+    const float inverse = part > 0.0f ? (p.norm ? __fdiv_rn(448.0f, top) : __frcp_rn(part)) : 0.0f, again = p.norm ? 0.0f : inverse;
+    const Pair r2 = pack2(inverse, inverse), s2 = pack2(-part, -part), again2 = pack2(again, again);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int col = v * step + t * 8;
@@ -233,12 +241,12 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const Pair n = mul2(f[v][i], r2);
-          unpack2(fma2(fma2(n, s2, f[v][i]), r2, n), s[2 * i], s[2 * i + 1]);
+          unpack2(fma2(fma2(n, s2, f[v][i]), again2, n), s[2 * i], s[2 * i + 1]);
         }
       } else {
         from_pairs(f[v], s);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = scale > 0.0f ? __fdiv_rn(s[e], scale) : fabsf(s[e]) < INFINITY ? 0.0f : s[e];  // (no scale: a row with none finite but zeros)
+        for (int e = 0; e < 8; ++e) s[e] = part > 0.0f ? __fdiv_rn(s[e], part) : fabsf(s[e]) < INFINITY ? 0.0f : s[e];  // (none: a row with none finite but zeros)
       }
       row_store8<TY>(y, col, p.n, p.y_vec, pack8<TY>(s));
     }
