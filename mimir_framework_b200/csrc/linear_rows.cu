@@ -6,7 +6,8 @@
 // A CTA has as many features as make one CTA for each SM, a multiple of eight up to 128: the instructions always work on 128 rows of shared
 // memory, of which those behind the CTA's own are whatever comes next there and end in lanes that nobody reads.  Where few features would have
 // every CTA read all of x, the CTAs of a cluster (up to eight) share n_in instead; their sums meet in shared memory: each CTA
-// finishes some of the rows and gets what the others have of them, added up in a fixed order, so that a result has the same bits every time.
+// finishes some of the rows and gets what all have of them, added up in the order of the shares, so that a result has the same bits every time and
+// wherever its row is in the call.
 //   warp 0 TMA, warp 1 instructions, the other eight or sixteen results: 32 features and sixteen rows of x at a time.
 #include <algorithm>
 #include <cmath>
@@ -33,7 +34,7 @@ struct RowParams {
   int features;                     // of a CTA (a multiple of 8)
   int cluster;                      // CTAs that share n_in
   int stages, stage_bytes;
-  int parts_at;                     // other CTAs' sums: where in shared memory (0: the ring, when it is done with)
+  int parts_at;                     // the cluster's sums: where in shared memory (0: the ring, when it is done with)
   int turn_at;                      // where results are turned around, TURN bytes for four warps: the ring or behind the sums in it
   int tmem_cols, early;
 };
@@ -312,9 +313,8 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
       int who = 0, r0 = 0, r1 = share_begin(units, 1, rp.cluster);  // who finishes a unit, and that one's units
       for (int u = four; u < units; u += FOURS) {
         while (u >= r1) r0 = r1, r1 = share_begin(units, ++who + 1, rp.cluster);
-        if (who == rank) continue;
         // [sender][gate, up][unit][four rows][feature][row]
-        const int wide = r1 - r0, at = rp.parts_at + ((rank < who ? rank : rank - 1) * G * wide + u - r0) * UNIT * RM * 4 + (quad * 32 + lane) * 16;
+        const int wide = r1 - r0, at = rp.parts_at + (rank * G * wide + u - r0) * UNIT * RM * 4 + (quad * 32 + lane) * 16;
         const uint32_t dst = mapa_shared(smem_u32(smem + at), static_cast<uint32_t>(who));
         float z[16], y[16];
         tmem_ld_32x16(lanes + static_cast<uint32_t>(u * UNIT), z);
@@ -348,9 +348,14 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
       float* turn = turns + flip * UNIT * RM;
       if (busy) {
         float z[16], y[16];
-        tmem_ld_32x16(lanes + static_cast<uint32_t>(u * UNIT), z);
-        if constexpr (GATED) tmem_ld_32x16(lanes + static_cast<uint32_t>(n + u * UNIT), y);
-        for (int o = 0; o < rp.cluster - 1; ++o) {
+        if (rp.cluster == 1) {
+          tmem_ld_32x16(lanes + static_cast<uint32_t>(u * UNIT), z);
+          if constexpr (GATED) tmem_ld_32x16(lanes + static_cast<uint32_t>(n + u * UNIT), y);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) z[j] = y[j] = 0.0f;
+        }
+        for (int o = 0; o < rp.cluster && rp.cluster > 1; ++o) {
           const float4* from = parts + (o * G * wide + u - u0) * 4 * RM;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -422,7 +427,7 @@ bool shape_of(const MimirLinear& a, bool gated, int features, int cluster, int p
   s->tmem_cols = 32;
   while (s->tmem_cols < (f32 ? 3 : 1) * g * s->rows_tile) s->tmem_cols *= 2;
   if (s->tmem_cols > 512 / per_sm) return false;
-  const int units = s->rows_tile / UNIT, parts = (cluster - 1) * ((units + cluster - 1) / cluster) * UNIT * g * RM * 4;
+  const int units = s->rows_tile / UNIT, parts = cluster == 1 ? 0 : cluster * ((units + cluster - 1) / cluster) * UNIT * g * RM * 4;
   s->stage_bytes = (g * features + s->rows_tile) * LIN_BLOCK;
   // (an instruction reads 128 rows from the start of the features' that it is given)
   const int pad = std::max(0, RM - features - s->rows_tile) * LIN_BLOCK;
@@ -474,7 +479,7 @@ const ClusterTable* active_clusters() {
 
 // The quickest shape by an estimate in us.  A round of CTAs loads (at most 120 KB an us each, 18.4 MB in all; a ring that does not hold all of a
 // CTA's blocks is waited for 0.34 us at a time) and multiplies (an instruction of 128 x N takes 46 cycles, from N = 61 on 0.75 N, a block 70 more),
-// or waits for the weights from memory; then come 0.42 us for each unit of 16 rows that a warp finishes, and 1.85 and more for the meeting of a
+// or waits for the weights from memory, up to a tenth longer where SMs idle; then come 0.42 us for each unit of 16 rows that a warp finishes, and 1.85 and more for the meeting of a
 // cluster; of equals, CTAs of middling size.  The numbers are a fit to 228 products (1 to 2 048 rows, n_in 512 to 16 384, n_out 640 to 32 000, 16 and 8 bits, gated or not, up to 40
 // shapes each): the shape taken, or the kernel of tiles instead, is on average 2 % slower than the quickest, at worst 25 % (39 us against 49).
 RowShape row_shape(const MimirLinear& a, bool gated) {
@@ -482,7 +487,7 @@ RowShape row_shape(const MimirLinear& a, bool gated) {
   best.us = 1e30;
   const ClusterTable* active = active_clusters();
   if (!active) return best;
-  const int g = gated ? 2 : 1;
+  const int g = gated ? 2 : 1, sms = ctx().sm_count;
   const double blocks = std::ceil(static_cast<double>(a.n_in) * type_bytes(a.type) / LIN_BLOCK), hbm = blocks * LIN_BLOCK * g * a.n_out / 6.55e6;
   for (int cluster = 1; cluster <= MAX_CLUSTER; ++cluster)
     for (int features = RM; features >= 16; features -= 8)
@@ -493,7 +498,8 @@ RowShape row_shape(const MimirLinear& a, bool gated) {
         if (at_once <= 0) continue;
         const double load = std::max(s.stage_bytes / 120e3, s.stages < mine ? 0.34 / s.stages : 0.0);
         const double mma = (70.0 + g * 4 * std::max(46.0, 0.75 * s.rows_tile)) / 1850.0;
-        const double loop = std::max({rounds * mine * std::max(load, mma) * per_sm, hbm, s.ctas * mine * s.stage_bytes / 18.4e6});
+        const double busy = s.ctas / (std::ceil(static_cast<double>(s.ctas) / sms) * sms);  // share of the SMs, over the time
+        const double loop = std::max({rounds * mine * std::max(load, mma) * per_sm, hbm * (1.1 - 0.1 * busy), s.ctas * mine * s.stage_bytes / 18.4e6});
         const int turns = per_sm == 2 ? 2 : 4, units = ((s.rows_tile / UNIT + cluster - 1) / cluster + turns - 1) / turns;
         const double meet = cluster == 1 ? 0.0 : 1.85 + 0.019 * s.rows_tile * g * (cluster - 1) / cluster + (s.parts_at ? 0.0 : 2.0);
         s.us = 1.9 + loop + (0.23 + 0.42 * g * units + meet) * (per_sm == 1 ? rounds : (rounds + 1) / 2) + 0.003 * std::abs(features - 64);

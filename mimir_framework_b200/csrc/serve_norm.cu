@@ -125,7 +125,8 @@ __device__ __forceinline__ float root_reciprocal(float x) {
 // A row from the sums s that its threads hold on: V vectors of eight elements each; WARP: a row to a warp, else to the CTA.  Instructions bound it
 // where memory does not, so two elements go through one wherever there is such a one (8 192 rows of 4 096 with residual to codes took 37 M
 // instructions and 47 us element by element, 42 so).  A row that is not `live` takes part in the meetings and leaves nothing.
-template <int TX, int TY, int V, bool WARP>
+// NORM: 0, 1, or -1, which is what the call says (the ring's registers do not hold both kinds of codes).
+template <int TX, int TY, int V, bool WARP, int NORM = -1>
 __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, Pair (&f)[V][4], float (&buf)[2][32]) {
   if (p.sum && live) {
     char* const sum = p.sum + row * p.sum_row;
@@ -136,8 +137,9 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
       row_store8<TX>(sum, v * step + t * 8, p.n, p.sum_vec, pack8<TX>(s));
     }
   }
+  const bool norm = NORM < 0 ? p.norm != 0 : NORM == 1;
   float root = 1.0f;  // that the elements still lack
-  if (p.norm) {
+  if (norm) {
     Pair q2 = pack2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -230,7 +232,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
     // just between two codes.  Of a norm's values products with 448 / largest (`again` is zero), which is nearer to the quotients by the
     // largest itself: of 33 M codes 20 % fewer fall on the other side of a border than by the rounded scale.
     const bool quick = finite && (part == 0.0f || part > 0x1p-80f);
-    const float inverse = part > 0.0f ? (p.norm ? __fdiv_rn(448.0f, top) : __frcp_rn(part)) : 0.0f, again = p.norm ? 0.0f : inverse;
+    const float inverse = part > 0.0f ? (norm ? __fdiv_rn(448.0f, top) : __frcp_rn(part)) : 0.0f, again = norm ? 0.0f : inverse;
     const Pair r2 = pack2(inverse, inverse), s2 = pack2(-part, -part), again2 = pack2(again, again);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -241,7 +243,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const Pair n = mul2(f[v][i], r2);
-          unpack2(fma2(fma2(n, s2, f[v][i]), again2, n), s[2 * i], s[2 * i + 1]);
+          unpack2(NORM == 1 ? n : fma2(fma2(n, s2, f[v][i]), again2, n), s[2 * i], s[2 * i + 1]);
         }
       } else {
         from_pairs(f[v], s);
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WAR
 // The same for many long rows of 16 bits without a residual: few CTAs fit into the registers, so the rows come through a ring in shared memory by
 // bulk copies asked for several rows ahead, and what is on its way does not stand still while a row's threads meet.  5 003 rows of 12 288 halves
 // to codes 38 us, without it 46 (with a residual 65 against 54, and for rows that more CTAs hold 63 against 40: not there).
-template <int TX, int TY>
+template <int TX, int TY, int NORM>
 __global__ void __launch_bounds__(512, 2) norm_rows_ring_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t bars[NR_MAX_STAGES];
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(512, 2) norm_rows_ring_kernel(const __grid_con
       ask(static_cast<int>(next), stage);
       next += apart;
     }
-    finish_row<TX, TY, 4, false>(p, static_cast<int>(row), ok, t, step, f, buf);
+    finish_row<TX, TY, 4, false, NORM>(p, static_cast<int>(row), ok, t, step, f, buf);
     if (++stage == p.stages) { stage = 0; phase ^= 1; }
   }
 }
@@ -354,14 +356,17 @@ int launch_as(const NormParams& p, int threads, cudaStream_t st) {
     const size_t row_bytes = static_cast<size_t>(p.n) * type_bytes(TX);
     const unsigned at_once = static_cast<unsigned>(ctx().sm_count * 2);
     if (p.x_vec && !p.residual && row_bytes % 16 == 0 && grid > 2 * at_once) {
-      auto kern = norm_rows_ring_kernel<TX, TY>;
-      static PerDeviceOnce once;
-      MB_TRY(once.run([&]() -> int {
-        MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NR_RING));
-        return MIMIR_B200_OK;
-      }));
       q.stages = static_cast<int>(std::min<size_t>(NR_RING / row_bytes, NR_MAX_STAGES));  // (rows of up to 32 KB: three at least)
-      MB_TRY(launch_pdl(kern, dim3(at_once), dim3(static_cast<unsigned>(threads)), q.stages * row_bytes, st, 1, q));
+      auto run = [&](auto kern, PerDeviceOnce& once) -> int {
+        MB_TRY(once.run([&]() -> int {
+          MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NR_RING));
+          return MIMIR_B200_OK;
+        }));
+        return launch_pdl(kern, dim3(at_once), dim3(static_cast<unsigned>(threads)), q.stages * row_bytes, st, 1, q);
+      };
+      static PerDeviceOnce plain, normed;
+      if (p.norm) MB_TRY((run(norm_rows_ring_kernel<TX, TY, 1>, normed)));
+      else MB_TRY((run(norm_rows_ring_kernel<TX, TY, 0>, plain)));
       count_launch();
       return MIMIR_B200_OK;
     }

@@ -7,7 +7,7 @@ import torch
 
 from mimir_framework_b200 import abi
 from layer_ref import ACTS, NORM_UNITS, Operand, act, act_off, check_product, d, e4m3_half_step, linear_args, norm_rows, normal, padded, product, rounded
-from serving_ref import TORCH, Pages, attention, half_step, sample
+from serving_ref import TORCH, Pages, half_step, sample
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16, I8, E4M3 = abi.T_F32, abi.T_F16, abi.T_BF16, abi.T_I8, abi.T_E4M3
@@ -257,3 +257,235 @@ def test_pointers_are_looked_at(backend):
     # no rows: nothing is looked at
     backend.dev_linear(backend.linear(**(good | dict(rows=0, x=None, out=None))))
     backend.dev_norm_rows(backend.norm_rows(**(norm | dict(rows=0, x=None))))
+
+
+# ---- sizes between the two kernels, and every division of the inputs -----------------------------------------------------------------------
+@pytest.mark.parametrize("type_,out_type", [(BF16, F32), (E4M3, F32), (F16, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("rows,n_in,n_out", [(700, 8, 3000), (1111, 129, 1500), (2049, 257, 513), (900, 5000, 1300), (5000, 64, 40), (770, 1024, 4096), (258, 3000, 4096), (130, 8192, 130)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_products_of_many_shapes(backend, rows, n_in, n_out, type_, out_type, gated):
+    check_product(backend, rows, n_in, n_out, type_, out_type, name="gelu" if gated else "none", residual=not gated, gated=gated, seed=rows)
+
+
+@pytest.mark.parametrize("type_", [BF16, E4M3])
+@pytest.mark.parametrize("n_in", [512, 1000, 2048, 4096, 8000, 20000])
+@pytest.mark.parametrize("n_out", [8, 100, 520, 4096])
+def test_products_of_few_rows_whose_inputs_are_shared_out(backend, n_in, n_out, type_):
+    """From one CTA for all of n_in to eight of them, with as many rows as make one unit or several."""
+    for rows in (1, 16, 48, 100, 160):
+        check_product(backend, rows, n_in, n_out, type_, F32 if rows % 3 else BF16, residual=rows > 16, seed=rows + n_in)
+        if n_out < 4096:
+            check_product(backend, rows, n_in, n_out, type_, BF16, name="silu", gated=True, seed=rows + n_in)
+
+
+def test_weights_beyond_32_bits_of_offset(backend):
+    stride, n_out, n_in = 1 << 27, 18, 200
+    big = torch.empty(n_out, stride, dtype=torch.bfloat16, device="cuda")
+    w = normal(n_out, n_in, seed=1, dtype=torch.bfloat16)
+    big[:, :n_in] = w
+    for rows in (3, 1500):
+        x = normal(rows, n_in, seed=2, dtype=torch.bfloat16)
+        got, want = torch.empty(rows, n_out, device="cuda"), torch.empty(rows, n_out, device="cuda")
+        backend.dev_linear(backend.linear(x.data_ptr(), big.data_ptr(), got.data_ptr(), rows, n_in, n_out, BF16, F32, n_in, stride, n_out))
+        backend.dev_linear(backend.linear(x.data_ptr(), w.data_ptr(), want.data_ptr(), rows, n_in, n_out, BF16, F32, n_in, n_in, n_out))
+        torch.cuda.synchronize()
+        backend.check_device()
+        assert torch.equal(got, want)
+
+
+# ---- streams and graphs ----------------------------------------------------------------------------------------------------------------------
+def test_calls_of_several_streams_at_once(backend):
+    """Clusters that share inputs, single CTAs, pairs and norms beside one another: the results are those of one call after the other."""
+    sizes = [(40, 4096, 1024, BF16), (1500, 1024, 1536, F16), (3, 2048, 20000, E4M3), (300, 4096, 2048, E4M3)]
+    jobs = []
+    for i, (rows, n_in, n_out, type_) in enumerate(sizes):
+        x, w, u = Operand(rows, n_in, type_, i), Operand(n_out, n_in, type_, i + 10, 0.02), Operand(n_out, n_in, type_, i + 20, 0.02)
+        out = torch.empty(2, rows, n_out, device="cuda", dtype=torch.bfloat16)
+        a = linear_args(x, w, out[0], type_, BF16, rows, n_in, n_out)
+        g = linear_args(x, w, out[1], type_, BF16, rows, n_in, n_out, up=u.at(), up_stride=u.stride, up_scale=u.scale_at(), activation=abi.ELT_SILU)
+        y, scale = torch.empty(rows, n_out, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(rows, device="cuda")
+        norm = backend.norm_rows(out[0].data_ptr(), y.data_ptr(), rows, n_out, BF16, E4M3, n_out, n_out, y_scale=scale.data_ptr())
+        jobs.append((a, g, norm, out, y, scale, (x, w, u)))
+
+    def run(job, stream):
+        backend.dev_linear(job[0], stream)
+        backend.dev_norm_rows(job[2], stream)
+        backend.dev_gated_linear(job[1], stream)
+
+    for job in jobs:
+        run(job, 0)
+    torch.cuda.synchronize()
+    want = [(job[3].clone(), job[4].view(torch.uint8).clone(), job[5].clone()) for job in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(20):
+        for job, s in zip(jobs, streams):
+            run(job, s.cuda_stream)
+    torch.cuda.synchronize()
+    backend.check_device()
+    for job, (o, y, s) in zip(jobs, want):
+        assert torch.equal(job[3], o) and torch.equal(job[4].view(torch.uint8), y) and torch.equal(job[5], s)
+    # two graphs at once, on new inputs in the old buffers
+    graphs = []
+    for job, s in zip(jobs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            run(job, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for job in jobs:
+        job[3].zero_(), job[5].zero_()
+        x = job[6][0].x
+        x.copy_(x.flip(0))
+    torch.cuda.synchronize()
+    for g, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            g.replay()
+            g.replay()
+    torch.cuda.synchronize()
+    backend.check_device()
+    for job, (o, y, s) in zip(jobs, want):
+        x = job[6][0]
+        if x.scale is None:  # (8-bit rows keep their scales' places)
+            assert torch.equal(job[3], o.flip(1)) and torch.equal(job[5], s.flip(0))
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("coded", [False, True])
+def test_a_layer_and_its_tokens(backend, coded):
+    """A layer of a small model as it serves: norm, projection, rotary positions, cache, attention, projection with the residual, norm with the
+    residual's sum, gated block, logits, a token; a prompt's chunk and then single tokens, the steps captured once and replayed.  Each call is held against
+    its definition over what it then read."""
+    heads, kv_heads, dim, page, vocab, width, hidden = 6, 2, 64, 16, 301, 384, 1000
+    prompt, steps, type_ = [20, 5, 33], 3, BF16
+    bf = torch.bfloat16
+    p = Pages(prompt, [n + steps for n in prompt], kv_heads, dim, page, F16 if coded else BF16, seed=3)
+    wide = (heads + 2 * kv_heads) * dim
+    embed = normal(vocab, width, seed=1, dtype=bf)
+    op = E4M3 if coded else BF16
+    weights = {name: Operand(o, i, op, 20 + k, 1 / math.sqrt(i)) for k, (name, i, o) in enumerate(
+        [("qkv", width, wide), ("out", heads * dim, width), ("gate", width, hidden), ("up", width, hidden), ("down", hidden, width), ("head", width, vocab)])}
+    gamma = [1.0 + normal(width, seed=40 + i, scale=0.1) for i in range(3)]
+    plan = backend.rope_plan(dim, base=500000.0)
+    stream = torch.cuda.Stream()
+
+    def buffers(rows):
+        n = sum(rows)
+        b = {"rows": torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32, device="cuda"), "kv": torch.zeros(3, dtype=torch.int32, device="cuda"),
+             "pos": torch.zeros(n, dtype=torch.int32, device="cuda"), "tok": torch.zeros(n, dtype=torch.int64, device="cuda"), "u": torch.zeros(3, device="cuda"),
+             "last": torch.zeros(3, dtype=torch.int64, device="cuda"), "ids": torch.zeros(3, dtype=torch.int32, device="cuda"), "logits": torch.zeros(3, vocab, device="cuda")}
+        for name, size in (("x", width), ("qkv", wide), ("turned", wide), ("att", heads * dim), ("mid", width), ("sum", width), ("h", hidden), ("end", width)):
+            b[name] = torch.zeros(n, size, dtype=bf, device="cuda")
+        b["tail"] = torch.zeros(3, width, dtype=bf, device="cuda")
+        for name, rows_of, size in (("n1", n, width), ("n2", n, width), ("n3", 3, width), ("a8", n, heads * dim), ("h8", n, hidden)):
+            # (rows of 8-bit operands start on 16 bytes)
+            b[name] = torch.zeros(rows_of, -(-size // 16) * 16, dtype=TORCH[op], device="cuda")[:, :size]
+            b[name + "s"] = torch.zeros(rows_of, device="cuda")
+        return b
+
+    def norm(b, x, y, gamma_, s, residual=None, total=None, norm=True):
+        backend.dev_norm_rows(backend.norm_rows(
+            b[x].data_ptr(), b[y].data_ptr(), b[x].shape[0], b[x].shape[1], type_, op, b[x].stride(0), b[y].stride(0), None if gamma_ is None else gamma_.data_ptr(),
+            None if residual is None else b[residual].data_ptr(), width, None if total is None else b[total].data_ptr(), width,
+            b[y + "s"].data_ptr() if coded else None, norm), s)
+
+    def operand(b, name):
+        class X:
+            x, stride, scale = b[name], b[name].stride(0), b[name + "s"] if coded else None
+            value = property(lambda self: d(self.x) if self.scale is None else d(self.x) * d(self.scale)[:, None])
+            def at(self): return self.x.data_ptr()
+            def scale_at(self): return None if self.scale is None else self.scale.data_ptr()
+        return X()
+
+    def linear(b, x, w, y, s, residual=None, gated=False, out_type=BF16):
+        o, i, ww = b[y].shape[1], weights[w].x.shape[1], weights[w]
+        more = {}
+        if residual:
+            more = dict(residual=b[residual].data_ptr(), residual_stride=b[residual].stride(0))
+        if gated:
+            up = weights["up"]
+            more = dict(up=up.at(), up_stride=up.stride, up_scale=up.scale_at(), activation=abi.ELT_SILU)
+        a = linear_args(operand(b, x), ww, b[y], op, out_type, b[x].shape[0], i, o, **more)
+        (backend.dev_gated_linear if gated else backend.dev_linear)(a, s)
+
+    def step(b, rows):
+        s = torch.cuda.current_stream().cuda_stream
+        batch = backend.paged_batch(b["rows"].data_ptr(), b["kv"].data_ptr(), p.dev[2].data_ptr(), p.width, 3, sum(rows), max(rows), 64)
+        torch.index_select(embed, 0, b["tok"], out=b["x"])
+        norm(b, "x", "n1", gamma[0], s)
+        linear(b, "n1", "qkv", "qkv", s)
+        b["turned"].copy_(b["qkv"])
+        q = b["turned"]
+        backend.dev_rope(plan, b["pos"].data_ptr(), q.data_ptr(), q.data_ptr(), sum(rows), heads + kv_heads, dim, (wide, dim), (wide, dim), type_, s)
+        backend.dev_cache_write(p.cache(), batch, q[:, heads * dim :].data_ptr(), q[:, (heads + kv_heads) * dim :].data_ptr(), type_, wide, dim, s)
+        a = backend.paged_attention(q.data_ptr(), b["att"].data_ptr(), type_, heads, wide, dim, heads * dim, dim, dim**-0.5)
+        assert backend.paged_attention_workspace(p.cache(), batch, a) == 0
+        backend.dev_paged_attention(p.cache(), batch, a, s)
+        norm(b, "att", "a8", None, s, norm=False)
+        linear(b, "a8", "out", "mid", s, residual="x")
+        norm(b, "mid", "n2", gamma[1], s, residual="x", total="sum")
+        linear(b, "n2", "gate", "h", s, gated=True)
+        norm(b, "h", "h8", None, s, norm=False)
+        linear(b, "h8", "down", "end", s, residual="sum")
+        torch.index_select(b["end"], 0, b["last"], out=b["tail"])
+        norm(b, "tail", "n3", gamma[2], s)
+        linear(b, "n3", "head", "logits", s, out_type=F32)
+        backend.dev_sample_rows(b["logits"].data_ptr(), F32, 3, vocab, vocab, None, None, None, None, b["u"].data_ptr(), b["ids"].data_ptr(), None, s)
+
+    def check_linear(b, x, w, y, residual=None, gated=False, out_type=BF16):
+        xo = operand(b, x)
+        z, off = product(xo, weights[w], None, op, out_type)
+        if gated:
+            z2, off2 = product(xo, weights["up"], None, op, out_type)
+            v, off = act(z, "silu"), act_off(z, off, "silu")
+            off, z = off * (np.abs(z2) + off2) + np.abs(v) * off2 + np.abs(v * z2) * 2.0**-24, v * z2
+        if residual:
+            z = z + d(b[residual])
+            off = off + np.abs(z) * 2.0**-24
+        assert np.all(np.abs(d(b[y]) - z) <= rounded(z, off, out_type)), (x, w, y)
+
+    def check(b):
+        scale = lambda n: b[n + "s"] if coded else None  # noqa: E731
+        check_norm(b["x"], None, gamma[0], True, 1e-5, type_, op, b["n1"], None, scale("n1"))
+        check_linear(b, "n1", "qkv", "qkv")
+        check_norm(b["att"], None, None, False, 0, type_, op, b["a8"], None, scale("a8"))
+        check_linear(b, "a8", "out", "mid", residual="x")
+        check_norm(b["mid"], b["x"], gamma[1], True, 1e-5, type_, op, b["n2"], b["sum"], scale("n2"))
+        check_linear(b, "n2", "gate", "h", gated=True)
+        check_norm(b["h"], None, None, False, 0, type_, op, b["h8"], None, scale("h8"))
+        check_linear(b, "h8", "down", "end", residual="sum")
+        check_norm(b["tail"], None, gamma[2], True, 1e-5, type_, op, b["n3"], None, scale("n3"))
+        check_linear(b, "n3", "head", "logits", out_type=F32)
+
+    rng = np.random.default_rng(0)
+    tokens = [list(rng.integers(0, vocab, n)) for n in prompt]
+    one, graph = buffers([1, 1, 1]), None
+    for i in range(steps + 1):
+        rows = prompt if i == 0 else [1, 1, 1]
+        b = buffers(rows) if i == 0 else one
+        lens = [n + i for n in prompt]
+        b["tok"].copy_(torch.tensor(sum(([*t[-r:]] for t, r in zip(tokens, rows)), [])))
+        b["pos"].copy_(torch.tensor(np.concatenate([np.arange(n - r, n) for n, r in zip(lens, rows)]), dtype=torch.int32))
+        b["kv"].copy_(torch.tensor(lens, dtype=torch.int32))
+        b["last"].copy_(torch.tensor(np.cumsum(rows) - 1))
+        u = rng.random(3).astype(np.float32)
+        b["u"].copy_(torch.from_numpy(u))
+        torch.cuda.synchronize()
+        if i == 0:
+            step(b, rows)
+        elif graph is None:
+            with torch.cuda.stream(stream):
+                step(b, rows)  # (what torch sets up at first use)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step(b, rows)
+            graph.replay()
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        backend.check_device()
+        check(b)
+        logits = d(b["logits"])
+        for s in range(3):
+            want_id, _, gap = sample(logits[s], 1.0, 0, 1.0, 0.0, float(u[s]))
+            assert gap <= 1e-11 or int(b["ids"][s]) == want_id
+            tokens[s].append(int(b["ids"][s]))
