@@ -192,6 +192,7 @@ int check_linear(const char* what, const MimirLinear* a, bool gated) {
   MB_TRY(check_row_stride(what, "out", a->out_stride, a->rows, a->n_out));
   if (a->x_stride % unit || a->w_stride % unit || (gated && a->up_stride % unit))
     return fail(MIMIR_B200_E_UNSUPPORTED, "%s: strides of operands are multiples of 16 bytes", what);
+  if (a->out && (a->out == a->x || a->out == a->w || a->out == a->up)) return fail(MIMIR_B200_E_INVALID, "%s: out is an operand", what);
   if (a->residual && a->residual == a->out && a->residual_stride != a->out_stride) return fail(MIMIR_B200_E_INVALID, "%s: in place with two strides", what);
   return MIMIR_B200_OK;
 }

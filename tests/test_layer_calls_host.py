@@ -56,7 +56,7 @@ def test_norm_rows_refuses(change, status):
     (dict(activation=abi.ELT_MISH), abi.E_UNSUPPORTED), (dict(activation=-2), abi.E_UNSUPPORTED), (dict(x_scale=4), abi.E_INVALID), (dict(w_scale=4), abi.E_INVALID),
     (dict(up_scale=4), abi.E_INVALID), (dict(x_stride=60), abi.E_INVALID), (dict(x_stride=68), abi.E_UNSUPPORTED), (dict(w_stride=65), abi.E_UNSUPPORTED),
     (dict(w_stride=0), abi.E_INVALID), (dict(out_stride=39), abi.E_INVALID), (dict(rows=(1 << 24) + 1), abi.E_INVALID), (dict(n_in=1 << 25, x_stride=1 << 25, w_stride=1 << 25), abi.E_INVALID),
-    (dict(rows=1 << 24, n_out=1 << 17, out_stride=1 << 17), abi.E_INVALID)])
+    (dict(rows=1 << 24, n_out=1 << 17, out_stride=1 << 17), abi.E_INVALID), (dict(out=16), abi.E_INVALID), (dict(out=32), abi.E_INVALID)])
 def test_products_refuse(change, status):
     refused(rt.dev_linear, LINEAR, change, status)
     refused(rt.dev_gated_linear, GATED, change, status)
@@ -69,6 +69,7 @@ def test_each_product_has_its_own_parts():
     refused(rt.dev_linear, LINEAR, dict(residual=48, residual_stride=48), abi.E_INVALID)
     refused(rt.dev_gated_linear, GATED, dict(residual=64, residual_stride=40), abi.E_INVALID)
     refused(rt.dev_gated_linear, GATED, dict(up_stride=60), abi.E_INVALID)
+    refused(rt.dev_gated_linear, GATED, dict(out=64), abi.E_INVALID)
     refused(rt.dev_gated_linear, GATED, dict(up_stride=65), abi.E_UNSUPPORTED)
     for missing in ("x_scale", "w_scale"):
         refused(rt.dev_linear, CODED, {missing: None}, abi.E_INVALID)
