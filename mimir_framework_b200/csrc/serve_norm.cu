@@ -29,40 +29,93 @@ struct NormParams {
   float* y_scale;
   long long x_row, residual_row, sum_row, y_row;  // bytes
   int rows, n, norm, early, stages;
-  bool x_vec, residual_vec, sum_vec, gamma_vec, y_vec;  // rows start on 16 bytes
+  bool vec;  // all rows (and gamma) start on 16 bytes, codes on 8
   float eps, inv_n;
   int* err_word;
 };
 
-// Eight elements from column `col` on, those from n on zero.
-template <int T>
-__device__ __forceinline__ Raw8<T> row_load8(const char* row, int col, int n, bool vec) {
-  const char* p = row + static_cast<long long>(col) * type_bytes(T);
-  if (vec && col + 8 <= n) return load8<T>(p);
+// 16 bytes from byte `at` (even, below 16, the same for a row) of two times 16
+__device__ __forceinline__ uint4 bytes_from(const uint4& a, const uint4& b, int at) {
+  uint32_t w[5];
+  switch (at >> 2) {
+    case 0: w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x; break;
+    case 1: w[0] = a.y, w[1] = a.z, w[2] = a.w, w[3] = b.x, w[4] = b.y; break;
+    case 2: w[0] = a.z, w[1] = a.w, w[2] = b.x, w[3] = b.y, w[4] = b.z; break;
+    default: w[0] = a.w, w[1] = b.x, w[2] = b.y, w[3] = b.z, w[4] = b.w;
+  }
+  if (!(at & 2)) return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint4(__funnelshift_r(w[0], w[1], 16), __funnelshift_r(w[1], w[2], 16), __funnelshift_r(w[2], w[3], 16), __funnelshift_r(w[3], w[4], 16));
+}
+
+// A thread's eight elements of a vector, those from n on zero.  VEC: all rows start on 16 bytes.  Else neighbours from column `col` on, or (`apart` > 0,
+// where x is F32) every `apart`-th, so that a warp's lanes have neighbours.  Rows of 16 bits off their boundary come in the two times 16 bytes that hold a vector (both
+// hold some of it) and leave as whole 16 bytes that a lane makes up with its neighbour's: every lane of a warp has to call.  (5 638 rows of 5 871
+// halves with residual 67 us; element by element 137, 122 with lanes side by side.)
+template <int T, bool VEC>
+__device__ __forceinline__ Raw8<T> row_load8(const char* row, int col, int n, int apart) {
+  const char* const p = row + static_cast<long long>(col) * type_bytes(T);
+  const int off = VEC ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+  if ((VEC || apart == 0) && col + 8 <= n && off == 0) return load8<T>(p);
   Raw8<T> r;
+  if constexpr (type_bytes(T) == 2 && !VEC) {
+    if (col + 8 <= n) {
+      const uint4 v = bytes_from(*reinterpret_cast<const uint4*>(p - off), *reinterpret_cast<const uint4*>(p - off + 16), off);
+      r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+      return r;
+    }
+  }
+  const int step = !VEC && apart ? apart : 1;
 #pragma unroll
   for (uint32_t& w : r.w) w = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (col + e >= n) break;
-    if constexpr (type_bytes(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-    else r.w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+    const int at = col + e * step;
+    if (at >= n) break;
+    if constexpr (type_bytes(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(row)[at];
+    else r.w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[at]) << (16 * (e & 1));
   }
   return r;
 }
-template <int T>
-__device__ __forceinline__ void row_store8(char* row, int col, int n, bool vec, const Raw8<T>& r) {
-  char* p = row + static_cast<long long>(col) * type_bytes(T);
-  if (vec && col + 8 <= n) {
+template <int T, bool VEC>
+__device__ __forceinline__ void row_store8(char* row, int col, int n, int apart, const Raw8<T>& r) {
+  char* const p = row + static_cast<long long>(col) * type_bytes(T);
+  const bool whole = col + 8 <= n;
+  int first = 0, last = 8;  // the elements that go one by one
+  if constexpr (VEC) {
+    if (whole) {
+      store8<T>(p, r);
+      return;
+    }
+  } else if constexpr (type_bytes(T) == 2) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);  // (the same for all of a row)
+    if (apart == 0 && off) {
+      const int lane = threadIdx.x & 31;
+      const uint4 mine = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+      uint4 before;
+      before.x = __shfl_up_sync(0xffffffffu, mine.x, 1), before.y = __shfl_up_sync(0xffffffffu, mine.y, 1);
+      before.z = __shfl_up_sync(0xffffffffu, mine.z, 1), before.w = __shfl_up_sync(0xffffffffu, mine.w, 1);
+      const bool next_whole = __shfl_down_sync(0xffffffffu, static_cast<int>(whole), 1) && lane < 31;
+      if (whole && lane > 0) {
+        *reinterpret_cast<uint4*>(p - off) = bytes_from(before, mine, 16 - off);
+        first = 8 - off / 2;
+      }
+      if (whole && next_whole) last = 8 - off / 2;  // (the next lane has the rest)
+    } else if (apart == 0 && whole) {
+      store8<T>(p, r);
+      return;
+    }
+  } else if (apart == 0 && whole && (reinterpret_cast<uintptr_t>(p) & (type_bytes(T) == 1 ? 7 : 15)) == 0) {
     store8<T>(p, r);
     return;
   }
+  const int step = !VEC && apart ? apart : 1;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (col + e >= n) break;
-    if constexpr (type_bytes(T) == 4) reinterpret_cast<uint32_t*>(p)[e] = r.w[e];
-    else if constexpr (type_bytes(T) == 2) reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(r.w[e / 2] >> (16 * (e & 1)));
-    else reinterpret_cast<uint8_t*>(p)[e] = static_cast<uint8_t>(r.w[e / 4] >> (8 * (e & 3)));
+    const int at = col + e * step;
+    if (e < first || e >= last || at >= n) continue;
+    if constexpr (type_bytes(T) == 4) reinterpret_cast<uint32_t*>(row)[at] = r.w[e];
+    else if constexpr (type_bytes(T) == 2) reinterpret_cast<uint16_t*>(row)[at] = static_cast<uint16_t>(r.w[e / 2] >> (16 * (e & 1)));
+    else reinterpret_cast<uint8_t*>(row)[at] = static_cast<uint8_t>(r.w[e / 4] >> (8 * (e & 3)));
   }
 }
 
@@ -126,15 +179,16 @@ __device__ __forceinline__ float root_reciprocal(float x) {
 // where memory does not, so two elements go through one wherever there is such a one (8 192 rows of 4 096 with residual to codes took 37 M
 // instructions and 47 us element by element, 42 so).  A row that is not `live` takes part in the meetings and leaves nothing.
 // NORM: 0, 1, or -1, which is what the call says (the ring's registers do not hold both kinds of codes).
-template <int TX, int TY, int V, bool WARP, int NORM = -1>
-__device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, Pair (&f)[V][4], float (&buf)[2][32]) {
+template <int TX, int TY, int V, bool WARP, bool VEC, int NORM = -1>
+__device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[2][32]) {
+  const int col0 = !VEC && apart ? t : t * 8;
   if (p.sum && live) {
     char* const sum = p.sum + row * p.sum_row;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float s[8];
       from_pairs(f[v], s);
-      row_store8<TX>(sum, v * step + t * 8, p.n, p.sum_vec, pack8<TX>(s));
+      row_store8<TX, VEC>(sum, v * step + col0, p.n, apart, pack8<TX>(s));
     }
   }
   const bool norm = NORM < 0 ? p.norm != 0 : NORM == 1;
@@ -189,14 +243,14 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
     const Pair r2 = pack2(r, r);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int col = v * step + t * 8;
+      const int col = v * step + col0;
       if (!later) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], r2);
       }
       if (p.gamma) {
         Pair g[4];
-        to_pairs<MIMIR_B200_T_F32>(row_load8<MIMIR_B200_T_F32>(reinterpret_cast<const char*>(p.gamma), col, p.n, p.gamma_vec), g);
+        to_pairs<MIMIR_B200_T_F32>(row_load8<MIMIR_B200_T_F32, VEC>(reinterpret_cast<const char*>(p.gamma), col, p.n, apart), g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], g[i]);
       }
@@ -236,7 +290,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
     const Pair r2 = pack2(inverse, inverse), s2 = pack2(-part, -part), again2 = pack2(again, again);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int col = v * step + t * 8;
+      const int col = v * step + col0;
       if (col >= p.n || !live) break;
       float s[8];
       if (quick) {
@@ -250,14 +304,14 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = part > 0.0f ? __fdiv_rn(s[e], part) : fabsf(s[e]) < INFINITY ? 0.0f : s[e];  // (none: a row with none finite but zeros)
       }
-      row_store8<TY>(y, col, p.n, p.y_vec, pack8<TY>(s));
+      row_store8<TY, VEC>(y, col, p.n, apart, pack8<TY>(s));
     }
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float s[8];
       from_pairs(f[v], s);
-      if (live) row_store8<TY>(y, v * step + t * 8, p.n, p.y_vec, pack8<TY>(s));
+      if (live) row_store8<TY, VEC>(y, v * step + col0, p.n, apart, pack8<TY>(s));
     }
   }
 }
@@ -269,7 +323,7 @@ constexpr int norm_threads() { return WARP ? NR_WARP_THREADS : V == 2 && TX == M
 template <int TX, bool WARP, int V>
 constexpr int norm_ctas() { return WARP ? (V == 4 ? 4 : 8) : V == 2 ? (TX == MIMIR_B200_T_F32 ? 2 : 3) : V == 4 ? 2 : 1; }
 
-template <int TX, int TY, int V, bool WARP>
+template <int TX, int TY, int V, bool WARP, bool VEC>
 __global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WARP, V>()) norm_rows_serve_kernel(const __grid_constant__ NormParams p) {
   __shared__ __align__(16) float buf[2][32];
   pdl_early_if(p.early);
@@ -278,13 +332,14 @@ __global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WAR
   const int row = WARP ? blockIdx.x * (NR_WARP_THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
   if (WARP && row >= p.rows) return;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x, step = (WARP ? 32 : blockDim.x) * 8;
+  const int apart = VEC || TX != MIMIR_B200_T_F32 ? 0 : step / 8, col0 = apart ? t : t * 8;
   const char* const x = p.x + row * p.x_row;
   Pair f[V][4];
   Raw8<TX> raw[V], res[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    raw[v] = row_load8<TX>(x, v * step + t * 8, p.n, p.x_vec);
-    if (p.residual) res[v] = row_load8<TX>(p.residual + row * p.residual_row, v * step + t * 8, p.n, p.residual_vec);
+    raw[v] = row_load8<TX, VEC>(x, v * step + col0, p.n, apart);
+    if (p.residual) res[v] = row_load8<TX, VEC>(p.residual + row * p.residual_row, v * step + col0, p.n, apart);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -297,7 +352,7 @@ __global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WAR
     }
   }
   if (!WARP) __syncthreads();  // (the words of no warp)
-  finish_row<TX, TY, V, WARP>(p, row, true, t, step, f, buf);
+  finish_row<TX, TY, V, WARP, VEC>(p, row, true, t, step, apart, f, buf);
 }
 
 // The same for many long rows of 16 bits without a residual: few CTAs fit into the registers, so the rows come through a ring in shared memory by
@@ -336,13 +391,13 @@ __global__ void __launch_bounds__(512, 2) norm_rows_ring_kernel(const __grid_con
     const char* x = reinterpret_cast<const char*>(ring + stage * bytes);
     Pair f[4][4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) to_pairs<TX>(row_load8<TX>(x, v * step + t * 8, p.n, true), f[v]);
+    for (int v = 0; v < 4; ++v) to_pairs<TX>(row_load8<TX, true>(x, v * step + t * 8, p.n, 0), f[v]);
     __syncthreads();
     if (t == 0 && ok && next < p.rows) {
       ask(static_cast<int>(next), stage);
       next += apart;
     }
-    finish_row<TX, TY, 4, false, NORM>(p, static_cast<int>(row), ok, t, step, f, buf);
+    finish_row<TX, TY, 4, false, true, NORM>(p, static_cast<int>(row), ok, t, step, 0, f, buf);
     if (++stage == p.stages) { stage = 0; phase ^= 1; }
   }
 }
@@ -355,7 +410,7 @@ int launch_as(const NormParams& p, int threads, cudaStream_t st) {
   if constexpr (!WARP && V == 4 && TX != MIMIR_B200_T_F32) {
     const size_t row_bytes = static_cast<size_t>(p.n) * type_bytes(TX);
     const unsigned at_once = static_cast<unsigned>(ctx().sm_count * 2);
-    if (p.x_vec && !p.residual && row_bytes % 16 == 0 && grid > 2 * at_once) {
+    if (p.vec && !p.residual && row_bytes % 16 == 0 && grid > 2 * at_once) {
       q.stages = static_cast<int>(std::min<size_t>(NR_RING / row_bytes, NR_MAX_STAGES));  // (rows of up to 32 KB: three at least)
       auto run = [&](auto kern, PerDeviceOnce& once) -> int {
         MB_TRY(once.run([&]() -> int {
@@ -372,7 +427,8 @@ int launch_as(const NormParams& p, int threads, cudaStream_t st) {
     }
   }
   q.early = pdl_small_grid(grid);
-  MB_TRY(launch_pdl(norm_rows_serve_kernel<TX, TY, V, WARP>, dim3(grid), dim3(static_cast<unsigned>(threads)), 0, st, 1, q));
+  MB_TRY(launch_pdl(p.vec ? norm_rows_serve_kernel<TX, TY, V, WARP, true> : norm_rows_serve_kernel<TX, TY, V, WARP, false>, dim3(grid),
+                    dim3(static_cast<unsigned>(threads)), 0, st, 1, q));
   count_launch();
   return MIMIR_B200_OK;
 }
@@ -410,8 +466,8 @@ int launch_norm_rows(const MimirNormRows& a, cudaStream_t st) {
   p.gamma = a.gamma, p.y = static_cast<char*>(a.y), p.y_scale = a.y_scale;
   p.x_row = a.x_stride * xs, p.residual_row = a.residual_stride * xs, p.sum_row = a.sum_stride * xs, p.y_row = a.y_stride * ys;
   p.rows = a.rows, p.n = a.n, p.norm = a.norm, p.eps = a.eps, p.inv_n = 1.0f / static_cast<float>(a.n), p.err_word = ctx().dev_error_word;
-  p.x_vec = vectors_at(p.x, p.x_row, 16), p.residual_vec = vectors_at(p.residual, p.residual_row, 16), p.sum_vec = vectors_at(p.sum, p.sum_row, 16);
-  p.gamma_vec = vectors_at(p.gamma, 0, 16), p.y_vec = vectors_at(p.y, p.y_row, ys == 1 ? 8 : 16);
+  p.vec = vectors_at(p.x, p.x_row, 16) && vectors_at(p.residual, p.residual_row, 16) && vectors_at(p.sum, p.sum_row, 16) && vectors_at(p.gamma, 0, 16) &&
+          vectors_at(p.y, p.y_row, ys == 1 ? 8 : 16);
   switch (a.type) {
     case MIMIR_B200_T_F32: return launch_to<MIMIR_B200_T_F32>(p, a.y_type, st);
     case MIMIR_B200_T_F16: return launch_to<MIMIR_B200_T_F16>(p, a.y_type, st);
