@@ -6,7 +6,9 @@
 // tensor memory.  The kernel is persistent, tensor memory holds two accumulators of 256 columns:
 //   warp 0     TMA into a ring of six stages of 32 KB a CTA
 //   warp 1     (the leader's) issues the instructions for both
-//   warps 2-9  results: two warps for each 32 rows, half of the columns each; 32 columns at a time through activation, gate and residual
+//   the others results: two or four warps for each 32 rows, as many parts of the columns; 32 columns at a time through activation, gate and residual
+// Four where results bound the kernel, with few inputs or rows off their boundary (12 153 x 192 x 1 728 25.4 us, with two 27.4; 3 040 x 4 162 x 2 190 off it
+// 55.5 against 64.9); two where the instructions do, as there are registers for 168 a thread then (4 096 inputs, gated, 377 us against 384).
 // Results of F32 are taken out every 256 inputs and added up in registers: the tensor core's additions truncate.
 #include <algorithm>
 #include <cmath>
@@ -19,10 +21,9 @@ namespace {
 
 constexpr int TM = 128, TN = 256;  // rows of a CTA, columns of an accumulator
 constexpr int STAGES = 6, A_BYTES = TM * LIN_BLOCK, W_BYTES = TN / 2 * LIN_BLOCK, STAGE = A_BYTES + W_BYTES;
-constexpr int THREADS = 320, EPI_WARPS = 8;
-constexpr int TURN = 32 * 17 * 4;     // a warp's tile for results that are turned around, 16 columns at a time
-constexpr int COLS = 256 * 4;         // scales and biases of a warp's columns
-constexpr int SMEM = STAGES * STAGE + EPI_WARPS * (TURN + COLS) + 256 + 1024;
+constexpr int TURNS = 8 * 32 * 17 * 4;  // the warps' tiles for results that are turned around, 16 columns of 32 rows (16 warps: of 16) at a time
+constexpr int COLS = 2 * TN * 4;        // scales and biases of the columns of four warps
+constexpr int SMEM = STAGES * STAGE + TURNS + 4 * COLS + 256 + 1024;
 static_assert(SMEM <= 232448, "exceeds the 227 KB of shared memory a CTA may use");
 
 struct TileParams {
@@ -62,6 +63,7 @@ __device__ __forceinline__ void scaled(float (&v)[32], float sx, const float* sc
 }
 
 // 32 results of this lane's row, columns col0 on, to where they belong
+template <int ROWS>
 __device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32], int row0, int col0, float* turn) {
   const int lane = threadIdx.x & 31, row = row0 + lane;
   const int size = p.out_type == MIMIR_B200_T_F32 ? 4 : 2;
@@ -121,45 +123,51 @@ __device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32],
     return;
   }
   // rows off their boundary, and the last columns: turned around, so that a warp's lanes write neighbours, 16 columns of two rows at a time
-  const int rows = min(32, p.rows - row0);
+  const int at = lane & 15;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int c0 = 0; c0 < 32; c0 += 16) {
+    const int col = col0 + c0 + at;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = v[h * 16 + j];
-    __syncwarp();
-    const int at = lane & 15, col = col0 + h * 16 + at;
-    if (col < p.n_out) {
-      char* o = p.out + row0 * p.out_row + static_cast<long long>(col) * size;
-      const char* r = p.residual ? p.residual + row0 * p.residual_row + static_cast<long long>(col) * size : nullptr;
+    for (int r0 = 0; r0 < 32; r0 += ROWS) {
+      if (ROWS == 32 || (lane & 16) == r0) {
 #pragma unroll
-      for (int i0 = 0; i0 < 32; i0 += 16) {
-        float q[8];
-        if (p.residual) {
+        for (int j = 0; j < 16; ++j) turn[(lane & (ROWS - 1)) * 17 + j] = v[c0 + j];
+      }
+      __syncwarp();
+      const int rows = min(ROWS, p.rows - row0 - r0);
+      if (col < p.n_out) {
+        char* o = p.out + (row0 + r0) * p.out_row + static_cast<long long>(col) * size;
+        const char* r = p.residual ? p.residual + (row0 + r0) * p.residual_row + static_cast<long long>(col) * size : nullptr;
+#pragma unroll
+        for (int i0 = 0; i0 < ROWS; i0 += 16) {
+          float q[8];
+          if (p.residual) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int k = i0 + 2 * i + (lane >> 4);
+              q[i] = k < rows ? load_typed(r + k * p.residual_row, p.out_type) : 0.0f;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int k = i0 + 2 * i + (lane >> 4);
-            q[i] = k < rows ? load_typed(r + k * p.residual_row, p.out_type) : 0.0f;
+            if (k < rows) store_typed(o + k * p.out_row, p.out_type, p.residual ? turn[k * 17 + at] + q[i] : turn[k * 17 + at]);
           }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = i0 + 2 * i + (lane >> 4);
-          if (k < rows) store_typed(o + k * p.out_row, p.out_type, p.residual ? turn[k * 17 + at] + q[i] : turn[k * 17 + at]);
-        }
       }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
-template <bool F8, bool GATED, bool F32>
-__global__ void __launch_bounds__(THREADS, 1)
+template <bool F8, bool GATED, bool F32, int PARTS>
+__global__ void __launch_bounds__(64 + 128 * PARTS, 1)
 linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_up,
                     const __grid_constant__ TileParams tp) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* turns = reinterpret_cast<float*>(smem + STAGES * STAGE);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + EPI_WARPS * (TURN + COLS));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE + TURNS + 4 * COLS);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* acc_full = empty_bar + STAGES;
   uint64_t* acc_empty = acc_full + 2;
@@ -171,6 +179,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int rank = static_cast<int>(cluster_ctarank());
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1, all = tp.tiles_m * tp.tiles_n, items = 2 * all - tp.full;
   constexpr int OUT = GATED ? TN / 2 : TN;  // features of a tile
+  constexpr int EPI_WARPS = 4 * PARTS, WARP_COLS = COLS / PARTS, TURN = TURNS / EPI_WARPS;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -275,8 +284,8 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   } else {
-    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-    float* const turn = turns + ew * ((TURN + COLS) / 4);
+    const int ew = warp - 2, quad = warp & 3, part = ew >> 2;
+    float* const turn = turns + ew * ((TURN + WARP_COLS) / 4);
     float* const cols = turn + TURN / 4;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -296,16 +305,16 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       int tm, tn;
       const int cut = tile_of(tp, t, tm, tn);
       const int row0 = (2 * tm + rank) * TM + quad * 32;
-      const int wide = cut >= 0 ? OUT / 2 : OUT;             // features of this item
-      const int mine = half * (wide / 2), nch = wide / 64;   // this warp's first, and how many times 32
+      const int wide = cut >= 0 ? OUT / 2 : OUT;  // features of this item
+      const int each = max(32, wide / PARTS), mine = part * each, nch = mine < wide ? each / 32 : 0;  // this warp's, its first, and how many times 32
       const int col00 = tn * OUT + (cut > 0 ? OUT / 2 : 0) + mine;
       float sx = 1.0f;
       if (F8 && row0 + lane < p.rows) sx = __ldg(p.x_scale + row0 + lane);
-      // the columns' scales and biases while the sums are made: [bias][of up][scale][of up], as many as the warp has columns (a gated pair: 64, else 128)
-      constexpr int EACH = GATED ? 64 : 128;
+      // the columns' scales and biases while the sums are made: [bias][of up][scale][of up], as many as the warp has columns (a gated pair: half)
+      constexpr int EACH = OUT / PARTS;
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < WARP_COLS / 128; ++i) {
         const int which = i * 32 / EACH, col = col00 + i * 32 % EACH + lane;
         if (!F8 && which >= (GATED ? 2 : 1)) break;
         const float* from = GATED ? (which == 0 ? p.bias : which == 1 ? p.up_bias : which == 2 ? p.w_scale : p.up_scale) : which == 0 ? p.bias : p.w_scale;
@@ -321,24 +330,25 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 32; ++j) z[j] *= u[j];
         }
-        write_out(p, z, row0, col0, turn);
+        write_out<64 / PARTS>(p, z, row0, col0, turn);
       };
       if constexpr (F32) {
-        float v[4][32];
+        constexpr int HELD = TN / PARTS / 32;
+        float v[HELD][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < HELD; ++i)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;
         for (int kb = 0; kb < p.kblocks && ok; kb += p.chunk) {
           const uint32_t at = take();
           if (!ok) break;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // (of a gated pair: two of the one, two of the other)
-            const int n = GATED ? i & 1 : i;
+          for (int i = 0; i < HELD; ++i) {
+            // (of a gated pair: first the one's, then the other's)
+            const int n = GATED ? i % (HELD / 2) : i;
             if (n >= nch) continue;
             float w[32];
-            tmem_ld_32x32(at + static_cast<uint32_t>(mine + n * 32 + (GATED && i >= 2 ? wide : 0)), w);
+            tmem_ld_32x32(at + static_cast<uint32_t>(mine + n * 32 + (GATED && i >= HELD / 2 ? wide : 0)), w);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[i][j] += w[j];
           }
@@ -346,8 +356,8 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < (GATED ? 2 : 4); ++i)
-          if (i < nch && col00 + i * 32 < p.n_out) finish(v[i], v[GATED ? i + 2 : i], col00 + i * 32);
+        for (int i = 0; i < (GATED ? HELD / 2 : HELD); ++i)
+          if (i < nch && col00 + i * 32 < p.n_out) finish(v[i], v[GATED ? i + HELD / 2 : i], col00 + i * 32);
       } else {
         const uint32_t at = take();
         if (!ok) break;
@@ -390,17 +400,23 @@ TileShape tile_shape(const MimirLinear& a, bool gated) {
   return s;
 }
 
-template <bool F8, bool GATED, bool F32>
+template <bool F8, bool GATED, bool F32, int PARTS>
 int launch_as(const CUtensorMap (&maps)[3], const TileParams& p, unsigned grid, cudaStream_t st) {
-  auto kern = linear_tiles_kernel<F8, GATED, F32>;
+  auto kern = linear_tiles_kernel<F8, GATED, F32, PARTS>;
   static PerDeviceOnce once;
   MB_TRY(once.run([&]() -> int {
     MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     return MIMIR_B200_OK;
   }));
-  MB_TRY(launch_pdl(kern, dim3(grid), dim3(THREADS), SMEM, st, 2, maps[0], maps[1], maps[2], p));
+  MB_TRY(launch_pdl(kern, dim3(grid), dim3(64 + 128 * PARTS), SMEM, st, 2, maps[0], maps[1], maps[2], p));
   count_launch();
   return MIMIR_B200_OK;
+}
+template <bool F8, bool GATED>
+int launch_for(const CUtensorMap (&maps)[3], const TileParams& p, unsigned grid, cudaStream_t st) {
+  if (p.l.out_type == MIMIR_B200_T_F32) return launch_as<F8, GATED, true, 2>(maps, p, grid, st);
+  const bool many = p.l.kblocks <= (GATED ? 8 : 24) || (!GATED && p.l.vec_out != 32);
+  return many ? launch_as<F8, GATED, false, 4>(maps, p, grid, st) : launch_as<F8, GATED, false, 2>(maps, p, grid, st);
 }
 
 }  // namespace
@@ -425,12 +441,8 @@ int launch_linear_tiles(const MimirLinear& a, const LinearParams& l, bool gated,
   p.l = l, p.tiles_m = static_cast<int>(s.tiles_m), p.tiles_n = static_cast<int>(s.tiles_n), p.full = static_cast<int>(s.full);
   p.group_n = p.tiles_n < 8 ? p.tiles_n : 8;
   const unsigned grid = static_cast<unsigned>(2 * (s.items < s.pairs ? s.items : s.pairs));
-  const bool f32 = a.out_type == MIMIR_B200_T_F32;
-  if (a.type == MIMIR_B200_T_E4M3)
-    return gated ? (f32 ? launch_as<true, true, true>(maps, p, grid, st) : launch_as<true, true, false>(maps, p, grid, st))
-                 : (f32 ? launch_as<true, false, true>(maps, p, grid, st) : launch_as<true, false, false>(maps, p, grid, st));
-  return gated ? (f32 ? launch_as<false, true, true>(maps, p, grid, st) : launch_as<false, true, false>(maps, p, grid, st))
-               : (f32 ? launch_as<false, false, true>(maps, p, grid, st) : launch_as<false, false, false>(maps, p, grid, st));
+  if (a.type == MIMIR_B200_T_E4M3) return gated ? launch_for<true, true>(maps, p, grid, st) : launch_for<true, false>(maps, p, grid, st);
+  return gated ? launch_for<false, true>(maps, p, grid, st) : launch_for<false, false>(maps, p, grid, st);
 }
 
 }  // namespace mb
