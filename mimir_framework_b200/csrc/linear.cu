@@ -32,6 +32,19 @@ int make_operand_map(CUtensorMap* map, const void* base, int type, long long row
   return MIMIR_B200_OK;
 }
 
+int make_result_map(CUtensorMap* map, const void* base, int type, long long rows, int n_out, long long stride) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MIMIR_B200_E_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const int size = type_bytes(type);
+  const long long apart = rows > 1 ? stride * size : (static_cast<long long>(n_out) * size + 15) / 16 * 16;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(n_out), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(apart)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(64 / size), 32}, steps[2] = {1, 1};
+  const CUresult r = fn(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MIMIR_B200_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return MIMIR_B200_OK;
+}
+
 int launch_linear(const MimirLinear& a, bool gated, cudaStream_t st) {
   LinearParams p = {};
   const int size = type_bytes(a.out_type), per_block = LIN_BLOCK / type_bytes(a.type);

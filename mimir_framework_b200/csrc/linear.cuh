@@ -42,6 +42,8 @@ double linear_rows_us(const MimirLinear& a, bool gated);
 int launch_linear_rows(const MimirLinear& a, const LinearParams& p, bool gated, cudaStream_t st);
 // tensor map of an operand: boxes of 128 bytes x `box_rows` rows, 128-byte swizzle, zeros beyond its rows and inputs
 int make_operand_map(CUtensorMap* map, const void* base, int type, long long rows, int n_in, long long stride, int box_rows);
+// of a result whose rows are on 16 bytes: boxes of 64 bytes x 32 rows, 64-byte swizzle
+int make_result_map(CUtensorMap* map, const void* base, int type, long long rows, int n_out, long long stride);
 
 namespace {
 
@@ -59,6 +61,11 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
   asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1)
                : "memory");
+}
+// Arrives in a CTA of the cluster.  What it orders is tensor memory, by the fences on both sides; a release at the cluster's scope would wait for every
+// store of the thread (0.6 us a tile).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 // 8-bit floats: 32 values of K an instruction
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {

@@ -4,7 +4,7 @@
 // and half of the weights' 256, so that a byte of operands in shared memory is used 256 times.  A gated pair's tile is 128 features of each matrix:
 // the leader's half of the N side is the gate's, the other's is up's, and a thread finds both of an output in its own row of
 // tensor memory.  The kernel is persistent, tensor memory holds two accumulators of 256 columns:
-//   warp 0     TMA into a ring of six stages of 32 KB a CTA
+//   warp 0     TMA into a ring of five stages of 32 KB a CTA
 //   warp 1     (the leader's) issues the instructions for both
 //   the others results: two or four warps for each 32 rows, as many parts of the columns; 32 columns at a time through activation, gate and residual
 // Four where results bound the kernel, with few inputs or rows off their boundary (12 153 x 192 x 1 728 25.4 us, with two 27.4; 3 040 x 4 162 x 2 190 off it
@@ -20,9 +20,10 @@ namespace mb {
 namespace {
 
 constexpr int TM = 128, TN = 256;  // rows of a CTA, columns of an accumulator
-constexpr int STAGES = 6, A_BYTES = TM * LIN_BLOCK, W_BYTES = TN / 2 * LIN_BLOCK, STAGE = A_BYTES + W_BYTES;
-constexpr int TURNS = 8 * 32 * 17 * 4;  // the warps' tiles for results that are turned around, 16 columns of 32 rows (16 warps: of 16) at a time
-constexpr int COLS = 2 * TN * 4;        // scales and biases of the columns of four warps
+constexpr int STAGES = 5, A_BYTES = TM * LIN_BLOCK, W_BYTES = TN / 2 * LIN_BLOCK, STAGE = A_BYTES + W_BYTES;
+constexpr int OUT_TILE = 32 * 64;     // 32 rows x 64 bytes of results on their way out
+constexpr int TURNS = 16 * OUT_TILE;  // eight warps: two such tiles each, or what turns 32 rows around; sixteen: one, or 16 rows
+constexpr int COLS = 2 * TN * 4;      // scales and biases of the columns of four warps
 constexpr int SMEM = STAGES * STAGE + TURNS + 4 * COLS + 256 + 1024;
 static_assert(SMEM <= 232448, "exceeds the 227 KB of shared memory a CTA may use");
 
@@ -63,66 +64,89 @@ __device__ __forceinline__ void scaled(float (&v)[32], float sx, const float* sc
 }
 
 // 32 results of this lane's row, columns col0 on, to where they belong
-template <int ROWS>
-__device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32], int row0, int col0, float* turn) {
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+template <int ROWS, int BUFFERS>
+__device__ __forceinline__ void write_out(const LinearParams& p, const CUtensorMap& map_out, float (&v)[32], int row0, int col0, float* turn, int& flip) {
   const int lane = threadIdx.x & 31, row = row0 + lane;
   const int size = p.out_type == MIMIR_B200_T_F32 ? 4 : 2;
-  const bool full = col0 + 32 <= p.n_out;
-  if (full && p.vec_out == 32 && (!p.residual || p.vec_res)) {
+  if (p.vec_out && (col0 + 32 <= p.n_out || (p.n_out * size) % 16 == 0)) {
+    // rows on 16 bytes: tiles of 32 rows x 64 bytes in shared memory (64-byte swizzle: no conflicts), each one copy, which stops at the last row and, where
+    // that is on 16 bytes too (else it would write behind it), the last column
     if (p.residual && row < p.rows) {
       const char* r = p.residual + row * p.residual_row + static_cast<long long>(col0) * size;
-      if (size == 4) {
+      if (p.vec_res && col0 + 32 <= p.n_out) {
+        if (size == 4) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          float q[8];
-          unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(r + j * 4), q);
+          for (int j = 0; j < 32; j += 8) {
+            float q[8];
+            unpack8<MIMIR_B200_T_F32>(load8<MIMIR_B200_T_F32>(r + j * 4), q);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[j + e] += q[e];
+            for (int e = 0; e < 8; ++e) v[j + e] += q[e];
+          }
+        } else {
+          Raw8<MIMIR_B200_T_F16> raw[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raw[j] = load8<MIMIR_B200_T_F16>(r + j * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float q[8];
+            if (p.out_type == MIMIR_B200_T_F16) {
+              unpack8<MIMIR_B200_T_F16>(raw[j], q);
+            } else {
+              Raw8<MIMIR_B200_T_BF16> b;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) b.w[e] = raw[j].w[e];
+              unpack8<MIMIR_B200_T_BF16>(b, q);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[8 * j + e] += q[e];
+          }
         }
       } else {
-        Raw8<MIMIR_B200_T_F16> raw[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j] = load8<MIMIR_B200_T_F16>(r + j * 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float q[8];
-          if (p.out_type == MIMIR_B200_T_F16) {
-            unpack8<MIMIR_B200_T_F16>(raw[j], q);
-          } else {
-            Raw8<MIMIR_B200_T_BF16> b;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b.w[e] = raw[j].w[e];
-            unpack8<MIMIR_B200_T_BF16>(b, q);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[8 * j + e] += q[e];
-        }
+        for (int j = 0; j < 32; ++j)
+          if (col0 + j < p.n_out) v[j] += load_typed(r + j * size, p.out_type);
       }
     }
-    char* o = p.out + row * p.out_row + static_cast<long long>(col0) * size;
-    if (row >= p.rows) {
-    } else if (size == 4) {
+    const int copies = size == 4 ? 2 : 1;
 #pragma unroll
-      for (int j = 0; j < 32; j += 8) st_global_v8(reinterpret_cast<float*>(o) + j, &v[j]);
-    } else {
+    for (int h = 0; h < 2; ++h) {
+      if (h == copies) break;
       uint32_t w[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        if (p.out_type == MIMIR_B200_T_F16) {
-          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        if (size == 4) {
+          w[j] = __float_as_uint(v[16 * h + j]);
+        } else if (p.out_type == MIMIR_B200_T_F16) {
+          const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&x);
         } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&x);
         }
       }
-      st_global_v8_b32(o, &w[0]);
-      st_global_v8_b32(o + 32, &w[8]);
+      uint8_t* const tile = reinterpret_cast<uint8_t*>(turn) + flip * OUT_TILE;
+      if (BUFFERS == 2) flip ^= 1;
+      if (lane == 0) bulk_wait_read<BUFFERS - 1>();  // the copy that was there has read it
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(tile + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (row0 < p.rows && col0 + 16 * h < p.n_out) tma_store_2d(&map_out, tile, col0 + 16 * h, row0);
+        bulk_commit();
+      }
     }
-    __syncwarp();
     return;
   }
   // rows off their boundary, and the last columns: turned around, so that a warp's lanes write neighbours, 16 columns of two rows at a time
+  if (p.vec_out) {
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+  }
   const int at = lane & 15;
 #pragma unroll
   for (int c0 = 0; c0 < 32; c0 += 16) {
@@ -163,7 +187,7 @@ __device__ __forceinline__ void write_out(const LinearParams& p, float (&v)[32],
 template <bool F8, bool GATED, bool F32, int PARTS>
 __global__ void __launch_bounds__(64 + 128 * PARTS, 1)
 linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_up,
-                    const __grid_constant__ TileParams tp) {
+                    const __grid_constant__ CUtensorMap map_out, const __grid_constant__ TileParams tp) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* turns = reinterpret_cast<float*>(smem + STAGES * STAGE);
@@ -180,6 +204,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1, all = tp.tiles_m * tp.tiles_n, items = 2 * all - tp.full;
   constexpr int OUT = GATED ? TN / 2 : TN;  // features of a tile
   constexpr int EPI_WARPS = 4 * PARTS, WARP_COLS = COLS / PARTS, TURN = TURNS / EPI_WARPS;
+  static_assert(TURN >= (64 / PARTS) * 17 * 4, "a warp's results are turned around in it");
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -285,9 +310,9 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
   } else {
     const int ew = warp - 2, quad = warp & 3, part = ew >> 2;
-    float* const turn = turns + ew * ((TURN + WARP_COLS) / 4);
-    float* const cols = turn + TURN / 4;
-    int acc = 0;
+    float* const turn = turns + ew * (TURN / 4);
+    float* const cols = turns + TURNS / 4 + ew * (WARP_COLS / 4);
+    int acc = 0, flip = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     auto take = [&]() -> uint32_t {
@@ -298,29 +323,43 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     auto give_back = [&] {
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+      if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&acc_empty[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     };
-    for (int t = first; t < items && ok; t += step) {
-      int tm, tn;
-      const int cut = tile_of(tp, t, tm, tn);
-      const int row0 = (2 * tm + rank) * TM + quad * 32;
-      const int wide = cut >= 0 ? OUT / 2 : OUT;  // features of this item
-      const int each = max(32, wide / PARTS), mine = part * each, nch = mine < wide ? each / 32 : 0;  // this warp's, its first, and how many times 32
-      const int col00 = tn * OUT + (cut > 0 ? OUT / 2 : 0) + mine;
-      float sx = 1.0f;
-      if (F8 && row0 + lane < p.rows) sx = __ldg(p.x_scale + row0 + lane);
-      // the columns' scales and biases while the sums are made: [bias][of up][scale][of up], as many as the warp has columns (a gated pair: half)
-      constexpr int EACH = OUT / PARTS;
-      __syncwarp();
+    // What a tile's results need besides its sums is on its way while the tile before it is finished: scales and biases of the warp's columns ([bias][of
+    // up][scale][of up], EACH of them, in shared memory when their tile comes) and the scale of the lane's row.
+    constexpr int EACH = OUT / PARTS, HOLD = WARP_COLS / 128;
+    float next_cols[HOLD], next_sx = 1.0f;
+    // this warp's columns of a tile, from its first on, as many as `each` (none where mine >= wide)
+    auto my_columns = [&](int tn, int cut, int& wide, int& each, int& mine) -> int {
+      wide = cut >= 0 ? OUT / 2 : OUT, each = max(32, wide / PARTS), mine = part * each;
+      return tn * OUT + (cut > 0 ? OUT / 2 : 0) + mine;
+    };
+    auto fetch = [&](int t) {
+      if (t >= items) return;
+      int tm, tn, wide, each, mine;
+      const int cut = tile_of(tp, t, tm, tn), col00 = my_columns(tn, cut, wide, each, mine), row = (2 * tm + rank) * TM + quad * 32 + lane;
+      if (F8 && row < p.rows) next_sx = __ldg(p.x_scale + row);
 #pragma unroll
-      for (int i = 0; i < WARP_COLS / 128; ++i) {
+      for (int i = 0; i < HOLD; ++i) {
         const int which = i * 32 / EACH, col = col00 + i * 32 % EACH + lane;
         if (!F8 && which >= (GATED ? 2 : 1)) break;
         const float* from = GATED ? (which == 0 ? p.bias : which == 1 ? p.up_bias : which == 2 ? p.w_scale : p.up_scale) : which == 0 ? p.bias : p.w_scale;
-        cols[i * 32 + lane] = from && col < p.n_out ? __ldg(from + col) : 0.0f;
+        next_cols[i] = from && col < p.n_out ? __ldg(from + col) : 0.0f;
       }
+    };
+    fetch(first);
+    for (int t = first; t < items && ok; t += step) {
+      int tm, tn, wide, each, mine;
+      const int cut = tile_of(tp, t, tm, tn), col00 = my_columns(tn, cut, wide, each, mine), nch = mine < wide ? each / 32 : 0;
+      const int row0 = (2 * tm + rank) * TM + quad * 32;
+      const float sx = next_sx;
       __syncwarp();
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i)
+        if (F8 || i * 32 / EACH < (GATED ? 2 : 1)) cols[i * 32 + lane] = next_cols[i];
+      __syncwarp();
+      fetch(t + step);
       const float* const my_cols = cols - col00;  // (+ column)
       auto finish = [&](float (&z)[32], float (&u)[32], int col0) {
         scaled<F8>(z, sx, my_cols + (GATED ? 2 : 1) * EACH + col0, my_cols + col0);
@@ -330,7 +369,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 32; ++j) z[j] *= u[j];
         }
-        write_out<64 / PARTS>(p, z, row0, col0, turn);
+        write_out<64 / PARTS, 4 / PARTS>(p, map_out, z, row0, col0, turn, flip);
       };
       if constexpr (F32) {
         constexpr int HELD = TN / PARTS / 32;
@@ -372,6 +411,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         give_back();
       }
     }
+    if (lane == 0) bulk_wait_read<0>();  // no copy still reads shared memory when the CTA leaves
   }
 
   tcgen05_fence_before();
@@ -401,21 +441,21 @@ TileShape tile_shape(const MimirLinear& a, bool gated) {
 }
 
 template <bool F8, bool GATED, bool F32, int PARTS>
-int launch_as(const CUtensorMap (&maps)[3], const TileParams& p, unsigned grid, cudaStream_t st) {
+int launch_as(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
   auto kern = linear_tiles_kernel<F8, GATED, F32, PARTS>;
   static PerDeviceOnce once;
   MB_TRY(once.run([&]() -> int {
     MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     return MIMIR_B200_OK;
   }));
-  MB_TRY(launch_pdl(kern, dim3(grid), dim3(64 + 128 * PARTS), SMEM, st, 2, maps[0], maps[1], maps[2], p));
+  MB_TRY(launch_pdl(kern, dim3(grid), dim3(64 + 128 * PARTS), SMEM, st, 2, maps[0], maps[1], maps[2], maps[3], p));
   count_launch();
   return MIMIR_B200_OK;
 }
 template <bool F8, bool GATED>
-int launch_for(const CUtensorMap (&maps)[3], const TileParams& p, unsigned grid, cudaStream_t st) {
+int launch_for(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
   if (p.l.out_type == MIMIR_B200_T_F32) return launch_as<F8, GATED, true, 2>(maps, p, grid, st);
-  const bool many = p.l.kblocks <= (GATED ? 8 : 24) || (!GATED && p.l.vec_out != 32);
+  const bool many = p.l.kblocks <= (GATED ? 8 : 24) || (!GATED && !p.l.vec_out);
   return many ? launch_as<F8, GATED, false, 4>(maps, p, grid, st) : launch_as<F8, GATED, false, 2>(maps, p, grid, st);
 }
 
@@ -432,11 +472,13 @@ double linear_tiles_us(const MimirLinear& a, bool gated) {
 
 int launch_linear_tiles(const MimirLinear& a, const LinearParams& l, bool gated, cudaStream_t st) {
   const TileShape s = tile_shape(a, gated);
-  CUtensorMap maps[3];
+  CUtensorMap maps[4];
   MB_TRY(make_operand_map(&maps[0], a.x, a.type, a.rows, a.n_in, a.x_stride, TM));
   MB_TRY(make_operand_map(&maps[1], a.w, a.type, a.n_out, a.n_in, a.w_stride, LIN_W_BOX));
   maps[2] = maps[1];
   if (gated) MB_TRY(make_operand_map(&maps[2], a.up, a.type, a.n_out, a.n_in, a.up_stride, LIN_W_BOX));
+  maps[3] = maps[0];
+  if (l.vec_out) MB_TRY(make_result_map(&maps[3], a.out, a.out_type, a.rows, a.n_out, a.out_stride));
   TileParams p = {};
   p.l = l, p.tiles_m = static_cast<int>(s.tiles_m), p.tiles_n = static_cast<int>(s.tiles_n), p.full = static_cast<int>(s.full);
   p.group_n = p.tiles_n < 8 ? p.tiles_n : 8;
