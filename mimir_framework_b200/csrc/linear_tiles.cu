@@ -7,8 +7,9 @@
 //   warp 0     TMA into a ring of five stages of 32 KB a CTA
 //   warp 1     (the leader's) issues the instructions for both
 //   the others results: two or four warps for each 32 rows, as many parts of the columns; 32 columns at a time through activation, gate and residual
-// Four where results bound the kernel, with few inputs or rows off their boundary (12 153 x 192 x 1 728 25.4 us, with two 27.4; 3 040 x 4 162 x 2 190 off it
-// 55.5 against 64.9); two where the instructions do, as there are registers for 168 a thread then (4 096 inputs, gated, 377 us against 384).
+// Four where the results bound the kernel, with few inputs, rows off their boundary or a residual (rows x inputs x features, with four and with two: 12 153 x
+// 192 x 1 728 16.4 us, 18.1; 4 486 x 1 344 x 11 456 with residual 119, 134; off the boundary 3 040 x 4 162 x 2 190 with residual 57, 65, gated 4 000 x 1 024
+// x 4 001 59, 69); two where the instructions do, as a thread then has 168 registers (8 192 x 1 024 x 4 096 50.5, 49.5; gated 8 192 x 512 x 4 096 63, 59).
 // Results of F32 are taken out every 256 inputs and added up in registers: the tensor core's additions truncate.
 #include <algorithm>
 #include <cmath>
@@ -455,7 +456,7 @@ int launch_as(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, 
 template <bool F8, bool GATED>
 int launch_for(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
   if (p.l.out_type == MIMIR_B200_T_F32) return launch_as<F8, GATED, true, 2>(maps, p, grid, st);
-  const bool many = p.l.kblocks <= (GATED ? 8 : 24) || (!GATED && !p.l.vec_out);
+  const bool many = p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (K blocks: both sides at the top)
   return many ? launch_as<F8, GATED, false, 4>(maps, p, grid, st) : launch_as<F8, GATED, false, 2>(maps, p, grid, st);
 }
 
