@@ -22,7 +22,7 @@ namespace {
 constexpr int RM = 128;  // rows of an instruction: features of a CTA at most
 constexpr int MAX_STAGES = 24, EARLY = 4, AHEAD = 4;
 constexpr int MAX_CLUSTER = 8, UNIT = 16, TURN = 2 * UNIT * RM * 4;  // (two turns of a unit for four warps)
-constexpr int STATIC = 3072, DYNAMIC = 232448 - STATIC, DYNAMIC_TWO = (228 * 1024) / 2 - 1024 - STATIC;  // shared memory of a CTA, one or two to an SM
+constexpr int STATIC = 3 * 1024, DYNAMIC = 232448 - STATIC, DYNAMIC_TWO = (228 * 1024) / 2 - 1024 - STATIC;  // shared memory of a CTA, one or two to an SM
 // A CTA of a cluster waits for others that may still be asking for tensor memory.  So that none of them can be kept from it by a CTA that waits
 // in the same way, two such CTAs never share an SM: each takes more than half of its shared memory (and more than the other kernels
 // of clusters leave, which take at least 104 KB a CTA).

@@ -177,7 +177,7 @@ __device__ __forceinline__ float root_reciprocal(float x) {
 
 // A row from the sums s that its threads hold on: V vectors of eight elements each; WARP: a row to a warp, else to the CTA.  Instructions bound it
 // where memory does not, so two elements go through one wherever there is such a one (8 192 rows of 4 096 with residual to codes took 37 M
-// instructions and 47 us element by element, 42 so).  A row that is not `live` takes part in the meetings and leaves nothing.
+// instructions and 47 us element by element, 29 M and 40 us so).  A row that is not `live` takes part in the meetings and leaves nothing.
 // NORM: 0, 1, or -1, which is what the call says (the ring's registers do not hold both kinds of codes).
 template <int TX, int TY, int V, bool WARP, bool VEC, int NORM = -1>
 __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[2][32]) {
