@@ -47,13 +47,13 @@ int make_result_map(CUtensorMap* map, const void* base, int type, long long rows
 
 int launch_linear(const MimirLinear& a, bool gated, cudaStream_t st) {
   LinearParams p = {};
-  const int size = type_bytes(a.out_type), per_block = LIN_BLOCK / type_bytes(a.type);
+  const int size = type_bytes(a.out_type);
   p.x_scale = a.x_scale, p.w_scale = a.w_scale, p.up_scale = a.up_scale, p.bias = a.bias, p.up_bias = a.up_bias;
   p.residual = static_cast<const char*>(a.residual), p.out = static_cast<char*>(a.out);
   p.residual_row = a.residual_stride * size, p.out_row = a.out_stride * size;
   p.rows = a.rows, p.n_out = a.n_out, p.out_type = a.out_type, p.act = a.activation;
-  p.kblocks = (a.n_in + per_block - 1) / per_block;
-  p.chunk = a.out_type == MIMIR_B200_T_F32 ? LIN_CHUNK / per_block : p.kblocks;
+  p.kblocks = linear_kblocks(a);
+  p.chunk = linear_chunk(a);
   p.formats = a.type == MIMIR_B200_T_BF16 ? (1u << 7) | (1u << 10) : 0u;  // (half, E4M3: 0)
   p.vec_out = on(a.out, p.out_row, 32) ? 32 : on(a.out, p.out_row, 16) ? 16 : 0;
   p.vec_res = on(a.residual, p.residual_row, 32) ? 32 : on(a.residual, p.residual_row, 16) ? 16 : 0;

@@ -17,7 +17,11 @@ namespace mb {
 
 constexpr int LIN_BLOCK = 128;   // bytes of a row in a K block
 constexpr int LIN_W_BOX = 64;    // weight rows of a TMA box
-constexpr int LIN_CHUNK = 256;   // inputs that results of F32 add up in the tensor core before they are taken out
+// How much is added up in the tensor core before the sum is taken out and added rounded, since an instruction truncates, by up to 2^-22 of the magnitudes:
+// for results of F32 256 inputs (2^-18; E4M3 2^-19), of 16 bits 64 K blocks, 256 instructions (2^-14, an eighth of fp16's half step, at worst; a sum whose
+// terms have either sign loses some 2^-17 of itself).  With 16 blocks products of 2 048 rows took 3 to 5 % longer, in 8 bits 6 to 12 %; with 64 those
+// of more inputs 1 to 3 %, the others nothing.
+constexpr int LIN_CHUNK_F32 = 256, LIN_CHUNK_BLOCKS = 64;
 
 struct LinearParams {
   const float* x_scale;
@@ -29,11 +33,15 @@ struct LinearParams {
   char* out;
   long long residual_row, out_row;  // bytes
   int rows, n_out, out_type, act;
-  int kblocks, chunk;               // K blocks of a product, and of an accumulation in tensor memory
+  int kblocks, chunk;               // K blocks of a product, and at most of a sum in tensor memory
   uint32_t formats;                 // instruction descriptor: operand formats
   int vec_out, vec_res;             // result, residual: all rows on 32 bytes, on 16, or neither (0)
   int* err_word;
 };
+
+// K blocks of a product, and of a sum in tensor memory at most
+inline int linear_kblocks(const MimirLinear& a) { return static_cast<int>((static_cast<long long>(a.n_in) * type_bytes(a.type) + LIN_BLOCK - 1) / LIN_BLOCK); }
+inline int linear_chunk(const MimirLinear& a) { return a.out_type == MIMIR_B200_T_F32 ? LIN_CHUNK_F32 * type_bytes(a.type) / LIN_BLOCK : LIN_CHUNK_BLOCKS; }
 
 // linear_tiles.cu (many rows): tiles of 256 rows x 256 features; linear_rows.cu (few): 128 features and up to 256 rows
 double linear_tiles_us(const MimirLinear& a, bool gated);

@@ -82,8 +82,9 @@ __device__ __forceinline__ void add_eight(const Eight& e, int type, float (&v)[8
 }
 
 // FOURS: how many times four warps take the results.  Sixteen warps where a CTA has the SM to itself: each has its units one after the other, some
-// 0.9 us for 16 rows of a gated pair.
-template <bool F8, bool GATED, bool F32, int FOURS>
+// 0.9 us for 16 rows of a gated pair.  HELD: not 0 where the CTA's share of n_in is more than a sum in tensor memory
+// takes (linear.cuh): how many times 16 sums a thread holds then.
+template <bool F8, bool GATED, int HELD, int FOURS>
 __global__ void __launch_bounds__(64 + 128 * FOURS, FOURS == 2 ? 2 : 1)
 linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_up,
                    const __grid_constant__ RowParams rp) {
@@ -155,7 +156,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
   pdl_early_if(rp.early);
   pdl_wait();
 
-  // tensor memory: the sums; behind them (results of F32) two regions that the instructions add up in
+  // tensor memory: the sums; HELD: two such regions that the instructions add up in by turns, the whole in the first at the end
   const uint32_t region = static_cast<uint32_t>(G * n);
   const int quad = warp & 3, four = (warp - 2) >> 2;
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -183,12 +184,12 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     bool ready = false, ok = true;
     for (int b = b0; b < b1 && ok;) {
       uint32_t d = tmem;
-      if constexpr (F32) {
+      if constexpr (HELD > 0) {
         if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.err_word, 113)) break;
         tcgen05_fence_after();
-        d = tmem + (1 + acc) * region;
+        d = tmem + acc * region;
       }
-      const int from = b, end = F32 ? min(b1, b + p.chunk) : b1;
+      const int from = b, end = HELD ? min(b1, b + p.chunk) : b1;
       for (; b < end; ++b) {
         if (!__all_sync(0xffffffffu, ready) && !mbar_wait_warp(&full_bar[stage], phase, abort_flag, p.err_word, 114)) { ok = false; break; }
         tcgen05_fence_after();
@@ -214,7 +215,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         __syncwarp();
       }
       if (!ok) break;
-      if (one) umma_commit(&acc_full[F32 ? acc : 0]);
+      if (one) umma_commit(&acc_full[acc]);
       __syncwarp();
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -256,11 +257,10 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
       if (i < n) x_scales[i] = x_row0 + i < p.rows ? __ldg(p.x_scale + x_row0 + i) : 0.0f;
     }
     __syncwarp();
-    if constexpr (F32) {
-      // sums of a chunk at a time out of tensor memory, added up rounded, and the whole back into its first region
+    if constexpr (HELD > 0) {
+      // sums of a chunk at a time out of tensor memory, added up rounded, and the whole back into its first region (a warp's columns are its own)
       int acc = 0;
       uint32_t acc_phase = 0;
-      constexpr int HELD = 8 / FOURS;
       float v[HELD][16];  // 16 rows each, of a gated pair first the one, then the other
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
@@ -275,7 +275,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
           const uint32_t col = static_cast<uint32_t>((FOURS * i + four) * 16);
           if (col >= region || !busy) continue;
           float w[16];
-          tmem_ld_32x16(lanes + (1 + acc) * region + col, w);
+          tmem_ld_32x16(lanes + acc * region + col, w);
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[i][j] += w[j];
         }
@@ -298,8 +298,8 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     } else {
       ok = mbar_wait_warp(&acc_full[0], 0, abort_flag, p.err_word, 115);
     }
-    // (the rows' scales are there; sums of F32 change hands between a lane's two warps)
-    if (F8 || F32) result_warps_sync(RESULT_THREADS);
+    // (the rows' scales are there; sums taken out change hands between a lane's warps)
+    if (F8 || HELD > 0) result_warps_sync(RESULT_THREADS);
     tcgen05_fence_after();
   }
   if (rp.cluster > 1) {
@@ -407,6 +407,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
 struct RowShape {
   int rows_tile, row_tiles, features, cluster, per_sm, stages, stage_bytes, parts_at, turn_at, tmem_cols;
+  bool chunks;
   size_t smem;
   long long ctas;
   double us;
@@ -415,23 +416,23 @@ struct RowShape {
 // The shape of a launch with that many features to a CTA, `cluster` CTAs that share n_in, per_sm of them on an SM; false where it does not fit.
 bool shape_of(const MimirLinear& a, bool gated, int features, int cluster, int per_sm, RowShape* s) {
   const int g = gated ? 2 : 1, f32 = a.out_type == MIMIR_B200_T_F32;
-  // (of F32 two more regions that the sums are made in, and 64 of a thread's registers)
   const int most = (f32 ? 128 : 256) / g;
   s->row_tiles = (a.rows + most - 1) / most;
   s->rows_tile = round_up((a.rows + s->row_tiles - 1) / s->row_tiles, UNIT);
   s->features = features, s->cluster = cluster, s->per_sm = per_sm;
   s->ctas = static_cast<long long>(s->row_tiles) * ((a.n_out + features - 1) / features) * cluster;
-  const int kblocks = static_cast<int>((static_cast<long long>(a.n_in) * type_bytes(a.type) + LIN_BLOCK - 1) / LIN_BLOCK);
+  const int kblocks = linear_kblocks(a), need = (kblocks + cluster - 1) / cluster;  // stages that a CTA can fill at all
   if (cluster > 1 && per_sm > 1) return false;
   if (s->ctas > 0x3fffffffLL || (cluster > 1 && kblocks < 2 * cluster)) return false;
+  s->chunks = need > linear_chunk(a);
   s->tmem_cols = 32;
-  while (s->tmem_cols < (f32 ? 3 : 1) * g * s->rows_tile) s->tmem_cols *= 2;
+  while (s->tmem_cols < (s->chunks ? 2 : 1) * g * s->rows_tile) s->tmem_cols *= 2;
   if (s->tmem_cols > 512 / per_sm) return false;
   const int units = s->rows_tile / UNIT, parts = cluster == 1 ? 0 : cluster * ((units + cluster - 1) / cluster) * UNIT * g * RM * 4;
   s->stage_bytes = (g * features + s->rows_tile) * LIN_BLOCK;
   // (an instruction reads 128 rows from the start of the features' that it is given)
   const int pad = std::max(0, RM - features - s->rows_tile) * LIN_BLOCK;
-  const int space = (per_sm == 2 ? DYNAMIC_TWO : DYNAMIC) - 1024, need = (kblocks + cluster - 1) / cluster;  // stages that a CTA can fill at all
+  const int space = (per_sm == 2 ? DYNAMIC_TWO : DYNAMIC) - 1024;
   const int turns = (per_sm == 2 ? 2 : 4) * TURN;
   auto stages_in = [&](int bytes) { return bytes < 0 ? 0 : std::min(std::min(bytes / s->stage_bytes, MAX_STAGES), need); };
   s->stages = stages_in(space - pad - parts);
@@ -508,9 +509,9 @@ RowShape row_shape(const MimirLinear& a, bool gated) {
   return best;
 }
 
-template <bool F8, bool GATED, bool F32, int FOURS>
+template <bool F8, bool GATED, int HELD, int FOURS>
 int launch_as(const CUtensorMap (&maps)[3], const RowParams& p, const RowShape& s, cudaStream_t st) {
-  auto kern = linear_rows_kernel<F8, GATED, F32, FOURS>;
+  auto kern = linear_rows_kernel<F8, GATED, HELD, FOURS>;
   static PerDeviceOnce once;
   MB_TRY(once.run([&]() -> int {
     MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DYNAMIC));
@@ -522,8 +523,13 @@ int launch_as(const CUtensorMap (&maps)[3], const RowParams& p, const RowShape& 
 }
 template <bool F8, bool GATED>
 int launch_for(const CUtensorMap (&maps)[3], const RowParams& p, const RowShape& s, cudaStream_t st) {
-  if (p.l.out_type == MIMIR_B200_T_F32) return s.per_sm == 2 ? launch_as<F8, GATED, true, 2>(maps, p, s, st) : launch_as<F8, GATED, true, 4>(maps, p, s, st);
-  return s.per_sm == 2 ? launch_as<F8, GATED, false, 2>(maps, p, s, st) : launch_as<F8, GATED, false, 4>(maps, p, s, st);
+  const int region = (GATED ? 2 : 1) * s.rows_tile;  // (at most 256, of two CTAs to an SM 128: tensor memory)
+  if (s.per_sm == 2) {
+    if (!s.chunks) return launch_as<F8, GATED, 0, 2>(maps, p, s, st);
+    return region <= 64 ? launch_as<F8, GATED, 2, 2>(maps, p, s, st) : launch_as<F8, GATED, 4, 2>(maps, p, s, st);
+  }
+  if (!s.chunks) return launch_as<F8, GATED, 0, 4>(maps, p, s, st);
+  return region <= 128 ? launch_as<F8, GATED, 2, 4>(maps, p, s, st) : launch_as<F8, GATED, 4, 4>(maps, p, s, st);
 }
 
 // The shapes that this thread asked for last (looking through all of them takes longer than a launch).

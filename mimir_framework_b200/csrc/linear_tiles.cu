@@ -10,7 +10,7 @@
 // Four where the results bound the kernel, with few inputs, rows off their boundary or a residual (rows x inputs x features, with four and with two: 12 153 x
 // 192 x 1 728 16.4 us, 18.1; 4 486 x 1 344 x 11 456 with residual 119, 134; off the boundary 3 040 x 4 162 x 2 190 with residual 57, 65, gated 4 000 x 1 024
 // x 4 001 59, 69); two where the instructions do, as a thread then has 168 registers (8 192 x 1 024 x 4 096 50.5, 49.5; gated 8 192 x 512 x 4 096 63, 59).
-// Results of F32 are taken out every 256 inputs and added up in registers: the tensor core's additions truncate.
+// Sums of more inputs than linear.cuh leaves to the tensor core are taken out a chunk at a time and added up in registers (CHUNKS).
 #include <algorithm>
 #include <cmath>
 
@@ -185,7 +185,7 @@ __device__ __forceinline__ void write_out(const LinearParams& p, const CUtensorM
   }
 }
 
-template <bool F8, bool GATED, bool F32, int PARTS>
+template <bool F8, bool GATED, bool CHUNKS, int PARTS>
 __global__ void __launch_bounds__(64 + 128 * PARTS, 1)
 linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_up,
                     const __grid_constant__ CUtensorMap map_out, const __grid_constant__ TileParams tp) {
@@ -372,7 +372,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
         write_out<64 / PARTS, 4 / PARTS>(p, map_out, z, row0, col0, turn, flip);
       };
-      if constexpr (F32) {
+      if constexpr (CHUNKS) {
         constexpr int HELD = TN / PARTS / 32;
         float v[HELD][32];
 #pragma unroll
@@ -441,9 +441,9 @@ TileShape tile_shape(const MimirLinear& a, bool gated) {
   return s;
 }
 
-template <bool F8, bool GATED, bool F32, int PARTS>
+template <bool F8, bool GATED, bool CHUNKS, int PARTS>
 int launch_as(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
-  auto kern = linear_tiles_kernel<F8, GATED, F32, PARTS>;
+  auto kern = linear_tiles_kernel<F8, GATED, CHUNKS, PARTS>;
   static PerDeviceOnce once;
   MB_TRY(once.run([&]() -> int {
     MB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
@@ -455,8 +455,9 @@ int launch_as(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, 
 }
 template <bool F8, bool GATED>
 int launch_for(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
-  if (p.l.out_type == MIMIR_B200_T_F32) return launch_as<F8, GATED, true, 2>(maps, p, grid, st);
-  const bool many = p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (K blocks: both sides at the top)
+  const bool chunks = p.l.kblocks > p.l.chunk, f32 = p.l.out_type == MIMIR_B200_T_F32;
+  const bool many = !f32 && p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (K blocks: both sides at the top)
+  if (chunks) return many ? launch_as<F8, GATED, true, 4>(maps, p, grid, st) : launch_as<F8, GATED, true, 2>(maps, p, grid, st);
   return many ? launch_as<F8, GATED, false, 4>(maps, p, grid, st) : launch_as<F8, GATED, false, 2>(maps, p, grid, st);
 }
 
