@@ -18,10 +18,10 @@ namespace mb {
 constexpr int LIN_BLOCK = 128;   // bytes of a row in a K block
 constexpr int LIN_W_BOX = 64;    // weight rows of a TMA box
 // How much is added up in the tensor core before the sum is taken out and added rounded, since an instruction truncates, by up to 2^-22 of the magnitudes:
-// for results of F32 256 inputs (2^-18; E4M3 2^-19), of 16 bits 64 K blocks, 256 instructions (2^-14, an eighth of fp16's half step, at worst; a sum whose
-// terms have either sign loses some 2^-17 of itself).  With 16 blocks products of 2 048 rows took 3 to 5 % longer, in 8 bits 6 to 12 %; with 64 those
-// of more inputs 1 to 3 %, the others nothing.
-constexpr int LIN_CHUNK_F32 = 256, LIN_CHUNK_BLOCKS = 64;
+// for results of F32 256 inputs (2^-18; E4M3 2^-19), of 16 bits 96 K blocks, 384 instructions (2^-13.4, a fifth of fp16's half step, at worst; a sum whose
+// terms have either sign loses some 2^-17 of itself).  With 16 blocks products of 2 048 rows took 3 to 5 % longer, in 8 bits 6 to 12 %; with 96 only
+// those of more inputs do, 1 to 3 % (with 64 also rows off their boundary, where the results are the bound: 3 040 x 4 162 x 2 190 with residual 8 %).
+constexpr int LIN_CHUNK_F32 = 256, LIN_CHUNK_BLOCKS = 96;
 
 struct LinearParams {
   const float* x_scale;

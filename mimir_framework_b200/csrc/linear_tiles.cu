@@ -455,9 +455,8 @@ int launch_as(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, 
 }
 template <bool F8, bool GATED>
 int launch_for(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
-  const bool chunks = p.l.kblocks > p.l.chunk, f32 = p.l.out_type == MIMIR_B200_T_F32;
-  const bool many = !f32 && p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (K blocks: both sides at the top)
-  if (chunks) return many ? launch_as<F8, GATED, true, 4>(maps, p, grid, st) : launch_as<F8, GATED, true, 2>(maps, p, grid, st);
+  if (p.l.kblocks > p.l.chunk) return launch_as<F8, GATED, true, 2>(maps, p, grid, st);
+  const bool many = p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (K blocks: both sides at the top)
   return many ? launch_as<F8, GATED, false, 4>(maps, p, grid, st) : launch_as<F8, GATED, false, 2>(maps, p, grid, st);
 }
 
