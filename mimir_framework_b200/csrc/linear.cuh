@@ -103,16 +103,50 @@ __device__ __forceinline__ float relu_nan(float x) {
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + 2^t): an exponential and a reciprocal of 2^-22 each; rounding t costs |t| 2^-24 of 2^t
-__device__ __forceinline__ float logistic(float t) {
-  float e, r;
+// 1 / (1 + 2^t): an exponential of 2^-22, a reciprocal of 2^-23 and an addition; below 2^-126 zero.  With d: 2^t (1 + d) for a small d, t up to 126.9
+__device__ __forceinline__ float exp2_fast(float t) {
+  float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return e;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float sigmoid_fast(float x) { return logistic(x * -1.442695041f); }
+__device__ __forceinline__ float logistic(float t) { return reciprocal_fast(1.0f + exp2_fast(t)); }
+__device__ __forceinline__ float logistic(float t, float d) {
+  const float e = exp2_fast(t);
+  return reciprocal_fast(1.0f + fmaf(e, d, e));
+}
+// 1 / (1 + exp(-x)).  Rounding t alone would cost |x| 2^-24 of the exponential, so what it loses goes back in, as in silu2 (epilogue.cuh).
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  const float n = x > 64.0f ? -64.0f : -x, t = fminf(n * 1.44269504f, 126.9f);
+  return logistic(t, fmaf(t, 1.904654e-9f, fmaf(t, -0.693147182f, n)));
+}
+// GELU of two values as gelu_ref has it, x / (1 + exp(-2u)), for results of F32: the exponent -2u log2 e = C x (1 + K x^2) is some 460 where the result
+// is about to vanish, and each of its roundings would cost as many units of the exponential, so every product's rest is kept (by fused
+// multiply-adds) and put back in.  (4 096 x 1 024 x 4 096 57 us; with gelu_ref, 1e-6 of the value off at x = -5, 49.)
+__device__ __forceinline__ void gelu2_f32(float& x0, float& x1) {
+  // (the exponential is 0 or beyond fp32 from 16 on; not a number comes back in with the last product)
+  const float a0 = fminf(fmaxf(x0, -16.0f), 16.0f), a1 = fminf(fmaxf(x1, -16.0f), 16.0f);
+  auto both = [](float v) { return pack2(v, v); };
+  const unsigned long long a = pack2(a0, a1), ns = mul2(a, pack2(-a0, -a1)), s_rest = fma2(a, a, ns);  // ns: -x^2
+  const unsigned long long nq = fma2(both(0.044715f), ns, both(-1.0f));                                // -(1 + K x^2)
+  unsigned long long q_rest = fma2(both(-0.044715f), ns, add2(nq, both(1.0f)));
+  q_rest = fma2(both(0.044715f), s_rest, fma2(both(-1.5461444e-9f), ns, q_rest));
+  const unsigned long long h = mul2(a, both(-2.3022082f)), nh = mul2(a, both(2.3022082f));             // C x
+  const unsigned long long nh_rest = fma2(a, both(1.2948402e-8f), fma2(a, both(2.3022082f), h));
+  const unsigned long long nt = mul2(h, nq);                                                           // -C x (1 + K x^2)
+  const unsigned long long d = mul2(fma2(nh_rest, nq, fma2(h, q_rest, fma2(nh, nq, nt))), both(0.693147182f));
+  float t0, t1, r0, r1;
+  unpack2(nt, t0, t1);
+  const unsigned long long e = pack2(exp2_fast(fminf(-t0, 126.9f)), exp2_fast(fminf(-t1, 126.9f)));
+  unpack2(add2(fma2(e, d, e), both(1.0f)), r0, r1);
+  unpack2(mul2(pack2(x0, x1), pack2(reciprocal_fast(r0), reciprocal_fast(r1))), x0, x1);
+}
 // tanh |x| = 1 - 2 / (1 + exp(2 |x|)), from 1/2 on, where the difference loses a bit; below its series x - x^3 / 3 + 2 x^5 / 15 - ... (next term 1e-7 of the
-// value at 1/2).  (tanhf, called for each element: 3 000 x 192 x 5 800 74 us.)
+// value at 1/2).  (tanhf, called for each element: 3 000 x 192 x 5 800 74 us, so 25.)
 __device__ __forceinline__ float tanh_fast(float x) {
   const float a = fabsf(x), s = x * x;
   float p = 3.5921281e-3f;            // 21844 / 6081075
@@ -124,13 +158,19 @@ __device__ __forceinline__ float tanh_fast(float x) {
   const float small = fmaf(x * s, p, x), large = fmaf(-2.0f, logistic(a * 2.885390082f), 1.0f);
   return a < 0.5f ? small : copysignf(large, x);
 }
+// Within 10 units of 2^-24 of its value for results of F32; GELU of 16 bits within its exponent's |2u| 2^-22 besides.
 template <int N>
-__device__ __forceinline__ void activate(float (&v)[N], int act) {
+__device__ __forceinline__ void activate(float (&v)[N], int act, int out_type) {
   switch (act) {
     case -1: break;
     case MIMIR_B200_ELT_GELU:
+      if (out_type == MIMIR_B200_T_F32) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = gelu_ref(v[j]);
+        for (int j = 0; j < N; j += 2) gelu2_f32(v[j], v[j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = gelu_ref(v[j]);
+      }
       break;
     case MIMIR_B200_ELT_SILU:
 #pragma unroll

@@ -378,7 +378,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             if constexpr (GATED) y[j] += up_bias;
           }
         }
-        activate(z, p.act);
+        activate(z, p.act, p.out_type);
 #pragma unroll
         for (int j = 0; j < 16; ++j) turn[j * RM + quad * 32 + lane] = GATED ? z[j] * y[j] : z[j];
       }

@@ -364,7 +364,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const float* const my_cols = cols - col00;  // (+ column)
       auto finish = [&](float (&z)[32], float (&u)[32], int col0) {
         scaled<F8>(z, sx, my_cols + (GATED ? 2 : 1) * EACH + col0, my_cols + col0);
-        activate(z, p.act);
+        activate(z, p.act, p.out_type);
         if constexpr (GATED) {
           scaled<F8>(u, sx, my_cols + 3 * EACH + col0, my_cols + EACH + col0);
 #pragma unroll

@@ -91,3 +91,63 @@ def test_sums_of_either_sign(backend, n_in, type_, out_type):
         v = z.clamp_min(0) * y
         far = ((out.double() - v).abs() / (off + half_step(out_type) * (v.abs() + off) + tiny)).max().item()
         assert far <= 1, (rows, n_out, far)
+
+
+# ---- activations ------------------------------------------------------------------------------------------------------------------------
+def arguments():
+    """Every size that fp32 has to tell apart, both signs; the last ones are for the ends of the range."""
+    g = torch.Generator("cuda").manual_seed(1)
+    small = torch.exp2(torch.rand(16384, generator=g, device="cuda") * 37 - 30)
+    line = torch.linspace(-110, 110, 32764, device="cuda")
+    return torch.cat([small, -small, line, torch.tensor([0.0, 1e30, -1e30, 64.0], device="cuda")])
+
+
+def exact_act(z, name):
+    if name == "gelu":
+        return z / (1 + torch.exp(-2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z**3)))
+    if name == "tanh":
+        return torch.tanh(z)
+    return (z if name == "silu" else 1) / (1 + torch.exp(-z))
+
+
+@pytest.mark.parametrize("name", ["gelu", "silu", "tanh", "sigmoid"])
+@pytest.mark.parametrize("rows", [1, 300, 5000])
+@pytest.mark.parametrize("gated", [False, True])
+def test_activations_of_f32_results(backend, name, rows, gated):
+    """Over the whole range, by way of the bias: within an exponential of 2^-22, a reciprocal of 2^-23 and four roundings, 10 units of 2^-24 of the value
+    (tanh's difference 1 - 2 / (1 + e) takes 7 of the first six and one of its own).  A reciprocal below 2^-126 is zero."""
+    z = arguments()
+    n_in, n_out = 64, z.numel()
+    x, w = torch.zeros(rows, n_in, dtype=torch.bfloat16, device="cuda"), torch.ones(n_out, n_in, dtype=torch.bfloat16, device="cuda")
+    out, one = torch.empty(rows, n_out, device="cuda"), torch.ones(n_out, device="cuda")
+    more = dict(up=w.data_ptr(), up_stride=n_in, up_bias=one.data_ptr()) if gated else {}
+    a = backend.linear(x.data_ptr(), w.data_ptr(), out.data_ptr(), rows, n_in, n_out, BF16, F32, n_in, n_in, n_out, bias=z.data_ptr(), activation=ACTS[name], **more)
+    (backend.dev_gated_linear if gated else backend.dev_linear)(a)
+    torch.cuda.synchronize()
+    backend.check_device()
+    want = exact_act(z.double(), name)
+    want = torch.where(want.isnan(), 0.0, want)  # (-1e30 / infinity)
+    flushed = 2.0**-126 * (z.double().abs().clamp_max(128) if name in ("gelu", "silu") else 1.0)
+    bound = want.abs() * 10 * 2.0**-24 + flushed
+    assert (out == out[0]).all()
+    off = (out[0].double() - want).abs()
+    worst = torch.where(bound > 0, off / bound, 0.0).argmax()
+    assert (off <= bound).all(), (z[worst].item(), (off / bound)[worst].item())
+
+
+@pytest.mark.parametrize("name", ["gelu", "silu", "tanh", "sigmoid", "relu"])
+@pytest.mark.parametrize("out_type", [F32, F16])
+@pytest.mark.parametrize("rows", [2, 3000])
+def test_activations_of_infinities_and_of_what_is_not_a_number(backend, name, out_type, rows):
+    z = torch.tensor([math.inf, -math.inf, math.nan, 1.0, -math.nan, 0.0, -0.0, 3e38, -3e38] * 30, device="cuda")
+    x, w = torch.zeros(rows, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(z.numel(), 64, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty(rows, z.numel(), dtype=TORCH[out_type], device="cuda")
+    backend.dev_linear(backend.linear(x.data_ptr(), w.data_ptr(), out.data_ptr(), rows, 64, z.numel(), BF16, out_type, 64, 64, z.numel(), bias=z.data_ptr(), activation=ACTS[name]))
+    torch.cuda.synchronize()
+    backend.check_device()
+    top, nan, big = math.inf, math.nan, 3e38 if out_type == F32 else math.inf
+    want = {"relu": [top, 0, nan, 1, nan, 0, 0, big, 0], "tanh": [1, -1, nan, math.tanh(1), nan, 0, 0, 1, -1], "sigmoid": [1, 0, nan, 1 / (1 + math.exp(-1)), nan, 0.5, 0.5, 1, 0],
+            # (x / (1 + exp(..)) has no limit at -infinity that its own arithmetic finds)
+            "silu": [top, nan, nan, 1 / (1 + math.exp(-1)), nan, 0, 0, big, 0], "gelu": [top, nan, nan, 0.8411919906, nan, 0, 0, big, 0]}[name]
+    want = torch.tensor(want, device="cuda").repeat(30)
+    assert torch.allclose(out.float(), want.expand(rows, -1), rtol=2.0**-11, atol=1e-7, equal_nan=True)
