@@ -3,8 +3,8 @@
 //   s = x + residual,  v = s / sqrt(mean(s^2) + eps) * gamma,  y = v, or codes of 8 bits and their scale
 //
 // One pass: a row lies in the registers of the threads that share it (eight elements at a time, so that loads and stores are 16 bytes), its
-// sum of squares and, for codes, its largest magnitude are each one meeting of these threads.  Statistics are fp32.  Codes are those
-// of an IEEE division by the scale, as in the cache.
+// sum of squares and, for codes, its largest magnitude are each one meeting of these threads.  Statistics are fp32.  Codes of rows
+// without the norm are those of an IEEE division by the scale, as in the cache; of a norm's values see finish_row.
 #include <algorithm>
 
 #include "common.h"
@@ -236,18 +236,18 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
         r = root_reciprocal(fmaf(meet<WARP, false>(rest, buf[0]), p.inv_n, p.eps * down * down));
       }
     }
-    // For codes the root stays out of the elements, as it cancels in their quotients by the largest: a rounding less.  (Rows so large that s gamma
-    // might leave fp32's range take it in.)
-    const bool later = TY == MIMIR_B200_T_E4M3 && r > 0x1p-20f;
-    if (later) root = r;
+    // For codes only the root's power of two goes into the elements, which it leaves exact; the rest of it, from one to two, cancels in their
+    // quotients by the largest: a rounding less, and s gamma has v's range.  (No root: one of a mean that is zero, infinite or not a number.)
+    if (TY == MIMIR_B200_T_E4M3 && r > 0.0f && r < INFINITY) {
+      root = __uint_as_float((__float_as_uint(r) & 0x007fffffu) | 0x3f800000u);
+      r = __uint_as_float(__float_as_uint(r) & 0x7f800000u);
+    }
     const Pair r2 = pack2(r, r);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int col = v * step + col0;
-      if (!later) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], r2);
-      }
+      for (int i = 0; i < 4; ++i) f[v][i] = mul2(f[v][i], r2);
       if (p.gamma) {
         Pair g[4];
         to_pairs<MIMIR_B200_T_F32>(row_load8<MIMIR_B200_T_F32, VEC>(reinterpret_cast<const char*>(p.gamma), col, p.n, apart), g);
