@@ -18,6 +18,7 @@ namespace mb {
 namespace {
 
 constexpr int NR_WARP_THREADS = 128;  // of a CTA whose warps have a row each
+constexpr int MEETINGS = 3;           // of a row's threads, over words of their own (a CTA that meets has 96 threads at least)
 constexpr int NR_MAX_STAGES = 8, NR_RING = 108 * 1024;  // rows ahead at most, bytes of them in a CTA
 
 struct NormParams {
@@ -139,7 +140,8 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {
   return d;
 }
 
-// A number of each thread of a row, joined; every thread has the result (`buf`: 24 words of the CTA's, of one meeting).
+// A number of each thread of a row, joined; every thread has the result.  `buf`: 24 words of the CTA's.  Between two meetings over the same words
+// lies another one over others, or a barrier: a thread may still read when the next has gone on.
 template <bool WARP, bool MAX>
 __device__ __forceinline__ float meet(float v, float* buf) {
 #pragma unroll
@@ -180,7 +182,7 @@ __device__ __forceinline__ float root_reciprocal(float x) {
 // instructions and 47 us element by element, 29 M and 40 us so).  A row that is not `live` takes part in the meetings and leaves nothing.
 // NORM: 0, 1, or -1, which is what the call says (the ring's registers do not hold both kinds of codes).
 template <int TX, int TY, int V, bool WARP, bool VEC, int NORM = -1>
-__device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[2][32]) {
+__device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[MEETINGS][32]) {
   const int col0 = !VEC && apart ? t : t * 8;
   if (p.sum && live) {
     char* const sum = p.sum + row * p.sum_row;
@@ -217,7 +219,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
         for (int e = 0; e < 8; e += 2) top = max_abs3(s[e], s[e + 1], top);
       }
       if (!(top < INFINITY)) top = INFINITY;  // (not a number is as good as infinite here)
-      top = meet<WARP, true>(top, buf[1]);
+      top = meet<WARP, true>(top, buf[2]);
       if (top > 0.0f && top < INFINITY) {
         const int k = max(-100, min(126, ilogbf(top)));
         const float down = scalbnf(1.0f, -k);
@@ -325,9 +327,9 @@ constexpr int norm_ctas() { return WARP ? (V == 4 ? 4 : 8) : V == 2 ? (TX == MIM
 
 template <int TX, int TY, int V, bool WARP, bool VEC>
 __global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WARP, V>()) norm_rows_serve_kernel(const __grid_constant__ NormParams p) {
-  __shared__ __align__(16) float buf[2][32];
+  __shared__ __align__(16) float buf[MEETINGS][32];
   pdl_early_if(p.early);
-  if (!WARP && threadIdx.x < 64) buf[threadIdx.x >> 5][threadIdx.x & 31] = 0.0f;
+  if (!WARP && threadIdx.x < MEETINGS * 32) buf[threadIdx.x >> 5][threadIdx.x & 31] = 0.0f;
   pdl_wait();
   const int row = WARP ? blockIdx.x * (NR_WARP_THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
   if (WARP && row >= p.rows) return;
@@ -362,11 +364,11 @@ template <int TX, int TY, int NORM>
 __global__ void __launch_bounds__(512, 2) norm_rows_ring_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t bars[NR_MAX_STAGES];
-  __shared__ __align__(16) float buf[2][32];
+  __shared__ __align__(16) float buf[MEETINGS][32];
   __shared__ volatile int abort_word;
   const int t = threadIdx.x, step = blockDim.x * 8, apart = gridDim.x;
   const uint32_t bytes = static_cast<uint32_t>(p.n) * type_bytes(TX);
-  if (t < 64) buf[t >> 5][t & 31] = 0.0f;
+  if (t < MEETINGS * 32) buf[t >> 5][t & 31] = 0.0f;
   if (t == 0) {
     for (int s = 0; s < p.stages; ++s) mbar_init(&bars[s], 1);
     abort_word = 0;
