@@ -23,6 +23,8 @@ constexpr int LIN_W_BOX = 64;    // weight rows of a TMA box
 // those of more inputs do, 1 to 3 % (with 64 also rows off their boundary, where the results are the bound: 3 040 x 4 162 x 2 190 with residual 8 %).
 constexpr int LIN_CHUNK_F32 = 256, LIN_CHUNK_BLOCKS = 96;
 
+// (Scales and biases are read by ordinary loads behind pdl_wait: the norm that makes the scales may be the kernel before, still at work when this one starts,
+// and a load that goes by memory which does not change while the kernel runs has no claim to see them.)
 struct LinearParams {
   const float* x_scale;
   const float* w_scale;

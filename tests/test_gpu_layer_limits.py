@@ -1,4 +1,4 @@
-"""A layer's products where their sums are long."""
+"""A layer's products where their sums are long, their arguments far out, or their calls close together."""
 import math
 
 import pytest
@@ -151,3 +151,39 @@ def test_activations_of_infinities_and_of_what_is_not_a_number(backend, name, ou
             "silu": [top, nan, nan, 1 / (1 + math.exp(-1)), nan, 0, 0, big, 0], "gelu": [top, nan, nan, 0.8411919906, nan, 0, 0, big, 0]}[name]
     want = torch.tensor(want, device="cuda").repeat(30)
     assert torch.allclose(out.float(), want.expand(rows, -1), rtol=2.0**-11, atol=1e-7, equal_nan=True)
+
+
+# ---- calls that follow one another ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("rows,n_in,n_out", [(1, 512, 640), (40, 1024, 2048), (300, 512, 1024), (1100, 768, 512)])
+def test_scales_of_the_kernel_before(backend, rows, n_in, n_out, captured):
+    """Codes and scales made anew in the same buffers by the norm directly ahead of each product: every product takes its own, as with a pause between."""
+    turns = 24
+    xs = torch.stack([torch.randn(rows, n_in, generator=torch.Generator("cuda").manual_seed(i), device="cuda") * 2.0 ** (i % 7 - 3) for i in range(turns)])
+    w = Operand(n_out, n_in, E4M3, 1, 1 / math.sqrt(n_in))
+    codes, scales = torch.empty(rows, n_in, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(rows, device="cuda")
+    outs = [torch.empty(turns, rows, n_out, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+
+    def turn(i, out, stream):
+        backend.dev_norm_rows(backend.norm_rows(xs[i].data_ptr(), codes.data_ptr(), rows, n_in, F32, E4M3, n_in, n_in, y_scale=scales.data_ptr(), norm=False), stream)
+        backend.dev_linear(backend.linear(codes.data_ptr(), w.at(), out[i].data_ptr(), rows, n_in, n_out, E4M3, BF16, n_in, w.stride, n_out, x_scale=scales.data_ptr(), w_scale=w.scale_at()), stream)
+
+    for i in range(turns):
+        turn(i, outs[0], 0)
+        torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                for i in range(turns):
+                    turn(i, outs[1], torch.cuda.current_stream().cuda_stream)
+            graph.replay()
+            graph.replay()
+        else:
+            for _ in range(5):
+                for i in range(turns):
+                    turn(i, outs[1], stream.cuda_stream)
+    torch.cuda.synchronize()
+    backend.check_device()
+    assert torch.equal(outs[0], outs[1])
