@@ -23,7 +23,7 @@ constexpr int LIN_W_BOX = 64;    // weight rows of a TMA box
 // those of more inputs do, 1 to 3 % (with 64 also rows off their boundary, where the results are the bound: 3 040 x 4 162 x 2 190 with residual 8 %).
 constexpr int LIN_CHUNK_F32 = 256, LIN_CHUNK_BLOCKS = 96;
 
-// (Scales and biases are read by ordinary loads behind pdl_wait: the norm that makes the scales may be the kernel before, still at work when this one starts,
+// (Scales and biases are read by load_float, behind pdl_wait: the norm that makes the scales may be the kernel before, still at work when this one starts,
 // and a load that goes by memory which does not change while the kernel runs has no claim to see them.)
 struct LinearParams {
   const float* x_scale;
@@ -57,6 +57,11 @@ int make_result_map(CUtensorMap* map, const void* base, int type, long long rows
 
 namespace {
 
+__device__ __forceinline__ float load_float(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)

@@ -244,17 +244,17 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     if (!GATED && p.residual) fetch(mine);
     // all that the results need besides the sums, while these are made
     if (feature < limit) {
-      if constexpr (F8) w_scale = p.w_scale[feature];
-      if constexpr (F8 && GATED) up_scale = p.up_scale[feature];
-      if (p.bias) bias = p.bias[feature];
-      if (GATED && p.up_bias) up_bias = p.up_bias[feature];
+      if constexpr (F8) w_scale = load_float(p.w_scale + feature);
+      if constexpr (F8 && GATED) up_scale = load_float(p.up_scale + feature);
+      if (p.bias) bias = load_float(p.bias + feature);
+      if (GATED && p.up_bias) up_bias = load_float(p.up_bias + feature);
       if (!GATED && p.residual)  // (into L2)
         for (int i = u0 * UNIT + four; i < u1 * UNIT && x_row0 + i < p.rows; i += FOURS)
           prefetch_line(p.residual + (x_row0 + i) * p.residual_row + static_cast<long long>(feature) * size);
     }
     if constexpr (F8) {
       const int i = static_cast<int>(threadIdx.x) - 64;
-      if (i < n) x_scales[i] = x_row0 + i < p.rows ? p.x_scale[x_row0 + i] : 0.0f;
+      if (i < n) x_scales[i] = x_row0 + i < p.rows ? load_float(p.x_scale + x_row0 + i) : 0.0f;
     }
     __syncwarp();
     if constexpr (HELD > 0) {

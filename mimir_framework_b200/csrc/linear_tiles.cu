@@ -340,13 +340,13 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (t >= items) return;
       int tm, tn, wide, each, mine;
       const int cut = tile_of(tp, t, tm, tn), col00 = my_columns(tn, cut, wide, each, mine), row = (2 * tm + rank) * TM + quad * 32 + lane;
-      if (F8 && row < p.rows) next_sx = p.x_scale[row];
+      if (F8 && row < p.rows) next_sx = load_float(p.x_scale + row);
 #pragma unroll
       for (int i = 0; i < HOLD; ++i) {
         const int which = i * 32 / EACH, col = col00 + i * 32 % EACH + lane;
         if (!F8 && which >= (GATED ? 2 : 1)) break;
         const float* from = GATED ? (which == 0 ? p.bias : which == 1 ? p.up_bias : which == 2 ? p.w_scale : p.up_scale) : which == 0 ? p.bias : p.w_scale;
-        next_cols[i] = from && col < p.n_out ? from[col] : 0.0f;
+        next_cols[i] = from && col < p.n_out ? load_float(from + col) : 0.0f;
       }
     };
     fetch(first);
