@@ -91,11 +91,11 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
   constexpr int G = GATED ? 2 : 1, RESULT_THREADS = 128 * FOURS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 4];
+  __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 5];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_word;
   __shared__ float x_scales[F8 ? 256 : 1];
-  uint64_t *full_bar = bars, *empty_bar = bars + MAX_STAGES, *acc_full = bars + 2 * MAX_STAGES, *acc_empty = acc_full + 2;
+  uint64_t *full_bar = bars, *empty_bar = bars + MAX_STAGES, *acc_full = bars + 2 * MAX_STAGES, *drained = acc_full + 2, *acc_empty = acc_full + 3;
   volatile int* abort_flag = &abort_word;
 
   const LinearParams& p = rp.l;
@@ -122,9 +122,9 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     if (lane < rp.stages) {
       mbar_init(&full_bar[lane], 1);
       mbar_init(&empty_bar[lane], 1);
-    } else if (lane >= 28) {
-      mbar_init(&acc_full[lane - 28], lane < 30 ? 1 : RESULT_THREADS / 32);  // (acc_full[0, 1], acc_empty[0, 1])
-    } else if (lane == 27) {
+    } else if (lane >= 27) {
+      mbar_init(&acc_full[lane - 27], lane < 30 ? 1 : RESULT_THREADS / 32);  // (acc_full[0, 1], drained, acc_empty[0, 1])
+    } else if (lane == 26) {
       *abort_flag = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -165,16 +165,23 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     const bool one = elect_one();
     int stage = at_once == rp.stages ? 0 : at_once;
     uint32_t phase = at_once == rp.stages ? 1 : 0;
-    for (int b = b0 + at_once; b < b1; ++b) {
+    int issued = at_once;
+    for (; b0 + issued < b1; ++issued) {
       if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 111)) break;
-      if (one) load_block(stage, b);
+      if (one) load_block(stage, b0 + issued);
       __syncwarp();
       if (++stage == rp.stages) { stage = 0; phase ^= 1; }
     }
     // what was asked for has landed and been used (or the abort flag is up) before the ring becomes something else
-    for (int s = 0; s < rp.stages; ++s) {
-      if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 112)) break;
+    bool ok = true;
+    for (int s = 0; s < rp.stages && ok; ++s) {
+      ok = mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 112);
       if (++stage == rp.stages) { stage = 0; phase ^= 1; }
+    }
+    if (!ok) {  // a wait gave up: nothing may still be on its way into shared memory when the CTA ends
+      int still = 0;
+      for (int i = max(0, issued - rp.stages); i < issued; ++i)
+        mbar_wait_warp(&full_bar[i % rp.stages], static_cast<uint32_t>((i / rp.stages) & 1), &still, p.err_word, 116);
     }
   } else if (warp == 1) {
     const bool one = elect_one();
@@ -185,7 +192,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     for (int b = b0; b < b1 && ok;) {
       uint32_t d = tmem;
       if constexpr (HELD > 0) {
-        if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.err_word, 113)) break;
+        if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.err_word, 113)) { ok = false; break; }
         tcgen05_fence_after();
         d = tmem + acc * region;
       }
@@ -218,6 +225,12 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
       if (one) umma_commit(&acc_full[acc]);
       __syncwarp();
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+    if (!ok) {  // ... nor an instruction at work
+      int still = 0;
+      if (one) umma_commit(drained);
+      __syncwarp();
+      mbar_wait_warp(drained, 0, &still, p.err_word, 117);
     }
   }
 

@@ -196,7 +196,8 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* acc_full = empty_bar + STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* drained = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const LinearParams& p = tp.l;
@@ -216,6 +217,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 2 * EPI_WARPS);  // (the leader's collects both CTAs' warps)
     }
+    mbar_init(drained, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -235,7 +237,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const bool one = elect_one();
     const CUtensorMap* const wmap = GATED && rank ? &map_up : &map_w;
     constexpr int per_block = F8 ? LIN_BLOCK : LIN_BLOCK / 2;
-    int stage = 0;
+    int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int t = first; t < items && ok; t += step) {
@@ -257,13 +259,25 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           if (cut < 0) tma_load_2d_pair(base + A_BYTES + W_BYTES / 2, wmap, fb, kb * per_block, w_row + LIN_W_BOX);
         }
         __syncwarp();
+        if (issued < STAGES) ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
     }
     // what was asked for has landed and been used (or the abort flag is up) before the CTA leaves
+    int last = stage;
+    uint32_t last_phase = phase;
     for (int s = 0; s < STAGES; ++s) {
-      if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 102)) break;
+      if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.err_word, 102)) { ok = false; break; }
       if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    }
+    if (!ok && rank == 0) {
+      // a wait gave up: nothing may still be on its way into shared memory when the CTA ends (the barriers count both CTAs' copies, and the other leaves with
+      // this one)
+      int still = 0;
+      for (int s = 0; s < issued; ++s) {
+        if (--last < 0) { last = STAGES - 1; last_phase ^= 1; }
+        mbar_wait_warp(&full_bar[last], last_phase, &still, p.err_word, 106);
+      }
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -307,6 +321,12 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           __syncwarp();
           if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
+      }
+      if (!ok) {  // ... nor an instruction at work
+        int still = 0;
+        if (one) umma_commit_pair(mapa_shared(smem_u32(drained), 0));
+        __syncwarp();
+        mbar_wait_warp(drained, 0, &still, p.err_word, 107);
       }
     }
   } else {

@@ -179,12 +179,12 @@ __device__ __forceinline__ float root_reciprocal(float x) {
 
 // A row from the sums s that its threads hold on: V vectors of eight elements each; WARP: a row to a warp, else to the CTA.  Instructions bound it
 // where memory does not, so two elements go through one wherever there is such a one (8 192 rows of 4 096 with residual to codes took 37 M
-// instructions and 47 us element by element, 29 M and 40 us so).  A row that is not `live` takes part in the meetings and leaves nothing.
+// instructions and 47 us element by element, 29 M and 40 us so).
 // NORM: 0, 1, or -1, which is what the call says (the ring's registers do not hold both kinds of codes).
 template <int TX, int TY, int V, bool WARP, bool VEC, int NORM = -1>
-__device__ __forceinline__ void finish_row(const NormParams& p, int row, bool live, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[MEETINGS][32]) {
+__device__ __forceinline__ void finish_row(const NormParams& p, int row, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[MEETINGS][32]) {
   const int col0 = !VEC && apart ? t : t * 8;
-  if (p.sum && live) {
+  if (p.sum) {
     char* const sum = p.sum + row * p.sum_row;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -283,7 +283,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
       top = meet<WARP, true>(top, buf[0]);
     }
     const float part = __fmul_rn(top, 1.0f / 448.0f);
-    if (t == 0 && live) p.y_scale[row] = __fmul_rn(part, root);
+    if (t == 0) p.y_scale[row] = __fmul_rn(part, root);
     // Without the norm codes of the IEEE quotients by one reciprocal, as quotient_codes has them (a zero's sign aside): those of 16-bit values are often
     // just between two codes.  Of a norm's values products with 448 / largest (`again` is zero), which is nearer to the quotients by the
     // largest itself: of 33 M codes 20 % fewer fall on the other side of a border than by the rounded scale.
@@ -293,7 +293,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int col = v * step + col0;
-      if (col >= p.n || !live) break;
+      if (col >= p.n) break;
       float s[8];
       if (quick) {
 #pragma unroll
@@ -313,7 +313,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, bool li
     for (int v = 0; v < V; ++v) {
       float s[8];
       from_pairs(f[v], s);
-      if (live) row_store8<TY, VEC>(y, v * step + col0, p.n, apart, pack8<TY>(s));
+      row_store8<TY, VEC>(y, v * step + col0, p.n, apart, pack8<TY>(s));
     }
   }
 }
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(norm_threads<TX, WARP, V>(), norm_ctas<TX, WAR
     }
   }
   if (!WARP) __syncthreads();  // (the words of no warp)
-  finish_row<TX, TY, V, WARP, VEC>(p, row, true, t, step, apart, f, buf);
+  finish_row<TX, TY, V, WARP, VEC>(p, row, t, step, apart, f, buf);
 }
 
 // The same for many long rows of 16 bits without a residual: few CTAs fit into the registers, so the rows come through a ring in shared memory by
@@ -388,18 +388,26 @@ __global__ void __launch_bounds__(512, 2) norm_rows_ring_kernel(const __grid_con
   uint32_t phase = 0;
 #pragma unroll 1
   for (long long row = blockIdx.x; row < p.rows; row += apart) {
-    // (a thread whose wait gives up stays for the others' meetings, leaves nothing and asks for nothing more)
     const bool ok = mbar_wait(&bars[stage], phase, &abort_word, p.err_word, 121);
     const char* x = reinterpret_cast<const char*>(ring + stage * bytes);
     Pair f[4][4];
 #pragma unroll
     for (int v = 0; v < 4; ++v) to_pairs<TX>(row_load8<TX, true>(x, v * step + t * 8, p.n, 0), f[v]);
-    __syncthreads();
-    if (t == 0 && ok && next < p.rows) {
+    if (!__syncthreads_and(ok)) {  // a wait gave up: nothing may still be on its way into shared memory when the CTA ends
+      if (t == 0) {
+        int still = 0;
+        for (; row < next; row += apart) {
+          mbar_wait(&bars[stage], phase, &still, p.err_word, 122);
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+      }
+      break;
+    }
+    if (t == 0 && next < p.rows) {
       ask(static_cast<int>(next), stage);
       next += apart;
     }
-    finish_row<TX, TY, 4, false, true, NORM>(p, static_cast<int>(row), ok, t, step, 0, f, buf);
+    finish_row<TX, TY, 4, false, true, NORM>(p, static_cast<int>(row), t, step, 0, f, buf);
     if (++stage == p.stages) { stage = 0; phase ^= 1; }
   }
 }
