@@ -1,5 +1,9 @@
 """A layer's products where their sums are long, their arguments far out, or their calls close together."""
 import math
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -187,3 +191,151 @@ def test_scales_of_the_kernel_before(backend, rows, n_in, n_out, captured):
     torch.cuda.synchronize()
     backend.check_device()
     assert torch.equal(outs[0], outs[1])
+
+
+# ---- rows, and calls, that do not know of one another ----------------------------------------------------------------------------------------
+def run_product(backend, x, scale, w, u, type_, out_type, name, n_out, residual=None):
+    out = torch.empty(x.shape[0], n_out, dtype=TORCH[out_type], device="cuda")
+    more = dict(residual=residual.data_ptr(), residual_stride=n_out) if residual is not None else dict(up=u.at(), up_stride=u.stride, up_scale=u.scale_at())
+    a = backend.linear(x.data_ptr(), w.at(), out.data_ptr(), x.shape[0], w.x.shape[1], n_out, type_, out_type, x.stride(0), w.stride, n_out,
+                       x_scale=None if scale is None else scale.data_ptr(), w_scale=w.scale_at(), activation=ACTS[name], **more)
+    (backend.dev_linear if residual is not None else backend.dev_gated_linear)(a)
+    torch.cuda.synchronize()
+    return out
+
+
+def rows_of(t, order):
+    return t.view(torch.uint8 if t.dtype == torch.float8_e4m3fn else t.dtype)[order].view(t.dtype)
+
+
+@pytest.mark.parametrize("type_,out_type", [(BF16, BF16), (F16, F32), (E4M3, BF16), (E4M3, F32)])
+@pytest.mark.parametrize("rows", [2, 16, 33, 100, 250, 700, 2500])
+@pytest.mark.parametrize("n_in,n_out", [(1008, 500), (4096, 640), (13008, 200)])
+def test_a_row_has_its_result_wherever_it_is_and_whatever_is_beside_it(backend, n_in, n_out, rows, type_, out_type):
+    x, w, u = Operand(rows, n_in, type_, 1), Operand(n_out, n_in, type_, 2, 1 / math.sqrt(n_in)), Operand(n_out, n_in, type_, 3, 1 / math.sqrt(n_in))
+    other = Operand(rows, n_in, type_, 4, 3.0)
+    res = torch.randn(rows, n_out, device="cuda").to(TORCH[out_type])
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(rows)).cuda()
+    kept = torch.arange(rows, device="cuda") % 3 == 1
+    for residual in (res, None):
+        first = run_product(backend, x.x, x.scale, w, u, type_, out_type, "silu", n_out, residual)
+        moved = run_product(backend, rows_of(x.x, order), None if x.scale is None else x.scale[order], w, u, type_, out_type, "silu", n_out, None if residual is None else residual[order])
+        assert torch.equal(moved, first[order])
+        bits = torch.uint8 if type_ == E4M3 else x.x.dtype
+        mixed = torch.where(kept[:, None], x.x.view(bits), other.x.view(bits)).view(x.x.dtype)
+        scale = None if x.scale is None else torch.where(kept, x.scale, other.scale)
+        beside = run_product(backend, mixed, scale, w, u, type_, out_type, "silu", n_out, residual)
+        assert torch.equal(beside[kept], first[kept])
+    backend.check_device()
+
+
+@pytest.mark.parametrize("rows,n_in,n_out", [(3, 2048, 20000), (40, 4096, 1024), (300, 4096, 2048), (1500, 1024, 1536)])
+def test_replay_on_new_rows_of_8_bits(backend, rows, n_in, n_out):
+    x, w, u = Operand(rows, n_in, E4M3, 1), Operand(n_out, n_in, E4M3, 2, 0.02), Operand(n_out, n_in, E4M3, 3, 0.02)
+    out = torch.empty(2, rows, n_out, dtype=torch.bfloat16, device="cuda")
+    codes, scale = torch.empty(rows, n_out, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(rows, device="cuda")
+    a = linear_args(x, w, out[0], E4M3, BF16, rows, n_in, n_out)
+    g = linear_args(x, w, out[1], E4M3, BF16, rows, n_in, n_out, up=u.at(), up_stride=u.stride, up_scale=u.scale_at(), activation=ACTS["silu"])
+    norm = backend.norm_rows(out[0].data_ptr(), codes.data_ptr(), rows, n_out, BF16, E4M3, n_out, n_out, y_scale=scale.data_ptr())
+    stream = torch.cuda.Stream()
+
+    def run(s):
+        backend.dev_linear(a, s)
+        backend.dev_norm_rows(norm, s)
+        backend.dev_gated_linear(g, s)
+
+    run(0)
+    torch.cuda.synchronize()
+    want = [out.clone(), codes.view(torch.uint8).clone(), scale.clone()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run(torch.cuda.current_stream().cuda_stream)
+    x.x.view(torch.uint8).copy_(x.x.view(torch.uint8).flip(0))
+    x.scale.copy_(x.scale.flip(0))
+    out.zero_(), scale.zero_(), codes.view(torch.uint8).zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph.replay()
+        graph.replay()
+    torch.cuda.synchronize()
+    backend.check_device()
+    assert torch.equal(out, want[0].flip(1)) and torch.equal(codes.view(torch.uint8), want[1].flip(0)) and torch.equal(scale, want[2].flip(0))
+
+
+def test_calls_of_several_threads(backend):
+    """Each with its own stream and sizes, all at once: what a thread finds out about a launch's shape is its own."""
+    jobs = []
+    for i in range(6):
+        sizes = [(1 + 37 * j + i, 256 + 320 * ((i + j) % 5), 200 + 504 * ((i * j) % 4)) for j in range(8)]
+        made = [(Operand(r, k, E4M3 if (i + j) % 2 else BF16, j), Operand(n, k, E4M3 if (i + j) % 2 else BF16, j + 50, 0.05), torch.empty(2, r, n, device="cuda"))
+                for j, (r, k, n) in enumerate(sizes)]
+        jobs.append((sizes, made, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(job, turn, stream):
+        sizes, made, _ = job
+        for j, ((r, k, n), (x, w, out)) in enumerate(zip(sizes, made)):
+            backend.dev_linear(linear_args(x, w, out[turn], E4M3 if x.scale is not None else BF16, F32, r, k, n), stream)
+
+    def work(job):
+        try:
+            torch.cuda.set_device(0)
+            for _ in range(10):
+                run(job, 1, job[2].cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for job in jobs:
+        run(job, 0, 0)
+    torch.cuda.synchronize()
+    backend.check_device()
+    for _, made, _ in jobs:
+        for _, _, out in made:
+            assert torch.equal(out[0], out[1])
+
+
+FIRST = '''
+import sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+from mimir_framework_b200 import abi, runtime as rt
+rt.init(0)
+rows = {rows}
+g = torch.Generator("cuda").manual_seed(1)
+x = torch.randn(rows, 1024, generator=g, device="cuda").to(torch.bfloat16)
+w, u = (torch.randn(768, 1024, generator=g, device="cuda").mul_(0.03).to(torch.bfloat16) for _ in range(2))
+y, out, h = torch.empty_like(x), torch.empty(rows, 768, device="cuda"), torch.empty(rows, 768, device="cuda")
+norm = rt.norm_rows(x.data_ptr(), y.data_ptr(), rows, 1024, abi.T_BF16, abi.T_BF16, 1024, 1024)
+a = rt.linear(y.data_ptr(), w.data_ptr(), out.data_ptr(), rows, 1024, 768, abi.T_BF16, abi.T_F32, 1024, 1024, 768)
+p = rt.linear(y.data_ptr(), w.data_ptr(), h.data_ptr(), rows, 1024, 768, abi.T_BF16, abi.T_F32, 1024, 1024, 768, up=u.data_ptr(), up_stride=1024, activation=abi.ELT_SILU)
+def run(s):
+    rt.dev_norm_rows(norm, s), rt.dev_linear(a, s), rt.dev_gated_linear(p, s)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    run(torch.cuda.current_stream().cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (y, out, h)]
+for t in (y, out, h):
+    t.zero_()
+run(0)
+torch.cuda.synchronize()
+rt.check_device()
+assert all(torch.equal(s, t) for s, t in zip(got, (y, out, h))) and out.abs().max() > 0
+print("same")
+'''
+
+
+@pytest.mark.parametrize("rows", [3, 2000])
+def test_the_first_calls_of_a_process_are_captured(rows):
+    tests = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST.format(root=os.path.dirname(tests), tests=tests, rows=rows)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
