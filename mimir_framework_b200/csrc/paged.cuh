@@ -160,47 +160,6 @@ __device__ __forceinline__ Raw8<T> pack8(const float (&f)[8]) {
   return r;
 }
 
-// ---- codes of 8 bits ------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-__device__ __forceinline__ float min3_nan(float a, float b, float c) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// the largest magnitude of eight, not a number if one of them is none
-__device__ __forceinline__ float top_of_8(const float (&f)[8]) {
-  return fmaxf(max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max3_nan(f[6], f[7], f[7])),
-               -min3_nan(min3_nan(f[0], f[1], f[2]), min3_nan(f[3], f[4], f[5]), min3_nan(f[6], f[7], f[7])));
-}
-
-// Codes of f / s, correctly rounded quotients by one reciprocal for all of them: with r = 1 / s rounded to nearest (0 for s = 0), q = f r and
-// q + (f - q s) r with fused multiply-adds is the IEEE quotient (Markstein, IBM J. Res. Dev. 34, 1990), where nothing under- or overflows:
-// s above 2^-80, for smaller f the code is zero either way.  Quotients of 16-bit values are often just between two codes, so their last
-// bits count.  27 K tokens of 8 key heads of 128 to int8: 90 us with an IEEE division an element, 55 so.
-template <int CT>
-__device__ __forceinline__ Raw8<CT> quotient_codes(const float (&f)[8], float s, float r) {
-  float q[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float n = __fmul_rn(f[e], r);
-    q[e] = __fmaf_rn(__fmaf_rn(-n, s, f[e]), r, n);
-    if constexpr (CT != MIMIR_B200_T_I8) q[e] = copysignf(q[e], f[e]);  // (zeros)
-  }
-  if constexpr (CT != MIMIR_B200_T_I8) return pack8<CT>(q);
-  Raw8<CT> codes;
-  uint32_t w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(q[e] + 12582912.0f);  // 1.5 * 2^23: the nearest integer in the low bits, as two's complement
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    codes.w[i] = __byte_perm(__byte_perm(w[4 * i], w[4 * i + 1], 0x0040), __byte_perm(w[4 * i + 2], w[4 * i + 3], 0x0040), 0x5410);
-  return codes;
-}
-
 }  // namespace
 
 // the launches behind the C calls (serve.cu); arguments are checked there
