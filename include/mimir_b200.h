@@ -654,10 +654,11 @@ int mimir_b200_dev_sample_rows(const void* logits, int type, long long rows, int
 /* Rows between a layer's products.  s = x + residual (x alone where residual is NULL), in fp32; sum receives s in x's type.  With norm
  * != 0, v = s / sqrt(mean(s^2) + eps) * gamma over the n elements of the row, s before its rounding to sum; else v = s.  y receives v in
  * y_type: F32, F16, BF16, or E4M3 codes with one scale a row, y_scale = (largest finite magnitude of v) * (1 / 448 in fp32), codes of v / y_scale to
- * nearest: infinities become the largest code, what is not a number stays so.  Without the norm the quotient is the IEEE one, as dev_cache_write's;
- * of a norm's values its last bits depend on the order of the factors (s gamma is kept within fp32's range).  Sums of squares beyond that range are
- * formed once more with the row scaled down.  A row's own numbers decide about it alone.
- * sum may be x or residual, and y may be x or residual, with their stride and type; other overlaps are not allowed.  n up to 32 768. */
+ * nearest: infinities become the largest code, what is not a number stays so (zeros without eps among it: 0 / 0, and their scale is 0).
+ * Without the norm the quotient is the IEEE one, as dev_cache_write's; of a norm's values its last bits depend on the order of the factors.
+ * Sums of squares beyond fp32's range are formed once more with the row scaled down.  A row's own numbers decide about it alone.
+ * sum may be x or residual, and y may be x or residual, with their stride and type; other overlaps are not allowed.  n up to 32 768.  Rows of 16 bits
+ * that do not start on 16 bytes are read in whole 16 bytes: what lies beside them in these is read and dropped, and may be written meanwhile. */
 typedef struct MimirNormRows {
   const void* x;        /* [rows][n], rows x_stride elements apart */
   const void* residual; /* the same type, or NULL */

@@ -55,8 +55,7 @@ int launch_linear(const MimirLinear& a, bool gated, cudaStream_t st) {
   p.kblocks = linear_kblocks(a);
   p.chunk = linear_chunk(a);
   p.formats = a.type == MIMIR_B200_T_BF16 ? (1u << 7) | (1u << 10) : 0u;  // (half, E4M3: 0)
-  p.vec_out = on(a.out, p.out_row, 32) ? 32 : on(a.out, p.out_row, 16) ? 16 : 0;
-  p.vec_res = on(a.residual, p.residual_row, 32) ? 32 : on(a.residual, p.residual_row, 16) ? 16 : 0;
+  p.vec_out = on(a.out, p.out_row, 16), p.vec_res = on(a.residual, p.residual_row, 16);
   p.err_word = ctx().dev_error_word;
   return linear_rows_us(a, gated) <= linear_tiles_us(a, gated) ? launch_linear_rows(a, p, gated, st) : launch_linear_tiles(a, p, gated, st);
 }

@@ -18,10 +18,14 @@ namespace mb {
 constexpr int LIN_BLOCK = 128;   // bytes of a row in a K block
 constexpr int LIN_W_BOX = 64;    // weight rows of a TMA box
 // How much is added up in the tensor core before the sum is taken out and added rounded, since an instruction truncates, by up to 2^-22 of the magnitudes:
-// for results of F32 256 inputs (2^-18; E4M3 2^-19), of 16 bits 96 K blocks, 384 instructions (2^-13.4, a fifth of fp16's half step, at worst; a sum whose
-// terms have either sign loses some 2^-17 of itself).  With 16 blocks products of 2 048 rows took 3 to 5 % longer, in 8 bits 6 to 12 %; with 96 only
-// those of more inputs do, 1 to 3 % (with 64 also rows off their boundary, where the results are the bound: 3 040 x 4 162 x 2 190 with residual 8 %).
+// for results of F32 256 inputs (2^-18; E4M3 2^-19), of 16 bits 96 K blocks, 384 instructions (2^-13.4, a fifth of fp16's half step, at worst; a sum
+// whose terms have either sign loses some 2^-17 of itself).
+// F32, operands of bfloat16: 2.3e-7 of the result off from 256 inputs on (plain fp32 sums of 256 inputs 1.1e-7, of 4 096 6.1e-7).  With 128 inputs it would be
+// 1.2e-7, and 2 048 x 4 096 x 4 096 take 70 us instead of 58, 4 096 x 4 096 x 4 096 of E4M3, which loses nothing (4e-8 either way), 103 instead of 75.
+// 16 bits: with 16 blocks products of 2 048 rows took 3 to 5 % longer, in 8 bits 6 to 12 %; with 96 only those of more inputs do, 1 to 3 % (with 64 also
+// rows off their boundary, where the results are the bound: 3 040 x 4 162 x 2 190 with residual 8 %).
 constexpr int LIN_CHUNK_F32 = 256, LIN_CHUNK_BLOCKS = 96;
+static_assert(LIN_CHUNK_F32 % LIN_BLOCK == 0, "a sum is one K block at least, whatever the type");
 
 // (Scales and biases are read by load_float, behind pdl_wait: the norm that makes the scales may be the kernel before, still at work when this one starts,
 // and a load that goes by memory which does not change while the kernel runs has no claim to see them.)
@@ -37,7 +41,7 @@ struct LinearParams {
   int rows, n_out, out_type, act;
   int kblocks, chunk;               // K blocks of a product, and at most of a sum in tensor memory
   uint32_t formats;                 // instruction descriptor: operand formats
-  int vec_out, vec_res;             // result, residual: all rows on 32 bytes, on 16, or neither (0)
+  bool vec_out, vec_res;            // result, residual: all rows on 16 bytes
   int* err_word;
 };
 

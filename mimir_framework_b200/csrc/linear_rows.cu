@@ -11,7 +11,6 @@
 //   warp 0 TMA, warp 1 instructions, the other eight or sixteen results: 32 features and sixteen rows of x at a time.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "launch.cuh"
 #include "linear.cuh"
@@ -492,10 +491,12 @@ const ClusterTable* active_clusters() {
 }
 
 // The quickest shape by an estimate in us.  A round of CTAs loads (at most 120 KB an us each, 18.4 MB in all; a ring that does not hold all of a
-// CTA's blocks is waited for 0.34 us at a time) and multiplies (an instruction of 128 x N takes 46 cycles, from N = 61 on 0.75 N, a block 70 more),
-// or waits for the weights from memory, up to a tenth longer where SMs idle; then come 0.42 us for each unit of 16 rows that a warp finishes, and 1.85 and more for the meeting of a
-// cluster; of equals, CTAs of middling size.  The numbers are a fit to 228 products (1 to 2 048 rows, n_in 512 to 16 384, n_out 640 to 32 000, 16 and 8 bits, gated or not, up to 40
-// shapes each): the shape taken, or the kernel of tiles instead, is on average 2 % slower than the quickest, at worst 25 % (39 us against 49).
+// CTA's blocks is waited for 0.34 us at a time) and multiplies (an instruction of 128 x N takes 46 cycles, from N = 61 on 0.75 N, a block 70
+// more), or waits for the weights from memory, up to a tenth longer where SMs idle; then come 0.42 us for each unit of 16 rows that a warp
+// finishes, and 1.85 and more for the meeting of a cluster; of equals, CTAs of middling size.  The numbers were fitted to earlier forms of both
+// kernels.  With the present ones, over 228 products (1 to 2 048 rows, n_in 512 to 16 384, n_out 640 to 32 000, 16 and 8 bits, gated or not, up
+// to 46 shapes each): the shape taken, or the kernel of tiles instead, is on average 2.7 % slower than the quickest, half of them at most 0.4 %,
+// 20 more than 10 %, at worst 38 % (384 rows x 1 024 x 32 000 in 8 bits 29.2 us, in tiles 21.2).
 RowShape row_shape(const MimirLinear& a, bool gated) {
   RowShape best = {};
   best.us = 1e30;

@@ -7,9 +7,21 @@
 //   warp 0     TMA into a ring of five stages of 32 KB a CTA
 //   warp 1     (the leader's) issues the instructions for both
 //   the others results: two or four warps for each 32 rows, as many parts of the columns; 32 columns at a time through activation, gate and residual
-// Four where the results bound the kernel, with few inputs, rows off their boundary or a residual (rows x inputs x features, with four and with two: 12 153 x
-// 192 x 1 728 16.4 us, 18.1; 4 486 x 1 344 x 11 456 with residual 119, 134; off the boundary 3 040 x 4 162 x 2 190 with residual 57, 65, gated 4 000 x 1 024
-// x 4 001 59, 69); two where the instructions do, as a thread then has 168 registers (8 192 x 1 024 x 4 096 50.5, 49.5; gated 8 192 x 512 x 4 096 63, 59).
+// Four where the results bound the kernel, two where the instructions do, as a thread then has 168 registers.  The time with four over that with two, by the
+// K blocks of a product (8 192 rows x 4 096 features, off their boundary 4 000 x 4 001; without an activation, and with GELU):
+//                                           2          4          8         16         24         48         96
+//   16 bits                             .87 .78    .88 .80    .99 .80   1.05 .94  1.03 1.01  1.05  .98  1.03 1.00
+//   16 bits, residual                   .86 .77    .89 .78    .89 .82   1.02 .81  1.03  .90  1.01  .99   .99 1.01
+//   16 bits, off the boundary           .65 .69    .68 .70    .69 .71    .77 .73   .88  .79  1.02 1.05  1.01 1.02
+//   16 bits, off it with residual       .72 .72    .73 .72    .74 .73    .74 .74   .75  .74   .78  .82   .97  .96
+//   16 bits, gated                      .96 .90   1.03 .91   1.08 .93   1.15 1.04 1.02  .97  1.01 1.04  1.01 1.01
+//   16 bits, gated, off the boundary    .77 .78    .79 .79    .82 .80   1.01 .85  1.09 1.03  1.01 1.03  1.02 1.02
+//   E4M3                               1.00 .89   1.00 .90   1.00 .90   1.05 .95  1.05 1.03  1.02 1.00  1.03 1.01
+//   E4M3, residual                     1.00 .96   1.03 .97   1.06 .98   1.05 .98  1.06  .98  1.02 1.03   .95 1.02
+//   E4M3, off the boundary              .78 .76    .78 .77    .80 .78    .85 .80   .93  .86  1.04 1.02   .99 1.02
+//   E4M3, off it with residual          .70 .70    .71 .70    .71 .71    .73 .72   .74  .73   .85  .81  1.01  .95
+//   E4M3, gated                         .93 .90    .93 .91    .94 .91   1.02 1.12 1.01 1.01  1.08 1.03  1.02 1.01
+//   E4M3, gated, off the boundary       .78 .76    .80 .76    .81 .78    .85 .82  1.04 1.01  1.02 1.02  1.02  .99
 // Sums of more inputs than linear.cuh leaves to the tensor core are taken out a chunk at a time and added up in registers (CHUNKS).
 #include <algorithm>
 #include <cmath>
@@ -476,7 +488,7 @@ int launch_as(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, 
 template <bool F8, bool GATED>
 int launch_for(const CUtensorMap (&maps)[4], const TileParams& p, unsigned grid, cudaStream_t st) {
   if (p.l.kblocks > p.l.chunk) return launch_as<F8, GATED, true, 2>(maps, p, grid, st);
-  const bool many = p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (K blocks: both sides at the top)
+  const bool many = p.l.kblocks <= (p.l.vec_out ? (GATED ? 4 : p.l.residual ? 24 : 8) : p.l.residual ? 96 : 24);  // (both sides at the top)
   return many ? launch_as<F8, GATED, false, 4>(maps, p, grid, st) : launch_as<F8, GATED, false, 2>(maps, p, grid, st);
 }
 

@@ -179,7 +179,7 @@ __device__ __forceinline__ float root_reciprocal(float x) {
 
 // A row from the sums s that its threads hold on: V vectors of eight elements each; WARP: a row to a warp, else to the CTA.  Instructions bound it
 // where memory does not, so two elements go through one wherever there is such a one (8 192 rows of 4 096 with residual to codes took 37 M
-// instructions and 47 us element by element, 29 M and 40 us so).
+// instructions and 47 us element by element, 28 M and 40 us so).
 // NORM: 0, 1, or -1, which is what the call says (the ring's registers do not hold both kinds of codes).
 template <int TX, int TY, int V, bool WARP, bool VEC, int NORM = -1>
 __device__ __forceinline__ void finish_row(const NormParams& p, int row, int t, int step, int apart, Pair (&f)[V][4], float (&buf)[MEETINGS][32]) {
@@ -284,7 +284,7 @@ __device__ __forceinline__ void finish_row(const NormParams& p, int row, int t, 
     }
     const float part = __fmul_rn(top, 1.0f / 448.0f);
     if (t == 0) p.y_scale[row] = __fmul_rn(part, root);
-    // Without the norm codes of the IEEE quotients by one reciprocal, as quotient_codes has them (a zero's sign aside): those of 16-bit values are often
+    // Without the norm codes of the IEEE quotients by one reciprocal, as the cache's (a zero's sign aside): those of 16-bit values are often
     // just between two codes.  Of a norm's values products with 448 / largest (`again` is zero), which is nearer to the quotients by the
     // largest itself: of 33 M codes 20 % fewer fall on the other side of a border than by the rounded scale.
     const bool quick = finite && (part == 0.0f || part > 0x1p-80f);
